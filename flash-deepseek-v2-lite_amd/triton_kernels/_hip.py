@@ -87,6 +87,13 @@ _SIGS = {
     "dsv2_moe_grouped_gateup_shared_fp8": ([_p, _i32, _p, _p, _p, _i32, _i32, _p, _p, _p, _p, _i32, _p, _p, _p], _i32),
     "dsv2_moe_grouped_down_shared_fp8": ([_p, _i32, _p, _p, _i32, _i32, _p, _p, _p, _p, _p, _i32, _p, _p, _p], _i32),
     "dsv2_moe_combine_parts": ([_p, _p, _p, _i32, _p, _p, _p, _p, _f32, _p, _p], _i32),
+    "dsv2_paged_step": ([_p, _p, _i32, _p, _i64, _i32, _p, _i32, _i32, _i32, _p, _p, _p, _p, _p, _p], _i32),
+    "dsv2_paged_slots": ([_p, _p, _i32, _p, _i64, _i32, _i32, _i32, _p, _p, _p, _p, _p], _i32),
+    "dsv2_paged_write_fp4": ([_p, _i64, _i32, _p, _p, _i64, _i32, _i32, _p, _p], _i32),
+    "dsv2_paged_read_fp4": ([_p, _i64, _i32, _i32, _p, _i32, _p, _i64, _p, _p], _i32),
+    "dsv2_mla_paged_workspace_size": ([_i32, _i32, _i32, _i32, _i32], _i64),
+    "dsv2_mla_decode_paged_fp4": ([_p, _i64, _i64, _i32, _i32, _p, _i64, _i32, _i32, _p, _i64, _i32, _p, _i32, _p,
+                                   _i32, _f32, _p, _i64, _i64, _p, _i64, _p, _p], _i32),
 }
 
 EXPORTS = tuple(_SIGS)

@@ -37,6 +37,9 @@ extern "C" {
 
 /* bits a kernel ORs into the caller's device status word (int32, optional) */
 #define DSV2_DEVERR_CACHE_FULL 1  /* a cache write at or past a row's capacity was skipped */
+#define DSV2_DEVERR_NO_PAGE 2     /* a request of dsv2_paged_step found too few free pages    */
+#define DSV2_DEVERR_BAD_SLOT 4    /* a slot, page or position outside the pool or block table */
+#define DSV2_DEVERR_TOKENS 8      /* more new tokens than max_tokens                          */
 
 /* flags of dsv2_gemv_bf16 / dsv2_gemm_bf16 */
 #define DSV2_LINEAR_SWIGLU 1  /* W holds [gate; up] (2N rows): y = bf16(silu(bf16 g)) * bf16 u */
@@ -484,6 +487,67 @@ int dsv2_moe_combine(const void* ysorted, const int32_t* route_pos, const float*
 int dsv2_moe_combine_parts(const void* ysorted, const int32_t* route_pos, const float* weights, int rows,
                            const float* shared_parts, const void* residual, void* out, const void* next_norm_w,
                            float eps, void* xn_out, void* stream);
+
+/* ---- paged latent cache held in 4 bits ------------------------------------ */
+
+/* No reference counterpart (its cache is one expanded bf16 tensor, src/run.py:81-99).
+ *
+ * The cache of one layer is a pool of n_pages pages, page_stride bytes apart (>= 400 * page_size,
+ * 16-byte aligned); page_size is a power of two up to 1024, the same for all layers, and slot
+ * p * page_size + i names token i of page p.  A token takes 400 bytes: its 512 latent values as e2m1
+ * codes in blocks of 32, its 64 rotary keys in bf16 and one e8m0 scale per block.  A page holds
+ * page_size * 256 bytes of codes (two a byte, low nibble first), page_size * 128 bytes of rotary keys,
+ * page_size * 16 bytes of scales.  Block scale: the least power of two 2^e, -124 <= e <= 125, with
+ * max |x| <= 6 * 2^e (past 1.5 * 2^127 values saturate), byte e + 127; codes round to nearest, ties to
+ * even.  A block that holds an infinity or a NaN gets scale byte 255 and reads as NaN throughout.
+ *
+ * Request b's cached token t is token t % page_size of page block_table[b * table_stride + t / page_size].
+ */
+
+/* One step of the requests' lengths.  state [requests + 2]: the lengths, then head and count of the ring
+ * free_pages [n_pages] of free page numbers (free_pages[(head + i) % n_pages], i < count); delta
+ * [requests]: new tokens (> 0), tokens dropped from the end (< 0, at most all), or 0.  Pages follow:
+ * a growing request takes the ring's next pages into its table entries, a shrinking one puts its empty
+ * ones behind the count (free from the next step on).  state_out [requests + 2] (no overlap with
+ * state) is the state after the step, which reads nothing that it writes: repeated on the same state it
+ * gives the same.  New token i (requests in order, each one's tokens in order) gets slots[i],
+ * positions[i] and rows[i] = its request, i < max_tokens; entries past the last new token are -1.
+ * A request whose tokens do not fit the table's width, max_tokens or (a page needed) the free pages
+ * left by all requests before it keeps its length, its tokens get -1 and a DSV2_DEVERR_* bit is set.
+ * requests <= 4096. */
+int dsv2_paged_step(const int32_t* state, const int32_t* delta, int requests, int32_t* block_table,
+                    int64_t table_stride, int table_width, int32_t* free_pages, int n_pages, int page_size,
+                    int max_tokens, int32_t* state_out, int32_t* slots, int32_t* positions, int32_t* rows,
+                    int32_t* status, void* stream);
+
+/* Slots of the tokens [starts[b], starts[b] + counts[b]) of every request, one after the other, as in
+ * dsv2_paged_step; -1 past the last one and for positions or pages out of range. */
+int dsv2_paged_slots(const int32_t* starts, const int32_t* counts, int requests, const int32_t* block_table,
+                     int64_t table_stride, int table_width, int page_size, int max_tokens, int32_t* slots,
+                     int32_t* positions, int32_t* rows, int32_t* status, void* stream);
+
+/* Rounds row i (576 bf16: latent | rotary key, as dsv2_mla_prepare writes it) into slots[i] of the pool.
+ * A negative slot is skipped, one past the pool sets DSV2_DEVERR_BAD_SLOT; of two rows with one slot
+ * either may stay. */
+int dsv2_paged_write_fp4(const void* rows, int64_t row_stride, int n, const int32_t* slots, void* pages,
+                         int64_t page_stride, int n_pages, int page_size, int32_t* status, void* stream);
+
+/* The bf16 rows that slots hold (exact); zeros for a negative slot or one past the pool. */
+int dsv2_paged_read_fp4(const void* pages, int64_t page_stride, int n_pages, int page_size, const int32_t* slots,
+                        int n, void* out, int64_t out_stride, int32_t* status, void* stream);
+
+/* Absorbed-MLA attention of the queries q [tokens, heads, 576] (strides q_ts, q_hs; absorbed latent |
+ * rotated rotary part) over the requests' cached tokens: out[t, h, :512] = sum_s p_s latent_s, p = softmax
+ * of softmax_scale * q[t, h] . row_s.  Request b owns the query tokens [cu_q[b], cu_q[b + 1]), at most
+ * max_q of them (cu_q NULL: token b); they are its last cached ones: query j of n sees the tokens below
+ * lens[b] - n + j + 1.  A query that sees nothing gives zeros; query tokens of no request are left alone.
+ * workspace: dsv2_mla_paged_workspace_size bytes, 16-byte aligned. */
+int64_t dsv2_mla_paged_workspace_size(int requests, int max_q, int heads, int table_width, int page_size);
+int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_hs, int tokens, int heads, const void* pages,
+                              int64_t page_stride, int n_pages, int page_size, const int32_t* block_table,
+                              int64_t table_stride, int table_width, const int32_t* lens, int requests,
+                              const int32_t* cu_q, int max_q, float softmax_scale, void* out, int64_t out_ts,
+                              int64_t out_hs, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

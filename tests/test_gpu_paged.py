@@ -1,0 +1,577 @@
+"""The paged 4-bit latent cache on the GPU against plain implementations in 64 bits: block tables and
+slot maps exactly, the block format exactly (every bf16 value), attention within the bound that its
+roundings give, and the operators together as a serving loop uses them."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    from triton_kernels import _hip
+    from triton_kernels import paged_cache as P
+
+import paged_ref as R
+
+DEV = "cuda"
+BF = torch.bfloat16
+SCALE = 0.1147
+
+
+@pytest.fixture(autouse=True)
+def no_error_bits_left():
+    """No call but those that are meant to sets a device status bit."""
+    yield
+    P.check_paged_status()
+
+
+def rnd(*shape, seed=0, std=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device=DEV) * std).to(BF)
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def pool(n_pages, ps, fill=None):
+    """A pool of pages: every byte `fill`, or rows of normal values."""
+    pages = torch.full((n_pages, ps * R.TOKEN), 255 if fill is None else fill, dtype=torch.uint8, device=DEV)
+    if fill is None:
+        P.paged_cache_write_fp4(rnd(n_pages * ps, R.ROW, seed=n_pages), torch.arange(n_pages * ps, device=DEV).int(),
+                                pages)
+    return pages
+
+
+def batch(lens, ps, seed=0, spare=3, fill=None):
+    """(pages, table, the requests' rows in 64 bits): pages dealt out in random order; what no request
+    owns, the unused ends of their last pages included, is bytes 255 (NaN scales and keys)."""
+    rng = random.Random(seed)
+    need = [-(-n // ps) for n in lens]
+    order = list(range(sum(need) + spare))
+    rng.shuffle(order)
+    width = max(1, max(need))
+    table, at = [], 0
+    for n in need:
+        table.append(order[at:at + n] + [-1] * (width - n))
+        at += n
+    pages = torch.full((len(order), ps * R.TOKEN), 255, dtype=torch.uint8, device=DEV)
+    keys = []
+    for b, n in enumerate(lens):
+        rows = rnd(n, R.ROW, seed=seed * 1000 + b) if fill is None else fill(b, n)
+        t = torch.arange(n, device=DEV)
+        slots = i32(table[b])[t // ps].long() * ps + t % ps if n else t
+        P.paged_cache_write_fp4(rows, slots.int(), pages)
+        keys.append(R.held(rows))
+    return pages, i32(table), keys
+
+
+def same(got, want):
+    """Equal values, NaN where NaN."""
+    got, want = got.double(), want.double()
+    off = ~((got == want) | (got.isnan() & want.isnan()))
+    at = off.nonzero()[:4].tolist()
+    assert not at, [(i, float(got[tuple(i)]), float(want[tuple(i)])) for i in at] + [int(off.sum())]
+
+
+# --------------------------------------------------------------------------- block format
+def test_every_bf16_value_as_a_blocks_largest():
+    """Each of the 65,536 bf16 bit patterns as the first value of a block, 31 smaller ones beside it:
+    the bytes stand for the nearest values, blocks with inf or NaN read as NaN, reading is exact."""
+    bits = torch.arange(65536, device=DEV, dtype=torch.int32)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    top = bits.to(torch.int16).view(BF).float()
+    x = (torch.rand(65536, 32, device=DEV, generator=g) * 2 - 1) * torch.nan_to_num(top, 1.0, 1.0, 1.0)[:, None]
+    x = x.to(BF)
+    x[:, 0] = bits.to(torch.int16).view(BF)
+    # ties: halves of the code steps at the block's own scale
+    x[:, 1] = (x[:, 0].float() / 8).to(BF)
+    x[:, 2] = (x[:, 0].float() * 0.4375).to(BF)
+    rows = torch.cat([x.view(4096, 512), rnd(4096, 64)], 1)
+    pages = torch.zeros(64, 64 * R.TOKEN, dtype=torch.uint8, device=DEV)
+    slots = torch.randperm(4096, device=DEV).int()
+    P.paged_cache_write_fp4(rows, slots, pages)
+    want = R.held(rows)
+    same(R.stored(pages, slots, 64), want)
+    same(P.paged_cache_read_fp4(pages, slots), want)
+
+
+def test_every_code_between_its_neighbours():
+    """Values on a fine grid through one block scale: nearest code, ties to the even one."""
+    y = torch.arange(0, 256, device=DEV) / 32 - 3.96875
+    rows = torch.zeros(16, R.ROW, device=DEV)
+    rows[:, :512] = y.repeat(32).view(16, 512)
+    rows[:, 0:512:32] = 6.0
+    rows = rows.to(BF)
+    pages = torch.zeros(2, 16 * R.TOKEN, dtype=torch.uint8, device=DEV)
+    P.paged_cache_write_fp4(rows, torch.arange(16, device=DEV).int(), pages)
+    assert torch.equal(P.paged_cache_read_fp4(pages, torch.arange(16, device=DEV).int()).double(), R.held(rows))
+
+
+@pytest.mark.parametrize("ps", [1, 2, 16, 64, 1024])
+@pytest.mark.parametrize("n", [1, 3, 130])
+def test_write_and_read_by_slots(ps, n):
+    """Rows of a wider matrix into scattered slots of one layer of a page-major pool: the slots' bytes,
+    and no others, change; reading them back, unwritten and left-out ones, is exact."""
+    n_pages = max(3, 2 * n // ps + 1)
+    layers = torch.full((n_pages, 3, ps * R.TOKEN), 9, dtype=torch.uint8, device=DEV)
+    pages = layers[:, 1]
+    g = torch.Generator(device=DEV).manual_seed(n)
+    slots = torch.randperm(n_pages * ps, device=DEV, generator=g)[:n].int()
+    rows = rnd(n, 3648, seed=n)[:, 3648 - R.ROW:]
+    if n > 2:
+        slots[1] = -1
+        slots[n - 1] = -7
+    P.paged_cache_write_fp4(rows, slots, pages)
+    want = torch.full((n_pages * ps, R.ROW), -1.0, dtype=torch.float64, device=DEV)
+    live = slots >= 0
+    want[slots[live].long()] = R.held(rows)[live]
+    untouched = torch.ones(n_pages * ps, dtype=torch.bool, device=DEV)
+    untouched[slots[live].long()] = False
+    every = torch.arange(n_pages * ps, device=DEV)
+    got = R.stored(pages, every, ps)
+    assert torch.equal(got[~untouched], want[~untouched])
+    nine = R.stored(torch.full((1, R.TOKEN), 9, dtype=torch.uint8, device=DEV), torch.zeros(1, device=DEV), 1)
+    assert torch.equal(got[untouched], nine.expand(int(untouched.sum()), -1))
+    assert int((layers[:, 0] != 9).sum()) == 0 and int((layers[:, 2] != 9).sum()) == 0
+    out = torch.full((n, 600), 5.0, dtype=BF, device=DEV)
+    back = P.paged_cache_read_fp4(pages, slots, out=out[:, :R.ROW])
+    assert torch.equal(back[live].double(), R.held(rows)[live])
+    assert int((back[~live] != 0).sum()) == 0 and int((out[:, R.ROW:] != 5.0).sum()) == 0
+
+
+def test_slots_outside_the_pool_are_skipped_and_reported():
+    pages = pool(4, 16, fill=1)
+    before = pages.clone()
+    P.paged_cache_write_fp4(rnd(3, R.ROW), i32([64, 2 ** 31 - 1, -2 ** 31]), pages)
+    assert torch.equal(pages, before)
+    with pytest.raises(RuntimeError, match="outside the pool"):
+        P.check_paged_status()
+    got = P.paged_cache_read_fp4(pages, i32([64, 2 ** 31 - 1, -1]))
+    assert int((got != 0).sum()) == 0
+    with pytest.raises(RuntimeError, match="outside the pool"):
+        P.check_paged_status()
+
+
+def test_a_pool_past_four_gigabytes():
+    """Slots whose byte offsets pass 32 bits: written, read and attended."""
+    ps, n_pages = 64, 200_000  # 5.1 GB
+    pages = torch.empty(n_pages, ps * R.TOKEN, dtype=torch.uint8, device=DEV)
+    n = 100
+    table = i32([[n_pages - 1, 3]])
+    slots, _, _ = P.paged_slot_map(i32([0]), i32([n]), table, ps, n)
+    rows = rnd(n, R.ROW)
+    P.paged_cache_write_fp4(rows, slots, pages)
+    assert torch.equal(P.paged_cache_read_fp4(pages, slots).double(), R.held(rows))
+    q = rnd(1, 16, R.ROW, seed=1, std=0.3)
+    got = P.attention_decode_paged_fp4(q, pages, table, i32([n]), SCALE)
+    want, tol = R.attention(q[0], R.held(rows), n, SCALE)
+    assert ((got[0].double() - want).abs() <= tol).all()
+
+
+# --------------------------------------------------------------------------- block tables, slot maps
+def _state(alloc):
+    return i32(alloc.lens + [alloc.head, alloc.count])
+
+
+@pytest.mark.parametrize("n,ps,width,pages,cap", [(1, 64, 4, 9, 300), (5, 16, 7, 40, 90), (64, 32, 9, 400, 4000),
+                                                  (257, 1, 11, 1500, 900), (300, 64, 3, 500, 20000),
+                                                  (4096, 16, 4, 9000, 30000), (3, 1024, 2, 5, 3000)])
+def test_steps_follow_the_plain_allocator(n, ps, width, pages, cap):
+    """Random growth, truncation and retirement for several steps, pages, table columns and slots
+    running out at times; each step run twice on the same state."""
+    rng = random.Random(n * ps)
+    ring = list(range(pages))
+    rng.shuffle(ring)
+    ref = R.Allocator([0] * n, [[-5] * width for _ in range(n)], ring, rng.randrange(pages), pages, ps)
+    table, free, state = i32(ref.table), i32(ring), _state(ref)
+    errors = 0
+    for k in range(8):
+        room = width * ps
+        delta = []
+        for b in range(n):
+            kind = rng.random()
+            if kind < 0.35:
+                delta.append(1)
+            elif kind < 0.6:
+                delta.append(rng.randint(0, max(1, min(room, 2 * cap // n))))
+            elif kind < 0.75:
+                delta.append(-ref.lens[b])
+            elif kind < 0.9:
+                delta.append(-rng.randint(0, 2 * ps))
+            else:
+                delta.append(0)
+        d = i32(delta)
+        first = P.paged_cache_step(state, d, table, free, ps, cap)
+        after, slots, positions, rows = P.paged_cache_step(state, d, table, free, ps, cap)
+        want, e = ref.step(delta, cap)
+        errors |= e
+        assert all(torch.equal(x, y) for x, y in zip(first, (after, slots, positions, rows)))
+        assert after.tolist() == ref.lens + [ref.head, ref.count], k
+        assert [slots.tolist(), positions.tolist(), rows.tolist()] == want, k
+        assert free.tolist() == ref.ring and table.tolist() == ref.table, k
+        held = [p for b in range(n) for p in ref.table[b][:ref.pages(ref.lens[b])]]
+        spare = [ref.ring[(ref.head + i) % pages] for i in range(ref.count)]
+        assert sorted(held + spare) == list(range(pages))
+        state = after
+    if errors:
+        with pytest.raises(RuntimeError, match="were skipped"):
+            P.check_paged_status()
+
+
+def test_step_refuses_what_does_not_fit_request_by_request():
+    ps, width = 16, 4
+    ref = R.Allocator([64, 60, 0, 3, 0, 0], [list(range(4)), list(range(4, 8)), [9] * 4, [8, 9, 9, 9], [9] * 4, [9] * 4],
+                      list(range(10, 40)), 7, 3, ps)
+    table, free, state = i32(ref.table), i32(ref.ring), _state(ref)
+    # past the width; within a page; three pages; within a page; a page too many; a page, but none is left
+    delta = [1, 4, 48, 13, 1, 1]
+    after, slots, positions, rows = P.paged_cache_step(state, i32(delta), table, free, ps, 100)
+    want, _ = ref.step(delta, 100)
+    assert [slots.tolist(), positions.tolist(), rows.tolist()] == want and after.tolist()[:6] == [64, 64, 48, 16, 0, 0]
+    with pytest.raises(RuntimeError, match="outgrew its block table; no free page"):
+        P.check_paged_status()
+    huge = [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 0, 2 ** 31 - 1, -1]
+    ref2 = R.Allocator(ref.lens, ref.table, ref.ring, ref.head, ref.count, ps)
+    after2, slots, positions, rows = P.paged_cache_step(after, i32(huge), table, free, ps, 100)
+    want, _ = ref2.step(huge, 100)
+    assert after2.tolist() == ref2.lens + [ref2.head, ref2.count] and slots.tolist() == want[0]
+    with pytest.raises(RuntimeError, match="outgrew"):
+        P.check_paged_status()
+    # more tokens than slots: the request that passes them and those after it wait
+    after3, slots, _, rows = P.paged_cache_step(after2, i32([0, 5, 0, 0, 9, 1]), table, free, ps, 10)
+    assert after3.tolist()[:6] == [64, 5, 48, 16, 0, 0] and rows.tolist() == [1] * 5 + [-1] * 5
+    with pytest.raises(RuntimeError, match="max_tokens"):
+        P.check_paged_status()
+
+
+def test_step_with_corrupt_state_stays_in_bounds():
+    """A ring position, a count or a length out of range, a page number that is none: nothing outside
+    the tensors is touched, the slots are -1 and the status says so."""
+    guard = torch.full((3, 64), -3, dtype=torch.int32, device=DEV)
+    table, free = guard[1, :8].view(2, 4), guard[2, :6]
+    P.paged_cache_step(i32([-9, 2 ** 31 - 1, -4, 2 ** 31 - 1]), i32([5, -3]), table, free, 16, 8)
+    P.paged_cache_step(i32([3, 64, 99, -8]), i32([2, -64]), table, free, 16, 8)
+    assert int((guard[0] != -3).sum()) == 0 and int((guard[1, 8:] != -3).sum()) == 0
+    assert int((guard[2, 6:] != -3).sum()) == 0
+    with pytest.raises(RuntimeError, match="outside the pool"):
+        P.check_paged_status()
+
+
+@pytest.mark.parametrize("n", [1, 7, 256, 4096])
+def test_slot_map_of_ranges(n):
+    ps, width = 32, 6
+    rng = random.Random(n)
+    table = [[rng.randrange(1000) for _ in range(width)] for _ in range(n)]
+    starts = [rng.randint(0, 60) for _ in range(n)]
+    counts = [rng.choice([0, 0, 1, rng.randint(0, 100), -4]) for _ in range(n)]
+    want = [(table[b][t // ps] * ps + t % ps, t, b) for b in range(n) for t in range(starts[b], starts[b] + counts[b])]
+    total = len(want)
+    got = P.paged_slot_map(i32(starts), i32(counts), i32(table), ps, total + 4)
+    assert [list(x) for x in zip(*(want + [(-1,) * 3] * 4))] == [x.tolist() for x in got]
+    if total > 1:
+        short = P.paged_slot_map(i32(starts), i32(counts), i32(table), ps, total - 1)
+        assert [x.tolist() for x in short] == [x.tolist()[:total - 1] for x in got]
+        with pytest.raises(RuntimeError, match="more new tokens"):
+            P.check_paged_status()
+
+
+def test_slot_map_out_of_range():
+    table = i32([[3, -1], [4, 2 ** 30]])
+    slots, positions, rows = P.paged_slot_map(i32([-2, 15]), i32([3, 20]), table, 16, 30)
+    assert slots.tolist() == [-1] * 3 + [4 * 16 + 15] + [-1] * 26
+    with pytest.raises(RuntimeError, match="outside the pool or block table"):
+        P.check_paged_status()
+
+
+# --------------------------------------------------------------------------- attention
+def check(q, pages, table, lens, keys, nq=None, scale=SCALE, **kw):
+    """Attention of q [T, H, 576] against 64 bits, request by request."""
+    cu = None
+    if nq is not None:
+        cu = i32([sum(nq[:b]) for b in range(len(nq) + 1)])
+        kw = {"max_q": max(1, max(nq)), **kw}
+    got = P.attention_decode_paged_fp4(q, pages, table, i32(lens), scale, cu, **kw)
+    t = 0
+    for b, n in enumerate(nq or [1] * len(lens)):
+        for j in range(n):
+            want, tol = R.attention(q[t], keys[b], lens[b] - n + j + 1, scale)
+            off = (got[t].double() - want).abs()
+            assert (off <= tol).all(), (b, j, lens[b], float((off / tol.clamp(min=1e-300)).max()))
+            t += 1
+    return got
+
+
+@pytest.mark.parametrize("ps", [1, 16, 64, 1024])
+@pytest.mark.parametrize("lens", [[1], [0], [31, 32, 33, 0, 64], [63, 65, 127, 128, 129, 1, 5], [700, 0, 2049, 17]])
+def test_attention_lengths_and_pages(ps, lens):
+    pages, table, keys = batch(lens, ps, seed=len(lens))
+    check(rnd(len(lens), 16, R.ROW, seed=5, std=0.3), pages, table, lens, keys)
+
+
+@pytest.mark.parametrize("heads", [1, 3, 8, 16, 17, 40, 128])
+@pytest.mark.parametrize("nq", [[1, 1, 1], [3, 0, 5], [1, 2, 9]])
+def test_attention_heads_and_queries(heads, nq):
+    """Odd head counts; drafts of several tokens, one request without any, one with more of them than
+    it has tokens (the first ones then see nothing)."""
+    lens = [200, 70, 6]
+    pages, table, keys = batch(lens, 16, seed=heads)
+    check(rnd(sum(nq), heads, R.ROW, seed=heads, std=0.3), pages, table, lens, keys, nq)
+
+
+@pytest.mark.parametrize("lens", [[20000], [9000, 10, 15001], [513] * 40 + [12345], [2048] * 300])
+def test_attention_long_and_many(lens):
+    pages, table, keys = batch(lens, 64, seed=7)
+    check(rnd(len(lens), 16, R.ROW, seed=6, std=0.3), pages, table, lens, keys)
+
+
+@pytest.mark.parametrize("std", [0.0, 3.0, 30.0])
+def test_attention_flat_and_sharp(std):
+    """Equal scores, and scores whose softmax has one token left; a scale of its own."""
+    lens = [300, 1100]
+    pages, table, keys = batch(lens, 64, seed=2)
+    check(rnd(2, 16, R.ROW, seed=3, std=std), pages, table, lens, keys, scale=0.07)
+
+
+def test_attention_rising_scores():
+    """Each tile's scores above all before it: the running maximum moves every time."""
+    def fill(b, n):
+        x = rnd(n, R.ROW, seed=b)
+        x[:, 512:] = torch.linspace(-20, 20 + b, n, device=DEV)[:, None].to(BF)
+        return x
+
+    lens = [3000, 257]
+    pages, table, keys = batch(lens, 32, fill=fill)
+    q = rnd(2, 16, R.ROW, seed=4, std=0.1)
+    q[:, :8, 512:] = 0.4
+    q[:, 8:, 512:] = -0.4
+    check(q, pages, table, lens, keys)
+
+
+def test_attention_strides():
+    """Queries and outputs inside wider tensors, a block table inside a wider one, page-major layers."""
+    lens, ps = [40, 333, 90], 32
+    pages, table, keys = batch(lens, ps, seed=1)
+    layers = torch.full((pages.shape[0], 2, pages.shape[1]), 255, dtype=torch.uint8, device=DEV)
+    layers[:, 1] = pages
+    wide = torch.full((3, table.shape[1] + 5), 10 ** 9, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    q = rnd(16, 3, 640, seed=9, std=0.3).transpose(0, 1)[:, :, 64:]
+    out = torch.full((3, 20, 520), 7.0, dtype=BF, device=DEV)
+    got = check(q, layers[:, 1], wide[:, :table.shape[1]], lens, keys, out=out[:, 2:18, :512])
+    assert got.data_ptr() == out[:, 2:18].data_ptr()
+    assert int((out[:, :2] != 7).sum()) + int((out[:, 18:] != 7).sum()) + int((out[:, :, 512:] != 7).sum()) == 0
+
+
+def test_attention_leaves_query_tokens_of_no_request():
+    lens = [50, 60]
+    pages, table, keys = batch(lens, 16)
+    q = rnd(7, 16, R.ROW, std=0.3)
+    out = torch.full((7, 16, 512), 7.0, dtype=BF, device=DEV)
+    P.attention_decode_paged_fp4(q, pages, table, i32(lens), SCALE, i32([1, 3, 5]), 2, out)
+    assert int((out[0] != 7).sum()) == 0 and int((out[5:] != 7).sum()) == 0
+    for t, (b, seen) in enumerate([(0, 49), (0, 50), (1, 59), (1, 60)]):
+        want, tol = R.attention(q[1 + t], keys[b], seen, SCALE)
+        assert ((out[1 + t].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("what", ["latent", "latent_inf", "rope", "q"])
+def test_attention_nan_reaches_only_those_who_see_it(what):
+    """A NaN or an infinity in the last cached token: the queries before it stay as they are."""
+    lens, nq = [100, 40], [3, 2]
+
+    def fill(b, n):
+        x = rnd(n, R.ROW, seed=b)
+        if b == 0:
+            if what.startswith("latent"):
+                x[-1, 100] = float("nan") if what == "latent" else float("-inf")
+            elif what == "rope":
+                x[-1, 520] = float("nan")
+        return x
+
+    pages, table, keys = batch(lens, 32, fill=fill)
+    q = rnd(5, 16, R.ROW, std=0.3)
+    if what == "q":
+        q[2, 4, 7] = float("nan")
+    got = P.attention_decode_paged_fp4(q, pages, table, i32(lens), SCALE, i32([0, 3, 5]), 3)
+    t = 0
+    for b, n in enumerate(nq):
+        for j in range(n):
+            want, tol = R.attention(q[t], keys[b], lens[b] - n + j + 1, SCALE)
+            bad = want.isnan().any(-1)  # a NaN score makes the whole head NaN
+            assert torch.equal(bad, torch.tensor([t == 2 and (what != "q" or h == 4) for h in range(16)], device=DEV))
+            assert got[t][bad].isnan().all()
+            assert ((got[t].double() - want).abs() <= tol)[~bad].all()
+            t += 1
+
+
+def test_attention_infinite_scores():
+    """Scores of -inf count nothing; nothing but them is NaN, and so is a score of +inf."""
+    def fill(b, n):
+        x = rnd(n, R.ROW, seed=b)
+        x[:, 512:] = 0
+        at = {0: [3, 40], 1: list(range(n)), 2: [50]}[b]
+        x[at, 512] = float("-inf") if b < 2 else float("inf")
+        return x
+
+    lens = [60, 33, 64]
+    pages, table, keys = batch(lens, 16, fill=fill)
+    q = rnd(3, 16, R.ROW, std=0.3)
+    q[:, :, 512] = 1.0
+    got = P.attention_decode_paged_fp4(q, pages, table, i32(lens), SCALE)
+    keep = [t for t in range(60) if t not in (3, 40)]
+    want, tol = R.attention(q[0], keys[0][keep], 58, SCALE)
+    assert ((got[0].double() - want).abs() <= tol).all()
+    assert got[1].isnan().all() and got[2].isnan().all()
+
+
+def test_attention_skips_bad_pages_and_reports_them():
+    """Table entries that name no page hold tokens of zeros; lengths past the table stop at its end."""
+    lens = [100, 64]
+    pages, table, keys = batch(lens, 32)
+    table[0, 1] = pages.shape[0]
+    table[0, 3] = -2
+    keys[0][32:64] = 0
+    keys[0][96:] = 0
+    q = rnd(2, 16, R.ROW, std=0.3)
+    check(q, pages, table, lens, keys)
+    with pytest.raises(RuntimeError, match="outside the pool"):
+        P.check_paged_status()
+    table[0, 1], table[0, 3] = table[1, 0], table[1, 1]
+    keys[0][32:64] = keys[1][:32]
+    k0 = torch.cat([keys[0][:96], keys[1][32:64]])
+    got = P.attention_decode_paged_fp4(q, pages, table, i32([2 ** 31 - 1, -5]), SCALE)
+    want, tol = R.attention(q[0], k0, 128, SCALE)
+    assert ((got[0].double() - want).abs() <= tol).all() and int((got[1] != 0).sum()) == 0
+
+
+def test_attention_more_queries_than_max_q():
+    lens = [64]
+    pages, table, keys = batch(lens, 32)
+    q = rnd(4, 16, R.ROW, std=0.3)
+    out = torch.full((4, 16, 512), 7.0, dtype=BF, device=DEV)
+    P.attention_decode_paged_fp4(q, pages, table, i32(lens), SCALE, i32([0, 4]), 2, out)
+    for t in range(2):
+        want, tol = R.attention(q[t], keys[0], 61 + t, SCALE)
+        assert ((out[t].double() - want).abs() <= tol).all()
+    assert int((out[2:] != 7).sum()) == 0
+    with pytest.raises(RuntimeError, match="max_q"):
+        P.check_paged_status()
+
+
+def test_attention_is_the_same_every_time_and_on_every_stream():
+    """Same bits for the same call, alone or beside another one on a second stream."""
+    lens = [5000, 77, 3001, 900]
+    pages, table, _ = batch(lens, 64, seed=4)
+    q, q2 = rnd(4, 16, R.ROW, std=0.3), rnd(4, 16, R.ROW, seed=8, std=0.3)
+    n = i32(lens)
+    first, second = (P.attention_decode_paged_fp4(x, pages, table, n, SCALE) for x in (q, q2))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        with torch.cuda.stream(side):
+            b = P.attention_decode_paged_fp4(q2, pages, table, n, SCALE)
+        a = P.attention_decode_paged_fp4(q, pages, table, n, SCALE)
+        torch.cuda.synchronize()
+        assert torch.equal(a, first) and torch.equal(b, second)
+
+
+# --------------------------------------------------------------------------- together
+def test_serving_loop_eager_and_captured():
+    """Requests join, grow, are rolled back and end while one captured step (lengths, write, attention)
+    is replayed between eager calls; every step's output against 64 bits, pages never shared."""
+    ps, width, n_pages, rows = 16, 8, 40, 5
+    rng = random.Random(1)
+    ring = list(range(n_pages))
+    rng.shuffle(ring)
+    state = i32([0] * rows + [3, n_pages])
+    free, table = i32(ring), torch.full((rows, width), -1, dtype=torch.int32, device=DEV)
+    pages = torch.full((n_pages, ps * R.TOKEN), 255, dtype=torch.uint8, device=DEV)
+    delta, new, q = i32([0] * rows), rnd(rows, R.ROW), rnd(rows, 16, R.ROW, std=0.3)
+    keys = [torch.zeros(0, R.ROW, dtype=torch.float64, device=DEV) for _ in range(rows)]
+
+    def step(max_tokens, x):
+        after, slots, _, _ = P.paged_cache_step(state, delta, table, free, ps, max_tokens)
+        P.paged_cache_write_fp4(x, slots, pages)
+        state.copy_(after)
+        return P.attention_decode_paged_fp4(q, pages, table, state[:rows], SCALE), slots
+
+    def expect(out, d, x):
+        at = 0
+        for b in range(rows):
+            if d[b] > 0:
+                keys[b] = torch.cat([keys[b], R.held(x[at:at + d[b]])])
+                at += d[b]
+            elif d[b] < 0:
+                keys[b] = keys[b][:max(0, len(keys[b]) + d[b])]
+            want, tol = R.attention(q[b], keys[b], len(keys[b]), SCALE)
+            assert ((out[b].double() - want).abs() <= tol).all(), b
+        assert state.tolist()[:rows] == [len(k) for k in keys]
+        held = [p for b in range(rows) for p in table[b, :-(-len(keys[b]) // ps)].tolist()]
+        assert len(held) == len(set(held)) and len(held) + int(state[rows + 1]) == n_pages
+
+    def eager(d, seed):
+        x = rnd(max(1, sum(v for v in d if v > 0)), R.ROW, seed=seed)
+        delta.copy_(i32(d))
+        out, _ = step(x.shape[0], x)
+        expect(out, d, x)
+
+    eager([20, 0, 33, 7, 0], 11)
+    delta.fill_(0)
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(rows, new)
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        captured, slots = step(rows, new)
+    for k in range(6):
+        for i in range(4):  # the captured step appends one token to each live request
+            live = [1 if len(keys[b]) else 0 for b in range(rows)]
+            delta.copy_(i32(live))
+            q.copy_(rnd(rows, 16, R.ROW, seed=100 * k + i, std=0.3))
+            x = rnd(rows, R.ROW, seed=200 * k + i)
+            new.copy_(x)
+            graph.replay()
+            expect(captured, live, x)
+        # eager between the replays: a request joins, one is rolled back, one ends
+        d = [0] * rows
+        d[k % rows] = -len(keys[k % rows]) if len(keys[k % rows]) else 40
+        d[(k + 2) % rows] = -3 if len(keys[(k + 2) % rows]) else 18
+        eager(d, 300 + k)
+    everything, _, _ = P.paged_slot_map(i32([0] * rows), state[:rows].clone(), table, ps, int(state[:rows].sum()))
+    assert torch.equal(P.paged_cache_read_fp4(pages, everything).double(), torch.cat(keys))
+
+
+def test_calls_on_the_librarys_current_device_only_need_the_tensors():
+    """A lone page, a lone request, a lone token: the smallest call of each operator."""
+    pages = torch.zeros(1, R.TOKEN, dtype=torch.uint8, device=DEV)
+    table, free = i32([[-1]]), i32([0])
+    state, slots, pos, rows = P.paged_cache_step(i32([0, 0, 1]), i32([1]), table, free, 1, 1)
+    assert state.tolist() == [1, 0, 0] and slots.tolist() == pos.tolist() == rows.tolist() == [0]
+    x = rnd(1, R.ROW)
+    P.paged_cache_write_fp4(x, slots, pages)
+    assert torch.equal(P.paged_cache_read_fp4(pages, slots).double(), R.held(x))
+    q = rnd(1, 1, R.ROW)
+    got = P.attention_decode_paged_fp4(q, pages, table, state[:1], SCALE)
+    assert torch.equal(got[0, 0].double(), R.held(x)[0, :512])
+
+
+def test_empty_calls():
+    pages = pool(2, 16, fill=0)
+    e = torch.empty(0, dtype=torch.int32, device=DEV)
+    table = torch.empty(0, 3, dtype=torch.int32, device=DEV)
+    state, slots, _, _ = P.paged_cache_step(i32([1, 2]), e, table, i32([0, 1]), 16, 3)
+    assert state.tolist() == [1, 2] and slots.tolist() == [-1] * 3
+    assert P.paged_slot_map(e, e, table, 16, 2)[0].tolist() == [-1] * 2
+    P.paged_cache_write_fp4(torch.empty(0, R.ROW, dtype=BF, device=DEV), e, pages)
+    assert P.paged_cache_read_fp4(pages, e).shape == (0, R.ROW)
+    assert P.attention_decode_paged_fp4(torch.empty(0, 16, R.ROW, dtype=BF, device=DEV), pages, table, e,
+                                        SCALE).shape == (0, 16, 512)
+    out = P.paged_cache_step(i32([5, 0, 2]), i32([0]), i32([[0, 1]]), i32([0, 1]), 16, 0)
+    assert out[0].tolist() == [5, 0, 2] and out[1].shape == (0,)

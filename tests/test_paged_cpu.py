@@ -1,0 +1,153 @@
+"""The paged 4-bit latent cache without a GPU: what its functions and entry points refuse, before any
+launch, and the plain implementations that the GPU tests hold it to."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import paged_ref as R
+from triton_kernels import _hip
+from triton_kernels import paged_cache as P
+
+BF = torch.bfloat16
+
+
+def i32(*shape):
+    return torch.zeros(*shape, dtype=torch.int32)
+
+
+def good():
+    """Arguments that each function takes, by function."""
+    pages = torch.zeros(6, 16 * 400, dtype=torch.uint8)
+    return {
+        "paged_cache_step": [i32(6), i32(4), i32(4, 3), i32(6), 16, 9],
+        "paged_slot_map": [i32(4), i32(4), i32(4, 3), 16, 9],
+        "paged_cache_write_fp4": [torch.zeros(5, 576, dtype=BF), i32(5), pages],
+        "paged_cache_read_fp4": [pages, i32(5), torch.zeros(5, 576, dtype=BF)],
+        "attention_decode_paged_fp4": [torch.zeros(7, 16, 576, dtype=BF), pages, i32(4, 3), i32(4), 0.1, i32(5), 2,
+                                       torch.zeros(7, 16, 512, dtype=BF)],
+    }
+
+
+@pytest.mark.parametrize("name", sorted(good()))
+def test_functions_refuse_cpu_tensors(name):
+    with pytest.raises(NotImplementedError, match="requires CUDA"):
+        getattr(P, name)(*good()[name])
+
+
+PAGES = lambda *shape: torch.zeros(*shape, dtype=torch.uint8)  # noqa: E731
+REFUSED = [
+    ("paged_cache_step", 0, i32(5), ValueError, "state must be"),
+    ("paged_cache_step", 0, i32(6).long(), NotImplementedError, "state must be int32"),
+    ("paged_cache_step", 1, i32(4, 1), ValueError, "delta must be"),
+    ("paged_cache_step", 1, i32(8)[::2], NotImplementedError, "delta must be contiguous"),
+    ("paged_cache_step", 2, i32(3, 3), ValueError, "block_table must be"),
+    ("paged_cache_step", 2, i32(4, 0), ValueError, "block_table must be"),
+    ("paged_cache_step", 2, i32(3, 4).T, NotImplementedError, "block_table rows"),
+    ("paged_cache_step", 2, i32(1, 3).expand(4, 3), NotImplementedError, "block_table rows"),
+    ("paged_cache_step", 2, i32(4, 3).float(), NotImplementedError, "block_table must be int32"),
+    ("paged_cache_step", 3, i32(0), ValueError, "0 pages"),
+    ("paged_cache_step", 4, 48, ValueError, "power of two"),
+    ("paged_cache_step", 4, 2048, ValueError, "power of two"),
+    ("paged_cache_step", 4, 0, ValueError, "power of two"),
+    ("paged_cache_step", 5, -1, ValueError, "max_tokens"),
+    ("paged_slot_map", 0, i32(3), ValueError, "counts must be"),
+    ("paged_slot_map", 3, 12, ValueError, "power of two"),
+    ("paged_slot_map", 4, -3, ValueError, "max_tokens"),
+    ("paged_cache_write_fp4", 0, torch.zeros(5, 576), NotImplementedError, "rows must be bf16"),
+    ("paged_cache_write_fp4", 0, torch.zeros(5, 512, dtype=BF), ValueError, "rows must be"),
+    ("paged_cache_write_fp4", 0, torch.zeros(4, 576, dtype=BF), ValueError, "rows must be"),
+    ("paged_cache_write_fp4", 0, torch.zeros(576, 5, dtype=BF).T, NotImplementedError, "contiguous rows"),
+    ("paged_cache_write_fp4", 1, i32(5).long(), NotImplementedError, "slots must be int32"),
+    ("paged_cache_write_fp4", 2, PAGES(6, 16 * 400 + 16), ValueError, "pages must be"),
+    ("paged_cache_write_fp4", 2, PAGES(0, 400), ValueError, "pages must be"),
+    ("paged_cache_write_fp4", 2, PAGES(6, 400).to(torch.int8), NotImplementedError, "pages must be uint8"),
+    ("paged_cache_write_fp4", 2, PAGES(1, 400).expand(6, 400), NotImplementedError, "contiguous and apart"),
+    ("paged_cache_read_fp4", 2, torch.zeros(5, 576), NotImplementedError, "out must be bf16"),
+    ("paged_cache_read_fp4", 2, torch.zeros(1, 576, dtype=BF).expand(5, 576), NotImplementedError, "contiguous rows"),
+    ("attention_decode_paged_fp4", 0, torch.zeros(7, 16, 576), NotImplementedError, "bf16 only"),
+    ("attention_decode_paged_fp4", 0, torch.zeros(7, 16, 512, dtype=BF), ValueError, "expects q"),
+    ("attention_decode_paged_fp4", 0, torch.zeros(7, 129, 576, dtype=BF), ValueError, "expects q"),
+    ("attention_decode_paged_fp4", 0, torch.zeros(7, 576, 16, dtype=BF).transpose(1, 2), NotImplementedError,
+     "contiguous last"),
+    ("attention_decode_paged_fp4", 1, PAGES(6, 48 * 400), ValueError, "power of two"),
+    ("attention_decode_paged_fp4", 2, i32(5, 3), ValueError, "block_table must be"),
+    ("attention_decode_paged_fp4", 5, None, ValueError, "one query token a request"),
+    ("attention_decode_paged_fp4", 5, i32(4), ValueError, "cu_q must be"),
+    ("attention_decode_paged_fp4", 6, 0, ValueError, "max_q"),
+    ("attention_decode_paged_fp4", 7, torch.zeros(7, 16, 576, dtype=BF), ValueError, "out must be"),
+    ("attention_decode_paged_fp4", 7, torch.zeros(7, 1, 512, dtype=BF).expand(7, 16, 512), NotImplementedError,
+     "rows must be contiguous"),
+]
+
+
+@pytest.mark.parametrize("name,at,value,error,text", REFUSED)
+def test_functions_refuse_other_shapes_types_and_strides(monkeypatch, name, at, value, error, text):
+    monkeypatch.setattr(P, "require_cuda", lambda *a: None)
+    calls = []
+    monkeypatch.setattr(P, "_call", lambda dev, entry, *args: calls.append(entry))
+    getattr(P, name)(*good()[name])
+    assert len(calls) == 1
+    args = good()[name]
+    args[at] = value
+    with pytest.raises(error, match=text):
+        getattr(P, name)(*args)
+    assert len(calls) == 1
+
+
+def test_entry_points_refuse_bad_arguments_without_launching():
+    one, odd = 1 << 20, (1 << 20) + 8  # never read: every call below is refused on the host
+
+    def refused(match, entry, *args):
+        with pytest.raises(_hip.HipKernelError, match=match):
+            _hip.call(entry, *args, None, None)
+
+    step = [one, one, 4, one, 3, 3, one, 6, 16, 9, odd << 4, one, one, one]
+    for at, value, match in [(0, None, "null"), (2, 4097, "at most 4096"), (2, -1, "requests"), (4, 2, "block table"),
+                             (5, 0, "block table"), (7, 0, "pages"), (7, 2 ** 28, "pages"), (8, 24, "power of two"),
+                             (9, -1, "max_tokens"), (10, one + 8, "overlaps"), (11, None, "null")]:
+        refused(match, "dsv2_paged_step", *step[:at], value, *step[at + 1:])
+    slots = [one, one, 4, one, 3, 3, 16, 9, one, one, one]
+    for at, value, match in [(1, None, "null"), (2, 5000, "at most"), (5, 2 ** 28, "block table"), (6, 0, "power of two")]:
+        refused(match, "dsv2_paged_slots", *slots[:at], value, *slots[at + 1:])
+    write = [one, 576, 5, one, one, 6400, 6, 16]
+    for at, value, match in [(0, None, "null"), (0, odd, "alignment"), (1, 572, "bad shape"), (1, 580, "alignment"),
+                             (2, -1, "bad shape"), (4, None, "null"), (4, odd, "alignment"), (5, 6384, "takes 6400"),
+                             (5, 6408, "alignment"), (6, 0, "slots are int32"), (6, 2 ** 28, "slots are int32"),
+                             (7, 17, "power of two")]:
+        refused(match, "dsv2_paged_write_fp4", *write[:at], value, *write[at + 1:])
+    read = [one, 6400, 6, 16, one, 5, one, 576]
+    for at, value, match in [(4, None, "null"), (5, -1, "bad shape"), (6, odd, "alignment"), (7, 575, "bad shape")]:
+        refused(match, "dsv2_paged_read_fp4", *read[:at], value, *read[at + 1:])
+    size = _hip.lib.dsv2_mla_paged_workspace_size(4, 2, 16, 3, 16)
+    attn = [one, 9216, 576, 7, 16, one, 6400, 6, 16, one, 3, 3, one, 4, one, 2, 0.1, one, 8192, 512, one, size]
+    for at, value, match in [(0, None, "null"), (0, odd, "alignment"), (1, 9220, "alignment"), (3, -1, "bad shape"),
+                             (4, 0, "bad shape"), (4, 129, "bad shape"), (8, 40, "power of two"), (10, 2, "block table"),
+                             (11, 2 ** 28, "block table"), (12, None, "null"), (13, -1, "bad shape"),
+                             (14, None, "bad shape"), (15, 0, "bad shape"), (18, 8196, "alignment"),
+                             (20, None, "workspace"), (20, odd, "workspace"), (21, size - 1, "workspace")]:
+        refused(match, "dsv2_mla_decode_paged_fp4", *attn[:at], value, *attn[at + 1:])
+
+
+def test_the_plain_block_format():
+    """The reference of the GPU tests on values worked out by hand."""
+    x = torch.zeros(4, 576)
+    x[0, :4] = torch.tensor([6.0, 5.0, 2.5, -0.25])       # 6 is held: scale 1; ties 5 -> 4, 2.5 -> 2, 0.25 -> 0
+    x[1, :4] = torch.tensor([6.03125, 1.75, 0.5, -3.5])   # past 6: scale 2: 3, 0.875 -> 1, 0.25 -> 0, 1.75 -> 2
+    x[2, :3] = torch.tensor([float("inf"), 1.0, 2.0])
+    x[3, 32:35] = torch.tensor([3.0e38, -3.3e38, 1.0e38])  # past 1.5 * 2^127: saturated at 6 * 2^125
+    got = R.held(x.to(BF))
+    assert got[0, :4].tolist() == [6.0, 4.0, 2.0, 0.0]
+    assert got[1, :4].tolist() == [6.0, 2.0, 0.0, -4.0]
+    assert got[2, :32].isnan().all() and not got[2, 32:].isnan().any()
+    assert got[3, 32:34].tolist() == [6.0 * 2.0 ** 125, -6.0 * 2.0 ** 125]
+    assert got[3, 34] == 2.0 * 2.0 ** 125  # 1e38 / 2^125 = 2.35
+
+
+def test_the_plain_allocator_hands_out_and_takes_back():
+    b = R.Allocator([2, 1], [[5, -1], [6, -1]], [9, 4, 7], 2, 1, 2)
+    out, errors = b.step([1, -1], 3)
+    # request 0 takes page 7 (ring position 2); request 1's page goes behind it, to position 0
+    assert out == [[14, -1, -1], [2, -1, -1], [0, -1, -1]] and errors == 0
+    assert b.ring == [6, 4, 7] and (b.head, b.count) == (0, 1) and b.lens == [3, 0]
