@@ -267,7 +267,7 @@ def attention_decode_paged_fp4(q: torch.Tensor, pages: torch.Tensor, block_table
             raise NotImplementedError(f"{name}: out's rows must be contiguous and apart")
     if t == 0 or n == 0:
         return out
-    size = _hip.lib.dsv2_mla_paged_workspace_size(n, max_q, h, width, page_size)
+    size = _hip.lib.dsv2_mla_paged_workspace_size(n, max_q, h)
     ws = torch.empty(size, dtype=_U8, device=dev)
     _call(dev, "dsv2_mla_decode_paged_fp4", q.data_ptr(), q_ts, q_hs, t, h, pages.data_ptr(), page_stride, n_pages,
           page_size, block_table.data_ptr(), ts, width, lens.data_ptr(), n, None if cu_q is None else cu_q.data_ptr(),
