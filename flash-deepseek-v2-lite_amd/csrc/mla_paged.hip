@@ -3,8 +3,8 @@
 //   s_t = scale * q . (latent_t | rope_t),  p = softmax(s),  o = sum_t p_t latent_t
 //
 // One (query token, head) pair is a column; a request's columns are numbered token by token, and 16 of
-// them make the narrow side of v_mfma_f32_16x16x32_bf16 (S^T = K Q^T, O^T += V^T P^T).  An item is one
-// request and 16 of its columns: ceil(length / 32) tiles of 32 tokens.
+// them make the narrow side of the MFMAs (S^T = K Q^T, O^T += V^T P^T).  An item is one request and 16 of
+// its columns: ceil(length / 16) tiles of 16 tokens.
 //
 // Work is dealt out on the device, where the lengths are: every workgroup sums the items' tiles for
 // itself and takes an equal run of them, whatever requests it crosses.  An item that lies within one
@@ -15,15 +15,19 @@
 using namespace paged;
 
 namespace {
-constexpr int kTile = 32;
-constexpr int kWaves = 4;
-constexpr int kVRow = kLat + 16;       // padded LDS row of a token's latent (elements): 1,056 bytes
-constexpr int kORow = kLat + 4;        // padded LDS row of a column's output (floats)
+constexpr int kTile = 16;
+constexpr int kWaves = 8;
+constexpr int kThreads = 64 * kWaves;
+// LDS row of a token's latent: 1,056 bytes, with the halves of every 32 bytes swapped in rows 4-7 and
+// 12-15.  Eight rows' 16-byte writes of one block then fill 128 bytes, and so do the four rows' 32 bytes
+// of a transposed read
+constexpr int kVRow = kLat + 16;
+constexpr int kORow = kLat + 4;        // LDS row of a column's output (floats)
 constexpr int kWaveLds = kTile * kVRow * 2;
-static_assert(16 * kORow * 4 <= kWaveLds, "a wave's outputs take its tile's place");
+constexpr int kQLds = 18 * 64 * 16;    // the item's Q^T fragments
+static_assert(16 * kORow * 4 <= 2 * kWaveLds, "a wave's outputs take two tiles' place");
 constexpr int kWgs = 256;              // one workgroup per CU
-constexpr int kMinTiles = 8;           // tiles of a workgroup, at least
-constexpr int kMaxRequests = 4096;     // the running tile counts stand in LDS
+constexpr int kMinTiles = 16;          // tiles of a workgroup, at least
 constexpr int kPartFloats = 16 * kLat;
 
 struct PagedAttnArgs {
@@ -52,6 +56,8 @@ struct PagedAttnArgs {
 
 struct Request {
   int len, q0, nq, columns;
+  __device__ __forceinline__ int tiles() const { return (len + kTile - 1) / kTile; }
+  __device__ __forceinline__ int all_tiles() const { return tiles() * ((columns + 15) / 16); }
 };
 __device__ __forceinline__ Request request(const PagedAttnArgs& a, int b) {
   Request r;
@@ -67,34 +73,40 @@ __device__ __forceinline__ Request request(const PagedAttnArgs& a, int b) {
   return r;
 }
 
-// a tile's bytes: lane (li, kg) has 16-token blocks h = 0, 1's token li, latent blocks 4c + kg (32 codes
-// each), the token's 16 scales, rotary keys y * 32 + kg * 8 .. +8
+// a tile's bytes: lane (li, kg) has token li's latent blocks 4c + kg (32 codes each), its 16 scales and
+// its rotary keys y * 32 + kg * 8 .. +8
 struct Raw {
-  uint4 code[2][4];
-  uint4 rope[2][2];
-  uint4 scale[2];
-  bool ok[2];  // the token exists and its page is one
+  uint4 code[4];
+  uint4 rope[2];
+  uint4 scale;
+  bool ok;  // the token exists and its page is one
 };
+
+__device__ __forceinline__ floatx4_t mfma16x16x16(const uint2& a, const uint2& b, const floatx4_t& c) {
+  typedef short short4_t __attribute__((ext_vector_type(4)));
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4_t, a), __builtin_bit_cast(short4_t, b), c, 0, 0, 0);
+}
 }  // namespace
 
-__global__ __launch_bounds__(64 * kWaves, 1) void mla_paged_kernel(const PagedAttnArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ float ml[kWaves][16][2];
-  __shared__ int32_t wave_sum32[kWaves];
-  int32_t* ends = reinterpret_cast<int32_t*>(smem + kWaves * kWaveLds);
+  __shared__ int32_t wave_sums[kWaves];
+  __shared__ int32_t from_request[2];
+  uint4* const q_lds = reinterpret_cast<uint4*>(smem + kWaves * kWaveLds);
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, li = lane & 15, kg = lane >> 4;
 
-  // running tile counts of the requests (the host has checked that they stay within int32)
-  int total;
+  // the tiles of all requests (the host has checked that they stay within int32), and the request that
+  // this workgroup's run begins in
+  int first, last, per, b, b_start;
   {
-    const int per = (a.requests + 255) / 256;
-    const int b0 = min(tid * per, a.requests), b1 = min(b0 + per, a.requests);
+    const int chunk = (a.requests + kThreads - 1) / kThreads;
+    const int b0 = min(tid * chunk, a.requests), b1 = min(b0 + chunk, a.requests);
     int run = 0;
-    for (int b = b0; b < b1; ++b) {
-      const Request r = request(a, b);
+    for (int i = b0; i < b1; ++i) {
+      const Request r = request(a, i);
       if (r.nq > a.max_q && blockIdx.x == 0 && a.status) atomicOr(a.status, DSV2_DEVERR_TOKENS);
-      run += ((r.len + kTile - 1) / kTile) * ((r.columns + 15) / 16);
-      ends[b] = run;
+      run += r.all_tiles();
     }
     int scan = run;
 #pragma unroll
@@ -102,84 +114,80 @@ __global__ __launch_bounds__(64 * kWaves, 1) void mla_paged_kernel(const PagedAt
       const int u = __shfl_up(scan, o, DSV2_WAVE);
       if (lane >= o) scan += u;
     }
-    if (lane == 63) wave_sum32[wv] = scan;
+    if (lane == 63) wave_sums[wv] = scan;
     __syncthreads();
-    int before = scan - run;
-    total = 0;
+    int before = scan - run, total = 0;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
-      if (i < wv) before += wave_sum32[i];
-      total += wave_sum32[i];
+      if (i < wv) before += wave_sums[i];
+      total += wave_sums[i];
     }
-    for (int b = b0; b < b1; ++b) ends[b] += before;
+    per = max((total + kWgs - 1) / kWgs, kMinTiles);
+    if (blockIdx.x == 0 && tid == 0) a.starts[a.requests * a.columns16] = per;
+    const int64_t from = static_cast<int64_t>(blockIdx.x) * per;
+    if (from >= total) return;
+    first = static_cast<int>(from);
+    last = min(first + per, total);
+    if (before <= first && first < before + run) {
+      int i = b0;
+      for (;; ++i) {
+        const int n = request(a, i).all_tiles();
+        if (first < before + n) break;
+        before += n;
+      }
+      from_request[0] = i;
+      from_request[1] = before;
+    }
     __syncthreads();
-  }
-  const int per = max((total + kWgs - 1) / kWgs, kMinTiles);
-  if (blockIdx.x == 0 && tid == 0) a.starts[a.requests * a.columns16] = per;
-  const int64_t from = static_cast<int64_t>(blockIdx.x) * per;
-  if (from >= total) return;
-  const int first = static_cast<int>(from), last = min(first + per, total);
-  int b;
-  {
-    int lo = 0, hi = a.requests - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (ends[mid] > first)
-        hi = mid;
-      else
-        lo = mid + 1;
-    }
-    b = lo;
+    b = from_request[0];
+    b_start = from_request[1];
   }
 
   bf16_t* const vt = reinterpret_cast<bf16_t*>(smem + wv * kWaveLds);
+  Request r = request(a, b);
   for (int at = first; at < last;) {
-    while (ends[b] <= at) ++b;
-    const Request r = request(a, b);
-    const int tiles = (r.len + kTile - 1) / kTile;
-    const int b_start = b ? ends[b - 1] : 0;
+    while (at >= b_start + r.all_tiles()) {
+      b_start += r.all_tiles();
+      r = request(a, ++b);
+    }
+    const int tiles = r.tiles();
     const int ct = (at - b_start) / tiles;
     const int item = b_start + ct * tiles;  // its first tile
     const int t_first = at - item, t_last = min(last - item, tiles);
-    const int col = ct * 16 + li;
-    const bool live = col < r.columns;
-    const int j = live ? col / a.heads : 0, h = live ? col - j * a.heads : 0;
-    const int seen = live ? max(r.len - r.nq + j + 1, 0) : 0;
 
-    // Q^T fragments (B operand): column li; the k order of a block group's four products is the lanes'
-    // own: k-slot (kg, e) of product (c, x) is latent (4c + kg) * 32 + x * 8 + e
-    bf16x8_t qf[18];
-    {
-      const bf16_t* qc = a.q + (r.q0 + j) * a.q_ts + h * a.q_hs;
+    // Q^T fragments (B operand), once for all waves; the k order of a block group's four products is the
+    // lanes' own: k-slot (kg, e) of product (c, x) is latent (4c + kg) * 32 + x * 8 + e
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        qf[i] = as_bf16x8(keep_if(live, ldg16(qc + ((i >> 2) * 4 + kg) * 32 + (i & 3) * 8)));
-#pragma unroll
-      for (int y = 0; y < 2; ++y) qf[16 + y] = as_bf16x8(keep_if(live, ldg16(qc + kLat + y * 32 + kg * 8)));
+    for (int n = 0; n < (18 * 64 + kThreads - 1) / kThreads; ++n) {
+      const int f = tid + n * kThreads;
+      if (f < 18 * 64) {
+        const int i = f >> 6, cc = ct * 16 + li;
+        const int dim = i < 16 ? ((i >> 2) * 4 + kg) * 32 + (i & 3) * 8 : kLat + (i - 16) * 32 + kg * 8;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (cc < r.columns) v = ldg16(a.q + (r.q0 + cc / a.heads) * a.q_ts + (cc % a.heads) * a.q_hs + dim);
+        q_lds[f] = v;
+      }
     }
+    const int col = ct * 16 + li;
+    const int seen = col < r.columns ? max(r.len - r.nq + col / a.heads + 1, 0) : 0;
 
     const int32_t* row = a.table + b * a.ts;
-    auto load_pages = [&](int tile, int* pg) {
+    const int end = t_last - 1;
+    auto load_page = [&](int tile) { return row[min(min(tile, end) * kTile + li, r.len - 1) >> a.shift]; };
+    auto load_tile = [&](int tile, int pg, Raw& w) {
+      const int t = min(tile, end) * kTile + li;
+      const bool page = pg >= 0 && pg < a.n_pages;
+      w.ok = page && t < r.len;
+      if (!page && kg == 0 && t < r.len && a.status) atomicOr(a.status, DSV2_DEVERR_BAD_SLOT);
+      const int off = min(t, r.len - 1) & ((1 << a.shift) - 1);
+      const uint8_t* base = a.pages + (page ? pg : 0) * a.page_stride;
+      const uint8_t* code = base + off * kCodeB + kg * 16;
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) pg[hf] = row[min(tile * kTile + hf * 16 + li, r.len - 1) >> a.shift];
-    };
-    auto load_tile = [&](int tile, const int* pg, Raw& w) {
+      for (int c = 0; c < 4; ++c) w.code[c] = ldg16(code + c * 64);
+      const uint8_t* rope = base + (kCodeB << a.shift) + off * kRopeB + kg * 16;
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int t = tile * kTile + hf * 16 + li;
-        const bool page = pg[hf] >= 0 && pg[hf] < a.n_pages;
-        w.ok[hf] = page && t < r.len;
-        if (!page && kg == 0 && t < r.len && a.status) atomicOr(a.status, DSV2_DEVERR_BAD_SLOT);
-        const int off = min(t, r.len - 1) & ((1 << a.shift) - 1);
-        const uint8_t* base = a.pages + (page ? pg[hf] : 0) * a.page_stride;
-        const uint8_t* code = base + off * kCodeB + kg * 16;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) w.code[hf][c] = ldg16(code + c * 64);
-        const uint8_t* rope = base + (kCodeB << a.shift) + off * kRopeB + kg * 16;
-#pragma unroll
-        for (int y = 0; y < 2; ++y) w.rope[hf][y] = ldg16(rope + y * 64);
-        w.scale[hf] = ldg16(base + ((kCodeB + kRopeB) << a.shift) + off * kScaleB);
-      }
+      for (int y = 0; y < 2; ++y) w.rope[y] = ldg16(rope + y * 64);
+      w.scale = ldg16(base + ((kCodeB + kRopeB) << a.shift) + off * kScaleB);
     };
 
     float m_run = -__FLT_MAX__, l_run = 0.f;
@@ -188,47 +196,44 @@ __global__ __launch_bounds__(64 * kWaves, 1) void mla_paged_kernel(const PagedAt
     for (int f = 0; f < 32; ++f) acc[f] = floatx4_t{0.f, 0.f, 0.f, 0.f};
 
     auto tile_step = [&](int tile, Raw& w) {
-      floatx4_t sc[2];
+      uint32_t s[4];
+      const uint32_t sw[4] = {w.scale.x, w.scale.y, w.scale.z, w.scale.w};
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        uint32_t s[4];
-        const uint32_t sw[4] = {w.scale[hf].x, w.scale[hf].y, w.scale[hf].z, w.scale[hf].w};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s[c] = (sw[c] >> (8 * kg)) & 0xff;
-        // rare: a token past the end or on no page (zeros), a block of NaN (its codes are zeros; one
-        // rotary key becomes NaN instead, so that only the queries that see the token get NaN: a NaN
-        // latent times an unseen token's p = 0 would be one too)
-        const bool nan = max(max(s[0], s[1]), max(s[2], s[3])) == kNanScale;
-        if (__any(!w.ok[hf] || nan)) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            w.code[hf][c] = keep_if(w.ok[hf] && s[c] != kNanScale, w.code[hf][c]);
-            s[c] = w.ok[hf] && s[c] != kNanScale ? s[c] : 127;
-          }
-#pragma unroll
-          for (int y = 0; y < 2; ++y) w.rope[hf][y] = keep_if(w.ok[hf], w.rope[hf][y]);
-          if (nan && w.ok[hf]) w.rope[hf][0].x = 0x7fc07fc0u;
-        }
-        sc[hf] = floatx4_t{0.f, 0.f, 0.f, 0.f};
-        bf16_t* vr = vt + (hf * 16 + li) * kVRow + kg * 32;
+      for (int c = 0; c < 4; ++c) s[c] = (sw[c] >> (8 * kg)) & 0xff;
+      // rare: a token past the end or on no page (zeros), a block of NaN (its codes are zeros; one rotary
+      // key becomes NaN instead, so that only the queries that see the token get NaN: a NaN latent times
+      // an unseen token's p = 0 would be one too)
+      const bool nan = max(max(s[0], s[1]), max(s[2], s[3])) == kNanScale;
+      if (__any(!w.ok || nan)) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const uint32_t cw[4] = {w.code[hf][c].x, w.code[hf][c].y, w.code[hf][c].z, w.code[hf][c].w};
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const uint4 v = decode8(cw[x], s[c]);
-            *reinterpret_cast<uint4*>(vr + c * 128 + x * 8) = v;
-            sc[hf] = mfma16x16x32(as_bf16x8(v), qf[c * 4 + x], sc[hf]);
-          }
+          w.code[c] = keep_if(w.ok && s[c] != kNanScale, w.code[c]);
+          s[c] = w.ok && s[c] != kNanScale ? s[c] : 127;
         }
 #pragma unroll
-        for (int y = 0; y < 2; ++y) sc[hf] = mfma16x16x32(as_bf16x8(w.rope[hf][y]), qf[16 + y], sc[hf]);
+        for (int y = 0; y < 2; ++y) w.rope[y] = keep_if(w.ok, w.rope[y]);
+        if (nan && w.ok) w.rope[0].x = 0x7fc07fc0u;
       }
-      asm volatile("" ::: "memory");
-      float p[8], mx = -INFINITY;
+      floatx4_t sc = floatx4_t{0.f, 0.f, 0.f, 0.f};
+      bf16_t* vr = vt + li * kVRow + kg * 32;
+      const int swap = (li & 4) * 2;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        p[i] = tile * kTile + (i >> 2) * 16 + 4 * kg + (i & 3) < seen ? sc[i >> 2][i & 3] : -INFINITY;
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t cw[4] = {w.code[c].x, w.code[c].y, w.code[c].z, w.code[c].w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint4 v = decode8(cw[x], s[c]);
+          *reinterpret_cast<uint4*>(vr + c * 128 + ((x * 8) ^ swap)) = v;
+          sc = mfma16x16x32(as_bf16x8(v), as_bf16x8(q_lds[(c * 4 + x) * 64 + lane]), sc);
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < 2; ++y) sc = mfma16x16x32(as_bf16x8(w.rope[y]), as_bf16x8(q_lds[(16 + y) * 64 + lane]), sc);
+      asm volatile("" ::: "memory");
+      float p[4], mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = tile * kTile + 4 * kg + i < seen ? sc[i] : -INFINITY;
         mx = fmaxf(mx, p[i]);
       }
       mx = xor32_max(xor16_max(mx)) * a.scale_log2;
@@ -243,49 +248,43 @@ __global__ __launch_bounds__(64 * kWaves, 1) void mla_paged_kernel(const PagedAt
 #pragma unroll
         for (int f = 0; f < 32; ++f) acc[f] *= alpha;
       }
-      float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4; ++i) {
         p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], a.scale_log2, -m_run));
-        sum += p[i];
+        l_run += p[i];  // this lane's tokens; the lanes meet at the end
       }
-      l_run += sum;  // this lane's tokens; the lanes meet at the end
-      // P^T (B operand): column li, tokens 4 kg + e then 16 + 4 kg + e; the V^T fragments take the same
-      // tokens through two transposed reads (lane (li, kg) addresses token 4 kg + li / 4)
-      const bf16x8_t pb = as_bf16x8(pack8(p));
-      const bf16_t* vp = vt + (4 * kg + (li >> 2)) * kVRow + 4 * (li & 3);
+      // P^T (B operand): column li, tokens 4 kg + e; the V^T fragments take the same tokens through
+      // transposed reads (lane (li, kg) addresses token 4 kg + li / 4)
+      const uint2 pb = make_uint2(pack2(p[0], p[1]), pack2(p[2], p[3]));
+      const bf16_t* vp = vt + (4 * kg + (li >> 2)) * kVRow + ((4 * (li & 3)) ^ ((kg & 1) * 8));
 #pragma unroll
-      for (int f = 0; f < 32; ++f) {
-        const uint2 lo = lds_read_tr16(vp + f * 16), hi = lds_read_tr16(vp + f * 16 + 16 * kVRow);
-        acc[f] = mfma16x16x32(as_bf16x8(make_uint4(lo.x, lo.y, hi.x, hi.y)), pb, acc[f]);
-      }
+      for (int f = 0; f < 32; ++f) acc[f] = mfma16x16x16(lds_read_tr16(vp + f * 16), pb, acc[f]);
       asm volatile("" ::: "memory");
     };
 
-    // wave w takes tiles t_first + w, + 4, ...: one ahead in registers, its pages one further
+    // wave w takes tiles t_first + w, + 8, ...: one ahead in registers, its page number one further
     {
-      const int end = t_last - 1;
       int tile = t_first + wv;
-      int pg[2];
       Raw w0, w1;
-      load_pages(min(tile, end), pg);
-      load_tile(min(tile, end), pg, w0);
-      load_pages(min(tile + kWaves, end), pg);
+      int pg = load_page(tile);
+      load_tile(tile, pg, w0);
+      pg = load_page(tile + kWaves);
+      __syncthreads();  // Q
       while (tile < t_last) {
-        load_tile(min(tile + kWaves, end), pg, w1);
-        load_pages(min(tile + 2 * kWaves, end), pg);
+        load_tile(tile + kWaves, pg, w1);
+        pg = load_page(tile + 2 * kWaves);
         tile_step(tile, w0);
         tile += kWaves;
         if (tile >= t_last) break;
-        load_tile(min(tile + kWaves, end), pg, w0);
-        load_pages(min(tile + 2 * kWaves, end), pg);
+        load_tile(tile + kWaves, pg, w0);
+        pg = load_page(tile + 2 * kWaves);
         tile_step(tile, w1);
         tile += kWaves;
       }
     }
     l_run = xor32_sum(xor16_sum(l_run));
 
-    // the waves' parts meet in LDS, in each wave's own tile's place
+    // the waves' parts meet in LDS, in the tiles' place: the upper four's, then the sums of pairs
     if (kg == 0) {
       ml[wv][li][0] = m_run;
       ml[wv][li][1] = l_run;
@@ -294,13 +293,22 @@ __global__ __launch_bounds__(64 * kWaves, 1) void mla_paged_kernel(const PagedAt
     float m_all = ml[0][li][0];
 #pragma unroll
     for (int i = 1; i < kWaves; ++i) m_all = fmaxf(m_all, ml[i][li][0]);
-    {
-      const float weight = __builtin_amdgcn_exp2f(m_run - m_all);
-      float* o = reinterpret_cast<float*>(smem + wv * kWaveLds) + li * kORow + 4 * kg;
+    const float weight = __builtin_amdgcn_exp2f(m_run - m_all);
+    float* o_lds = reinterpret_cast<float*>(smem + (wv & 3) * 2 * kWaveLds) + li * kORow + 4 * kg;
+    if (wv >= 4) {
 #pragma unroll
       for (int f = 0; f < 32; ++f) {
         const floatx4_t v = acc[f] * weight;
-        *reinterpret_cast<float4*>(o + f * 16) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(o_lds + f * 16) = make_float4(v[0], v[1], v[2], v[3]);
+      }
+    }
+    __syncthreads();
+    if (wv < 4) {
+#pragma unroll
+      for (int f = 0; f < 32; ++f) {
+        const float4 u = *reinterpret_cast<const float4*>(o_lds + f * 16);
+        const floatx4_t v = acc[f] * weight;
+        *reinterpret_cast<float4*>(o_lds + f * 16) = make_float4(v[0] + u.x, v[1] + u.y, v[2] + u.z, v[3] + u.w);
       }
     }
     __syncthreads();
@@ -308,12 +316,13 @@ __global__ __launch_bounds__(64 * kWaves, 1) void mla_paged_kernel(const PagedAt
     const int slot = at == first ? 2 * blockIdx.x : 2 * blockIdx.x + 1;
     if (t_first == 0 && tid == 0) a.starts[b * a.columns16 + ct] = item;
 #pragma unroll
-    for (int i = 0; i < kPartFloats / 4 / 256; ++i) {
-      const int f = tid + 256 * i, c = f >> 7, d = (f & 127) * 4;
+    for (int i = 0; i < kPartFloats / 4 / kThreads; ++i) {
+      const int f = tid + kThreads * i, c = f >> 7, d = (f & 127) * 4;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int u = 0; u < kWaves; ++u) {
-        const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + u * kWaveLds) + c * kORow + d);
+      for (int u = 0; u < 4; ++u) {
+        const float4 x =
+            *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + u * 2 * kWaveLds) + c * kORow + d);
         v.x += x.x;
         v.y += x.y;
         v.z += x.z;
@@ -345,7 +354,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void mla_paged_kernel(const PagedAt
       a.part_ml[(slot * 16 + tid) * 2 + 1] = l;
     }
     at = item + t_last;
-    if (at < last) __syncthreads();  // the next item's tiles and maxima go where these were read
+    if (at < last) __syncthreads();  // the next item's tiles, queries and maxima go where these were read
   }
 }
 
@@ -433,7 +442,7 @@ extern "C" int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_
                                          void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
   if (const int rc = paged_check_pool("mla_decode_paged_fp4", pages, page_stride, n_pages, page_size)) return rc;
   DSV2_REQUIRE(q && block_table && lens && out, DSV2_E_NULL, "mla_decode_paged_fp4: null pointer");
-  DSV2_REQUIRE(tokens >= 0 && heads > 0 && heads <= 128 && requests >= 0 && requests <= kMaxRequests && max_q > 0 &&
+  DSV2_REQUIRE(tokens >= 0 && heads > 0 && heads <= 128 && requests >= 0 && requests <= 65535 && max_q > 0 &&
                    max_q <= 65535 && (cu_q || requests == tokens),
                DSV2_E_SHAPE, "mla_decode_paged_fp4: bad shape (%d query tokens, %d heads, %d requests, max_q %d)", tokens,
                heads, requests, max_q);
@@ -461,8 +470,7 @@ extern "C" int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_
                         status};
   const int64_t most = items * ((room + kTile - 1) / kTile);
   const int wgs = static_cast<int>(most / kMinTiles + 1 < kWgs ? most / kMinTiles + 1 : kWgs);
-  hipLaunchKernelGGL(mla_paged_kernel, dim3(wgs), dim3(64 * kWaves), kWaves * kWaveLds + requests * 4,
-                     (hipStream_t)stream, a);
+  hipLaunchKernelGGL(mla_paged_kernel, dim3(wgs), dim3(kThreads), kWaves * kWaveLds + kQLds, (hipStream_t)stream, a);
   if (const int rc = dsv2_launch_status("mla_decode_paged_fp4")) return rc;
   hipLaunchKernelGGL(mla_paged_merge_kernel, dim3((unsigned)items, 16, 4), dim3(256), 0, (hipStream_t)stream, a);
   return dsv2_launch_status("mla_decode_paged_fp4");

@@ -542,7 +542,7 @@ int dsv2_paged_read_fp4(const void* pages, int64_t page_stride, int n_pages, int
  * max_q of them (cu_q NULL: token b); they are its last cached ones: query j of n sees the tokens below
  * lens[b] - n + j + 1.  A query that sees nothing gives zeros; query tokens of no request are left alone.
  * Table entries that name no page stand for tokens of zeros (and set DSV2_DEVERR_BAD_SLOT); a request with
- * more than max_q query tokens has the first max_q done (and sets DSV2_DEVERR_TOKENS).  requests <= 4096.
+ * more than max_q query tokens has the first max_q done (and sets DSV2_DEVERR_TOKENS).
  * workspace: dsv2_mla_paged_workspace_size bytes, 16-byte aligned, not shared by calls that may overlap. */
 int64_t dsv2_mla_paged_workspace_size(int requests, int max_q, int heads);
 int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_hs, int tokens, int heads, const void* pages,

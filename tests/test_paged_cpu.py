@@ -124,7 +124,7 @@ def test_entry_points_refuse_bad_arguments_without_launching():
     attn = [one, 9216, 576, 7, 16, one, 6400, 6, 16, one, 3, 3, one, 4, one, 2, 0.1, one, 8192, 512, one, size]
     for at, value, match in [(0, None, "null"), (0, odd, "alignment"), (1, 9220, "alignment"), (3, -1, "bad shape"),
                              (4, 0, "bad shape"), (4, 129, "bad shape"), (8, 40, "power of two"), (10, 2, "block table"),
-                             (11, 2 ** 28, "block table"), (12, None, "null"), (13, -1, "bad shape"), (13, 4097, "bad shape"),
+                             (11, 2 ** 28, "block table"), (12, None, "null"), (13, -1, "bad shape"), (13, 65536, "bad shape"),
                              (14, None, "bad shape"), (15, 0, "bad shape"), (18, 8196, "alignment"),
                              (20, None, "workspace"), (20, odd, "workspace"), (21, size - 1, "workspace")]:
         refused(match, "dsv2_mla_decode_paged_fp4", *attn[:at], value, *attn[at + 1:])
