@@ -6,10 +6,12 @@
 // them make the narrow side of the MFMAs (S^T = K Q^T, O^T += V^T P^T).  An item is one request and 16 of
 // its columns: ceil(length / 16) tiles of 16 tokens.
 //
-// Work is dealt out on the device, where the lengths are: every workgroup sums the items' tiles for
-// itself and takes an equal run of them, whatever requests it crosses.  An item that lies within one
-// workgroup is finished there; of one that crosses into others each leaves its part (fp32 o, max, sum)
-// in the workspace and mla_paged_merge_kernel joins them.
+// Work is dealt out on the device, where the lengths are.  Items stand one after the other on a line, each
+// with its tiles and kItemCost more places for what an item costs beside them (queries, the waves' joining,
+// outputs); every workgroup sums the line for itself and takes an equal stretch of it.  A stretch's end
+// closer than kPiece tiles to an item's end moves there, so pieces fill the waves at least once and items
+// of less than two pieces are never cut.  An item within one workgroup is finished there; of one cut into
+// several each leaves its part (fp32 o, max, sum) in the workspace and mla_paged_merge_kernel joins them.
 #include "paged.h"
 
 using namespace paged;
@@ -27,7 +29,9 @@ constexpr int kWaveLds = kTile * kVRow * 2;
 constexpr int kQLds = 18 * 64 * 16;    // the item's Q^T fragments
 static_assert(16 * kORow * 4 <= 2 * kWaveLds, "a wave's outputs take two tiles' place");
 constexpr int kWgs = 256;              // one workgroup per CU
-constexpr int kMinTiles = 16;          // tiles of a workgroup, at least
+constexpr int kPiece = 8;              // tiles of a cut item's piece, at least: one a wave
+constexpr int kMinStretch = 2 * kPiece;
+constexpr int kItemCost = 16;
 constexpr int kPartFloats = 16 * kLat;
 
 struct PagedAttnArgs {
@@ -50,14 +54,18 @@ struct PagedAttnArgs {
   int64_t o_ts, o_hs;
   float* part_o;     // [2 * kWgs][16][512]
   float* part_ml;    // [2 * kWgs][16][2]
-  int32_t* starts;   // [requests * columns16 + 1]: an item's first tile; last: tiles of a workgroup
+  int4* cuts;        // [kWgs]: the item that a workgroup's first piece continues (request or -1, column
+                     // group) and the workgroups that it begins and ends in
   int32_t* status;
 };
 
 struct Request {
   int len, q0, nq, columns;
   __device__ __forceinline__ int tiles() const { return (len + kTile - 1) / kTile; }
-  __device__ __forceinline__ int all_tiles() const { return tiles() * ((columns + 15) / 16); }
+  // its places on the line of all items
+  __device__ __forceinline__ int places() const {
+    return len > 0 ? (tiles() + kItemCost) * ((columns + 15) / 16) : 0;
+  }
 };
 __device__ __forceinline__ Request request(const PagedAttnArgs& a, int b) {
   Request r;
@@ -92,21 +100,24 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ float ml[kWaves][16][2];
   __shared__ int32_t wave_sums[kWaves];
-  __shared__ int32_t from_request[2];
+  __shared__ int4 first_request[2];
   uint4* const q_lds = reinterpret_cast<uint4*>(smem + kWaves * kWaveLds);
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, li = lane & 15, kg = lane >> 4;
 
-  // the tiles of all requests (the host has checked that they stay within int32), and the request that
-  // this workgroup's run begins in
-  int first, last, per, b, b_start;
+  // the length of the line (the host has checked that it stays within int32), and the request that this
+  // workgroup's stretch begins in
+  int lo, hi, per, b, start;
+  Request r;
   {
     const int chunk = (a.requests + kThreads - 1) / kThreads;
     const int b0 = min(tid * chunk, a.requests), b1 = min(b0 + chunk, a.requests);
     int run = 0;
+    bool nothing = false;
     for (int i = b0; i < b1; ++i) {
-      const Request r = request(a, i);
+      r = request(a, i);
       if (r.nq > a.max_q && blockIdx.x == 0 && a.status) atomicOr(a.status, DSV2_DEVERR_TOKENS);
-      run += r.all_tiles();
+      nothing |= r.len == 0 && r.columns > 0;
+      run += r.places();
     }
     int scan = run;
 #pragma unroll
@@ -115,45 +126,66 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
       if (lane >= o) scan += u;
     }
     if (lane == 63) wave_sums[wv] = scan;
-    __syncthreads();
+    if (__syncthreads_or(nothing)) {  // requests with nothing cached: zeros
+      for (int i = blockIdx.x; i < a.requests; i += gridDim.x) {
+        const Request z = request(a, i);
+        if (z.len > 0) continue;
+        for (int f = tid; f < z.columns * (kLat / 8); f += kThreads) {
+          const int cc = f / (kLat / 8);
+          *reinterpret_cast<uint4*>(a.out + (z.q0 + cc / a.heads) * a.o_ts + (cc % a.heads) * a.o_hs +
+                                    f % (kLat / 8) * 8) = make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
     int before = scan - run, total = 0;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
       if (i < wv) before += wave_sums[i];
       total += wave_sums[i];
     }
-    per = max((total + kWgs - 1) / kWgs, kMinTiles);
-    if (blockIdx.x == 0 && tid == 0) a.starts[a.requests * a.columns16] = per;
+    per = max((total + kWgs - 1) / kWgs, kMinStretch);
     const int64_t from = static_cast<int64_t>(blockIdx.x) * per;
+    if (tid == 0) a.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
     if (from >= total) return;
-    first = static_cast<int>(from);
-    last = min(first + per, total);
-    if (before <= first && first < before + run) {
+    lo = static_cast<int>(from);
+    hi = min(lo + per, total);
+    if (before <= lo && lo < before + run) {
       int i = b0;
-      for (;; ++i) {
-        const int n = request(a, i).all_tiles();
-        if (first < before + n) break;
-        before += n;
-      }
-      from_request[0] = i;
-      from_request[1] = before;
+      if (b1 - b0 > 1)
+        for (;; ++i) {
+          r = request(a, i);
+          if (lo < before + r.places()) break;
+          before += r.places();
+        }
+      first_request[0] = make_int4(i, before, 0, 0);
+      first_request[1] = make_int4(r.len, r.q0, r.nq, r.columns);
     }
     __syncthreads();
-    b = from_request[0];
-    b_start = from_request[1];
+    const int4 u = first_request[0], v = first_request[1];
+    b = u.x;
+    start = u.y;
+    r.len = v.x;
+    r.q0 = v.y;
+    r.nq = v.z;
+    r.columns = v.w;
   }
 
   bf16_t* const vt = reinterpret_cast<bf16_t*>(smem + wv * kWaveLds);
-  Request r = request(a, b);
-  for (int at = first; at < last;) {
-    while (at >= b_start + r.all_tiles()) {
-      b_start += r.all_tiles();
+  int ct = (lo - start) / (r.tiles() + kItemCost);
+  start += ct * (r.tiles() + kItemCost);  // of the item
+  bool again = false;
+  for (; start < hi; start += r.tiles() + kItemCost, ++ct) {
+    while (ct * 16 >= r.columns || r.len == 0) {  // the next request: there is one, the line goes on
       r = request(a, ++b);
+      ct = 0;
     }
     const int tiles = r.tiles();
-    const int ct = (at - b_start) / tiles;
-    const int item = b_start + ct * tiles;  // its first tile
-    const int t_first = at - item, t_last = min(last - item, tiles);
+    // where this stretch cuts the item: an end within kPiece of one of the item's moves there
+    auto cut = [&](int t) { return t < kPiece ? 0 : (tiles - t < kPiece ? tiles : t); };
+    const int t_first = cut(lo - start), t_last = cut(hi - start);
+    if (t_first >= t_last) continue;
+    if (again) __syncthreads();  // the last item's outputs, queries and maxima lay where this one's go
+    again = true;
 
     // Q^T fragments (B operand), once for all waves; the k order of a block group's four products is the
     // lanes' own: k-slot (kg, e) of product (c, x) is latent (4c + kg) * 32 + x * 8 + e
@@ -270,16 +302,12 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
       load_tile(tile, pg, w0);
       pg = load_page(tile + kWaves);
       __syncthreads();  // Q
-      while (tile < t_last) {
+#pragma unroll 1
+      for (; tile < t_last; tile += kWaves) {
         load_tile(tile + kWaves, pg, w1);
         pg = load_page(tile + 2 * kWaves);
         tile_step(tile, w0);
-        tile += kWaves;
-        if (tile >= t_last) break;
-        load_tile(tile + kWaves, pg, w0);
-        pg = load_page(tile + 2 * kWaves);
-        tile_step(tile, w1);
-        tile += kWaves;
+        w0 = w1;
       }
     }
     l_run = xor32_sum(xor16_sum(l_run));
@@ -313,9 +341,16 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
     }
     __syncthreads();
     const bool whole = t_first == 0 && t_last == tiles;
-    const int slot = at == first ? 2 * blockIdx.x : 2 * blockIdx.x + 1;
-    if (t_first == 0 && tid == 0) a.starts[b * a.columns16 + ct] = item;
-#pragma unroll
+    const int slot = 2 * blockIdx.x + (t_first == 0);
+    if (t_first > 0 && tid == 0) {
+      // the workgroups that the item's first and last tiles went to
+      const int end = start + tiles;
+      int w0 = start / per, w1 = (end - 1) / per;
+      if ((w0 + 1) * per - start < kPiece) ++w0;
+      if (end - w1 * per < kPiece) --w1;
+      a.cuts[blockIdx.x] = make_int4(b, ct, w0, w1);
+    }
+#pragma unroll 1
     for (int i = 0; i < kPartFloats / 4 / kThreads; ++i) {
       const int f = tid + kThreads * i, c = f >> 7, d = (f & 127) * 4;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -353,76 +388,76 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
       a.part_ml[(slot * 16 + tid) * 2] = mm;
       a.part_ml[(slot * 16 + tid) * 2 + 1] = l;
     }
-    at = item + t_last;
-    if (at < last) __syncthreads();  // the next item's tiles, queries and maxima go where these were read
   }
 }
 
-// One workgroup per item, column and quarter of the features: joins the parts of an item that crossed
-// workgroups, writes zeros for a request with nothing cached, leaves finished items alone.  8 groups of 32
-// threads (4 features each) take every eighth part.
-__global__ __launch_bounds__(256) void mla_paged_merge_kernel(const PagedAttnArgs a) {
-  __shared__ float wgt[2 * kWgs];
-  __shared__ float red[8];
-  __shared__ float4 osum[8][32];
-  const int b = blockIdx.x / a.columns16, ct = blockIdx.x % a.columns16, c = blockIdx.y, tid = threadIdx.x;
-  const int lane = tid & 63, wv = tid >> 6;
+// Joins the parts of items that were cut.  Workgroup x stands for the cut between workgroups x and x + 1 of
+// the first launch: an item in n parts has n - 1 of them, which share its 16 x 512 outputs, so each reads
+// some 32 KB for each part more than one, however the parts are spread over items.
+__global__ __launch_bounds__(kThreads) void mla_paged_merge_kernel(const PagedAttnArgs a) {
+  __shared__ float weight[16][kWgs];   // of column (relative to the share's first) and part
+  __shared__ float4 sums[kThreads];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int4 item = a.cuts[blockIdx.x + 1];
+  if (item.x < 0) return;
+  const int b = item.x, ct = item.y, w0 = item.z, parts = item.w - w0 + 1;  // 2 .. kWgs
   const Request r = request(a, b);
-  const int cc = ct * 16 + c;
-  if (cc >= r.columns) return;
-  const int j = cc / a.heads, h = cc - j * a.heads;
-  const int d = blockIdx.z * 128 + (tid & 31) * 4;
-  bf16_t* o = a.out + (r.q0 + j) * a.o_ts + h * a.o_hs + d;
-  const int tiles = (r.len + kTile - 1) / kTile;
-  if (tiles == 0) {
-    if (tid < 32) *reinterpret_cast<uint2*>(o) = make_uint2(0, 0);
-    return;
-  }
-  const int per = a.starts[a.requests * a.columns16], item = a.starts[b * a.columns16 + ct];
-  const int w0 = item / per, w1 = (item + tiles - 1) / per;
-  if (w0 == w1) return;
-  const int parts = w1 - w0 + 1;  // <= kWgs
-  const int slot0 = item == w0 * per ? 2 * w0 : 2 * w0 + 1;
-  float m = -__FLT_MAX__, l = 0.f;
-  if (tid < parts) {
-    const int slot = tid ? 2 * (w0 + tid) : slot0;
-    m = a.part_ml[(slot * 16 + c) * 2];
-    l = a.part_ml[(slot * 16 + c) * 2 + 1];
-  }
-  float mm = wave_max(m);
-  if (lane == 0) red[wv] = mm;
-  __syncthreads();
-  mm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float w = __builtin_amdgcn_exp2f(m - mm);
-  const float ls = wave_sum(l * w);
-  if (lane == 0) red[4 + wv] = ls;
-  wgt[tid] = w;
-  __syncthreads();
-  const float lsum = (red[4] + red[5]) + (red[6] + red[7]);
-  const int grp = tid >> 5;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int p = grp; p < parts; p += 8) {
-    const int slot = p ? 2 * (w0 + p) : slot0;
-    const float4 x = *reinterpret_cast<const float4*>(a.part_o + static_cast<int64_t>(slot) * kPartFloats + c * kLat + d);
-    const float f = wgt[p];
-    v.x = __builtin_fmaf(f, x.x, v.x);
-    v.y = __builtin_fmaf(f, x.y, v.y);
-    v.z = __builtin_fmaf(f, x.z, v.z);
-    v.w = __builtin_fmaf(f, x.w, v.w);
-  }
-  osum[grp][tid & 31] = v;
-  __syncthreads();
-  if (tid < 32) {
-#pragma unroll
-    for (int g = 1; g < 8; ++g) {
-      v.x += osum[g][tid].x;
-      v.y += osum[g][tid].y;
-      v.z += osum[g][tid].z;
-      v.w += osum[g][tid].w;
+  const int share = (kPartFloats / 4 + parts - 2) / (parts - 1);  // groups of four outputs
+  const int f0 = (blockIdx.x - w0) * share, f1 = min(f0 + share, kPartFloats / 4);
+  if (f0 >= f1) return;
+  const int c0 = f0 >> 7, c1 = (f1 - 1) >> 7;
+  auto slot = [&](int p) { return 2 * (w0 + p) + (p == 0); };
+  for (int c = c0 + wv; c <= c1; c += kWaves) {
+    const int cc = ct * 16 + c;
+    float m = -__FLT_MAX__;
+    for (int p = lane; p < parts; p += 64) m = fmaxf(m, a.part_ml[(slot(p) * 16 + c) * 2]);
+    m = wave_max(m);
+    float l = 0.f;
+    for (int p = lane; p < parts; p += 64) {
+      const float2 x = *reinterpret_cast<const float2*>(a.part_ml + (slot(p) * 16 + c) * 2);
+      const float w = __builtin_amdgcn_exp2f(x.x - m);
+      weight[c - c0][p] = w;
+      l += x.y * w;
     }
-    const float inv = r.len - r.nq + j + 1 > 0 ? 1.0f / lsum : 0.f;
-    *reinterpret_cast<uint2*>(o) = make_uint2(pack2(v.x * inv, v.y * inv), pack2(v.z * inv, v.w * inv));
+    l = wave_sum(l);
+    const float inv = cc < r.columns && r.len - r.nq + cc / a.heads + 1 > 0 ? 1.0f / l : 0.f;
+    for (int p = lane; p < parts; p += 64) weight[c - c0][p] *= inv;
+  }
+  __syncthreads();
+  // threads in groups of the share's width, each group every so many parts
+  const int width = min(f1 - f0, kThreads), groups = kThreads / width, g = tid / width;
+  for (int f = f0 + tid % width; f < f1; f += width) {  // one pass with more than one group
+    const int c = f >> 7, d = (f & 127) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (groups == 1 && g > 0) break;
+    if (g < groups) {
+#pragma unroll 4
+      for (int p = g; p < parts; p += groups) {
+        const float4 x =
+            *reinterpret_cast<const float4*>(a.part_o + static_cast<int64_t>(slot(p)) * kPartFloats + c * kLat + d);
+        const float w = weight[c - c0][p];
+        v.x = __builtin_fmaf(w, x.x, v.x);
+        v.y = __builtin_fmaf(w, x.y, v.y);
+        v.z = __builtin_fmaf(w, x.z, v.z);
+        v.w = __builtin_fmaf(w, x.w, v.w);
+      }
+    }
+    if (groups > 1) {
+      sums[tid] = v;
+      __syncthreads();
+      if (g > 0) return;
+      for (int i = 1; i < groups; ++i) {
+        const float4 x = sums[i * width + tid];
+        v.x += x.x;
+        v.y += x.y;
+        v.z += x.z;
+        v.w += x.w;
+      }
+    }
+    const int cc = ct * 16 + c;
+    if (cc < r.columns)
+      *reinterpret_cast<uint2*>(a.out + (r.q0 + cc / a.heads) * a.o_ts + (cc % a.heads) * a.o_hs + d) =
+          make_uint2(pack2(v.x, v.y), pack2(v.z, v.w));
   }
 }
 
@@ -430,8 +465,7 @@ static int column_groups(int max_q, int heads) { return (max_q * heads + 15) / 1
 
 extern "C" int64_t dsv2_mla_paged_workspace_size(int requests, int max_q, int heads) {
   if (requests < 0 || max_q < 0 || heads < 0) return 0;
-  const int64_t starts = static_cast<int64_t>(requests) * ((static_cast<int64_t>(max_q) * heads + 15) / 16) + 1;
-  return 2 * kWgs * (kPartFloats + 32) * 4 + (starts * 4 + 15) / 16 * 16;
+  return kWgs * (2 * (kPartFloats + 32) * 4 + 16);
 }
 
 extern "C" int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_hs, int tokens, int heads,
@@ -455,7 +489,7 @@ extern "C" int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_
   const int groups = column_groups(max_q, heads), shift = page_shift(page_size);
   const int64_t items = static_cast<int64_t>(requests) * groups;
   const int64_t room = static_cast<int64_t>(table_width) << shift;
-  DSV2_REQUIRE(room <= INT32_MAX - kTile && items <= (1 << 22) && items <= INT32_MAX / ((room + kTile - 1) / kTile), DSV2_E_SHAPE,
+  DSV2_REQUIRE(room <= INT32_MAX - kTile && items <= INT32_MAX / ((room + kTile - 1) / kTile + kItemCost), DSV2_E_SHAPE,
                "mla_decode_paged_fp4: %d requests of up to %lld tokens, %d column groups each", requests, (long long)room,
                groups);
   DSV2_REQUIRE(workspace && dsv2_aligned16(workspace) &&
@@ -463,15 +497,16 @@ extern "C" int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_
                DSV2_E_SHAPE, "mla_decode_paged_fp4: workspace of %lld bytes", (long long)workspace_bytes);
   float* part_o = (float*)workspace;
   float* part_ml = part_o + 2 * kWgs * kPartFloats;
-  int32_t* starts = (int32_t*)(part_ml + 2 * kWgs * 32);
+  int4* cuts = (int4*)(part_ml + 2 * kWgs * 32);
   const PagedAttnArgs a{(const bf16_t*)q, q_ts, q_hs, tokens, heads, (const uint8_t*)pages, page_stride, n_pages,
                         shift, block_table, table_stride, table_width, lens, cu_q, max_q, requests, groups,
-                        softmax_scale * 1.4426950408889634f, (bf16_t*)out, out_ts, out_hs, part_o, part_ml, starts,
+                        softmax_scale * 1.4426950408889634f, (bf16_t*)out, out_ts, out_hs, part_o, part_ml, cuts,
                         status};
-  const int64_t most = items * ((room + kTile - 1) / kTile);
-  const int wgs = static_cast<int>(most / kMinTiles + 1 < kWgs ? most / kMinTiles + 1 : kWgs);
+  const int64_t tiles = (room + kTile - 1) / kTile, most = items * (tiles + kItemCost);
+  const int wgs = static_cast<int>(most / kMinStretch + 1 < kWgs ? most / kMinStretch + 1 : kWgs);
   hipLaunchKernelGGL(mla_paged_kernel, dim3(wgs), dim3(kThreads), kWaves * kWaveLds + kQLds, (hipStream_t)stream, a);
   if (const int rc = dsv2_launch_status("mla_decode_paged_fp4")) return rc;
-  hipLaunchKernelGGL(mla_paged_merge_kernel, dim3((unsigned)items, 16, 4), dim3(256), 0, (hipStream_t)stream, a);
+  if (wgs == 1 || tiles < 2 * kPiece) return DSV2_OK;  // no item of so few tiles is cut
+  hipLaunchKernelGGL(mla_paged_merge_kernel, dim3(wgs - 1), dim3(kThreads), 0, (hipStream_t)stream, a);
   return dsv2_launch_status("mla_decode_paged_fp4");
 }
