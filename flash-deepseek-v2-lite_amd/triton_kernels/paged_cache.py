@@ -20,7 +20,6 @@ from __future__ import annotations
 import torch
 
 from . import _hip
-from ._checks import require_cuda
 
 LAT, ROPE = 512, 64
 ROW = LAT + ROPE
@@ -28,89 +27,106 @@ TOKEN_BYTES = LAT // 2 + 2 * ROPE + LAT // 32  # 400
 MAX_REQUESTS = 4096
 MAX_HEADS = 128
 
+# These calls launch kernels of 2 to 10 us, so their own host time is looked at: a launch takes 3 us of it, a
+# torch.empty 1.3, an attribute of a tensor 0.05 to 0.1.
 _BF16, _I32, _U8 = torch.bfloat16, torch.int32, torch.uint8
-_STATUS: dict = {}  # device index -> int32 [1] status word of the functions below
+_PAGE_SIZES = frozenset(1 << i for i in range(11))
+_ENTRY = {n: getattr(_hip.lib, n) for n in ("dsv2_paged_step", "dsv2_paged_slots", "dsv2_paged_write_fp4",
+                                            "dsv2_paged_read_fp4", "dsv2_mla_decode_paged_fp4")}
+_WORKSPACE = {}  # (requests, max_q, heads) -> bytes
+_STATUS: dict = {}  # device index -> (int32 [1] status word of the functions below, its address)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _status(dev: torch.device) -> torch.Tensor:
-    st = _STATUS.get(dev.index)
-    if st is None:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("paged cache: the first call on a device must be outside graph capture")
-        st = _STATUS[dev.index] = torch.zeros(1, dtype=_I32, device=dev)
-        torch.cuda.current_stream(dev).synchronize()  # other streams' calls find it cleared
-    return st
+def _status(index: int) -> tuple[torch.Tensor, int]:
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("paged cache: the first call on a device must be outside graph capture")
+    st = torch.zeros(1, dtype=_I32, device=torch.device("cuda", index))
+    torch.cuda.current_stream(index).synchronize()  # other streams' calls find it cleared
+    return _STATUS.setdefault(index, (st, st.data_ptr()))
 
 
 def check_paged_status(device: torch.device | str = "cuda") -> None:
     """Raise if a call on `device` since the last check skipped something (synchronises)."""
-    dev = torch.device(device)
-    st = _STATUS.get(torch.cuda.current_device() if dev.index is None else dev.index)
-    bits = 0 if st is None else int(st.item())
+    index = torch.device(device).index
+    known = _STATUS.get(torch.cuda.current_device() if index is None else index)
+    bits = 0 if known is None else int(known[0].item())
     if not bits:
         return
-    st.zero_()
+    known[0].zero_()
     what = [text for bit, text in ((1, "a request outgrew its block table"), (2, "no free page was left"),
                                    (4, "a slot, page or position lay outside the pool or block table"),
                                    (8, "there were more new tokens than max_tokens or max_q")) if bits & bit]
     raise RuntimeError("paged cache: " + "; ".join(what) + "; those tokens were skipped")
 
 
-def _call(dev: torch.device, name: str, *args) -> None:
-    """The entry point on dev's current stream, with dev as the current device."""
-    if torch.cuda.current_device() == dev.index:
-        _hip.call(name, *args, _status(dev).data_ptr(), _hip.stream_ptr(dev))
-        return
-    with torch.cuda.device(dev):
-        _hip.call(name, *args, _status(dev).data_ptr(), _hip.stream_ptr(dev))
+def _call(index: int, entry: str, *args) -> None:
+    """The entry point on the device's current stream, with the device as the current one."""
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return _call(index, entry, *args)
+    known = _STATUS.get(index) or _status(index)
+    rc = _ENTRY[entry](*args, known[1], _hip._raw_stream(index))
+    if rc:
+        raise _hip.HipKernelError(f"{entry} failed (status {rc}): "
+                                  f"{_hip.lib.dsv2_last_error_message().decode(errors='replace')}")
 
 
-def _same_device(name: str, *ts: torch.Tensor) -> torch.device:
-    require_cuda(name, *ts)
-    dev = ts[0].device
-    for t in ts[1:]:
-        if t.device != dev:
-            raise ValueError(f"{name}: tensors on {dev} and {t.device}")
-    return dev
+def _device(name: str, *ts: torch.Tensor) -> int:
+    """The index of the one GPU that all tensors are on."""
+    index = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != index or index < 0:
+            if not t.is_cuda:
+                raise NotImplementedError(f"{name} requires CUDA (HIP) tensors")
+            raise ValueError(f"{name}: tensors on {ts[0].device} and {t.device}")
+    return index
 
 
-def _int32(name: str, what: str, t: torch.Tensor, n: int | None = None) -> None:
-    if t.dtype != _I32:
+def _int32(name: str, what: str, t: torch.Tensor, n: int | None = None) -> int:
+    """The length of an int32 vector (n, if given)."""
+    if t.dtype is not _I32:
         raise NotImplementedError(f"{name}: {what} must be int32")
-    if t.ndim != 1 or (n is not None and t.shape[0] != n):
-        raise ValueError(f"{name}: {what} must be [{'n' if n is None else n}]")
-    if t.shape[0] > 1 and t.stride(0) != 1:
+    shape = t.shape
+    if len(shape) != 1 or (n is not None and shape[0] != n):
+        raise ValueError(f"{name}: {what} must be [{'n' if n is None else n}], not {list(shape)}")
+    if not t.is_contiguous():
         raise NotImplementedError(f"{name}: {what} must be contiguous")
+    return shape[0]
 
 
 def _table(name: str, t: torch.Tensor, n: int) -> tuple[int, int]:
     """(row stride, width) of a block table."""
-    if t.dtype != _I32:
+    if t.dtype is not _I32:
         raise NotImplementedError(f"{name}: block_table must be int32")
-    if t.ndim != 2 or t.shape[0] != n or t.shape[1] == 0:
-        raise ValueError(f"{name}: block_table must be [{n}, pages of a request]")
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != n or shape[1] == 0:
+        raise ValueError(f"{name}: block_table must be [{n}, pages of a request], not {list(shape)}")
+    width = shape[1]
     rs, cs = t.stride()
-    width = t.shape[1]
     if cs != 1 and width > 1 or rs < width and n > 1:
         raise NotImplementedError(f"{name}: block_table rows must be contiguous and apart")
-    return max(rs, width), width
+    return (rs if rs > width else width), width
 
 
 def _pool(name: str, pages: torch.Tensor) -> tuple[int, int, int]:
     """(page stride in bytes, pages, page size) of a pool."""
-    if pages.dtype != _U8:
+    if pages.dtype is not _U8:
         raise NotImplementedError(f"{name}: pages must be uint8")
-    if pages.ndim != 2 or pages.shape[0] == 0 or pages.shape[1] == 0 or pages.shape[1] % TOKEN_BYTES:
-        raise ValueError(f"{name}: pages must be [n_pages, page_size * {TOKEN_BYTES}]")
-    n, width = pages.shape
-    ps, cs = pages.stride()
-    if cs != 1 or ps < width and n > 1:
+    shape = pages.shape
+    if len(shape) != 2 or shape[0] == 0 or shape[1] == 0 or shape[1] % TOKEN_BYTES:
+        raise ValueError(f"{name}: pages must be [n_pages, page_size * {TOKEN_BYTES}], not {list(shape)}")
+    n, width = shape
+    stride, cs = pages.stride()
+    if cs != 1 or stride < width and n > 1:
         raise NotImplementedError(f"{name}: pages must be contiguous and apart")
-    return max(ps, width), n, width // TOKEN_BYTES
+    page_size = width // TOKEN_BYTES
+    _page_size(name, page_size)
+    return (stride if stride > width else width), n, page_size
 
 
 def _page_size(name: str, page_size: int) -> None:
-    if page_size < 1 or page_size > 1024 or page_size & (page_size - 1):
+    if page_size not in _PAGE_SIZES:
         raise ValueError(f"{name}: page_size must be a power of two up to 1024, not {page_size}")
 
 
@@ -129,25 +145,23 @@ def paged_cache_step(state: torch.Tensor, delta: torch.Tensor, block_table: torc
     -1.  A request whose tokens do not fit the table, ``max_tokens`` or the free pages that the
     requests before it leave keeps its length; its tokens get -1 and check_paged_status raises."""
     name = "paged_cache_step"
-    dev = _same_device(name, state, delta, block_table, free_pages)
-    n = delta.shape[0] if delta.ndim == 1 else -1
-    _int32(name, "delta", delta)
+    index = _device(name, state, delta, block_table, free_pages)
+    n = _int32(name, "delta", delta)
     _int32(name, "state", state, n + 2)
-    _int32(name, "free_pages", free_pages)
+    pages = _int32(name, "free_pages", free_pages)
     _page_size(name, page_size)
     ts, width = _table(name, block_table, n)
-    if n > MAX_REQUESTS or free_pages.shape[0] == 0 or max_tokens < 0:
-        raise ValueError(f"{name}: {n} requests (at most {MAX_REQUESTS}), {free_pages.shape[0]} pages, max_tokens "
-                         f"{max_tokens}")
-    after = torch.empty(n + 2, dtype=_I32, device=dev)
-    maps = torch.empty((3, max_tokens), dtype=_I32, device=dev)
+    if n > MAX_REQUESTS or pages == 0 or max_tokens < 0:
+        raise ValueError(f"{name}: {n} requests (at most {MAX_REQUESTS}), {pages} pages, max_tokens {max_tokens}")
+    outs = state.new_empty(n + 2 + 3 * max_tokens)  # one allocation: the state, then the three maps
     if n == 0:
-        return after.copy_(state), *maps.fill_(-1).unbind(0)
-    at = maps.data_ptr()
-    _call(dev, "dsv2_paged_step", state.data_ptr(), delta.data_ptr(), n, block_table.data_ptr(), ts, width,
-          free_pages.data_ptr(), free_pages.shape[0], page_size, max_tokens, after.data_ptr(), at,
-          at + 4 * max_tokens, at + 8 * max_tokens)
-    return after, *maps.unbind(0)
+        outs.fill_(-1)[:2] = state
+    else:
+        at = outs.data_ptr()
+        maps, size = at + 4 * n + 8, 4 * max_tokens
+        _call(index, "dsv2_paged_step", state.data_ptr(), delta.data_ptr(), n, block_table.data_ptr(), ts, width,
+              free_pages.data_ptr(), pages, page_size, max_tokens, at, maps, maps + size, maps + 2 * size)
+    return torch.unsafe_split_with_sizes(outs, (n + 2, max_tokens, max_tokens, max_tokens))
 
 
 def paged_slot_map(starts: torch.Tensor, counts: torch.Tensor, block_table: torch.Tensor, page_size: int,
@@ -156,33 +170,33 @@ def paged_slot_map(starts: torch.Tensor, counts: torch.Tensor, block_table: torc
     after the other, int32 [max_tokens]; -1 from the last one on, and for positions or pages out of
     range."""
     name = "paged_slot_map"
-    dev = _same_device(name, starts, counts, block_table)
-    n = starts.shape[0] if starts.ndim == 1 else -1
-    _int32(name, "starts", starts)
+    index = _device(name, starts, counts, block_table)
+    n = _int32(name, "starts", starts)
     _int32(name, "counts", counts, n)
     _page_size(name, page_size)
     ts, width = _table(name, block_table, n)
     if n > MAX_REQUESTS or max_tokens < 0:
         raise ValueError(f"{name}: {n} requests (at most {MAX_REQUESTS}), max_tokens {max_tokens}")
-    maps = torch.empty((3, max_tokens), dtype=_I32, device=dev)
+    maps = starts.new_empty(3 * max_tokens)
     if n == 0 or max_tokens == 0:
-        return maps.fill_(-1).unbind(0)
-    at = maps.data_ptr()
-    _call(dev, "dsv2_paged_slots", starts.data_ptr(), counts.data_ptr(), n, block_table.data_ptr(), ts, width,
-          page_size, max_tokens, at, at + 4 * max_tokens, at + 8 * max_tokens)
-    return maps.unbind(0)
+        maps.fill_(-1)
+    else:
+        at, size = maps.data_ptr(), 4 * max_tokens
+        _call(index, "dsv2_paged_slots", starts.data_ptr(), counts.data_ptr(), n, block_table.data_ptr(), ts, width,
+              page_size, max_tokens, at, at + size, at + 2 * size)
+    return torch.unsafe_split_with_sizes(maps, (max_tokens, max_tokens, max_tokens))
 
 
 def _cache_rows(name: str, what: str, rows: torch.Tensor, n: int) -> int:
     """Row stride of [n, 576] bf16 cache rows."""
-    if rows.dtype != _BF16:
+    if rows.dtype is not _BF16:
         raise NotImplementedError(f"{name}: {what} must be bf16")
     if rows.shape != (n, ROW):
-        raise ValueError(f"{name}: {what} must be [{n}, {ROW}]")
+        raise ValueError(f"{name}: {what} must be [{n}, {ROW}], not {list(rows.shape)}")
     rs, cs = rows.stride()
     if cs != 1 or rs < ROW and n > 1:
         raise NotImplementedError(f"{name}: {what} must have contiguous rows")
-    return max(rs, ROW)
+    return rs if n > 1 else ROW
 
 
 def paged_cache_write_fp4(rows: torch.Tensor, slots: torch.Tensor, pages: torch.Tensor) -> None:
@@ -190,29 +204,28 @@ def paged_cache_write_fp4(rows: torch.Tensor, slots: torch.Tensor, pages: torch.
     multiple of 8) into ``slots`` (int32 [n]) of ``pages``; a row with a negative slot is left out.
     Of two rows with the same slot either may stay."""
     name = "paged_cache_write_fp4"
-    dev = _same_device(name, rows, slots, pages)
-    _int32(name, "slots", slots)
-    n = slots.shape[0]
+    index = _device(name, rows, slots, pages)
+    n = _int32(name, "slots", slots)
     rs = _cache_rows(name, "rows", rows, n)
     page_stride, n_pages, page_size = _pool(name, pages)
     if n:
-        _call(dev, "dsv2_paged_write_fp4", rows.data_ptr(), rs, n, slots.data_ptr(), pages.data_ptr(), page_stride,
+        _call(index, "dsv2_paged_write_fp4", rows.data_ptr(), rs, n, slots.data_ptr(), pages.data_ptr(), page_stride,
               n_pages, page_size)
 
 
 def paged_cache_read_fp4(pages: torch.Tensor, slots: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """The bf16 rows [n, 576] that ``slots`` (int32 [n]) hold, exactly; zeros for a negative slot."""
     name = "paged_cache_read_fp4"
-    dev = _same_device(name, pages, slots) if out is None else _same_device(name, pages, slots, out)
-    _int32(name, "slots", slots)
-    n = slots.shape[0]
+    index = _device(name, pages, slots)
+    n = _int32(name, "slots", slots)
     page_stride, n_pages, page_size = _pool(name, pages)
     if out is None:
-        out, os = torch.empty((n, ROW), dtype=_BF16, device=dev), ROW
+        out, os = torch.empty((n, ROW), dtype=_BF16, device=slots.device), ROW
     else:
+        _device(name, pages, out)
         os = _cache_rows(name, "out", out, n)
     if n:
-        _call(dev, "dsv2_paged_read_fp4", pages.data_ptr(), page_stride, n_pages, page_size, slots.data_ptr(), n,
+        _call(index, "dsv2_paged_read_fp4", pages.data_ptr(), page_stride, n_pages, page_size, slots.data_ptr(), n,
               out.data_ptr(), os)
     return out
 
@@ -230,46 +243,48 @@ def attention_decode_paged_fp4(q: torch.Tensor, pages: torch.Tensor, block_table
     gives zeros; query tokens past cu_q[B] are not written (in a fresh ``out`` they are undefined).
     Up to 128 heads; q and out may have any token and head strides that are multiples of 8."""
     name = "attention_decode_paged_fp4"
-    dev = _same_device(name, q, pages, block_table, lens)
-    if q.dtype != _BF16:
+    index = _device(name, q, pages, block_table, lens)
+    if q.dtype is not _BF16:
         raise NotImplementedError(f"{name} supports bf16 only")
-    if q.ndim != 3 or q.shape[2] != ROW or not 0 < q.shape[1] <= MAX_HEADS:
-        raise ValueError(f"{name} expects q [tokens, heads up to {MAX_HEADS}, {ROW}]")
-    t, h, _ = q.shape
-    _int32(name, "lens", lens)
-    n = lens.shape[0]
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != ROW or not 0 < shape[1] <= MAX_HEADS:
+        raise ValueError(f"{name} expects q [tokens, heads up to {MAX_HEADS}, {ROW}], not {list(shape)}")
+    t, h, _ = shape
+    n = _int32(name, "lens", lens)
     page_stride, n_pages, page_size = _pool(name, pages)
-    _page_size(name, page_size)
     ts, width = _table(name, block_table, n)
     if cu_q is None:
         if n != t or max_q != 1:
             raise ValueError(f"{name}: without cu_q there is one query token a request ({t} for {n})")
+        cu = None
     else:
-        _same_device(name, q, cu_q)
+        _device(name, q, cu_q)
         _int32(name, "cu_q", cu_q, n + 1)
         if max_q < 1:
             raise ValueError(f"{name}: max_q must be positive")
-        max_q = min(max_q, max(t, 1))
+        max_q, cu = min(max_q, max(t, 1)), cu_q.data_ptr()
     q_ts, q_hs, q_ds = q.stride()
     if q_ds != 1:
         raise NotImplementedError(f"{name} needs a contiguous last dimension")
     if out is None:
-        out = torch.empty((t, h, LAT), dtype=_BF16, device=dev)
+        out = q.new_empty((t, h, LAT))
         o_ts, o_hs = h * LAT, LAT
     else:
-        _same_device(name, q, out)
-        if out.dtype != _BF16:
+        _device(name, q, out)
+        if out.dtype is not _BF16:
             raise NotImplementedError(f"{name} writes bf16 only")
         if out.shape != (t, h, LAT):
-            raise ValueError(f"{name}: out must be [{t}, {h}, {LAT}]")
+            raise ValueError(f"{name}: out must be [{t}, {h}, {LAT}], not {list(out.shape)}")
         o_ts, o_hs, o_ds = out.stride()
         if o_ds != 1 or h > 1 and o_hs < LAT or t > 1 and o_ts < LAT:
             raise NotImplementedError(f"{name}: out's rows must be contiguous and apart")
     if t == 0 or n == 0:
         return out
-    size = _hip.lib.dsv2_mla_paged_workspace_size(n, max_q, h)
-    ws = torch.empty(size, dtype=_U8, device=dev)
-    _call(dev, "dsv2_mla_decode_paged_fp4", q.data_ptr(), q_ts, q_hs, t, h, pages.data_ptr(), page_stride, n_pages,
-          page_size, block_table.data_ptr(), ts, width, lens.data_ptr(), n, None if cu_q is None else cu_q.data_ptr(),
-          max_q, float(softmax_scale), out.data_ptr(), o_ts, o_hs, ws.data_ptr(), size)
+    size = _WORKSPACE.get((n, max_q, h))
+    if size is None:
+        size = _WORKSPACE[n, max_q, h] = _hip.lib.dsv2_mla_paged_workspace_size(n, max_q, h)
+    ws = pages.new_empty(size)
+    _call(index, "dsv2_mla_decode_paged_fp4", q.data_ptr(), q_ts, q_hs, t, h, pages.data_ptr(), page_stride, n_pages,
+          page_size, block_table.data_ptr(), ts, width, lens.data_ptr(), n, cu, max_q, softmax_scale, out.data_ptr(),
+          o_ts, o_hs, ws.data_ptr(), size)
     return out

@@ -84,9 +84,9 @@ REFUSED = [
 
 @pytest.mark.parametrize("name,at,value,error,text", REFUSED)
 def test_functions_refuse_other_shapes_types_and_strides(monkeypatch, name, at, value, error, text):
-    monkeypatch.setattr(P, "require_cuda", lambda *a: None)
+    monkeypatch.setattr(P, "_device", lambda *a: 0)
     calls = []
-    monkeypatch.setattr(P, "_call", lambda dev, entry, *args: calls.append(entry))
+    monkeypatch.setattr(P, "_call", lambda index, entry, *args: calls.append(entry))
     getattr(P, name)(*good()[name])
     assert len(calls) == 1
     args = good()[name]
