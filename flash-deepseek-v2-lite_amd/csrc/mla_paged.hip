@@ -54,8 +54,8 @@ struct PagedAttnArgs {
   int64_t o_ts, o_hs;
   float* part_o;     // [2 * kWgs][16][512]
   float* part_ml;    // [2 * kWgs][16][2]
-  int4* cuts;        // [kWgs]: the item that a workgroup's first piece continues (request or -1, column
-                     // group) and the workgroups that it begins and ends in
+  int4* cuts;        // [kWgs][2]: the item that a workgroup's first piece continues (first column or -1, its
+                     // request's columns, the workgroups that it begins and ends in) and its request
   int32_t* status;
 };
 
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
     }
     per = max((total + kWgs - 1) / kWgs, kMinStretch);
     const int64_t from = static_cast<int64_t>(blockIdx.x) * per;
-    if (tid == 0) a.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (tid == 0) a.cuts[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
     if (from >= total) return;
     lo = static_cast<int>(from);
     hi = min(lo + per, total);
@@ -348,7 +348,8 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
       int w0 = start / per, w1 = (end - 1) / per;
       if ((w0 + 1) * per - start < kPiece) ++w0;
       if (end - w1 * per < kPiece) --w1;
-      a.cuts[blockIdx.x] = make_int4(b, ct, w0, w1);
+      a.cuts[2 * blockIdx.x] = make_int4(ct * 16, r.columns, w0, w1);
+      a.cuts[2 * blockIdx.x + 1] = make_int4(r.len, r.nq, r.q0, 0);
     }
 #pragma unroll 1
     for (int i = 0; i < kPartFloats / 4 / kThreads; ++i) {
@@ -393,71 +394,97 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
 
 // Joins the parts of items that were cut.  Workgroup x stands for the cut between workgroups x and x + 1 of
 // the first launch: an item in n parts has n - 1 of them, which share its 16 x 512 outputs, so each reads
-// some 32 KB for each part more than one, however the parts are spread over items.
-__global__ __launch_bounds__(kThreads) void mla_paged_merge_kernel(const PagedAttnArgs a) {
+// some 32 KB for each part more than one, however the parts are spread over items.  Everything that it needs
+// is requested at once, when it knows its item: a thread's part of the outputs takes 8 loads at most (2 and 4
+// parts: 4 and 2 times all parts; 8: 8 parts; 256: every 56th part of 9 groups of four outputs, 5 loads).
+__global__ __launch_bounds__(512) void mla_paged_merge_kernel(const PagedAttnArgs a) {
+  constexpr int kLoads = 8, kLaneParts = kWgs / 64;
   __shared__ float weight[16][kWgs];   // of column (relative to the share's first) and part
-  __shared__ float4 sums[kThreads];
+  __shared__ float4 sums[512];
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const int4 item = a.cuts[blockIdx.x + 1];
+  const int4 item = a.cuts[2 * (blockIdx.x + 1)], req = a.cuts[2 * (blockIdx.x + 1) + 1];
   if (item.x < 0) return;
-  const int b = item.x, ct = item.y, w0 = item.z, parts = item.w - w0 + 1;  // 2 .. kWgs
-  const Request r = request(a, b);
+  const int col0 = item.x, columns = item.y, w0 = item.z, parts = item.w - w0 + 1;  // 2 .. kWgs
   const int share = (kPartFloats / 4 + parts - 2) / (parts - 1);  // groups of four outputs
   const int f0 = (blockIdx.x - w0) * share, f1 = min(f0 + share, kPartFloats / 4);
   if (f0 >= f1) return;
   const int c0 = f0 >> 7, c1 = (f1 - 1) >> 7;
   auto slot = [&](int p) { return 2 * (w0 + p) + (p == 0); };
-  for (int c = c0 + wv; c <= c1; c += kWaves) {
-    const int cc = ct * 16 + c;
-    float m = -__FLT_MAX__;
-    for (int p = lane; p < parts; p += 64) m = fmaxf(m, a.part_ml[(slot(p) * 16 + c) * 2]);
+  float2 ml[2][kLaneParts];  // wave w: columns c0 + w and c0 + w + 8, lane l: parts l, l + 64, ...
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int k = 0; k < kLaneParts; ++k) {
+      const int c = c0 + wv + 8 * i, p = lane + 64 * k;
+      ml[i][k] = make_float2(-__FLT_MAX__, 0.f);
+      if (c <= c1 && p < parts) ml[i][k] = *reinterpret_cast<const float2*>(a.part_ml + (slot(p) * 16 + c) * 2);
+    }
+  // threads in groups of the share's width, each group every so many parts; a share wider than the
+  // workgroup goes in passes
+  const int width = min(f1 - f0, 512), groups = 512 / width, g = tid / width;
+  const int in_pass = (parts + groups - 1) / groups, loads = (f1 - f0 + width - 1) / width * in_pass;
+  float4 x[kLoads];
+#pragma unroll
+  for (int k = 0; k < kLoads; ++k) {
+    const int f = f0 + tid - g * width + k / in_pass * width, p = g + k % in_pass * groups;
+    x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (k < loads && g < groups && f < f1 && p < parts)
+      x[k] = *reinterpret_cast<const float4*>(a.part_o + static_cast<int64_t>(slot(p)) * kPartFloats + f * 4);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int c = c0 + wv + 8 * i;
+    if (c > c1) break;
+    float m = ml[i][0].x;
+#pragma unroll
+    for (int k = 1; k < kLaneParts; ++k) m = fmaxf(m, ml[i][k].x);
     m = wave_max(m);
-    float l = 0.f;
-    for (int p = lane; p < parts; p += 64) {
-      const float2 x = *reinterpret_cast<const float2*>(a.part_ml + (slot(p) * 16 + c) * 2);
-      const float w = __builtin_amdgcn_exp2f(x.x - m);
-      weight[c - c0][p] = w;
-      l += x.y * w;
+    float l = 0.f, w[kLaneParts];
+#pragma unroll
+    for (int k = 0; k < kLaneParts; ++k) {
+      w[k] = __builtin_amdgcn_exp2f(ml[i][k].x - m);
+      l += ml[i][k].y * w[k];
     }
     l = wave_sum(l);
-    const float inv = cc < r.columns && r.len - r.nq + cc / a.heads + 1 > 0 ? 1.0f / l : 0.f;
-    for (int p = lane; p < parts; p += 64) weight[c - c0][p] *= inv;
+    const int cc = col0 + c;
+    const float inv = cc < columns && req.x - req.y + cc / a.heads + 1 > 0 ? 1.0f / l : 0.f;
+#pragma unroll
+    for (int k = 0; k < kLaneParts; ++k)
+      if (lane + 64 * k < parts) weight[c - c0][lane + 64 * k] = w[k] * inv;
   }
   __syncthreads();
-  // threads in groups of the share's width, each group every so many parts
-  const int width = min(f1 - f0, kThreads), groups = kThreads / width, g = tid / width;
-  for (int f = f0 + tid % width; f < f1; f += width) {  // one pass with more than one group
-    const int c = f >> 7, d = (f & 127) * 4;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (groups == 1 && g > 0) break;
-    if (g < groups) {
-#pragma unroll 4
-      for (int p = g; p < parts; p += groups) {
-        const float4 x =
-            *reinterpret_cast<const float4*>(a.part_o + static_cast<int64_t>(slot(p)) * kPartFloats + c * kLat + d);
-        const float w = weight[c - c0][p];
-        v.x = __builtin_fmaf(w, x.x, v.x);
-        v.y = __builtin_fmaf(w, x.y, v.y);
-        v.z = __builtin_fmaf(w, x.z, v.z);
-        v.w = __builtin_fmaf(w, x.w, v.w);
-      }
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < kLoads; ++k) {
+    if (k >= loads) break;
+    const int f = f0 + tid - g * width + k / in_pass * width, p = g + k % in_pass * groups;
+    const bool mine = g < groups && f < f1 && p < parts;
+    const int c = f >> 7;
+    if (mine) {
+      const float w = weight[c - c0][p];
+      v.x = __builtin_fmaf(w, x[k].x, v.x);
+      v.y = __builtin_fmaf(w, x[k].y, v.y);
+      v.z = __builtin_fmaf(w, x[k].z, v.z);
+      v.w = __builtin_fmaf(w, x[k].w, v.w);
     }
-    if (groups > 1) {
+    if (k % in_pass != in_pass - 1) continue;
+    if (groups > 1) {  // one pass
       sums[tid] = v;
       __syncthreads();
       if (g > 0) return;
       for (int i = 1; i < groups; ++i) {
-        const float4 x = sums[i * width + tid];
-        v.x += x.x;
-        v.y += x.y;
-        v.z += x.z;
-        v.w += x.w;
+        const float4 u = sums[i * width + tid];
+        v.x += u.x;
+        v.y += u.y;
+        v.z += u.z;
+        v.w += u.w;
       }
     }
-    const int cc = ct * 16 + c;
-    if (cc < r.columns)
-      *reinterpret_cast<uint2*>(a.out + (r.q0 + cc / a.heads) * a.o_ts + (cc % a.heads) * a.o_hs + d) =
+    const int cc = col0 + c;
+    if (g == 0 && f < f1 && cc < columns)
+      *reinterpret_cast<uint2*>(a.out + (req.z + cc / a.heads) * a.o_ts + (cc % a.heads) * a.o_hs + (f & 127) * 4) =
           make_uint2(pack2(v.x, v.y), pack2(v.z, v.w));
+    v = make_float4(0.f, 0.f, 0.f, 0.f);
   }
 }
 
@@ -465,7 +492,7 @@ static int column_groups(int max_q, int heads) { return (max_q * heads + 15) / 1
 
 extern "C" int64_t dsv2_mla_paged_workspace_size(int requests, int max_q, int heads) {
   if (requests < 0 || max_q < 0 || heads < 0) return 0;
-  return kWgs * (2 * (kPartFloats + 32) * 4 + 16);
+  return kWgs * (2 * (kPartFloats + 32) * 4 + 32);
 }
 
 extern "C" int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_hs, int tokens, int heads,
@@ -507,6 +534,6 @@ extern "C" int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_
   hipLaunchKernelGGL(mla_paged_kernel, dim3(wgs), dim3(kThreads), kWaves * kWaveLds + kQLds, (hipStream_t)stream, a);
   if (const int rc = dsv2_launch_status("mla_decode_paged_fp4")) return rc;
   if (wgs == 1 || tiles < 2 * kPiece) return DSV2_OK;  // no item of so few tiles is cut
-  hipLaunchKernelGGL(mla_paged_merge_kernel, dim3(wgs - 1), dim3(kThreads), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(mla_paged_merge_kernel, dim3(wgs - 1), dim3(512), 0, (hipStream_t)stream, a);
   return dsv2_launch_status("mla_decode_paged_fp4");
 }
