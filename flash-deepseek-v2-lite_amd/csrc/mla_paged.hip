@@ -59,6 +59,9 @@ struct PagedAttnArgs {
   int32_t* status;
 };
 
+// a value that all lanes have, to scalar registers: what follows from it stays off the vector units
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 struct Request {
   int len, q0, nq, columns;
   __device__ __forceinline__ int tiles() const { return (len + kTile - 1) / kTile; }
@@ -67,6 +70,9 @@ struct Request {
     return len > 0 ? (tiles() + kItemCost) * ((columns + 15) / 16) : 0;
   }
 };
+__device__ __forceinline__ Request uniform(const Request& r) {
+  return {uniform(r.len), uniform(r.q0), uniform(r.nq), uniform(r.columns)};
+}
 __device__ __forceinline__ Request request(const PagedAttnArgs& a, int b) {
   Request r;
   const int64_t room = static_cast<int64_t>(a.width) << a.shift;
@@ -96,13 +102,17 @@ __device__ __forceinline__ floatx4_t mfma16x16x16(const uint2& a, const uint2& b
 }
 }  // namespace
 
+// kOnePage (pages of at least a tile, whose tiles then lie in one page each): a tile's address is the wave's, in
+// scalar registers, and the lanes' offsets never change; with smaller pages every lane has its own
+template <bool kOnePage>
 __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ float ml[kWaves][16][2];
   __shared__ int32_t wave_sums[kWaves];
   __shared__ int4 first_request[2];
   uint4* const q_lds = reinterpret_cast<uint4*>(smem + kWaves * kWaveLds);
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, li = lane & 15, kg = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6), li = lane & 15,
+            kg = lane >> 4;
 
   // the length of the line (the host has checked that it stays within int32), and the request that this
   // workgroup's stretch begins in
@@ -143,6 +153,7 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
       if (i < wv) before += wave_sums[i];
       total += wave_sums[i];
     }
+    total = uniform(total);
     per = max((total + kWgs - 1) / kWgs, kMinStretch);
     const int64_t from = static_cast<int64_t>(blockIdx.x) * per;
     if (tid == 0) a.cuts[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
@@ -162,12 +173,9 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
     }
     __syncthreads();
     const int4 u = first_request[0], v = first_request[1];
-    b = u.x;
-    start = u.y;
-    r.len = v.x;
-    r.q0 = v.y;
-    r.nq = v.z;
-    r.columns = v.w;
+    b = uniform(u.x);
+    start = uniform(u.y);
+    r = uniform(Request{v.x, v.y, v.z, v.w});
   }
 
   bf16_t* const vt = reinterpret_cast<bf16_t*>(smem + wv * kWaveLds);
@@ -179,6 +187,11 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
       r = request(a, ++b);
       ct = 0;
     }
+    // (the compiler does not see that these are the same for all lanes)
+    r = uniform(r);
+    b = uniform(b);
+    ct = uniform(ct);
+    start = uniform(start);
     const int tiles = r.tiles();
     // where this stretch cuts the item: an end within kPiece of one of the item's moves there
     auto cut = [&](int t) { return t < kPiece ? 0 : (tiles - t < kPiece ? tiles : t); };
@@ -205,21 +218,27 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
 
     const int32_t* row = a.table + b * a.ts;
     const int end = t_last - 1;
-    auto load_page = [&](int tile) { return row[min(min(tile, end) * kTile + li, r.len - 1) >> a.shift]; };
+    auto load_page = [&](int tile) {
+      const int t = min(tile, end) * kTile;
+      return row[(kOnePage ? t : min(t + li, r.len - 1)) >> a.shift];
+    };
     auto load_tile = [&](int tile, int pg, Raw& w) {
-      const int t = min(tile, end) * kTile + li;
+      const int t0 = min(tile, end) * kTile;
+      if (kOnePage) pg = uniform(pg);
       const bool page = pg >= 0 && pg < a.n_pages;
-      w.ok = page && t < r.len;
-      if (!page && kg == 0 && t < r.len && a.status) atomicOr(a.status, DSV2_DEVERR_BAD_SLOT);
-      const int off = min(t, r.len - 1) & ((1 << a.shift) - 1);
+      const int t = kOnePage ? t0 : min(t0 + li, r.len - 1);
+      w.ok = page && t0 + li < r.len;
+      if (!page && kg == 0 && t0 + li < r.len && a.status) atomicOr(a.status, DSV2_DEVERR_BAD_SLOT);
+      const int off = t & ((1 << a.shift) - 1);
       const uint8_t* base = a.pages + (page ? pg : 0) * a.page_stride;
-      const uint8_t* code = base + off * kCodeB + kg * 16;
+      const uint8_t *code = base + off * kCodeB, *rope = base + (kCodeB << a.shift) + off * kRopeB,
+                    *scale = base + ((kCodeB + kRopeB) << a.shift) + off * kScaleB;
+      const uint32_t token = kOnePage ? li : 0;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) w.code[c] = ldg16(code + c * 64);
-      const uint8_t* rope = base + (kCodeB << a.shift) + off * kRopeB + kg * 16;
+      for (int c = 0; c < 4; ++c) w.code[c] = ldg16(code + (token * kCodeB + kg * 16 + c * 64));
 #pragma unroll
-      for (int y = 0; y < 2; ++y) w.rope[y] = ldg16(rope + y * 64);
-      w.scale = ldg16(base + ((kCodeB + kRopeB) << a.shift) + off * kScaleB);
+      for (int y = 0; y < 2; ++y) w.rope[y] = ldg16(rope + (token * kRopeB + kg * 16 + y * 64));
+      w.scale = ldg16(scale + token * kScaleB);
     };
 
     float m_run = -__FLT_MAX__, l_run = 0.f;
@@ -531,7 +550,10 @@ extern "C" int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_
                         status};
   const int64_t tiles = (room + kTile - 1) / kTile, most = items * (tiles + kItemCost);
   const int wgs = static_cast<int>(most / kMinStretch + 1 < kWgs ? most / kMinStretch + 1 : kWgs);
-  hipLaunchKernelGGL(mla_paged_kernel, dim3(wgs), dim3(kThreads), kWaves * kWaveLds + kQLds, (hipStream_t)stream, a);
+  if ((1 << shift) >= kTile)
+    hipLaunchKernelGGL(mla_paged_kernel<true>, dim3(wgs), dim3(kThreads), kWaves * kWaveLds + kQLds, (hipStream_t)stream, a);
+  else
+    hipLaunchKernelGGL(mla_paged_kernel<false>, dim3(wgs), dim3(kThreads), kWaves * kWaveLds + kQLds, (hipStream_t)stream, a);
   if (const int rc = dsv2_launch_status("mla_decode_paged_fp4")) return rc;
   if (wgs == 1 || tiles < 2 * kPiece) return DSV2_OK;  // no item of so few tiles is cut
   hipLaunchKernelGGL(mla_paged_merge_kernel, dim3(wgs - 1), dim3(512), 0, (hipStream_t)stream, a);
