@@ -31,7 +31,9 @@ static_assert(16 * kORow * 4 <= 2 * kWaveLds, "a wave's outputs take two tiles' 
 constexpr int kWgs = 256;              // one workgroup per CU
 constexpr int kPiece = 8;              // tiles of a cut item's piece, at least: one a wave
 constexpr int kMinStretch = 2 * kPiece;
-constexpr int kItemCost = 16;
+// A piece takes what 32 more tiles would, 20,000 cycles (MI355X, 128 x 256..8,192 tokens, both launches: 67.5 us
+// with 16, 64.7 with 24, 64.0 with 32, 63.5 with 40; 39 x 1,043..8,347 32.4 / 30.7 / 30.3 / 30.6)
+constexpr int kItemCost = 32;
 constexpr int kPartFloats = 16 * kLat;
 
 struct PagedAttnArgs {
@@ -507,10 +509,7 @@ __global__ __launch_bounds__(512) void mla_paged_merge_kernel(const PagedAttnArg
   }
 }
 
-static int column_groups(int max_q, int heads) { return (max_q * heads + 15) / 16; }
-
-extern "C" int64_t dsv2_mla_paged_workspace_size(int requests, int max_q, int heads) {
-  if (requests < 0 || max_q < 0 || heads < 0) return 0;
+extern "C" int64_t dsv2_mla_paged_workspace_size(void) {
   return kWgs * (2 * (kPartFloats + 32) * 4 + 32);
 }
 
@@ -532,14 +531,14 @@ extern "C" int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_
                DSV2_E_ALIGN, "mla_decode_paged_fp4: alignment");
   if (tokens == 0 || requests == 0) return DSV2_OK;
   if (!cu_q) max_q = 1;
-  const int groups = column_groups(max_q, heads), shift = page_shift(page_size);
+  const int groups = (max_q * heads + 15) / 16, shift = page_shift(page_size);
   const int64_t items = static_cast<int64_t>(requests) * groups;
   const int64_t room = static_cast<int64_t>(table_width) << shift;
-  DSV2_REQUIRE(room <= INT32_MAX - kTile && items <= INT32_MAX / ((room + kTile - 1) / kTile + kItemCost), DSV2_E_SHAPE,
+  DSV2_REQUIRE(room <= INT32_MAX - kTile && items <= INT32_MAX / 2 / ((room + kTile - 1) / kTile + kItemCost), DSV2_E_SHAPE,
                "mla_decode_paged_fp4: %d requests of up to %lld tokens, %d column groups each", requests, (long long)room,
                groups);
   DSV2_REQUIRE(workspace && dsv2_aligned16(workspace) &&
-                   workspace_bytes >= dsv2_mla_paged_workspace_size(requests, max_q, heads),
+                   workspace_bytes >= dsv2_mla_paged_workspace_size(),
                DSV2_E_SHAPE, "mla_decode_paged_fp4: workspace of %lld bytes", (long long)workspace_bytes);
   float* part_o = (float*)workspace;
   float* part_ml = part_o + 2 * kWgs * kPartFloats;

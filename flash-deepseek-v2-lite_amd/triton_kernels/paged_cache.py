@@ -33,7 +33,7 @@ _BF16, _I32, _U8 = torch.bfloat16, torch.int32, torch.uint8
 _PAGE_SIZES = frozenset(1 << i for i in range(11))
 _ENTRY = {n: getattr(_hip.lib, n) for n in ("dsv2_paged_step", "dsv2_paged_slots", "dsv2_paged_write_fp4",
                                             "dsv2_paged_read_fp4", "dsv2_mla_decode_paged_fp4")}
-_WORKSPACE = {}  # (requests, max_q, heads) -> bytes
+_WORKSPACE = _hip.lib.dsv2_mla_paged_workspace_size()  # bytes
 _STATUS: dict = {}  # device index -> (int32 [1] status word of the functions below, its address)
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
@@ -280,11 +280,8 @@ def attention_decode_paged_fp4(q: torch.Tensor, pages: torch.Tensor, block_table
             raise NotImplementedError(f"{name}: out's rows must be contiguous and apart")
     if t == 0 or n == 0:
         return out
-    size = _WORKSPACE.get((n, max_q, h))
-    if size is None:
-        size = _WORKSPACE[n, max_q, h] = _hip.lib.dsv2_mla_paged_workspace_size(n, max_q, h)
-    ws = pages.new_empty(size)
+    ws = pages.new_empty(_WORKSPACE)
     _call(index, "dsv2_mla_decode_paged_fp4", q.data_ptr(), q_ts, q_hs, t, h, pages.data_ptr(), page_stride, n_pages,
           page_size, block_table.data_ptr(), ts, width, lens.data_ptr(), n, cu, max_q, softmax_scale, out.data_ptr(),
-          o_ts, o_hs, ws.data_ptr(), size)
+          o_ts, o_hs, ws.data_ptr(), _WORKSPACE)
     return out

@@ -544,7 +544,7 @@ int dsv2_paged_read_fp4(const void* pages, int64_t page_stride, int n_pages, int
  * Table entries that name no page stand for tokens of zeros (and set DSV2_DEVERR_BAD_SLOT); a request with
  * more than max_q query tokens has the first max_q done (and sets DSV2_DEVERR_TOKENS).
  * workspace: dsv2_mla_paged_workspace_size bytes, 16-byte aligned, not shared by calls that may overlap. */
-int64_t dsv2_mla_paged_workspace_size(int requests, int max_q, int heads);
+int64_t dsv2_mla_paged_workspace_size(void);
 int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_hs, int tokens, int heads, const void* pages,
                               int64_t page_stride, int n_pages, int page_size, const int32_t* block_table,
                               int64_t table_stride, int table_width, const int32_t* lens, int requests,

@@ -120,7 +120,7 @@ def test_entry_points_refuse_bad_arguments_without_launching():
     read = [one, 6400, 6, 16, one, 5, one, 576]
     for at, value, match in [(4, None, "null"), (5, -1, "bad shape"), (6, odd, "alignment"), (7, 575, "bad shape")]:
         refused(match, "dsv2_paged_read_fp4", *read[:at], value, *read[at + 1:])
-    size = _hip.lib.dsv2_mla_paged_workspace_size(4, 2, 16)
+    size = _hip.lib.dsv2_mla_paged_workspace_size()
     attn = [one, 9216, 576, 7, 16, one, 6400, 6, 16, one, 3, 3, one, 4, one, 2, 0.1, one, 8192, 512, one, size]
     for at, value, match in [(0, None, "null"), (0, odd, "alignment"), (1, 9220, "alignment"), (3, -1, "bad shape"),
                              (4, 0, "bad shape"), (4, 129, "bad shape"), (8, 40, "power of two"), (10, 2, "block table"),
