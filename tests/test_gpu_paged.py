@@ -575,3 +575,75 @@ def test_empty_calls():
                                         SCALE).shape == (0, 16, 512)
     out = P.paged_cache_step(i32([5, 0, 2]), i32([0]), i32([[0, 1]]), i32([0, 1]), 16, 0)
     assert out[0].tolist() == [5, 0, 2] and out[1].shape == (0,)
+
+
+# --------------------------------------------------------------------------- dsv2lite.PagedLatentCache
+def test_paged_latent_cache_beside_the_compressed_one():
+    """Prompts and decode steps of two layers through PagedLatentCache, the new rows and absorbed queries by
+    dsv2_mla_prepare_qlat into a staging buffer, against 64 bits on the rows that the pages hold and against
+    dsv2_mla_decode_rows over a bf16 cache of the same rows."""
+    from dsv2lite import DSV2Config, PagedLatentCache
+    from dsv2lite.rope import cos_sin_tables
+
+    cfg, B, layers = DSV2Config(), 4, 2
+    cache = PagedLatentCache(layers, B, max_len=300, n_pages=24, page_size=32)
+    cos, sin = cos_sin_tables(cfg, 512, device=DEV)
+    kvw, w_ukt = (rnd(512, seed=1, std=0.1) + 1).to(BF), rnd(16, 512, 128, std=0.05, seed=2)
+    ptr = lambda t: t.data_ptr()  # noqa: E731
+
+    def prepare(qkva, positions):
+        """Cache rows [n, 576] and queries [n, 16, 576]: every row of the staging buffer a sequence of its own."""
+        n = qkva.shape[0]
+        rows, q = torch.zeros(n, 576, dtype=BF, device=DEV), torch.zeros(n, 16, 576, dtype=BF, device=DEV)
+        base = torch.arange(n, device=DEV) - positions
+        _hip.call("dsv2_mla_prepare_qlat", ptr(qkva), 3648, n, ptr(positions), ptr(base), ptr(positions + 1), ptr(kvw),
+                  1e-6, ptr(cos), ptr(sin), 512, ptr(w_ukt), ptr(rows), ptr(q), None, _hip.stream_ptr())
+        return rows, q
+
+    for step, delta in enumerate([[70, 5, 0, 130], [1, 1, 0, 1], [1, 1, 33, 1], [1, -6, 1, 1], [1, 0, 1, 1]]):
+        n = sum(d for d in delta if d > 0)
+        slots, positions, rows_of = cache.step(i32(delta), n)
+        lens = cache.lens.tolist()
+        for layer in range(layers):
+            new, q = prepare(rnd(n, 3648, seed=10 * step + layer), positions)
+            cache.write(layer, new, slots)
+            assert torch.equal(cache.read(layer, slots).double(), R.held(new))
+            # the last new token of each request that grew asks; the others ask with the first token's query
+            last = [max([i for i, b in enumerate(rows_of.tolist()) if b == r], default=0) for r in range(B)]
+            qb = q[last]
+            got = cache.attend(layer, qb, cfg.softmax_scale)
+            every, _, _ = cache.slots_of(torch.zeros_like(cache.lens), cache.lens, sum(lens))
+            held = cache.read(layer, every)
+            keys = held.double().split(lens)
+            base = i32([sum(lens[:b]) for b in range(B)]).long()
+            plain = torch.zeros(B, 8192, dtype=BF, device=DEV)
+            _hip.call("dsv2_mla_decode_rows", ptr(qb), ptr(held), ptr(base), ptr(cache.lens - 1), ptr(cache.lens), B,
+                      cfg.softmax_scale, ptr(plain), 8192, _hip.stream_ptr())
+            for b in range(B):
+                want, tol = R.attention(qb[b], keys[b], lens[b], cfg.softmax_scale)
+                assert ((got[b].double() - want).abs() <= tol).all(), (step, layer, b)
+                if lens[b]:
+                    assert ((got[b].double() - plain[b].view(16, 512).double()).abs() <= 2 * tol).all(), (step, layer, b)
+    assert cache.lens.tolist() == [74, 1, 35, 134] and cache.free_tokens() == (24 - 3 - 1 - 2 - 5) * 32
+    cache.check_status()
+
+
+def test_paged_latent_cache_snapshot_and_overflow():
+    from dsv2lite import PagedLatentCache
+
+    cache = PagedLatentCache(1, 3, max_len=64, n_pages=5, page_size=16)
+    slots, _, _ = cache.step(i32([20, 30, 1]), 51)
+    rows = rnd(51, R.ROW)
+    cache.write(0, rows, slots)
+    snap = cache.snapshot()
+    first = cache.step(i32([-20, 2, 15]), 17)
+    assert cache.lens.tolist() == [0, 32, 16] and cache.free_tokens() == 2 * 16
+    cache.restore(snap)
+    again = cache.step(i32([-20, 2, 15]), 17)
+    assert all(torch.equal(x, y) for x, y in zip(first, again))
+    assert torch.equal(cache.read(0, slots[20:50]).double(), R.held(rows[20:50]))
+    cache.check_status()
+    cache.step(i32([33, 0, 49]), 82)  # a page too many; past max_len
+    assert cache.lens.tolist() == [0, 32, 16]
+    with pytest.raises(RuntimeError, match="outgrew its block table; no free page"):
+        cache.check_status()

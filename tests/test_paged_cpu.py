@@ -151,3 +151,22 @@ def test_the_plain_allocator_hands_out_and_takes_back():
     # request 0 takes page 7 (ring position 2); request 1's page goes behind it, to position 0
     assert out == [[14, -1, -1], [2, -1, -1], [0, -1, -1]] and errors == 0
     assert b.ring == [6, 4, 7] and (b.head, b.count) == (0, 1) and b.lens == [3, 0]
+
+
+def test_paged_latent_cache_shapes_and_refusals():
+    from dsv2lite import PagedLatentCache
+
+    c = PagedLatentCache(3, 5, max_len=100, n_pages=7, page_size=32, device="cpu")
+    assert c.pages.shape == (3, 7, 32 * 400) and c.block_table.shape == (5, 4)
+    assert c.state.tolist() == [0, 0, 0, 0, 0, 0, 7] and c.lens.data_ptr() == c.state.data_ptr()
+    snap = c.snapshot()
+    c.state.fill_(9)
+    c.restore(snap)
+    assert c.state.tolist() == [0, 0, 0, 0, 0, 0, 7] and c.free_tokens() == 224
+    with pytest.raises(NotImplementedError, match="requires CUDA"):
+        c.step(i32(5), 5)
+    for kw, text in [(dict(page_size=48), "power of two"), (dict(page_size=2048), "power of two"),
+                     (dict(requests=4097), "at most 4096"), (dict(n_pages=0), "positive"), (dict(max_len=0), "positive"),
+                     (dict(n_pages=2 ** 26), "int32")]:
+        with pytest.raises(ValueError, match=text):
+            PagedLatentCache(**{**dict(n_layers=1, requests=2, max_len=10, n_pages=3, page_size=32, device="cpu"), **kw})
