@@ -40,6 +40,7 @@ struct PagedAttnArgs {
   const bf16_t* q;
   int64_t q_ts, q_hs;
   int tokens, heads;
+  uint32_t heads_inv;  // ceil(2^32 / heads), 0 for one head
   const uint8_t* pages;
   int64_t page_stride;
   int n_pages, shift;
@@ -60,6 +61,17 @@ struct PagedAttnArgs {
                      // request's columns, the workgroups that it begins and ends in) and its request
   int32_t* status;
 };
+
+// column / heads: exact for columns below 2^25 and up to 128 heads (the product is less than column / 2^32 * 128 above
+// the quotient times 2^32); a division by a run-time value takes some 40 instructions
+__device__ __forceinline__ int token_of(const PagedAttnArgs& a, int column) {
+  return a.heads_inv ? static_cast<int>(__umulhi(static_cast<uint32_t>(column), a.heads_inv)) : column;
+}
+// the output row of a column of the request whose first query token is q0
+__device__ __forceinline__ bf16_t* out_row(const PagedAttnArgs& a, int q0, int column) {
+  const int j = token_of(a, column);
+  return a.out + (q0 + j) * a.o_ts + (column - j * a.heads) * a.o_hs;
+}
 
 // a value that all lanes have, to scalar registers: what follows from it stays off the vector units
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -143,9 +155,7 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
         const Request z = request(a, i);
         if (z.len > 0) continue;
         for (int f = tid; f < z.columns * (kLat / 8); f += kThreads) {
-          const int cc = f / (kLat / 8);
-          *reinterpret_cast<uint4*>(a.out + (z.q0 + cc / a.heads) * a.o_ts + (cc % a.heads) * a.o_hs +
-                                    f % (kLat / 8) * 8) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(out_row(a, z.q0, f / (kLat / 8)) + f % (kLat / 8) * 8) = make_uint4(0, 0, 0, 0);
         }
       }
     }
@@ -204,19 +214,19 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
 
     // Q^T fragments (B operand), once for all waves; the k order of a block group's four products is the
     // lanes' own: k-slot (kg, e) of product (c, x) is latent (4c + kg) * 32 + x * 8 + e
+    const int cc = ct * 16 + li, token = token_of(a, cc);
+    const int seen = cc < r.columns ? max(r.len - r.nq + token + 1, 0) : 0;
 #pragma unroll
     for (int n = 0; n < (18 * 64 + kThreads - 1) / kThreads; ++n) {
       const int f = tid + n * kThreads;
       if (f < 18 * 64) {
-        const int i = f >> 6, cc = ct * 16 + li;
+        const int i = f >> 6;
         const int dim = i < 16 ? ((i >> 2) * 4 + kg) * 32 + (i & 3) * 8 : kLat + (i - 16) * 32 + kg * 8;
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (cc < r.columns) v = ldg16(a.q + (r.q0 + cc / a.heads) * a.q_ts + (cc % a.heads) * a.q_hs + dim);
+        if (cc < r.columns) v = ldg16(a.q + (r.q0 + token) * a.q_ts + (cc - token * a.heads) * a.q_hs + dim);
         q_lds[f] = v;
       }
     }
-    const int col = ct * 16 + li;
-    const int seen = col < r.columns ? max(r.len - r.nq + col / a.heads + 1, 0) : 0;
 
     const int32_t* row = a.table + b * a.ts;
     const int end = t_last - 1;
@@ -396,10 +406,8 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
       for (int u = 1; u < kWaves; ++u) mm = fmaxf(mm, ml[u][c][0]);
 #pragma unroll
       for (int u = 0; u < kWaves; ++u) l += ml[u][c][1] * __builtin_amdgcn_exp2f(ml[u][c][0] - mm);
-      const int jj = cc / a.heads, hh = cc - jj * a.heads;
-      const float inv = r.len - r.nq + jj + 1 > 0 ? 1.0f / l : 0.f;
-      *reinterpret_cast<uint2*>(a.out + (r.q0 + jj) * a.o_ts + hh * a.o_hs + d) =
-          make_uint2(pack2(v.x * inv, v.y * inv), pack2(v.z * inv, v.w * inv));
+      const float inv = r.len - r.nq + token_of(a, cc) + 1 > 0 ? 1.0f / l : 0.f;
+      *reinterpret_cast<uint2*>(out_row(a, r.q0, cc) + d) = make_uint2(pack2(v.x * inv, v.y * inv), pack2(v.z * inv, v.w * inv));
     }
     if (!whole && tid < 16) {
       float mm = ml[0][tid][0], l = 0.f;
@@ -445,12 +453,21 @@ __global__ __launch_bounds__(512) void mla_paged_merge_kernel(const PagedAttnArg
   const int width = min(f1 - f0, 512), groups = 512 / width, g = tid / width;
   const int in_pass = (parts + groups - 1) / groups, loads = (f1 - f0 + width - 1) / width * in_pass;
   float4 x[kLoads];
+  int f = f0 + tid - g * width, p = g, pass = 0;  // of the next load
+  auto advance = [&] {
+    p += groups;
+    if (++pass < in_pass) return false;
+    pass = 0;
+    p = g;
+    f += width;
+    return true;
+  };
 #pragma unroll
   for (int k = 0; k < kLoads; ++k) {
-    const int f = f0 + tid - g * width + k / in_pass * width, p = g + k % in_pass * groups;
     x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (k < loads && g < groups && f < f1 && p < parts)
       x[k] = *reinterpret_cast<const float4*>(a.part_o + static_cast<int64_t>(slot(p)) * kPartFloats + f * 4);
+    advance();
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -468,43 +485,57 @@ __global__ __launch_bounds__(512) void mla_paged_merge_kernel(const PagedAttnArg
     }
     l = wave_sum(l);
     const int cc = col0 + c;
-    const float inv = cc < columns && req.x - req.y + cc / a.heads + 1 > 0 ? 1.0f / l : 0.f;
+    const float inv = cc < columns && req.x - req.y + token_of(a, cc) + 1 > 0 ? 1.0f / l : 0.f;
 #pragma unroll
     for (int k = 0; k < kLaneParts; ++k)
       if (lane + 64 * k < parts) weight[c - c0][lane + 64 * k] = w[k] * inv;
   }
   __syncthreads();
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  f = f0 + tid - g * width;
+  p = g;
+  pass = 0;
 #pragma unroll
   for (int k = 0; k < kLoads; ++k) {
     if (k >= loads) break;
-    const int f = f0 + tid - g * width + k / in_pass * width, p = g + k % in_pass * groups;
-    const bool mine = g < groups && f < f1 && p < parts;
-    const int c = f >> 7;
-    if (mine) {
+    const int at = f, c = at >> 7;
+    if (g < groups && at < f1 && p < parts) {
       const float w = weight[c - c0][p];
       v.x = __builtin_fmaf(w, x[k].x, v.x);
       v.y = __builtin_fmaf(w, x[k].y, v.y);
       v.z = __builtin_fmaf(w, x[k].z, v.z);
       v.w = __builtin_fmaf(w, x[k].w, v.w);
     }
-    if (k % in_pass != in_pass - 1) continue;
-    if (groups > 1) {  // one pass
+    if (!advance()) continue;
+    if (groups > 1) {  // one pass: the groups' sums by eights, then those
+      auto add = [&](int from, int by) {
+        for (int i = from; i < groups; i += by) {
+          const float4 u = sums[i * width + tid - g * width];
+          v.x += u.x;
+          v.y += u.y;
+          v.z += u.z;
+          v.w += u.w;
+        }
+      };
       sums[tid] = v;
       __syncthreads();
-      if (g > 0) return;
-      for (int i = 1; i < groups; ++i) {
-        const float4 u = sums[i * width + tid];
-        v.x += u.x;
-        v.y += u.y;
-        v.z += u.z;
-        v.w += u.w;
+      if (g < 8) add(g + 8, 8);
+      __syncthreads();
+      if (g < 8) sums[tid] = v;
+      __syncthreads();
+      if (g == 0) {
+        for (int i = 1; i < min(groups, 8); ++i) {
+          const float4 u = sums[i * width + tid];
+          v.x += u.x;
+          v.y += u.y;
+          v.z += u.z;
+          v.w += u.w;
+        }
       }
     }
     const int cc = col0 + c;
-    if (g == 0 && f < f1 && cc < columns)
-      *reinterpret_cast<uint2*>(a.out + (req.z + cc / a.heads) * a.o_ts + (cc % a.heads) * a.o_hs + (f & 127) * 4) =
-          make_uint2(pack2(v.x, v.y), pack2(v.z, v.w));
+    if (g == 0 && at < f1 && cc < columns)
+      *reinterpret_cast<uint2*>(out_row(a, req.z, cc) + (at & 127) * 4) = make_uint2(pack2(v.x, v.y), pack2(v.z, v.w));
     v = make_float4(0.f, 0.f, 0.f, 0.f);
   }
 }
@@ -543,7 +574,8 @@ extern "C" int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_
   float* part_o = (float*)workspace;
   float* part_ml = part_o + 2 * kWgs * kPartFloats;
   int4* cuts = (int4*)(part_ml + 2 * kWgs * 32);
-  const PagedAttnArgs a{(const bf16_t*)q, q_ts, q_hs, tokens, heads, (const uint8_t*)pages, page_stride, n_pages,
+  const PagedAttnArgs a{(const bf16_t*)q, q_ts, q_hs, tokens, heads,
+                        heads == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + heads - 1) / heads), (const uint8_t*)pages, page_stride, n_pages,
                         shift, block_table, table_stride, table_width, lens, cu_q, max_q, requests, groups,
                         softmax_scale * 1.4426950408889634f, (bf16_t*)out, out_ts, out_hs, part_o, part_ml, cuts,
                         status};
