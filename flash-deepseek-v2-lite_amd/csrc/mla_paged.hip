@@ -334,12 +334,13 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
       pg = load_page(tile + kWaves);
       __syncthreads();  // Q
 #pragma unroll 1
-      for (; tile < t_last; tile += kWaves) {
+      for (; tile + kWaves < t_last; tile += kWaves) {
         load_tile(tile + kWaves, pg, w1);
         pg = load_page(tile + 2 * kWaves);
         tile_step(tile, w0);
         w0 = w1;
       }
+      if (tile < t_last) tile_step(tile, w0);
     }
     l_run = xor32_sum(xor16_sum(l_run));
 
