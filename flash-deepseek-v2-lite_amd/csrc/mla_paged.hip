@@ -558,6 +558,9 @@ extern "C" int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_
                DSV2_E_SHAPE, "mla_decode_paged_fp4: bad shape (%d query tokens, %d heads, %d requests, max_q %d)", tokens,
                heads, requests, max_q);
   DSV2_REQUIRE(table_width > 0 && table_stride >= table_width, DSV2_E_SHAPE, "mla_decode_paged_fp4: block table");
+  // the largest product is the largest score only then; zero or an infinity would make masked scores NaN
+  DSV2_REQUIRE(softmax_scale > 0.f && softmax_scale <= 1e30f, DSV2_E_SHAPE,
+               "mla_decode_paged_fp4: softmax_scale %g is not in (0, 1e30]", softmax_scale);
   DSV2_REQUIRE(dsv2_aligned16(q) && dsv2_aligned16(out) && q_ts % 8 == 0 && q_hs % 8 == 0 && out_ts % 8 == 0 &&
                    out_hs % 8 == 0,
                DSV2_E_ALIGN, "mla_decode_paged_fp4: alignment");

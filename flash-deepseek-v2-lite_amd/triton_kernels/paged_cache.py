@@ -263,6 +263,8 @@ def attention_decode_paged_fp4(q: torch.Tensor, pages: torch.Tensor, block_table
         if max_q < 1:
             raise ValueError(f"{name}: max_q must be positive")
         max_q, cu = min(max_q, max(t, 1)), cu_q.data_ptr()
+    if not 0.0 < softmax_scale <= 1e30:
+        raise ValueError(f"{name}: softmax_scale must be positive and finite, not {softmax_scale}")
     q_ts, q_hs, q_ds = q.stride()
     if q_ds != 1:
         raise NotImplementedError(f"{name} needs a contiguous last dimension")

@@ -538,7 +538,7 @@ int dsv2_paged_read_fp4(const void* pages, int64_t page_stride, int n_pages, int
 
 /* Absorbed-MLA attention of the queries q [tokens, heads, 576] (strides q_ts, q_hs; absorbed latent |
  * rotated rotary part) over the requests' cached tokens: out[t, h, :512] = sum_s p_s latent_s, p = softmax
- * of softmax_scale * q[t, h] . row_s.  Request b owns the query tokens [cu_q[b], cu_q[b + 1]), at most
+ * of softmax_scale * q[t, h] . row_s, softmax_scale in (0, 1e30].  Request b owns the query tokens [cu_q[b], cu_q[b + 1]), at most
  * max_q of them (cu_q NULL: token b); they are its last cached ones: query j of n sees the tokens below
  * lens[b] - n + j + 1.  A query that sees nothing gives zeros; query tokens of no request are left alone.
  * Table entries that name no page stand for tokens of zeros (and set DSV2_DEVERR_BAD_SLOT); a request with

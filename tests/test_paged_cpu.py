@@ -73,6 +73,10 @@ REFUSED = [
      "contiguous last"),
     ("attention_decode_paged_fp4", 1, PAGES(6, 48 * 400), ValueError, "power of two"),
     ("attention_decode_paged_fp4", 2, i32(5, 3), ValueError, "block_table must be"),
+    ("attention_decode_paged_fp4", 4, 0.0, ValueError, "softmax_scale must be positive"),
+    ("attention_decode_paged_fp4", 4, -0.1, ValueError, "softmax_scale must be positive"),
+    ("attention_decode_paged_fp4", 4, float("inf"), ValueError, "softmax_scale must be positive"),
+    ("attention_decode_paged_fp4", 4, float("nan"), ValueError, "softmax_scale must be positive"),
     ("attention_decode_paged_fp4", 5, None, ValueError, "one query token a request"),
     ("attention_decode_paged_fp4", 5, i32(4), ValueError, "cu_q must be"),
     ("attention_decode_paged_fp4", 6, 0, ValueError, "max_q"),
@@ -125,7 +129,9 @@ def test_entry_points_refuse_bad_arguments_without_launching():
     for at, value, match in [(0, None, "null"), (0, odd, "alignment"), (1, 9220, "alignment"), (3, -1, "bad shape"),
                              (4, 0, "bad shape"), (4, 129, "bad shape"), (8, 40, "power of two"), (10, 2, "block table"),
                              (11, 2 ** 28, "block table"), (12, None, "null"), (13, -1, "bad shape"), (13, 65536, "bad shape"),
-                             (14, None, "bad shape"), (15, 0, "bad shape"), (18, 8196, "alignment"),
+                             (14, None, "bad shape"), (15, 0, "bad shape"),
+                             (16, 0.0, "softmax_scale"), (16, -1.0, "softmax_scale"), (16, float("inf"), "softmax_scale"),
+                             (16, float("nan"), "softmax_scale"), (18, 8196, "alignment"),
                              (20, None, "workspace"), (20, odd, "workspace"), (21, size - 1, "workspace")]:
         refused(match, "dsv2_mla_decode_paged_fp4", *attn[:at], value, *attn[at + 1:])
 
