@@ -329,6 +329,22 @@ def test_attention_long_and_many(lens):
     check(rnd(len(lens), 16, R.ROW, seed=6, std=0.3), pages, table, lens, keys)
 
 
+@pytest.mark.parametrize("live", [[0, 1, 4095], [63, 64, 65, 1000, 2047], [4095], list(range(5, 4096, 130))])
+def test_attention_of_few_live_rows_among_many_idle_ones(live):
+    lens = [0] * 4096
+    for i, b in enumerate(live):
+        lens[b] = 1 + 37 * i
+    pages, table, keys = batch([lens[b] for b in live], 16, seed=len(live))
+    wide = torch.full((4096, table.shape[1]), -1, dtype=torch.int32, device=DEV)
+    wide[live] = table
+    q = rnd(4096, 16, R.ROW, seed=3, std=0.3)
+    got = P.attention_decode_paged_fp4(q, pages, wide, i32(lens), SCALE)
+    assert int((got[[b for b in range(4096) if not lens[b]]] != 0).sum()) == 0
+    for i, b in enumerate(live):
+        want, tol = R.attention(q[b], keys[i], lens[b], SCALE)
+        assert ((got[b].double() - want).abs() <= tol).all(), b
+
+
 @pytest.mark.parametrize("std", [0.0, 3.0, 30.0])
 def test_attention_flat_and_sharp(std):
     """Equal scores, and scores whose softmax has one token left; a scale of its own."""
