@@ -47,13 +47,18 @@ def _status(index: int) -> tuple[torch.Tensor, int]:
 
 
 def check_paged_status(device: torch.device | str = "cuda") -> None:
-    """Raise if a call on `device` since the last check skipped something (synchronises)."""
+    """Raise if a call on `device` since the last check skipped something (waits for all its streams)."""
     index = torch.device(device).index
-    known = _STATUS.get(torch.cuda.current_device() if index is None else index)
-    bits = 0 if known is None else int(known[0].item())
+    index = torch.cuda.current_device() if index is None else index
+    known = _STATUS.get(index)
+    if known is None:
+        return
+    torch.cuda.synchronize(index)  # calls on any stream
+    bits = int(known[0].item())
     if not bits:
         return
     known[0].zero_()
+    torch.cuda.synchronize(index)  # before a later call on another stream sets one
     what = [text for bit, text in ((1, "a request outgrew its block table"), (2, "no free page was left"),
                                    (4, "a slot, page or position lay outside the pool or block table"),
                                    (8, "there were more new tokens than max_tokens or max_q")) if bits & bit]

@@ -496,6 +496,23 @@ def test_attention_is_the_same_every_time_and_on_every_stream():
         assert torch.equal(a, first) and torch.equal(b, second)
 
 
+def test_check_sees_calls_on_every_stream():
+    """The check waits for work that is still queued on a stream other than the current one."""
+    pages = pool(4, 16, fill=1)
+    rows, slots = rnd(3, R.ROW), i32([64, 0, 1])
+    busy = torch.zeros(1 << 28, device=DEV)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            busy.add_(1)
+        P.paged_cache_write_fp4(rows, slots, pages)
+    with pytest.raises(RuntimeError, match="outside the pool"):
+        P.check_paged_status()
+    torch.cuda.synchronize()
+    P.check_paged_status()
+
+
 # --------------------------------------------------------------------------- together
 def test_serving_loop_eager_and_captured():
     """Requests join, grow, are rolled back and end while one captured step (lengths, write, attention)
