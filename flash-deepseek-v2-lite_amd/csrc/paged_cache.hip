@@ -405,7 +405,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(const uint8_t* __restri
 extern "C" int dsv2_paged_write_fp4(const void* rows, int64_t row_stride, int n, const int32_t* slots, void* pages,
                                     int64_t page_stride, int n_pages, int page_size, int32_t* status, void* stream) {
   if (const int rc = paged_check_pool("paged_write_fp4", pages, page_stride, n_pages, page_size)) return rc;
-  DSV2_REQUIRE(n >= 0 && row_stride >= kRow, DSV2_E_SHAPE, "paged_write_fp4: bad shape");
+  DSV2_REQUIRE(n >= 0 && (row_stride >= kRow || row_stride == 0), DSV2_E_SHAPE, "paged_write_fp4: bad shape");
   if (n == 0) return DSV2_OK;
   DSV2_REQUIRE(rows && slots, DSV2_E_NULL, "paged_write_fp4: null pointer");
   DSV2_REQUIRE(dsv2_aligned16(rows) && row_stride % 8 == 0, DSV2_E_ALIGN, "paged_write_fp4: rows alignment");

@@ -193,21 +193,21 @@ def paged_slot_map(starts: torch.Tensor, counts: torch.Tensor, block_table: torc
 
 
 def _cache_rows(name: str, what: str, rows: torch.Tensor, n: int) -> int:
-    """Row stride of [n, 576] bf16 cache rows."""
+    """Row stride of [n, 576] bf16 cache rows; 0 for one row that is read for all."""
     if rows.dtype is not _BF16:
         raise NotImplementedError(f"{name}: {what} must be bf16")
     if rows.shape != (n, ROW):
         raise ValueError(f"{name}: {what} must be [{n}, {ROW}], not {list(rows.shape)}")
     rs, cs = rows.stride()
-    if cs != 1 or rs < ROW and n > 1:
+    if cs != 1 or rs < ROW and n > 1 and (rs or what == "out"):
         raise NotImplementedError(f"{name}: {what} must have contiguous rows")
     return rs if n > 1 else ROW
 
 
 def paged_cache_write_fp4(rows: torch.Tensor, slots: torch.Tensor, pages: torch.Tensor) -> None:
-    """Round cache rows (bf16 [n, 576]: normalised latent | rotated key, any row stride that is a
-    multiple of 8) into ``slots`` (int32 [n]) of ``pages``; a row with a negative slot is left out.
-    Of two rows with the same slot either may stay."""
+    """Round cache rows (bf16 [n, 576]: normalised latent | rotated key, a row stride that is a
+    multiple of 8, or 0 for one row) into ``slots`` (int32 [n]) of ``pages``; a row with a negative slot is left out.
+    Rows with the same slot have to be the same: of different ones a mixture may stay."""
     name = "paged_cache_write_fp4"
     index = _device(name, rows, slots, pages)
     n = _int32(name, "slots", slots)

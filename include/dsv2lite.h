@@ -526,9 +526,10 @@ int dsv2_paged_slots(const int32_t* starts, const int32_t* counts, int requests,
                      int64_t table_stride, int table_width, int page_size, int max_tokens, int32_t* slots,
                      int32_t* positions, int32_t* rows, int32_t* status, void* stream);
 
-/* Rounds row i (576 bf16: latent | rotary key, as dsv2_mla_prepare writes it) into slots[i] of the pool.
- * A negative slot is skipped, one past the pool sets DSV2_DEVERR_BAD_SLOT; of two rows with one slot
- * either may stay. */
+/* Rounds row i (576 bf16: latent | rotary key, as dsv2_mla_prepare writes it) into slots[i] of the pool
+ * (row_stride 0: the same row into all).
+ * A negative slot is skipped, one past the pool sets DSV2_DEVERR_BAD_SLOT.  Rows with one slot have to be
+ * the same: of different ones a mixture may stay. */
 int dsv2_paged_write_fp4(const void* rows, int64_t row_stride, int n, const int32_t* slots, void* pages,
                          int64_t page_stride, int n_pages, int page_size, int32_t* status, void* stream);
 

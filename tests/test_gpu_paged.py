@@ -144,6 +144,17 @@ def test_write_and_read_by_slots(ps, n):
     assert int((back[~live] != 0).sum()) == 0 and int((out[:, R.ROW:] != 5.0).sum()) == 0
 
 
+def test_the_same_row_written_to_one_slot_many_times():
+    """A padded batch repeats its last row and slot."""
+    rows, slots = rnd(1, R.ROW).expand(300, R.ROW), i32([37] * 300)
+    pages = pool(4, 16, fill=9)
+    P.paged_cache_write_fp4(rows, slots, pages)
+    same(P.paged_cache_read_fp4(pages, slots), R.held(rows))
+    want = torch.full_like(pages, 9)
+    P.paged_cache_write_fp4(rows[:1], slots[:1], want)
+    assert torch.equal(pages, want)
+
+
 def test_slots_outside_the_pool_are_skipped_and_reported():
     pages = pool(4, 16, fill=1)
     before = pages.clone()
