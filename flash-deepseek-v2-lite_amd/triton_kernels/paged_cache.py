@@ -26,6 +26,7 @@ ROW = LAT + ROPE
 TOKEN_BYTES = LAT // 2 + 2 * ROPE + LAT // 32  # 400
 MAX_REQUESTS = 4096
 MAX_HEADS = 128
+MAX_TOKENS = 2 ** 31 - 1
 
 # These calls launch kernels of 2 to 10 us, so their own host time is looked at: a launch takes 3 us of it, a
 # torch.empty 1.3, an attribute of a tensor 0.05 to 0.1.
@@ -156,7 +157,7 @@ def paged_cache_step(state: torch.Tensor, delta: torch.Tensor, block_table: torc
     pages = _int32(name, "free_pages", free_pages)
     _page_size(name, page_size)
     ts, width = _table(name, block_table, n)
-    if n > MAX_REQUESTS or pages == 0 or max_tokens < 0:
+    if n > MAX_REQUESTS or pages == 0 or not 0 <= max_tokens <= MAX_TOKENS:
         raise ValueError(f"{name}: {n} requests (at most {MAX_REQUESTS}), {pages} pages, max_tokens {max_tokens}")
     outs = state.new_empty(n + 2 + 3 * max_tokens)  # one allocation: the state, then the three maps
     if n == 0:
@@ -180,7 +181,7 @@ def paged_slot_map(starts: torch.Tensor, counts: torch.Tensor, block_table: torc
     _int32(name, "counts", counts, n)
     _page_size(name, page_size)
     ts, width = _table(name, block_table, n)
-    if n > MAX_REQUESTS or max_tokens < 0:
+    if n > MAX_REQUESTS or not 0 <= max_tokens <= MAX_TOKENS:
         raise ValueError(f"{name}: {n} requests (at most {MAX_REQUESTS}), max_tokens {max_tokens}")
     maps = starts.new_empty(3 * max_tokens)
     if n == 0 or max_tokens == 0:
@@ -273,6 +274,10 @@ def attention_decode_paged_fp4(q: torch.Tensor, pages: torch.Tensor, block_table
     q_ts, q_hs, q_ds = q.stride()
     if q_ds != 1:
         raise NotImplementedError(f"{name} needs a contiguous last dimension")
+    if t == 1:  # strides that are never taken may be anything
+        q_ts = 0
+    if h == 1:
+        q_hs = 0
     if out is None:
         out = q.new_empty((t, h, LAT))
         o_ts, o_hs = h * LAT, LAT
@@ -285,6 +290,10 @@ def attention_decode_paged_fp4(q: torch.Tensor, pages: torch.Tensor, block_table
         o_ts, o_hs, o_ds = out.stride()
         if o_ds != 1 or h > 1 and o_hs < LAT or t > 1 and o_ts < LAT:
             raise NotImplementedError(f"{name}: out's rows must be contiguous and apart")
+        if t == 1:
+            o_ts = 0
+        if h == 1:
+            o_hs = 0
     if t == 0 or n == 0:
         return out
     ws = pages.new_empty(_WORKSPACE)

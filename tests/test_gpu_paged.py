@@ -394,6 +394,20 @@ def test_attention_strides():
     assert int((out[:, :2] != 7).sum()) + int((out[:, 18:] != 7).sum()) + int((out[:, :, 512:] != 7).sum()) == 0
 
 
+@pytest.mark.parametrize("tokens,heads", [(1, 16), (5, 1), (1, 1)])
+def test_attention_of_one_token_or_head_takes_any_stride_of_it(tokens, heads):
+    lens = [90, 1, 33, 0, 20][:tokens]
+    pages, table, keys = batch(lens, 16)
+    kept = rnd(tokens, heads, R.ROW, seed=tokens, std=0.3)
+    odd = (4 if tokens == 1 else heads * 584, 3 if heads == 1 else 584, 1)
+    q = torch.zeros(tokens * heads * 584, dtype=BF, device=DEV).as_strided((tokens, heads, R.ROW), odd)
+    q.copy_(kept)
+    room = torch.full((tokens * heads * 520,), 7.0, dtype=BF, device=DEV)
+    out = room.as_strided((tokens, heads, 512), (4 if tokens == 1 else heads * 520, 3 if heads == 1 else 520, 1))
+    got = check(q, pages, table, lens, keys, out=out)
+    assert torch.equal(got, P.attention_decode_paged_fp4(kept, pages, table, i32(lens), SCALE))
+
+
 def test_attention_leaves_query_tokens_of_no_request():
     lens = [50, 60]
     pages, table, keys = batch(lens, 16)

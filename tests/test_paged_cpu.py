@@ -52,6 +52,8 @@ REFUSED = [
     ("paged_cache_step", 4, 2048, ValueError, "power of two"),
     ("paged_cache_step", 4, 0, ValueError, "power of two"),
     ("paged_cache_step", 5, -1, ValueError, "max_tokens"),
+    ("paged_cache_step", 5, 2 ** 31, ValueError, "max_tokens"),
+    ("paged_slot_map", 4, 2 ** 32 + 9, ValueError, "max_tokens"),
     ("paged_slot_map", 0, i32(3), ValueError, "counts must be"),
     ("paged_slot_map", 3, 12, ValueError, "power of two"),
     ("paged_slot_map", 4, -3, ValueError, "max_tokens"),
