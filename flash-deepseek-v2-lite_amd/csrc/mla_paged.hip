@@ -12,6 +12,17 @@
 // closer than kPiece tiles to an item's end moves there, so pieces fill the waves at least once and items
 // of less than two pieces are never cut.  An item within one workgroup is finished there; of one cut into
 // several each leaves its part (fp32 o, max, sum) in the workspace and mla_paged_merge_kernel joins them.
+//
+// A token's 400 bytes give 2 * 16 * (576 + 512) operations a column group, 87 a byte: the matrix cores' rate would
+// allow 200, so the pages' bytes bound it.  A wave takes a tile of 16 tokens at a time: it decodes a block of codes
+// once, into registers (the K side of the scores) and into its own rows of LDS, where the outputs' products read them
+// transposed (the V side); scores and outputs are fp32, the running maximum and sum stay in the wave, and the eight
+// waves meet once, at a piece's end.  Splitting the outputs over the waves instead needs no such end, but its barriers
+// keep the waves in step: 65.5 us where this takes 60.5.
+//
+// MI355X, both launches: 128 requests of 256 to 8,192 tokens, 16 heads: 60.5 us for 221 MB (3.6 TB/s; 38.8 us at the
+// rate of a copy, 5.69 TB/s); the loop itself runs at that rate, some 20 us are launches (3), the first loads (4), the
+// waves' meeting (5) and the merge (6).  One request of 150,000: 26.1 us; of 140: 11.1.
 #include "paged.h"
 
 using namespace paged;
@@ -33,8 +44,8 @@ static_assert(16 * kORow * 4 <= 2 * kWaveLds, "a wave's outputs take two tiles' 
 constexpr int kWgs = 256;              // one workgroup per CU
 constexpr int kPiece = 8;              // tiles of a cut item's piece, at least: one a wave
 constexpr int kMinStretch = 2 * kPiece;
-// A piece takes what 32 more tiles would, 20,000 cycles (MI355X, 128 x 256..8,192 tokens, both launches: 67.5 us
-// with 16, 64.7 with 24, 64.0 with 32, 63.5 with 40; 39 x 1,043..8,347 32.4 / 30.7 / 30.3 / 30.6)
+// A piece takes what some 32 more tiles would, 20,000 cycles (MI355X, 128 x 256..8,192 tokens, both launches: 62.8 us
+// with 16, 60.2 with 24, 60.5 with 32, 61.7 with 40; 12 x 1,440..24,485 26.8 / 26.0 / 25.9 / 26.2)
 constexpr int kItemCost = 32;
 constexpr int kPartFloats = 16 * kLat;
 
@@ -477,6 +488,9 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
 // some 32 KB for each part more than one, however the parts are spread over items.  Everything that it needs
 // is requested at once, when it knows its item: a thread's part of the outputs takes 8 loads at most (2 and 4
 // parts: 4 and 2 times all parts; 8: 8 parts; 256: every 56th part of 9 groups of four outputs, 5 loads).
+// Bound by three loads that wait for one another (cuts; maxima and sums with the parts; outputs) and its launch: 5.6 us
+// on MI355X for 255 cuts of one item, 6.1 for some 200 of 128.  Joining in the workgroup that ends last would save the
+// launch, but needs counters that are zero at each call's start, which two captured graphs would share.
 __global__ __launch_bounds__(512) void mla_paged_merge_kernel(const PagedAttnArgs a) {
   constexpr int kLoads = 8, kLaneParts = kWgs / 64;
   __shared__ float weight[16][kWgs];   // of column (relative to the share's first) and part
