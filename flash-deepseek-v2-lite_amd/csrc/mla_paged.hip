@@ -48,6 +48,10 @@ constexpr int kMinStretch = 2 * kPiece;
 // with 16, 60.2 with 24, 60.5 with 32, 61.7 with 40; 12 x 1,440..24,485 26.8 / 26.0 / 25.9 / 26.2)
 constexpr int kItemCost = 32;
 constexpr int kPartFloats = 16 * kLat;
+// Up to 128 requests every wave sums the line for itself, without LDS or barriers; more are shared by the workgroup
+// (MI355X, one request, to the first item: 1,850 cycles where the workgroup takes 3,400; with room for 256 requests
+// 2,480, for 64 some 1,700)
+constexpr int kFew = 2;
 
 struct PagedAttnArgs {
   const bf16_t* q;
@@ -100,16 +104,22 @@ struct Request {
 __device__ __forceinline__ Request uniform(const Request& r) {
   return {uniform(r.len), uniform(r.q0), uniform(r.nq), uniform(r.columns)};
 }
+__device__ __forceinline__ Request of_lane(const Request& r, int lane) {
+  return {__builtin_amdgcn_readlane(r.len, lane), __builtin_amdgcn_readlane(r.q0, lane),
+          __builtin_amdgcn_readlane(r.nq, lane), __builtin_amdgcn_readlane(r.columns, lane)};
+}
 __device__ __forceinline__ Request request(const PagedAttnArgs& a, int b) {
   Request r;
-  const int64_t room = static_cast<int64_t>(a.width) << a.shift;
-  r.len = static_cast<int>(min(static_cast<int64_t>(max(a.lens[b], 0)), room));
+  const int len = a.lens[b];
   r.q0 = b;
-  r.nq = 1;
+  int end = b + 1;
   if (a.cu_q) {
     r.q0 = a.cu_q[b];
-    r.nq = r.q0 >= 0 ? max(min(a.cu_q[b + 1], a.tokens) - r.q0, 0) : 0;
+    end = a.cu_q[b + 1];
+    pin(end);  // all three are requested before the first is waited for
   }
+  r.len = min(max(len, 0), a.width << a.shift);  // the host has checked that this is an int32
+  r.nq = r.q0 >= 0 ? max(min(end, a.tokens) - r.q0, 0) : 0;
   r.columns = min(r.nq, a.max_q) * a.heads;
   return r;
 }
@@ -146,24 +156,12 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
   int lo, hi, per, b, start;
   Request r;
   {
-    const int chunk = (a.requests + kThreads - 1) / kThreads;
-    const int b0 = min(tid * chunk, a.requests), b1 = min(b0 + chunk, a.requests);
-    int run = 0;
-    bool nothing = false;
-    for (int i = b0; i < b1; ++i) {
-      r = request(a, i);
+    auto seen = [&](const Request& r) {
       if (r.nq > a.max_q && blockIdx.x == 0 && a.status) atomicOr(a.status, DSV2_DEVERR_TOKENS);
-      nothing |= r.len == 0 && r.columns > 0;
-      run += r.places();
-    }
-    int scan = run;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(scan, o, DSV2_WAVE);
-      if (lane >= o) scan += u;
-    }
-    if (lane == 63) wave_sums[wv] = scan;
-    if (__syncthreads_or(nothing)) {  // requests with nothing cached: zeros
+      return r.len == 0 && r.columns > 0;
+    };
+    // requests with nothing cached: zeros
+    auto clear = [&] {
       for (int i = blockIdx.x; i < a.requests; i += gridDim.x) {
         const Request z = request(a, i);
         if (z.len > 0) continue;
@@ -171,41 +169,88 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
           *reinterpret_cast<uint4*>(out_row(a, z.q0, f / (kLat / 8)) + f % (kLat / 8) * 8) = make_uint4(0, 0, 0, 0);
         }
       }
-    }
-    int before = scan - run, total = 0;
+    };
+    // false: no stretch is left for this workgroup
+    auto stretch = [&](int total) {
+      per = max((total + kWgs - 1) / kWgs, kMinStretch);
+      const int64_t from = static_cast<int64_t>(blockIdx.x) * per;
+      if (tid == 0) a.cuts[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
+      if (from >= total) return false;
+      lo = static_cast<int>(from);
+      hi = min(lo + per, total);
+      return true;
+    };
+    if (a.requests <= kFew * 64) {
+      // every wave for itself: lane l has requests l, l + 64, ...
+      Request u[kFew];
+      int run[kFew], scan[kFew], total = 0;
+      bool nothing = false;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      if (i < wv) before += wave_sums[i];
-      total += wave_sums[i];
+      for (int k = 0; k < kFew; ++k) u[k] = request(a, min(64 * k + lane, a.requests - 1));
+#pragma unroll
+      for (int k = 0; k < kFew; ++k) {
+        const bool is = 64 * k + lane < a.requests;
+        nothing |= is && seen(u[k]);
+        run[k] = is ? u[k].places() : 0;
+        scan[k] = wave_scan(run[k]) + total;
+        total = __builtin_amdgcn_readlane(scan[k], 63);
+      }
+      if (__any(nothing)) clear();
+      if (!stretch(total)) return;
+#pragma unroll
+      for (int k = 0; k < kFew; ++k) {
+        const uint64_t has = __ballot(scan[k] - run[k] <= lo && lo < scan[k]);
+        if (!has) continue;
+        const int at = __builtin_ctzll(has);
+        b = 64 * k + at;
+        start = __builtin_amdgcn_readlane(scan[k] - run[k], at);
+        r = of_lane(u[k], at);
+      }
+    } else {
+      const int chunk = (a.requests + kThreads - 1) / kThreads;
+      const int b0 = min(tid * chunk, a.requests), b1 = min(b0 + chunk, a.requests);
+      int run = 0;
+      bool nothing = false;
+      for (int i = b0; i < b1; ++i) {
+        r = request(a, i);
+        nothing |= seen(r);
+        run += r.places();
+      }
+      const int scan = wave_scan(run);
+      if (lane == 63) wave_sums[wv] = scan;
+      if (__syncthreads_or(nothing)) clear();
+      int before = scan - run, total = 0;
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) {
+        if (i < wv) before += wave_sums[i];
+        total += wave_sums[i];
+      }
+      if (!stretch(uniform(total))) return;
+      if (before <= lo && lo < before + run) {
+        int i = b0;
+        if (b1 - b0 > 1)
+          for (;; ++i) {
+            r = request(a, i);
+            if (lo < before + r.places()) break;
+            before += r.places();
+          }
+        first_request[0] = make_int4(i, before, 0, 0);
+        first_request[1] = make_int4(r.len, r.q0, r.nq, r.columns);
+      }
+      __syncthreads();
+      const int4 u = first_request[0], v = first_request[1];
+      b = uniform(u.x);
+      start = uniform(u.y);
+      r = uniform(Request{v.x, v.y, v.z, v.w});
     }
-    total = uniform(total);
-    per = max((total + kWgs - 1) / kWgs, kMinStretch);
-    const int64_t from = static_cast<int64_t>(blockIdx.x) * per;
-    if (tid == 0) a.cuts[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
-    if (from >= total) return;
-    lo = static_cast<int>(from);
-    hi = min(lo + per, total);
-    if (before <= lo && lo < before + run) {
-      int i = b0;
-      if (b1 - b0 > 1)
-        for (;; ++i) {
-          r = request(a, i);
-          if (lo < before + r.places()) break;
-          before += r.places();
-        }
-      first_request[0] = make_int4(i, before, 0, 0);
-      first_request[1] = make_int4(r.len, r.q0, r.nq, r.columns);
-    }
-    __syncthreads();
-    const int4 u = first_request[0], v = first_request[1];
-    b = uniform(u.x);
-    start = uniform(u.y);
-    r = uniform(Request{v.x, v.y, v.z, v.w});
   }
 
   bf16_t* const vt = reinterpret_cast<bf16_t*>(smem + wv * kWaveLds);
-  int ct = (lo - start) / (r.tiles() + kItemCost);
-  start += ct * (r.tiles() + kItemCost);  // of the item
+  int ct = 0;
+  if (r.columns > 16) {
+    ct = (lo - start) / (r.tiles() + kItemCost);
+    start += ct * (r.tiles() + kItemCost);  // of the item
+  }
   bool again = false;
   for (; start < hi; start += r.tiles() + kItemCost, ++ct) {
     if (ct * 16 >= r.columns) {
@@ -220,8 +265,7 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
       if (!has) return;
       const int at = __builtin_ctzll(has);
       b += at;
-      r = Request{__builtin_amdgcn_readlane(r.len, at), __builtin_amdgcn_readlane(r.q0, at),
-                  __builtin_amdgcn_readlane(r.nq, at), __builtin_amdgcn_readlane(r.columns, at)};
+      r = of_lane(r, at);
       ct = 0;
     }
     // (the compiler does not see that these are the same for all lanes)
@@ -452,9 +496,11 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
     if (t_first > 0 && tid == 0) {
       // the workgroups that the item's first and last tiles went to
       const int end = start + tiles;
-      int w0 = start / per, w1 = (end - 1) / per;
-      if ((w0 + 1) * per - start < kPiece) ++w0;
-      if (end - w1 * per < kPiece) --w1;
+      int by = per;
+      asm volatile("" : "+s"(by));  // the divisions are only done here
+      int w0 = start / by, w1 = (end - 1) / by;
+      if ((w0 + 1) * by - start < kPiece) ++w0;
+      if (end - w1 * by < kPiece) --w1;
       a.cuts[2 * blockIdx.x] = make_int4(ct * 16, r.columns, w0, w1);
       a.cuts[2 * blockIdx.x + 1] = make_int4(r.len, r.nq, r.q0, 0);
     }

@@ -41,6 +41,20 @@ __device__ __forceinline__ TokenAt token_at(int slot, int shift, int64_t page_st
           base + (static_cast<int64_t>(kCodeB + kRopeB) << shift) + off * kScaleB};
 }
 
+// the sums of v over lanes 0 .. l, by register moves between the lanes (six LDS-routed shuffles take 800 cycles)
+template <typename Add>
+__device__ __forceinline__ int wave_scan(int v, Add add) {
+  v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));  // row_shr 1, 2, 4, 8: within 16 lanes
+  v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+  v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+  v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+  v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));  // lane 15 (47) to lanes 16-31 (48-63)
+  return add(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));  // lane 31 to lanes 32-63
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  return wave_scan(v, [](int x, int y) { return x + y; });
+}
+
 // 8 codes (one dword, low nibble first) of a block with scale byte s as 8 bf16: the values are exact
 __device__ __forceinline__ uint4 decode8(uint32_t codes, uint32_t s) {
   const float scale = __uint_as_float(s << 23);

@@ -43,23 +43,14 @@ __device__ __forceinline__ void block_scan(const uint32_t* v, uint32_t* before, 
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   uint32_t x[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) x[k] = v[k];
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const uint32_t u = __shfl_up(x[k], o, DSV2_WAVE);
-      if (lane >= o) x[k] = add_sat(x[k], u);
-    }
-  }
+  for (int k = 0; k < K; ++k) x[k] = wave_scan(v[k], [](uint32_t a, uint32_t b) { return add_sat(a, b); });
   if (lane == 63) {
 #pragma unroll
     for (int k = 0; k < K; ++k) red[w * K + k] = x[k];
   }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const uint32_t u = __shfl_up(x[k], 1, DSV2_WAVE);
-    before[k] = lane ? u : 0;
+    before[k] = __builtin_amdgcn_update_dpp(0, x[k], 0x138, 0xf, 0xf, false);  // the lane before this one's, 0 before lane 0
   }
   __syncthreads();
 #pragma unroll
