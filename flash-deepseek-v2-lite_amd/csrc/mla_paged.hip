@@ -84,6 +84,10 @@ struct PagedAttnArgs {
 __device__ __forceinline__ int token_of(const PagedAttnArgs& a, int column) {
   return a.heads_inv ? static_cast<int>(__umulhi(static_cast<uint32_t>(column), a.heads_inv)) : column;
 }
+// n / d for 0 <= n < 2^20, d > 0: (n + 1/2) / d is 1 / (2 d) from the next whole number, its error below (n + 1/2) / d / 2^22
+__device__ __forceinline__ int quotient(int n, int d) {
+  return static_cast<int>((static_cast<float>(n) + 0.5f) * __builtin_amdgcn_rcpf(static_cast<float>(d)));
+}
 // the output row of a column of the request whose first query token is q0
 __device__ __forceinline__ bf16_t* out_row(const PagedAttnArgs& a, int q0, int column) {
   const int j = token_of(a, column);
@@ -545,7 +549,7 @@ __global__ __launch_bounds__(512) void mla_paged_merge_kernel(const PagedAttnArg
   const int4 item = a.cuts[2 * (blockIdx.x + 1)], req = a.cuts[2 * (blockIdx.x + 1) + 1];
   if (item.x < 0) return;
   const int col0 = item.x, columns = item.y, w0 = item.z, parts = item.w - w0 + 1;  // 2 .. kWgs
-  const int share = (kPartFloats / 4 + parts - 2) / (parts - 1);  // groups of four outputs
+  const int share = quotient(kPartFloats / 4 + parts - 2, parts - 1);  // groups of four outputs
   const int f0 = (blockIdx.x - w0) * share, f1 = min(f0 + share, kPartFloats / 4);
   if (f0 >= f1) return;
   const int c0 = f0 >> 7, c1 = (f1 - 1) >> 7;
@@ -561,8 +565,8 @@ __global__ __launch_bounds__(512) void mla_paged_merge_kernel(const PagedAttnArg
     }
   // threads in groups of the share's width, each group every so many parts; a share wider than the
   // workgroup goes in passes
-  const int width = min(f1 - f0, 512), groups = 512 / width, g = tid / width;
-  const int in_pass = (parts + groups - 1) / groups, loads = (f1 - f0 + width - 1) / width * in_pass;
+  const int width = min(f1 - f0, 512), groups = quotient(512, width), g = quotient(tid, width);
+  const int in_pass = quotient(parts + groups - 1, groups), loads = quotient(f1 - f0 + width - 1, width) * in_pass;
   float4 x[kLoads];
   int f = f0 + tid - g * width, p = g, pass = 0;  // of the next load
   auto advance = [&] {
