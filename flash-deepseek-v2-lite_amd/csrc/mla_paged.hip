@@ -22,7 +22,7 @@
 //
 // MI355X, both launches: 128 requests of 256 to 8,192 tokens, 16 heads: 60.5 us for 221 MB (3.6 TB/s; 38.8 us at the
 // rate of a copy, 5.69 TB/s); the loop itself runs at that rate, some 20 us are launches (3), the first loads (4), the
-// waves' meeting (5) and the merge (6).  One request of 150,000: 26.1 us; of 140: 11.1.
+// waves' meeting (5) and the merge (6).  One request of 150,000: 25.4 us; of 140: 10.2.
 #include "paged.h"
 
 using namespace paged;
@@ -306,7 +306,8 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
       const int off = t & ((1 << a.shift) - 1);
       const uint8_t* base = a.pages + (page ? pg : 0) * a.page_stride;
       if (kOnePage) {
-        const auto buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, tile < t_last ? kTokenB << a.shift : 0, 0x27000);
+        const auto buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0,
+                                                           tile < t_last ? kTokenB << a.shift : 0, 0x27000);
         auto load = [&](int lane_at, int at) {
           return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buf, lane_at, at, 0));
         };
@@ -538,8 +539,8 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
 // some 32 KB for each part more than one, however the parts are spread over items.  Everything that it needs
 // is requested at once, when it knows its item: a thread's part of the outputs takes 8 loads at most (2 and 4
 // parts: 4 and 2 times all parts; 8: 8 parts; 256: every 56th part of 9 groups of four outputs, 5 loads).
-// Bound by three loads that wait for one another (cuts; maxima and sums with the parts; outputs) and its launch: 5.6 us
-// on MI355X for 255 cuts of one item, 6.1 for some 200 of 128.  Joining in the workgroup that ends last would save the
+// Bound by two loads that wait for one another (cuts; maxima, sums and parts) and its launch: 5.3 us on MI355X for 255
+// cuts of one item, 5.8 for some 200 of 128.  Joining in the workgroup that ends last would save the
 // launch, but needs counters that are zero at each call's start, which two captured graphs would share.
 __global__ __launch_bounds__(512) void mla_paged_merge_kernel(const PagedAttnArgs a) {
   constexpr int kLoads = 8, kLaneParts = kWgs / 64;
@@ -693,8 +694,8 @@ extern "C" int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_
   float* part_ml = part_o + 2 * kWgs * kPartFloats;
   int4* cuts = (int4*)(part_ml + 2 * kWgs * 32);
   const PagedAttnArgs a{(const bf16_t*)q, q_ts, q_hs, tokens, heads,
-                        heads == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + heads - 1) / heads), (const uint8_t*)pages, page_stride, n_pages,
-                        shift, block_table, table_stride, table_width, lens, cu_q, max_q, requests, groups,
+                        heads == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + heads - 1) / heads),
+                        (const uint8_t*)pages, page_stride, n_pages, shift, block_table, table_stride, table_width, lens, cu_q, max_q, requests, groups,
                         softmax_scale * 1.4426950408889634f, (bf16_t*)out, out_ts, out_hs, part_o, part_ml, cuts,
                         status};
   const int64_t tiles = (room + kTile - 1) / kTile, most = items * (tiles + kItemCost);

@@ -96,8 +96,8 @@ struct PlanArgs {
 // pages that empties go behind the ring's free stretch in the order of requests and pages.
 //
 // Integer sums, a handful of bytes: bound by the launch and a few dependent loads and barriers (MI355X, in a graph:
-// 8 requests 3.5 us, of which an empty launch takes 1.7; 1,024 requests with 263,000 new tokens 9.9 us, 3.2 MB
-// written; ranges of 5 requests 2.9, of 256 with 525,000 tokens 5.7 us, 6.3 MB).
+// 8 requests 3.3 us, of which an empty launch takes 1.7; 1,024 requests with 263,000 new tokens 9.3 us, 3.2 MB
+// written; ranges of 5 requests 2.7, of 256 with 525,000 tokens 5.4 us, 6.3 MB).
 template <bool STEP, int kThreads>
 __global__ __launch_bounds__(kThreads) void paged_plan_kernel(const PlanArgs a) {
   constexpr int K = STEP ? 3 : 1;
@@ -257,9 +257,9 @@ static int plan_launch(const char* what, bool step, const PlanArgs& a, int page_
   DSV2_REQUIRE(a.width > 0 && a.width <= (INT32_MAX >> a.shift) && a.ts >= a.width, DSV2_E_SHAPE,
                "%s: block table of %d columns", what, a.width);
   DSV2_REQUIRE(a.tokens >= 0, DSV2_E_SHAPE, "%s: max_tokens %d", what, a.tokens);
-  // Every workgroup repeats the scan, so many requests go with few, large workgroups (MI355X, 1,024 requests
-  // with 263,000 new tokens: 512 workgroups of 256 threads 13.2 us, 2,048 13.0, 256 of 1,024 10.0; 64 requests
-  // with 64,000 tokens 3.8 with 1,024 threads, 3.4 with 256).  What a step takes back only the device knows:
+  // Every workgroup repeats the scan, so many requests go with few, large workgroups (MI355X, scans by
+  // shuffles then: 1,024 requests with 263,000 new tokens: 512 workgroups of 256 threads 13.2 us, 2,048 13.0, 256 of
+  // 1,024 10.0; 64 requests with 64,000 tokens 3.8 with 1,024 threads, 3.4 with 256).  What a step takes back only the device knows:
   // room for 8 pages a request (1,000 requests, 62 of which end with 62 pages: 7.7 us, with none 10.7).
   const bool many = a.n > kManyRequests;
   const int threads = many ? 1024 : 256, most = many ? 256 : 1024;
