@@ -695,15 +695,16 @@ extern "C" int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_
   int4* cuts = (int4*)(part_ml + 2 * kWgs * 32);
   const PagedAttnArgs a{(const bf16_t*)q, q_ts, q_hs, tokens, heads,
                         heads == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + heads - 1) / heads),
-                        (const uint8_t*)pages, page_stride, n_pages, shift, block_table, table_stride, table_width, lens, cu_q, max_q, requests, groups,
-                        softmax_scale * 1.4426950408889634f, (bf16_t*)out, out_ts, out_hs, part_o, part_ml, cuts,
+                        (const uint8_t*)pages, page_stride, n_pages, shift, block_table, table_stride,
+                        table_width, lens, cu_q, max_q, requests, groups, softmax_scale * 1.4426950408889634f, (bf16_t*)out, out_ts, out_hs, part_o, part_ml, cuts,
                         status};
   const int64_t tiles = (room + kTile - 1) / kTile, most = items * (tiles + kItemCost);
   const int wgs = static_cast<int>(most / kMinStretch + 1 < kWgs ? most / kMinStretch + 1 : kWgs);
-  if ((1 << shift) >= kTile)
-    hipLaunchKernelGGL(mla_paged_kernel<true>, dim3(wgs), dim3(kThreads), kWaves * kWaveLds + kQLds, (hipStream_t)stream, a);
+  constexpr int kLds = kWaves * kWaveLds + kQLds;
+  if (page_size >= kTile)
+    hipLaunchKernelGGL(mla_paged_kernel<true>, dim3(wgs), dim3(kThreads), kLds, (hipStream_t)stream, a);
   else
-    hipLaunchKernelGGL(mla_paged_kernel<false>, dim3(wgs), dim3(kThreads), kWaves * kWaveLds + kQLds, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(mla_paged_kernel<false>, dim3(wgs), dim3(kThreads), kLds, (hipStream_t)stream, a);
   if (const int rc = dsv2_launch_status("mla_decode_paged_fp4")) return rc;
   if (wgs == 1 || tiles < 2 * kPiece) return DSV2_OK;  // no item of so few tiles is cut
   hipLaunchKernelGGL(mla_paged_merge_kernel, dim3(wgs - 1), dim3(512), 0, (hipStream_t)stream, a);

@@ -356,6 +356,17 @@ def test_attention_of_few_live_rows_among_many_idle_ones(live):
         assert ((got[b].double() - want).abs() <= tol).all(), b
 
 
+@pytest.mark.parametrize("requests", [2, 63, 64, 65, 127, 128, 129, 192, 513])
+@pytest.mark.parametrize("drafts", [False, True])
+def test_attention_numbers_of_requests(requests, drafts):
+    """Lengths, empty ones among them, and query counts that differ from request to request."""
+    lens = [(b * 29) % 71 if b % 5 else 0 for b in range(requests)]
+    lens[-1] = 300
+    nq = [(b * 7) % 4 for b in range(requests)] if drafts else None
+    pages, table, keys = batch(lens, 32, seed=requests)
+    check(rnd(sum(nq) if drafts else requests, 4, R.ROW, seed=requests, std=0.3), pages, table, lens, keys, nq)
+
+
 @pytest.mark.parametrize("std", [0.0, 3.0, 30.0])
 def test_attention_flat_and_sharp(std):
     """Equal scores, and scores whose softmax has one token left; a scale of its own."""
