@@ -22,7 +22,7 @@
 //
 // MI355X, both launches: 128 requests of 256 to 8,192 tokens, 16 heads: 60.5 us for 221 MB (3.6 TB/s; 38.8 us at the
 // rate of a copy, 5.69 TB/s); the loop itself runs at that rate, some 20 us are launches (3), the first loads (4), the
-// waves' meeting (5) and the merge (6).  One request of 150,000: 25.4 us; of 140: 10.2.
+// waves' meeting (5) and the merge (6).  One request of 150,000: 25.6 us; of 140: 10.4.
 #include "paged.h"
 
 using namespace paged;
@@ -48,9 +48,9 @@ constexpr int kMinStretch = 2 * kPiece;
 // with 16, 60.2 with 24, 60.5 with 32, 61.7 with 40; 12 x 1,440..24,485 26.8 / 26.0 / 25.9 / 26.2)
 constexpr int kItemCost = 32;
 constexpr int kPartFloats = 16 * kLat;
-// Up to 128 requests every wave sums the line for itself, without LDS or barriers; more are shared by the workgroup
-// (MI355X, one request, to the first item: 1,850 cycles where the workgroup takes 3,400; with room for 256 requests
-// 2,480, for 64 some 1,700)
+// Up to 128 requests one wave sums the line; more are shared by the workgroup (MI355X, one request, to the first item,
+// each wave summing for itself: 1,850 cycles where the workgroup takes 3,400; with room for 256 requests 2,480, for 64
+// some 1,700; one wave for all, which cannot part the waves, takes 0.2 us more)
 constexpr int kFew = 2;
 
 struct PagedAttnArgs {
@@ -150,7 +150,9 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ float ml[kWaves][16][2];
   __shared__ int32_t wave_sums[kWaves];
-  __shared__ int4 first_request[2];
+  // what one wave or thread has found for all, so that the waves never part, whatever another stream does to the
+  // lengths meanwhile: a request, in turns (place on the line; itself)
+  __shared__ int4 found[2][2];
   uint4* const q_lds = reinterpret_cast<uint4*>(smem + kWaves * kWaveLds);
   const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6), li = lane & 15,
             kg = lane >> 4;
@@ -174,42 +176,44 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
         }
       }
     };
-    // false: no stretch is left for this workgroup
+    // this workgroup's stretch of the line; none: lo == hi == total
     auto stretch = [&](int total) {
       per = max((total + kWgs - 1) / kWgs, kMinStretch);
       const int64_t from = static_cast<int64_t>(blockIdx.x) * per;
-      if (tid == 0) a.cuts[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
-      if (from >= total) return false;
-      lo = static_cast<int>(from);
+      lo = static_cast<int>(min(from, static_cast<int64_t>(total)));
       hi = min(lo + per, total);
-      return true;
     };
+    if (tid == 0) a.cuts[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
     if (a.requests <= kFew * 64) {
-      // every wave for itself: lane l has requests l, l + 64, ...
-      Request u[kFew];
-      int run[kFew], scan[kFew], total = 0;
-      bool nothing = false;
+      // one wave: lane l has requests l, l + 64, ...
+      if (wv == 0) {
+        Request u[kFew];
+        int run[kFew], scan[kFew], total = 0;
+        bool nothing = false;
 #pragma unroll
-      for (int k = 0; k < kFew; ++k) u[k] = request(a, min(64 * k + lane, a.requests - 1));
+        for (int k = 0; k < kFew; ++k) u[k] = request(a, min(64 * k + lane, a.requests - 1));
 #pragma unroll
-      for (int k = 0; k < kFew; ++k) {
-        const bool is = 64 * k + lane < a.requests;
-        nothing |= is && seen(u[k]);
-        run[k] = is ? u[k].places() : 0;
-        scan[k] = wave_scan(run[k]) + total;
-        total = __builtin_amdgcn_readlane(scan[k], 63);
+        for (int k = 0; k < kFew; ++k) {
+          const bool is = 64 * k + lane < a.requests;
+          nothing |= is && seen(u[k]);
+          run[k] = is ? u[k].places() : 0;
+          scan[k] = wave_scan(run[k]) + total;
+          total = __builtin_amdgcn_readlane(scan[k], 63);
+        }
+        stretch(total);
+        const bool none = __any(nothing);
+        if (lane == 0) found[0][0] = make_int4(0, 0, total, none);
+#pragma unroll
+        for (int k = 0; k < kFew; ++k) {
+          if (scan[k] - run[k] <= lo && lo < scan[k]) {
+            found[0][0] = make_int4(64 * k + lane, scan[k] - run[k], total, none);
+            found[0][1] = make_int4(u[k].len, u[k].q0, u[k].nq, u[k].columns);
+          }
+        }
       }
-      if (__any(nothing)) clear();
-      if (!stretch(total)) return;
-#pragma unroll
-      for (int k = 0; k < kFew; ++k) {
-        const uint64_t has = __ballot(scan[k] - run[k] <= lo && lo < scan[k]);
-        if (!has) continue;
-        const int at = __builtin_ctzll(has);
-        b = 64 * k + at;
-        start = __builtin_amdgcn_readlane(scan[k] - run[k], at);
-        r = of_lane(u[k], at);
-      }
+      __syncthreads();
+      if (found[0][0].w) clear();
+      stretch(uniform(found[0][0].z));
     } else {
       const int chunk = (a.requests + kThreads - 1) / kThreads;
       const int b0 = min(tid * chunk, a.requests), b1 = min(b0 + chunk, a.requests);
@@ -229,24 +233,25 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
         if (i < wv) before += wave_sums[i];
         total += wave_sums[i];
       }
-      if (!stretch(uniform(total))) return;
+      stretch(uniform(total));
       if (before <= lo && lo < before + run) {
         int i = b0;
         if (b1 - b0 > 1)
           for (;; ++i) {
             r = request(a, i);
-            if (lo < before + r.places()) break;
+            if (i + 1 == b1 || lo < before + r.places()) break;
             before += r.places();
           }
-        first_request[0] = make_int4(i, before, 0, 0);
-        first_request[1] = make_int4(r.len, r.q0, r.nq, r.columns);
+        found[0][0] = make_int4(i, before, 0, 0);
+        found[0][1] = make_int4(r.len, r.q0, r.nq, r.columns);
       }
       __syncthreads();
-      const int4 u = first_request[0], v = first_request[1];
-      b = uniform(u.x);
-      start = uniform(u.y);
-      r = uniform(Request{v.x, v.y, v.z, v.w});
     }
+    if (lo >= hi) return;
+    const int4 u = found[0][0], v = found[0][1];
+    b = uniform(u.x);
+    start = uniform(u.y);
+    r = uniform(Request{v.x, v.y, v.z, v.w});
   }
 
   bf16_t* const vt = reinterpret_cast<bf16_t*>(smem + wv * kWaveLds);
@@ -256,20 +261,29 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
     start += ct * (r.tiles() + kItemCost);  // of the item
   }
   bool again = false;
+  int turn = 0;
   for (; start < hi; start += r.tiles() + kItemCost, ++ct) {
     if (ct * 16 >= r.columns) {
       // the next request that has places (there is one, the line goes on), looked for 64 at a time: of a server's
       // rows most may be idle (8 of 4,096 in use: 71 us one after the other, 33 so)
-      uint64_t has = 0;
-      for (++b; b < a.requests; b += 64) {
-        r = request(a, min(b + lane, a.requests - 1));
-        has = __ballot(b + lane < a.requests && r.places() > 0);
-        if (has) break;
+      turn ^= 1;
+      if (wv == 0) {
+        uint64_t has = 0;
+        for (++b; b < a.requests; b += 64) {
+          r = request(a, min(b + lane, a.requests - 1));
+          has = __ballot(b + lane < a.requests && r.places() > 0);
+          if (has) break;
+        }
+        if (has ? lane == __builtin_ctzll(has) : lane == 0) {
+          found[turn][0] = make_int4(has ? b + lane : -1, 0, 0, 0);
+          found[turn][1] = make_int4(r.len, r.q0, r.nq, r.columns);
+        }
       }
-      if (!has) return;
-      const int at = __builtin_ctzll(has);
-      b += at;
-      r = of_lane(r, at);
+      __syncthreads();
+      const int4 v = found[turn][1];
+      b = uniform(found[turn][0].x);
+      if (b < 0) return;
+      r = uniform(Request{v.x, v.y, v.z, v.w});
       ct = 0;
     }
     // (the compiler does not see that these are the same for all lanes)
