@@ -461,6 +461,34 @@ def test_attention_nan_reaches_only_those_who_see_it(what):
             t += 1
 
 
+def test_attention_weights_add_up_to_one():
+    """One token far above the rest, p of which is anything up to 2^8 for the maximum that its wave kept from an
+    earlier tile: its rounding must not scale the output.  Two tokens count, 0 with latents 4 and 128 (the same
+    wave's next tile) with 6 and a weight 2^5 to 2^8 times as large, so o = 6 - 2w."""
+    heads, n = 128, 129
+    x = torch.zeros(n, R.ROW, device=DEV)
+    x[:, :512] = 6.0
+    x[0, :512] = 4.0
+    x[1:128, 513] = -2.0 ** 14
+    x[128, 512] = 64.0
+    pages = torch.zeros(3, 64 * R.TOKEN, dtype=torch.uint8, device=DEV)
+    P.paged_cache_write_fp4(x.to(BF), torch.arange(n, device=DEV).int(), pages)
+    q = torch.zeros(1, heads, R.ROW, device=DEV)
+    q[0, :, 512] = torch.linspace(5, 7.9, heads, device=DEV) * 0.6931471805599453 / 64 / 0.125
+    q[0, :, 513] = 1.0
+    q = q.to(BF)
+    got = P.attention_decode_paged_fp4(q, pages, i32([[0, 1, 2]]), i32([n]), 0.125)
+    keys = x.to(BF).double()
+    p = torch.softmax(q[0].double() @ keys.T * 0.125, -1)
+    want = p @ keys[:, :512]
+    # the output's rounding (steps of 2^-5 between 4 and 8, half of one), each weight's to bf16 about the output
+    # (2^-8), fp32 sums, exp2 and division (2^-18)
+    spread = (p[:, :, None] * (keys[None, :, :512] - want[:, None]).abs()).sum(1)
+    tol = 2.0 ** -6 + 2.0 ** -8 * spread + 2.0 ** -18 * 6
+    off = (got[0].double() - want).abs()
+    assert (off <= tol).all(), float((off / tol).max())
+
+
 def test_attention_infinite_scores():
     """Scores of -inf count nothing; nothing but them is NaN, and so is a score of +inf."""
     def fill(b, n):
