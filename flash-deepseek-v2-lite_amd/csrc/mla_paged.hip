@@ -400,20 +400,21 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
         p[i] = tile * kTile + 4 * kg + i < seen ? sc[i] : -INFINITY;
         mx = fmaxf(mx, p[i]);
       }
-      mx = xor32_max(xor16_max(mx)) * a.scale_log2;
-      // lazy rescaling: the running maximum (log2 units) moves, and o and l are rescaled, only where a
-      // tile exceeds it by more than 8, so p <= 256; it starts below every finite score
-      const bool grow = mx > m_run + 8.f;
+      mx = xor32_max(xor16_max(mx));
+      // lazy rescaling: the running maximum (a score, not scaled yet) moves, and o and l are rescaled, only where a
+      // tile exceeds it by more than 8 in log2 units, so p <= 256; it starts below every finite score.  Differences
+      // are scaled, not scores: those are exact next to the maximum, however large the scores are or become when scaled
+      const bool grow = (mx - m_run) * a.scale_log2 > 8.f;
       if (__any(grow)) {
         const float m_new = grow ? mx : m_run;
-        const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+        const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * a.scale_log2);
         l_run *= alpha;
         m_run = m_new;
 #pragma unroll
         for (int f = 0; f < 32; ++f) acc[f] *= alpha;
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], a.scale_log2, -m_run));
+      for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f((p[i] - m_run) * a.scale_log2);
       // P^T (B operand): column li, tokens 4 kg + e; the V^T fragments take the same tokens through
       // transposed reads (lane (li, kg) addresses token 4 kg + li / 4).  p is rounded to bf16, which the products take
       // (2^-8 of a weight at most), and l sums the rounded values in fp32, so the weights add up to one: a token that
@@ -492,9 +493,9 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) m_all = fmaxf(m_all, part[i] = ml[i][li][0]);
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) l_all += ml[i][li][1] * __builtin_amdgcn_exp2f(part[i] - m_all);
+    for (int i = 0; i < kWaves; ++i) l_all += ml[i][li][1] * __builtin_amdgcn_exp2f((part[i] - m_all) * a.scale_log2);
     const bool whole = t_first == 0 && t_last == tiles;
-    float weight = __builtin_amdgcn_exp2f(m_run - m_all);
+    float weight = __builtin_amdgcn_exp2f((m_run - m_all) * a.scale_log2);
     if (whole) weight *= seen > 0 ? 1.0f / l_all : 0.f;
     float* o_lds = reinterpret_cast<float*>(smem + (wv & 3) * 2 * kWaveLds) + li * kORow + 4 * kg;
     if (wv >= 4) {
@@ -613,7 +614,7 @@ __global__ __launch_bounds__(512) void mla_paged_merge_kernel(const PagedAttnArg
     float l = 0.f, w[kLaneParts];
 #pragma unroll
     for (int k = 0; k < kLaneParts; ++k) {
-      w[k] = __builtin_amdgcn_exp2f(ml[i][k].x - m);
+      w[k] = __builtin_amdgcn_exp2f((ml[i][k].x - m) * a.scale_log2);
       l += ml[i][k].y * w[k];
     }
     l = wave_sum(l);

@@ -461,6 +461,32 @@ def test_attention_nan_reaches_only_those_who_see_it(what):
             t += 1
 
 
+@pytest.mark.parametrize("scale,size", [(1e30, 1.0), (0.125, 2.0 ** 33), (0.125, 2.0 ** 70), (1e-30, 2.0 ** 60),
+                                        (1e-42, 1.0)])
+@pytest.mark.parametrize("n", [1, 200, 5000])
+def test_attention_scores_of_any_size(scale, size, n):
+    """Scores that pass fp32 when scaled, whose fp32 steps are wider than exp2's range, and hardly any scores at all.
+    Each is one product, so exact; the two largest are equal."""
+    t = torch.arange(n, device=DEV)
+    x = rnd(n, R.ROW, seed=n)
+    x[:, 512:] = 0
+    x[:, 512] = ((1 + (t % 128) / 128) * torch.exp2((t // 128).float() - 20)).to(BF)
+    x[0, 512] = x[-1, 512]
+    x = x[torch.randperm(n, device=DEV, generator=torch.Generator(device=DEV).manual_seed(n))]
+    pages = torch.zeros(-(-n // 64), 64 * R.TOKEN, dtype=torch.uint8, device=DEV)
+    P.paged_cache_write_fp4(x, t.int(), pages)
+    q = torch.zeros(1, 16, R.ROW, device=DEV)
+    q[0, :, 512] = torch.where(torch.arange(16, device=DEV) % 2 > 0, -size, size)
+    q = q.to(BF)
+    table = torch.arange(pages.shape[0], device=DEV).int()[None]
+    got = P.attention_decode_paged_fp4(q, pages, table, i32([n]), scale)
+    keys = R.held(x)
+    p = torch.softmax(q[0].double() @ keys.T * scale, -1)
+    want, mass = p @ keys[:, :512], p @ keys[:, :512].abs()
+    # the output's rounding and the weights' (2^-8 each); differences, scaling, exp2 and fp32 sums 2^-16
+    assert ((got[0].double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 * 1.01 + 2.0 ** -16) * mass).all()
+
+
 def test_attention_weights_add_up_to_one():
     """One token far above the rest, p of which is anything up to 2^8 for the maximum that its wave kept from an
     earlier tile: its rounding must not scale the output.  Two tokens count, 0 with latents 4 and 128 (the same
