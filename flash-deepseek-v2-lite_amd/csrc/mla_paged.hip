@@ -24,6 +24,7 @@
 // rate of a copy, 5.69 TB/s); the loop itself runs at that rate, some 20 us are launches (3), the first loads (4), the
 // waves' meeting (5) and the merge (6).  One request of 150,000: 25.6 us; of 140: 10.4.
 #include "paged.h"
+#include "paged_line.h"
 
 using namespace paged;
 
@@ -42,7 +43,6 @@ constexpr int kQAhead = 3, kVAhead = 6;  // fragments that are read ahead of the
 constexpr int kQLoads = (18 + kWaves - 1) / kWaves;
 static_assert(16 * kORow * 4 <= 2 * kWaveLds, "a wave's outputs take two tiles' place");
 constexpr int kWgs = 256;              // one workgroup per CU
-constexpr int kPiece = 8;              // tiles of a cut item's piece, at least: one a wave
 constexpr int kMinStretch = 2 * kPiece;
 // A piece takes what some 32 more tiles would, 20,000 cycles (MI355X, 128 x 256..8,192 tokens, both launches: 62.8 us
 // with 16, 60.2 with 24, 60.5 with 32, 61.7 with 40; 12 x 1,440..24,485 26.8 / 26.0 / 25.9 / 26.2)
@@ -292,9 +292,7 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
     ct = uniform(ct);
     start = uniform(start);
     const int tiles = r.tiles();
-    // where this stretch cuts the item: an end within kPiece of one of the item's moves there
-    auto cut = [&](int t) { return t < kPiece ? 0 : (tiles - t < kPiece ? tiles : t); };
-    const int t_first = cut(lo - start), t_last = cut(hi - start);
+    const int t_first = cut_at(lo - start, tiles), t_last = cut_at(hi - start, tiles);
     if (t_first >= t_last) continue;
     if (again) __syncthreads();  // the last item's outputs, queries and maxima lay where this one's go
     again = true;
@@ -517,14 +515,10 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
     __syncthreads();
     const int slot = 2 * blockIdx.x + (t_first == 0);
     if (t_first > 0 && tid == 0) {
-      // the workgroups that the item's first and last tiles went to
-      const int end = start + tiles;
       int by = per;
       asm volatile("" : "+s"(by));  // the divisions are only done here
-      int w0 = start / by, w1 = (end - 1) / by;
-      if ((w0 + 1) * by - start < kPiece) ++w0;
-      if (end - w1 * by < kPiece) --w1;
-      a.cuts[2 * blockIdx.x] = make_int4(ct * 16, r.columns, w0, w1);
+      const Parts parts = parts_of(start, tiles, by, gridDim.x);
+      a.cuts[2 * blockIdx.x] = make_int4(ct * 16, r.columns, parts.first, parts.last);
       a.cuts[2 * blockIdx.x + 1] = make_int4(r.len, r.nq, r.q0, 0);
     }
 #pragma unroll 1

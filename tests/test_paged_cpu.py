@@ -3,6 +3,12 @@ launch, and the plain implementations that the GPU tests hold it to."""
 
 from __future__ import annotations
 
+import ctypes
+import os
+import random
+import shutil
+import subprocess
+
 import pytest
 import torch
 
@@ -178,3 +184,87 @@ def test_paged_latent_cache_shapes_and_refusals():
                      (dict(n_pages=2 ** 26), "int32")]:
         with pytest.raises(ValueError, match=text):
             PagedLatentCache(**{**dict(n_layers=1, requests=2, max_len=10, n_pages=3, page_size=32, device="cpu"), **kw})
+
+
+# --------------------------------------------------------------------------- the attention's line of items
+ITEM_COST, WGS = 32, 256
+
+
+@pytest.fixture(scope="module")
+def line(tmp_path_factory):
+    """csrc/paged_line.h, the arithmetic that the attention kernel cuts items with, in a host library."""
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        pytest.skip("no host compiler")
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(P.__file__))), "csrc")
+    where = tmp_path_factory.mktemp("line")
+    src, lib = where / "line.cpp", where / "line.so"
+    src.write_text('#include "paged_line.h"\n'
+                   'extern "C" int cut_at(int t, int tiles) { return paged::cut_at(t, tiles); }\n'
+                   'extern "C" void parts_of(int s, int n, int per, int wgs, int* out) {\n'
+                   '  const paged::Parts p = paged::parts_of(s, n, per, wgs);\n'
+                   '  out[0] = p.first;\n'
+                   '  out[1] = p.last;\n'
+                   '}\n')
+    subprocess.run([cxx, "-std=c++17", "-O1", "-shared", "-fPIC", "-I", csrc, str(src), "-o", str(lib)], check=True)
+    return ctypes.CDLL(str(lib))
+
+
+def _parts(line, start, tiles, per, wgs):
+    out = (ctypes.c_int * 2)()
+    line.parts_of(start, tiles, per, wgs, out)
+    return out[0], out[1]
+
+
+def _grid(items, per):
+    return min(WGS, max(1, sum(n + ITEM_COST for n in items)) // 16 + 1)
+
+
+def _random_items(rng):
+    return [rng.choice([rng.randint(1, 12), rng.randint(1, 40), rng.randint(1, 600), rng.randint(1, 12000)])
+            for _ in range(rng.choice([1, 2, 7, 40, 300]))]
+
+
+def test_every_tile_of_every_item_goes_to_one_piece_and_the_merge_knows_them(line):
+    rng = random.Random(5)
+    for _ in range(150):
+        items = _random_items(rng)
+        total = sum(n + ITEM_COST for n in items)
+        per = max(-(-total // WGS), 16)
+        wgs = _grid(items, per)
+        start = 0
+        for tiles in items:
+            pieces = []
+            for w in range(start // per, min(wgs, (start + tiles + ITEM_COST) // per + 1)):
+                lo, hi = min(w * per, total), min((w + 1) * per, total)
+                first, last = line.cut_at(lo - start, tiles), line.cut_at(hi - start, tiles)
+                if first < last:
+                    pieces.append((w, first, last))
+            assert [p[1] for p in pieces] == [0] + [p[2] for p in pieces[:-1]] and pieces[-1][2] == tiles
+            if len(pieces) > 1:
+                assert min(p[2] - p[1] for p in pieces) >= 8
+                assert [p[0] for p in pieces] == list(range(pieces[0][0], pieces[-1][0] + 1))
+                assert _parts(line, start, tiles, per, wgs) == (pieces[0][0], pieces[-1][0])
+            start += tiles + ITEM_COST
+
+
+def test_an_item_that_grew_after_the_line_was_summed_is_joined_of_existing_parts(line):
+    """A length that another stream changes while the attention runs may be read twice: the item's end then lies
+    past the line, by a request's whole room at most."""
+    rng = random.Random(6)
+    found = 0
+    for _ in range(3000):
+        items = _random_items(rng)
+        total = sum(n + ITEM_COST for n in items)
+        per = max(-(-total // WGS), 16)
+        wgs = _grid(items, per)
+        w = rng.randrange(wgs)
+        lo, hi = min(w * per, total), min((w + 1) * per, total)
+        start = rng.randint(max(0, lo - rng.choice([20, 500, 100000])), lo)
+        tiles = rng.choice([rng.randint(1, 100), rng.randint(1, 10 ** 6)])
+        first, last = line.cut_at(lo - start, tiles), line.cut_at(hi - start, tiles)
+        if lo < hi and 0 < first < last:  # this workgroup tells the merge of the item
+            p0, p1 = _parts(line, start, tiles, per, wgs)
+            assert 0 <= p0 < w <= p1 < wgs, (items, start, tiles, w)
+            found += 1
+    assert found > 500
