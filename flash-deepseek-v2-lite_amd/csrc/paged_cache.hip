@@ -447,3 +447,11 @@ extern "C" int dsv2_paged_read_fp4(const void* pages, int64_t page_stride, int n
                        status);
   return dsv2_launch_status("paged_read_fp4");
 }
+
+__global__ void paged_take_status_kernel(int32_t* bits, int32_t* status) { *bits = atomicExch(status, 0); }
+
+extern "C" int dsv2_paged_take_status(int32_t* bits, int32_t* status, void* stream) {
+  DSV2_REQUIRE(bits && status, DSV2_E_NULL, "paged_take_status: null pointer");
+  hipLaunchKernelGGL(paged_take_status_kernel, dim3(1), dim3(1), 0, (hipStream_t)stream, bits, status);
+  return dsv2_launch_status("paged_take_status");
+}

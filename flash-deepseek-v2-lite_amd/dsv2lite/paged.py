@@ -42,34 +42,35 @@ class PagedLatentCache:
         self.state = torch.zeros(requests + 2, dtype=torch.int32, device=device)
         self.state[-1] = n_pages
         self.lens = self.state[:requests]
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)  # what this cache's calls had to skip
 
     def step(self, delta: torch.Tensor, max_tokens: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """Change every request's length by ``delta`` (int32 [requests]; negative: tokens dropped from its end, at
         most all, which ends it) and give the new tokens, requests in order, their (slots, positions, rows), -1
         behind the last one.  A request that does not fit keeps its length (``check_status``)."""
         after, slots, positions, rows = ops.paged_cache_step(self.state, delta, self.block_table, self.free_pages,
-                                                             self.page_size, max_tokens)
+                                                             self.page_size, max_tokens, self.status)
         self.state.copy_(after)
         return slots, positions, rows
 
     def slots_of(self, starts: torch.Tensor, counts: torch.Tensor, max_tokens: int) -> tuple[torch.Tensor, ...]:
         """(slots, positions, rows) of the cached tokens [starts[b], starts[b] + counts[b]) of every request."""
-        return ops.paged_slot_map(starts, counts, self.block_table, self.page_size, max_tokens)
+        return ops.paged_slot_map(starts, counts, self.block_table, self.page_size, max_tokens, self.status)
 
     def write(self, layer: int, rows: torch.Tensor, slots: torch.Tensor) -> None:
         """Round cache rows [n, 576] (normalised latent | rotated key) into a layer's slots."""
-        ops.paged_cache_write_fp4(rows, slots, self.pages[layer])
+        ops.paged_cache_write_fp4(rows, slots, self.pages[layer], self.status)
 
     def read(self, layer: int, slots: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """The bf16 rows [n, 576] that a layer's slots hold."""
-        return ops.paged_cache_read_fp4(self.pages[layer], slots, out)
+        return ops.paged_cache_read_fp4(self.pages[layer], slots, out, self.status)
 
     def attend(self, layer: int, q: torch.Tensor, softmax_scale: float, cu_q: torch.Tensor | None = None,
                max_q: int = 1, out: torch.Tensor | None = None) -> torch.Tensor:
         """Latent attention outputs [tokens, heads, 512] of absorbed queries [tokens, heads, 576] over a layer: one
         query token per request, or ``cu_q``'s, the requests' last cached tokens."""
         return ops.attention_decode_paged_fp4(q, self.pages[layer], self.block_table, self.lens, softmax_scale, cu_q,
-                                              max_q, out)
+                                              max_q, out, self.status)
 
     def snapshot(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """Lengths, block table and free pages; the tokens themselves stay where they are, so a snapshot holds until
@@ -85,5 +86,5 @@ class PagedLatentCache:
         return int(self.state[-1].item()) * self.page_size
 
     def check_status(self) -> None:
-        """Raise if a call on this device skipped tokens since the last check (synchronises)."""
-        ops.check_paged_status(self.state.device)
+        """Raise if a call of this cache skipped tokens since the last check (waits for the device)."""
+        ops.check_paged_status(status=self.status)

@@ -91,6 +91,7 @@ _SIGS = {
     "dsv2_paged_slots": ([_p, _p, _i32, _p, _i64, _i32, _i32, _i32, _p, _p, _p, _p, _p], _i32),
     "dsv2_paged_write_fp4": ([_p, _i64, _i32, _p, _p, _i64, _i32, _i32, _p, _p], _i32),
     "dsv2_paged_read_fp4": ([_p, _i64, _i32, _i32, _p, _i32, _p, _i64, _p, _p], _i32),
+    "dsv2_paged_take_status": ([_p, _p, _p], _i32),
     "dsv2_mla_paged_workspace_size": ([], _i64),
     "dsv2_mla_decode_paged_fp4": ([_p, _i64, _i64, _i32, _i32, _p, _i64, _i32, _i32, _p, _i64, _i32, _p, _i32, _p,
                                    _i32, _f32, _p, _i64, _i64, _p, _i64, _p, _p], _i32),

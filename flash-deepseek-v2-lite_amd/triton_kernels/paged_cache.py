@@ -12,7 +12,9 @@ Slot ``p * page_size + i`` names token i of page p.  Token t of request b lies i
 ``block_table[b, t // page_size]``; one table serves all layers.
 
 Errors that only the device can see (no free page, a full block table, a slot outside the pool)
-skip what they concern and are reported by ``check_paged_status``.
+skip what they concern and are reported by ``check_paged_status``.  They are kept in ``status``, an int32
+[1] tensor of zeros on the same GPU that callers who share it pass to each call; without one the calls of
+a device share a word of the module's, whose first use has to be outside graph capture.
 """
 
 from __future__ import annotations
@@ -33,7 +35,7 @@ MAX_TOKENS = 2 ** 31 - 1
 _BF16, _I32, _U8 = torch.bfloat16, torch.int32, torch.uint8
 _PAGE_SIZES = frozenset(1 << i for i in range(11))
 _ENTRY = {n: getattr(_hip.lib, n) for n in ("dsv2_paged_step", "dsv2_paged_slots", "dsv2_paged_write_fp4",
-                                            "dsv2_paged_read_fp4", "dsv2_mla_decode_paged_fp4")}
+                                            "dsv2_paged_read_fp4", "dsv2_mla_decode_paged_fp4", "dsv2_paged_take_status")}
 _WORKSPACE = _hip.lib.dsv2_mla_paged_workspace_size()  # bytes
 _STATUS: dict = {}  # device index -> (int32 [1] status word of the functions below, its address)
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
@@ -47,32 +49,52 @@ def _status(index: int) -> tuple[torch.Tensor, int]:
     return _STATUS.setdefault(index, (st, st.data_ptr()))
 
 
-def check_paged_status(device: torch.device | str = "cuda") -> None:
-    """Raise if a call on `device` since the last check skipped something (waits for all its streams)."""
-    index = torch.device(device).index
-    index = torch.cuda.current_device() if index is None else index
-    known = _STATUS.get(index)
-    if known is None:
-        return
-    torch.cuda.synchronize(index)  # calls on any stream
-    bits = int(known[0].item())
+def check_paged_status(device: torch.device | str = "cuda", status: torch.Tensor | None = None) -> None:
+    """Raise if a call with this ``status`` (without one: a call on `device` without one) has skipped something since
+    the last check.  Waits for all streams of the device, on any of which such a call may be."""
+    name = "check_paged_status"
+    if status is None:
+        index = torch.device(device).index
+        index = torch.cuda.current_device() if index is None else index
+        known = _STATUS.get(index)
+        if known is None:
+            return
+        status = known[0]
+    index = _device(name, status)
+    at = _word(name, status, index)
+    torch.cuda.synchronize(index)
+    # read and cleared at once: what another thread's call finds meanwhile is left for the next check
+    taken = torch.empty_like(status)
+    _call(index, "dsv2_paged_take_status", taken.data_ptr(), at)
+    bits = int(taken.item())
     if not bits:
         return
-    known[0].zero_()
-    torch.cuda.synchronize(index)  # before a later call on another stream sets one
     what = [text for bit, text in ((1, "a request outgrew its block table"), (2, "no free page was left"),
                                    (4, "a slot, page or position lay outside the pool or block table"),
                                    (8, "there were more new tokens than max_tokens or max_q")) if bits & bit]
     raise RuntimeError("paged cache: " + "; ".join(what) + "; those tokens were skipped")
 
 
+def _word(name: str, status: torch.Tensor | None, index: int) -> int | None:
+    """The address of a call's own status word."""
+    if status is None:
+        return None
+    if status.dtype is not _I32 or status.numel() != 1:
+        raise ValueError(f"{name}: status must be int32 [1], not {status.dtype} {list(status.shape)}")
+    if status.get_device() != index:
+        raise ValueError(f"{name}: status on {status.device}")
+    return status.data_ptr()
+
+
 def _call(index: int, entry: str, *args) -> None:
-    """The entry point on the device's current stream, with the device as the current one."""
+    """The entry point on the device's current stream, with the device as the current one; the last argument is the
+    call's status word or None."""
     if _current_device() != index:
         with torch.cuda.device(index):
             return _call(index, entry, *args)
-    known = _STATUS.get(index) or _status(index)
-    rc = _ENTRY[entry](*args, known[1], _hip._raw_stream(index))
+    if args[-1] is None:
+        args = (*args[:-1], (_STATUS.get(index) or _status(index))[1])
+    rc = _ENTRY[entry](*args, _hip._raw_stream(index))
     if rc:
         raise _hip.HipKernelError(f"{entry} failed (status {rc}): "
                                   f"{_hip.lib.dsv2_last_error_message().decode(errors='replace')}")
@@ -137,7 +159,7 @@ def _page_size(name: str, page_size: int) -> None:
 
 
 def paged_cache_step(state: torch.Tensor, delta: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
-                     page_size: int, max_tokens: int) -> tuple[torch.Tensor, ...]:
+                     page_size: int, max_tokens: int, status: torch.Tensor | None = None) -> tuple[torch.Tensor, ...]:
     """One step of the requests' lengths; returns (state after the step, slots, positions, rows).
 
     ``state`` int32 [B + 2]: the B lengths, then head and count of the ring ``free_pages`` (int32
@@ -166,12 +188,14 @@ def paged_cache_step(state: torch.Tensor, delta: torch.Tensor, block_table: torc
         at = outs.data_ptr()
         maps, size = at + 4 * n + 8, 4 * max_tokens
         _call(index, "dsv2_paged_step", state.data_ptr(), delta.data_ptr(), n, block_table.data_ptr(), ts, width,
-              free_pages.data_ptr(), pages, page_size, max_tokens, at, maps, maps + size, maps + 2 * size)
+              free_pages.data_ptr(), pages, page_size, max_tokens, at, maps, maps + size, maps + 2 * size,
+              _word(name, status, index))
     return torch.unsafe_split_with_sizes(outs, (n + 2, max_tokens, max_tokens, max_tokens))
 
 
 def paged_slot_map(starts: torch.Tensor, counts: torch.Tensor, block_table: torch.Tensor, page_size: int,
-                   max_tokens: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                   max_tokens: int,
+                   status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(slots, positions, rows) of the tokens [starts[b], starts[b] + counts[b]) of every request, one
     after the other, int32 [max_tokens]; -1 from the last one on, and for positions or pages out of
     range."""
@@ -189,7 +213,7 @@ def paged_slot_map(starts: torch.Tensor, counts: torch.Tensor, block_table: torc
     else:
         at, size = maps.data_ptr(), 4 * max_tokens
         _call(index, "dsv2_paged_slots", starts.data_ptr(), counts.data_ptr(), n, block_table.data_ptr(), ts, width,
-              page_size, max_tokens, at, at + size, at + 2 * size)
+              page_size, max_tokens, at, at + size, at + 2 * size, _word(name, status, index))
     return torch.unsafe_split_with_sizes(maps, (max_tokens, max_tokens, max_tokens))
 
 
@@ -205,7 +229,8 @@ def _cache_rows(name: str, what: str, rows: torch.Tensor, n: int) -> int:
     return rs if n > 1 else ROW
 
 
-def paged_cache_write_fp4(rows: torch.Tensor, slots: torch.Tensor, pages: torch.Tensor) -> None:
+def paged_cache_write_fp4(rows: torch.Tensor, slots: torch.Tensor, pages: torch.Tensor,
+                          status: torch.Tensor | None = None) -> None:
     """Round cache rows (bf16 [n, 576]: normalised latent | rotated key, a row stride that is a
     multiple of 8, or 0 for one row) into ``slots`` (int32 [n]) of ``pages``; a row with a negative slot is left out.
     Rows with the same slot have to be the same: of different ones a mixture may stay."""
@@ -216,10 +241,11 @@ def paged_cache_write_fp4(rows: torch.Tensor, slots: torch.Tensor, pages: torch.
     page_stride, n_pages, page_size = _pool(name, pages)
     if n:
         _call(index, "dsv2_paged_write_fp4", rows.data_ptr(), rs, n, slots.data_ptr(), pages.data_ptr(), page_stride,
-              n_pages, page_size)
+              n_pages, page_size, _word(name, status, index))
 
 
-def paged_cache_read_fp4(pages: torch.Tensor, slots: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+def paged_cache_read_fp4(pages: torch.Tensor, slots: torch.Tensor, out: torch.Tensor | None = None,
+                         status: torch.Tensor | None = None) -> torch.Tensor:
     """The bf16 rows [n, 576] that ``slots`` (int32 [n]) hold, exactly; zeros for a negative slot."""
     name = "paged_cache_read_fp4"
     index = _device(name, pages, slots)
@@ -232,13 +258,14 @@ def paged_cache_read_fp4(pages: torch.Tensor, slots: torch.Tensor, out: torch.Te
         os = _cache_rows(name, "out", out, n)
     if n:
         _call(index, "dsv2_paged_read_fp4", pages.data_ptr(), page_stride, n_pages, page_size, slots.data_ptr(), n,
-              out.data_ptr(), os)
+              out.data_ptr(), os, _word(name, status, index))
     return out
 
 
 def attention_decode_paged_fp4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
                                softmax_scale: float, cu_q: torch.Tensor | None = None, max_q: int = 1,
-                               out: torch.Tensor | None = None) -> torch.Tensor:
+                               out: torch.Tensor | None = None,
+                               status: torch.Tensor | None = None) -> torch.Tensor:
     """Absorbed-MLA attention over the pages: q [T, H, 576] bf16 (q_nope W_UK | rotated q_pe) -> the
     latent outputs [T, H, 512] bf16 that W_UV takes, fp32 softmax over each request's ``lens[b]``
     cached tokens.
@@ -299,5 +326,5 @@ def attention_decode_paged_fp4(q: torch.Tensor, pages: torch.Tensor, block_table
     ws = pages.new_empty(_WORKSPACE)
     _call(index, "dsv2_mla_decode_paged_fp4", q.data_ptr(), q_ts, q_hs, t, h, pages.data_ptr(), page_stride, n_pages,
           page_size, block_table.data_ptr(), ts, width, lens.data_ptr(), n, cu, max_q, softmax_scale, out.data_ptr(),
-          o_ts, o_hs, ws.data_ptr(), _WORKSPACE)
+          o_ts, o_hs, ws.data_ptr(), _WORKSPACE, _word(name, status, index))
     return out

@@ -537,6 +537,10 @@ int dsv2_paged_write_fp4(const void* rows, int64_t row_stride, int n, const int3
 int dsv2_paged_read_fp4(const void* pages, int64_t page_stride, int n_pages, int page_size, const int32_t* slots,
                         int n, void* out, int64_t out_stride, int32_t* status, void* stream);
 
+/* bits = the status word, which is cleared in the same step: bits that a call on another stream sets
+ * meanwhile are in `bits` or left for the next time. */
+int dsv2_paged_take_status(int32_t* bits, int32_t* status, void* stream);
+
 /* Absorbed-MLA attention of the queries q [tokens, heads, 576] (strides q_ts, q_hs; absorbed latent |
  * rotated rotary part) over the requests' cached tokens: out[t, h, :512] = sum_s p_s latent_s, p = softmax
  * of softmax_scale * q[t, h] . row_s, softmax_scale in (0, 1e30].  Request b owns the query tokens [cu_q[b], cu_q[b + 1]), at most

@@ -770,3 +770,39 @@ def test_paged_latent_cache_snapshot_and_overflow():
     assert cache.lens.tolist() == [0, 32, 16]
     with pytest.raises(RuntimeError, match="outgrew its block table; no free page"):
         cache.check_status()
+
+
+def test_a_cache_reports_its_own_errors_only():
+    """Two caches of one device: the one that lost tokens says so, whoever is asked first, and the functions' common
+    word stays clear."""
+    from dsv2lite import PagedLatentCache
+
+    good, full = (PagedLatentCache(1, 2, max_len=64, n_pages=3, page_size=16) for _ in range(2))
+    slots, _, _ = good.step(i32([20, 1]), 21)
+    full.step(i32([64, 1]), 65)  # a page too many
+    good.write(0, rnd(21, R.ROW), slots)
+    good.check_status()
+    P.check_paged_status()
+    with pytest.raises(RuntimeError, match="no free page"):
+        full.check_status()
+    full.check_status()
+    full.read(0, i32([48]))
+    good.check_status()
+    with pytest.raises(RuntimeError, match="outside the pool"):
+        full.check_status()
+
+
+@pytest.mark.parametrize("name", ["step", "slots", "write", "read", "attention"])
+def test_each_function_reports_to_the_word_that_it_is_given(name):
+    pages, st = pool(3, 16, fill=0), i32([0])
+    {"step": lambda: P.paged_cache_step(i32([16, 0, 3]), i32([1]), i32([[0]]), i32([1, 2, 0]), 16, 1, status=st),
+     "slots": lambda: P.paged_slot_map(i32([15]), i32([2]), i32([[0]]), 16, 2, status=st),
+     "write": lambda: P.paged_cache_write_fp4(rnd(1, R.ROW), i32([48]), pages, status=st),
+     "read": lambda: P.paged_cache_read_fp4(pages, i32([48]), status=st),
+     "attention": lambda: P.attention_decode_paged_fp4(rnd(1, 16, R.ROW), pages, i32([[3]]), i32([5]), SCALE,
+                                                       status=st)}[name]()
+    P.check_paged_status()
+    with pytest.raises(RuntimeError, match="outgrew" if name == "step" else "outside the pool"):
+        P.check_paged_status(status=st)
+    P.check_paged_status(status=st)
+    assert st.tolist() == [0]

@@ -108,6 +108,26 @@ def test_functions_refuse_other_shapes_types_and_strides(monkeypatch, name, at, 
     assert len(calls) == 1
 
 
+@pytest.mark.parametrize("name", sorted(good()))
+def test_functions_refuse_a_status_word_of_another_type_shape_or_device(monkeypatch, name):
+    monkeypatch.setattr(P, "_device", lambda *a: -1)  # what get_device() says of a CPU tensor
+    calls = []
+    monkeypatch.setattr(P, "_call", lambda index, entry, *args: calls.append(args[-1]))
+    word = i32(1)
+    getattr(P, name)(*good()[name], status=word)
+    getattr(P, name)(*good()[name])
+    assert calls == [word.data_ptr(), None]
+    for bad in (i32(2), i32(0), i32(1).long()):
+        with pytest.raises(ValueError, match="status must be int32"):
+            getattr(P, name)(*good()[name], status=bad)
+    monkeypatch.setattr(P, "_device", lambda *a: 0)
+    with pytest.raises(ValueError, match="status on cpu"):
+        getattr(P, name)(*good()[name], status=word)
+    with pytest.raises(ValueError, match="status on cpu"):
+        P.check_paged_status(status=word)
+    assert len(calls) == 2
+
+
 def test_entry_points_refuse_bad_arguments_without_launching():
     one, odd = 1 << 20, (1 << 20) + 8  # never read: every call below is refused on the host
 
@@ -132,6 +152,9 @@ def test_entry_points_refuse_bad_arguments_without_launching():
     read = [one, 6400, 6, 16, one, 5, one, 576]
     for at, value, match in [(4, None, "null"), (5, -1, "bad shape"), (6, odd, "alignment"), (7, 575, "bad shape")]:
         refused(match, "dsv2_paged_read_fp4", *read[:at], value, *read[at + 1:])
+    for args in ((None, one), (one, None)):
+        with pytest.raises(_hip.HipKernelError, match="paged_take_status: null"):
+            _hip.call("dsv2_paged_take_status", *args, None)
     size = _hip.lib.dsv2_mla_paged_workspace_size()
     attn = [one, 9216, 576, 7, 16, one, 6400, 6, 16, one, 3, 3, one, 4, one, 2, 0.1, one, 8192, 512, one, size]
     for at, value, match in [(0, None, "null"), (0, odd, "alignment"), (1, 9220, "alignment"), (3, -1, "bad shape"),
