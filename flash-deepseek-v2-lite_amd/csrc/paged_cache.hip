@@ -21,11 +21,11 @@ int paged_check_pool(const char* what, const void* pages, int64_t page_stride, i
 namespace {
 constexpr int kMaxRequests = 4096;  // four int32 arrays of the requests in LDS
 constexpr int kManyRequests = 512;
-// sums of counts stay within int32: they stick at its largest value, past every size that is compared
-__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return min(a + b, 0x7fffffffu); }
+// sums of counts stick at the largest uint32, past every int32 that they are compared with
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
 
 // first index of ends[0, n) (ascending) that is past i; i < ends[n - 1]
-__device__ __forceinline__ int owner(const int32_t* ends, int n, int i) {
+__device__ __forceinline__ int owner(const uint32_t* ends, int n, uint32_t i) {
   int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
@@ -58,7 +58,7 @@ __device__ __forceinline__ void block_scan(const uint32_t* v, uint32_t* before, 
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     if (kWaves > 4) {
-      const int waves = wave_scan(lane < kWaves ? red[lane * K + k] : 0, sat);
+      const int waves = wave_scan(lane < kWaves ? red[lane * K + k] : 0u, sat);
       total[k] = __builtin_amdgcn_readlane(waves, kWaves - 1);
       if (w) before[k] = add_sat(before[k], __builtin_amdgcn_readlane(waves, w - 1));
     } else {
@@ -110,13 +110,13 @@ template <bool STEP, int kThreads>
 __global__ __launch_bounds__(kThreads) void paged_plan_kernel(const PlanArgs a) {
   constexpr int K = STEP ? 3 : 1;
   constexpr uint32_t kTaken = 0x80000000u;
-  extern __shared__ int32_t sums[];
+  extern __shared__ uint32_t sums[];
   __shared__ uint32_t red[kThreads / 64 * K];
   __shared__ int32_t taken_sum;
-  int32_t* tok_end = sums;              // tokens of requests [0, b]
-  int32_t* page_end = sums + a.n;       // STEP: pages they need
-  int32_t* back_end = sums + 2 * a.n;   // STEP: pages they give back
-  uint32_t* meta = reinterpret_cast<uint32_t*>(sums + 3 * a.n);  // STEP: old length; kTaken: the new tokens fit
+  uint32_t* tok_end = sums;             // tokens of requests [0, b]
+  uint32_t* page_end = sums + a.n;      // STEP: pages they need
+  uint32_t* back_end = sums + 2 * a.n;  // STEP: pages they give back
+  uint32_t* meta = sums + 3 * a.n;      // STEP: old length; kTaken: the new tokens fit
   const int tid = threadIdx.x;
   const int ps = 1 << a.shift;
   const int64_t room = static_cast<int64_t>(a.width) << a.shift;
@@ -132,6 +132,7 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(const PlanArgs a) 
   const int per = (a.n + kThreads - 1) / kThreads;
   const int b0 = min(tid * per, a.n), b1 = min(b0 + per, a.n);
   uint32_t run[K] = {};
+  int taken = 0, errors = 0;
   for (int b = b0; b < b1; ++b) {
     const int d = a.delta[b];
     run[0] = add_sat(run[0], max(d, 0));
@@ -140,6 +141,7 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(const PlanArgs a) 
       const int64_t len = min(max(static_cast<int64_t>(a.lens[b]), static_cast<int64_t>(0)), room);
       const int64_t want = len + d;
       const bool fits = d > 0 && want <= room;
+      if (d > 0 && !fits) errors |= DSV2_DEVERR_CACHE_FULL;
       if (fits) run[1] = add_sat(run[1], pages_of(want) - pages_of(len));
       if (d < 0) run[K - 1] = add_sat(run[K - 1], pages_of(len) - pages_of(max(want, static_cast<int64_t>(0))));
       page_end[b] = run[1 % K];
@@ -149,7 +151,6 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(const PlanArgs a) 
   }
   uint32_t before[K], total[K];
   block_scan<K, kThreads / 64>(run, before, total, red);
-  int taken = 0, errors = 0;
   uint32_t tok_last = 0, page_last = 0;
   for (int b = b0; b < b1; ++b) {
     const uint32_t t = tok_end[b], t_end = add_sat(before[0], t);
@@ -165,9 +166,7 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(const PlanArgs a) 
       const bool fits = m & kTaken;
       const bool ok = fits && t_end <= static_cast<uint32_t>(a.tokens) && (need == 0 || p_end <= static_cast<uint32_t>(count));
       if (ok) taken += need;
-      if (grows && !ok)
-        errors |= !fits ? DSV2_DEVERR_CACHE_FULL
-                        : (t_end > static_cast<uint32_t>(a.tokens) ? DSV2_DEVERR_TOKENS : DSV2_DEVERR_NO_PAGE);
+      if (fits && !ok) errors |= t_end > static_cast<uint32_t>(a.tokens) ? DSV2_DEVERR_TOKENS : DSV2_DEVERR_NO_PAGE;
       const int len = m & ~kTaken;
       meta[b] = ok ? m : len;
       if (blockIdx.x == 0) {

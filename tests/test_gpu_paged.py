@@ -260,6 +260,36 @@ def test_step_refuses_what_does_not_fit_request_by_request():
         P.check_paged_status()
 
 
+def test_step_and_slot_map_of_the_most_tokens_a_call_may_have():
+    """max_tokens of 2^31 - 1, and requests that ask for more together: the later one is refused."""
+    most = 2 ** 31 - 1
+    table, free = i32([[0, 0], [0, 0], [0, 0]]), i32([2, 1, 0])
+    after, slots, _, _ = P.paged_cache_step(i32([0, 0, 0, 0, 3]), i32([3, most, 2]), table, free, 16, most)
+    assert after.tolist() == [3, 0, 0, 1, 2] and slots[:3].tolist() == [32, 33, 34] and int(slots[3:].max()) == -1
+    with pytest.raises(RuntimeError, match="outgrew its block table; there were more new tokens"):
+        P.check_paged_status()
+    del slots
+    torch.cuda.empty_cache()
+    slots, _, rows = P.paged_slot_map(i32([0, 0, 1]), i32([1, most, most]), table, 16, most)
+    assert slots[:33].tolist() == [32] + [i % 16 for i in range(32)] and int(slots[33:].max()) == -1
+    assert rows[:34].tolist() == [0] + [1] * 32 + [-1]
+    with pytest.raises(RuntimeError, match="outside the pool or block table; there were more new tokens"):
+        P.check_paged_status()
+    del slots, rows
+    torch.cuda.empty_cache()
+
+
+def test_step_reports_every_reason_when_its_sums_are_full():
+    """A request that passes the table with the largest delta, one behind it (of the same thread's) past max_tokens."""
+    n = 300
+    delta = [0] * n
+    delta[0], delta[1] = 2 ** 31 - 1, 1
+    after, slots, _, _ = P.paged_cache_step(i32([0] * n + [0, 2]), i32(delta), i32([[0]] * n), i32([0, 1]), 16, 50)
+    assert after.tolist() == [0] * n + [0, 2] and slots.tolist() == [-1] * 50
+    with pytest.raises(RuntimeError, match="outgrew its block table; there were more new tokens"):
+        P.check_paged_status()
+
+
 def test_step_with_corrupt_state_stays_in_bounds():
     """A ring position, a count or a length out of range, a page number that is none: nothing outside
     the tensors is touched, the slots are -1 and the status says so."""
