@@ -422,9 +422,16 @@ extern "C" int dsv2_paged_write_fp4(const void* rows, int64_t row_stride, int n,
   DSV2_REQUIRE(rows && slots, DSV2_E_NULL, "paged_write_fp4: null pointer");
   DSV2_REQUIRE(dsv2_aligned16(rows) && row_stride % 8 == 0, DSV2_E_ALIGN, "paged_write_fp4: rows alignment");
   const int shift = page_shift(page_size);
-  hipLaunchKernelGGL(paged_write_kernel, dim3((n - 1) / 4 + 1), dim3(256), 0, (hipStream_t)stream, (const bf16_t*)rows,
-                     row_stride, n, slots, (uint8_t*)pages, page_stride, n_pages << shift, shift, status);
-  return dsv2_launch_status("paged_write_fp4");
+  // a launch has fewer than 2^32 threads, 64 for a row
+  constexpr int kMost = 1 << 25;
+  for (int64_t first = 0; first < n; first += kMost) {
+    const int some = n - first < kMost ? static_cast<int>(n - first) : kMost;
+    hipLaunchKernelGGL(paged_write_kernel, dim3((some - 1) / 4 + 1), dim3(256), 0, (hipStream_t)stream,
+                       (const bf16_t*)rows + first * row_stride, row_stride, some, slots + first, (uint8_t*)pages,
+                       page_stride, n_pages << shift, shift, status);
+    if (const int rc = dsv2_launch_status("paged_write_fp4")) return rc;
+  }
+  return DSV2_OK;
 }
 
 extern "C" int dsv2_paged_read_fp4(const void* pages, int64_t page_stride, int n_pages, int page_size,

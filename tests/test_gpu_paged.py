@@ -155,6 +155,19 @@ def test_the_same_row_written_to_one_slot_many_times():
     assert torch.equal(pages, want)
 
 
+def test_more_rows_than_a_launch_has_threads_for():
+    """2^26 + 1 slots of one row: the first, some around each 2^25 and the last are slots of the pool."""
+    n, pages = 2 ** 26 + 1, pool(2, 16, fill=9)
+    at = [0, 2 ** 25 - 1, 2 ** 25, 2 ** 25 + 1, 2 ** 26 - 1, 2 ** 26]
+    slots = torch.full((n,), -1, dtype=torch.int32, device=DEV)
+    slots[at] = i32([3, 0, 31, 16, 7, 20])
+    row = rnd(1, R.ROW)
+    P.paged_cache_write_fp4(row.expand(n, R.ROW), slots, pages)
+    want = pool(2, 16, fill=9)
+    P.paged_cache_write_fp4(row.expand(6, R.ROW), slots[at], want)
+    assert torch.equal(pages, want)
+
+
 def test_slots_outside_the_pool_are_skipped_and_reported():
     pages = pool(4, 16, fill=1)
     before = pages.clone()
