@@ -262,6 +262,18 @@ def paged_cache_read_fp4(pages: torch.Tensor, slots: torch.Tensor, out: torch.Te
     return out
 
 
+def _rows_apart(t: int, ts: int, h: int, hs: int) -> bool:
+    """No two of the t * h rows of 512 values, ts and hs apart, have a value in common."""
+    if h <= 1 or t <= 1:
+        return (h <= 1 or hs >= LAT) and (t <= 1 or ts >= LAT)
+    if min(ts, hs) < LAT:
+        return False
+    if ts >= (h - 1) * hs + LAT or hs >= (t - 1) * ts + LAT:  # one within the other
+        return True
+    # else the tokens next to every head's offset
+    return all(abs(j * hs - i * ts) >= LAT for j in range(1, h) for i in (j * hs // ts, j * hs // ts + 1) if i < t)
+
+
 def attention_decode_paged_fp4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
                                softmax_scale: float, cu_q: torch.Tensor | None = None, max_q: int = 1,
                                out: torch.Tensor | None = None,
@@ -315,7 +327,7 @@ def attention_decode_paged_fp4(q: torch.Tensor, pages: torch.Tensor, block_table
         if out.shape != (t, h, LAT):
             raise ValueError(f"{name}: out must be [{t}, {h}, {LAT}], not {list(out.shape)}")
         o_ts, o_hs, o_ds = out.stride()
-        if o_ds != 1 or h > 1 and o_hs < LAT or t > 1 and o_ts < LAT:
+        if o_ds != 1 or not _rows_apart(t, o_ts, h, o_hs):
             raise NotImplementedError(f"{name}: out's rows must be contiguous and apart")
         if t == 1:
             o_ts = 0

@@ -108,6 +108,28 @@ def test_functions_refuse_other_shapes_types_and_strides(monkeypatch, name, at, 
     assert len(calls) == 1
 
 
+@pytest.mark.parametrize("t,h", [(1, 1), (1, 5), (5, 1), (2, 2), (3, 4), (4, 3)])
+def test_attention_refuses_outputs_whose_rows_overlap(monkeypatch, t, h):
+    """Every pair of strides from a set, against all rows laid out."""
+    monkeypatch.setattr(P, "_device", lambda *a: 0)
+    calls = []
+    monkeypatch.setattr(P, "_call", lambda index, entry, *args: calls.append(entry))
+    q, pages, lens = torch.zeros(t, h, 576, dtype=BF), torch.zeros(6, 6400, dtype=torch.uint8), i32(t)
+    strides = [8, 504, 512, 520, 768, 1016, 1024, 1032, 1536, 2048, 2552, 4096]
+    for ts in strides:
+        for hs in strides:
+            at = sorted(i * ts + j * hs for i in range(t) for j in range(h))
+            apart = all(y - x >= 512 for x, y in zip(at, at[1:]))
+            out = torch.zeros(at[-1] + 512, dtype=BF).as_strided((t, h, 512), (ts, hs, 1))
+            del calls[:]
+            if apart:
+                P.attention_decode_paged_fp4(q, pages, i32(t, 3), lens, 0.1, out=out)
+            else:
+                with pytest.raises(NotImplementedError, match="rows must be contiguous and apart"):
+                    P.attention_decode_paged_fp4(q, pages, i32(t, 3), lens, 0.1, out=out)
+            assert len(calls) == apart, (ts, hs)
+
+
 @pytest.mark.parametrize("name", sorted(good()))
 def test_functions_refuse_a_status_word_of_another_type_shape_or_device(monkeypatch, name):
     monkeypatch.setattr(P, "_device", lambda *a: -1)  # what get_device() says of a CPU tensor
