@@ -9,9 +9,13 @@ functions are in ``triton_kernels.paged_cache``; this class keeps their tensors 
 A serving step, which may be captured in a graph (``delta`` and the rows then keep their tensors):
 
     slots, positions, rows = cache.step(delta, max_tokens)     # lengths, pages, where the tokens go
+    cu_q = cache.query_starts(delta)                           # which of them are whose
     for each layer:
         cache.write(layer, new_rows, slots)                    # [max_tokens, 576], as dsv2_mla_prepare writes them
-        latent = cache.attend(layer, q, softmax_scale)         # [requests, heads, 512], what W_UV takes
+        latent = cache.attend(layer, q, softmax_scale, cu_q, max_q)  # [max_tokens, heads, 512], what W_UV takes
+
+``new_rows`` and ``q`` are the new tokens', in the order of ``slots``: one request after the other, none of a
+request whose length does not grow.
 
 The reference keeps one expanded bf16 tensor of fixed length instead (src/run.py:81-99)."""
 
@@ -53,6 +57,14 @@ class PagedLatentCache:
         self.state.copy_(after)
         return slots, positions, rows
 
+    @staticmethod
+    def query_starts(delta: torch.Tensor) -> torch.Tensor:
+        """``attend``'s cu_q (int32 [requests + 1]) for a query of each new token of a step: request b's are
+        cu_q[b] .. cu_q[b + 1], at most max(delta) many.  One that the step refused keeps its places; what comes out
+        there means nothing, as rows[i] = -1 tells."""
+        ends = delta.clamp(min=0).cumsum(0).clamp(max=2 ** 31 - 1)  # the sums in 64 bits
+        return torch.cat([ends.new_zeros(1), ends]).int()
+
     def slots_of(self, starts: torch.Tensor, counts: torch.Tensor, max_tokens: int) -> tuple[torch.Tensor, ...]:
         """(slots, positions, rows) of the cached tokens [starts[b], starts[b] + counts[b]) of every request."""
         return ops.paged_slot_map(starts, counts, self.block_table, self.page_size, max_tokens, self.status)
@@ -67,8 +79,9 @@ class PagedLatentCache:
 
     def attend(self, layer: int, q: torch.Tensor, softmax_scale: float, cu_q: torch.Tensor | None = None,
                max_q: int = 1, out: torch.Tensor | None = None) -> torch.Tensor:
-        """Latent attention outputs [tokens, heads, 512] of absorbed queries [tokens, heads, 576] over a layer: one
-        query token per request, or ``cu_q``'s, the requests' last cached tokens."""
+        """Latent attention outputs [tokens, heads, 512] of absorbed queries [tokens, heads, 576] over a layer: the
+        requests' last cached tokens, ``cu_q[b]`` .. ``cu_q[b + 1]`` of them request b's (``query_starts``), or without
+        it row b for request b, idle requests included.  Rows past ``cu_q[-1]`` are not written."""
         return ops.attention_decode_paged_fp4(q, self.pages[layer], self.block_table, self.lens, softmax_scale, cu_q,
                                               max_q, out, self.status)
 

@@ -815,6 +815,73 @@ def test_paged_latent_cache_snapshot_and_overflow():
         cache.check_status()
 
 
+def test_queries_of_a_step_with_idle_requests_eager_and_captured():
+    """The new tokens' queries stand without gaps, whoever is idle, ends or is refused between them: every replay
+    of a captured step gives each the attention over its own request."""
+    from dsv2lite import PagedLatentCache
+
+    B, most, max_q, ps = 5, 9, 4, 16
+    cache = PagedLatentCache(1, B, max_len=96, n_pages=16, page_size=ps)
+    slots, _, _ = cache.step(i32([30, 0, 17, 60, 1]), 108)
+    first = rnd(108, R.ROW, seed=1)
+    cache.write(0, first, slots)
+    keys = list(R.held(first).split([30, 0, 17, 60, 1]))
+    delta, new, q = i32([0] * B), rnd(most, R.ROW, seed=2), rnd(most, 16, R.ROW, seed=3, std=0.3)
+    out = torch.zeros(most, 16, 512, dtype=BF, device=DEV)
+
+    def step():
+        slots, _, rows = cache.step(delta, most)
+        cache.write(0, new, slots)
+        cache.attend(0, q, SCALE, cache.query_starts(delta), max_q, out)
+        return rows
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rows = step()
+    deltas = [[1, 0, 1, 0, 1], [0, 0, 4, 1, 0], [1, 2, -18, 1, 3], [-31, 1, 0, 0, 1], [0, 1, 2, 4, 1], [4, 0, -4, 0, 4],
+              [1, 0, 0, 4, 1], [0, 0, 0, 0, 0], [1, 1, 1, 1, 1]]
+    for k, d in enumerate(deltas):
+        delta.copy_(i32(d))
+        new.copy_(rnd(most, R.ROW, seed=10 + k))
+        q.copy_(rnd(most, 16, R.ROW, seed=30 + k, std=0.3))
+        out.fill_(7.0)
+        if k == 3:
+            rows_now = step()  # an eager one among the replays
+        else:
+            graph.replay()
+            rows_now = rows
+        held, at = R.held(new), 0
+        for b in range(B):
+            keys[b] = torch.cat([keys[b], held[at:at + d[b]]]) if d[b] > 0 else keys[b][:max(0, len(keys[b]) + d[b])]
+            for j in range(max(d[b], 0)):
+                assert int(rows_now[at]) == b
+                want, tol = R.attention(q[at], keys[b], len(keys[b]) - d[b] + j + 1, SCALE)
+                assert ((out[at].double() - want).abs() <= tol).all(), (k, b, j)
+                at += 1
+        assert int((out[at:] != 7).sum()) == 0 and cache.lens.tolist() == [len(x) for x in keys]
+        cache.check_status()
+    # one that outgrows its room keeps its places among the others'
+    full, others = 96 - len(keys[3]) + 1, [1, 1, 0, 0, 1]
+    delta.copy_(i32(others[:3] + [full] + others[4:]))
+    big = rnd(full + 3, 16, R.ROW, seed=60, std=0.3)
+    x = rnd(full + 3, R.ROW, seed=61)
+    slots, _, rows_now = cache.step(delta, full + 3)
+    cache.write(0, x, slots)
+    got = cache.attend(0, big, SCALE, cache.query_starts(delta), full)
+    assert rows_now.tolist() == [0, 1] + [-1] * full + [4]
+    for at, b in ((0, 0), (1, 1), (full + 2, 4)):
+        keys[b] = torch.cat([keys[b], R.held(x[at:at + 1])])
+        want, tol = R.attention(big[at], keys[b], len(keys[b]), SCALE)
+        assert ((got[at].double() - want).abs() <= tol).all(), b
+    with pytest.raises(RuntimeError, match="outgrew"):
+        cache.check_status()
+
+
 def test_a_cache_reports_its_own_errors_only():
     """Two caches of one device: the one that lost tokens says so, whoever is asked first, and the functions' common
     word stays clear."""

@@ -174,9 +174,6 @@ def test_entry_points_refuse_bad_arguments_without_launching():
     read = [one, 6400, 6, 16, one, 5, one, 576]
     for at, value, match in [(4, None, "null"), (5, -1, "bad shape"), (6, odd, "alignment"), (7, 575, "bad shape")]:
         refused(match, "dsv2_paged_read_fp4", *read[:at], value, *read[at + 1:])
-    for args in ((None, one), (one, None)):
-        with pytest.raises(_hip.HipKernelError, match="paged_take_status: null"):
-            _hip.call("dsv2_paged_take_status", *args, None)
     size = _hip.lib.dsv2_mla_paged_workspace_size()
     attn = [one, 9216, 576, 7, 16, one, 6400, 6, 16, one, 3, 3, one, 4, one, 2, 0.1, one, 8192, 512, one, size]
     for at, value, match in [(0, None, "null"), (0, odd, "alignment"), (1, 9220, "alignment"), (3, -1, "bad shape"),
@@ -187,6 +184,12 @@ def test_entry_points_refuse_bad_arguments_without_launching():
                              (16, float("nan"), "softmax_scale"), (18, 8196, "alignment"),
                              (20, None, "workspace"), (20, odd, "workspace"), (21, size - 1, "workspace")]:
         refused(match, "dsv2_mla_decode_paged_fp4", *attn[:at], value, *attn[at + 1:])
+
+
+def test_take_status_refuses_null_pointers():
+    for args in ((None, 1 << 20), (1 << 20, None)):
+        with pytest.raises(_hip.HipKernelError, match="paged_take_status: null"):
+            _hip.call("dsv2_paged_take_status", *args, None)
 
 
 def test_the_plain_block_format():
@@ -229,6 +232,16 @@ def test_paged_latent_cache_shapes_and_refusals():
                      (dict(n_pages=2 ** 26), "int32")]:
         with pytest.raises(ValueError, match=text):
             PagedLatentCache(**{**dict(n_layers=1, requests=2, max_len=10, n_pages=3, page_size=32, device="cpu"), **kw})
+
+
+def test_query_starts_of_idle_shrinking_and_huge_steps():
+    from dsv2lite import PagedLatentCache
+
+    most = 2 ** 31 - 1
+    starts = PagedLatentCache.query_starts(torch.tensor([2, 0, -7, 3, 1], dtype=torch.int32))
+    assert starts.tolist() == [0, 2, 2, 2, 5, 6] and starts.dtype == torch.int32
+    starts = PagedLatentCache.query_starts(torch.tensor([1, most, 0, most, 5], dtype=torch.int32))
+    assert starts.tolist() == [0, 1] + [most] * 4
 
 
 # --------------------------------------------------------------------------- the attention's line of items
