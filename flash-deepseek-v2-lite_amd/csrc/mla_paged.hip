@@ -47,6 +47,10 @@ constexpr int kMinStretch = 2 * kPiece;
 // A piece takes what some 32 more tiles would, 20,000 cycles (MI355X, 128 x 256..8,192 tokens, both launches: 62.8 us
 // with 16, 60.2 with 24, 60.5 with 32, 61.7 with 40; 12 x 1,440..24,485 26.8 / 26.0 / 25.9 / 26.2)
 constexpr int kItemCost = 32;
+// The host refuses calls whose line would pass this (a request's columns, and all requests' by the query tokens that
+// there are).  Ranges of cu_q that overlap could still add up to more: sums stop here, and no index follows from more
+constexpr int kMostPlaces = 1 << 30;
+__device__ __forceinline__ int add_places(int a, int b) { return min(a + b, kMostPlaces); }
 constexpr int kPartFloats = 16 * kLat;
 // Up to 128 requests one wave sums the line; more are shared by the workgroup (MI355X, one request, to the first item,
 // each wave summing for itself: 1,850 cycles where the workgroup takes 3,400; with room for 256 requests 2,480, for 64
@@ -68,7 +72,6 @@ struct PagedAttnArgs {
   const int32_t* cu_q;
   int max_q;
   int requests;
-  int columns16;  // most column groups of a request
   float scale_log2;
   bf16_t* out;
   int64_t o_ts, o_hs;
@@ -197,7 +200,7 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
           const bool is = 64 * k + lane < a.requests;
           nothing |= is && seen(u[k]);
           run[k] = is ? u[k].places() : 0;
-          scan[k] = wave_scan(run[k]) + total;
+          scan[k] = add_places(wave_scan(run[k], add_places), total);
           total = __builtin_amdgcn_readlane(scan[k], 63);
         }
         stretch(total);
@@ -222,16 +225,16 @@ __global__ __launch_bounds__(kThreads, 2) void mla_paged_kernel(const PagedAttnA
       for (int i = b0; i < b1; ++i) {
         r = request(a, i);
         nothing |= seen(r);
-        run += r.places();
+        run = add_places(run, r.places());
       }
-      const int scan = wave_scan(run);
+      const int scan = wave_scan(run, add_places);
       if (lane == 63) wave_sums[wv] = scan;
       if (__syncthreads_or(nothing)) clear();
       int before = scan - run, total = 0;
 #pragma unroll
       for (int i = 0; i < kWaves; ++i) {
-        if (i < wv) before += wave_sums[i];
-        total += wave_sums[i];
+        if (i < wv) before = add_places(before, wave_sums[i]);
+        total = add_places(total, wave_sums[i]);
       }
       stretch(uniform(total));
       if (before <= lo && lo < before + run) {
@@ -693,12 +696,15 @@ extern "C" int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_
                DSV2_E_ALIGN, "mla_decode_paged_fp4: alignment");
   if (tokens == 0 || requests == 0) return DSV2_OK;
   if (!cu_q) max_q = 1;
-  const int groups = (max_q * heads + 15) / 16, shift = page_shift(page_size);
-  const int64_t items = static_cast<int64_t>(requests) * groups;
+  // column groups of a request and of all: no more than the query tokens have, one a request rounded up
+  const int groups = ((max_q < tokens ? max_q : tokens) * heads + 15) / 16, shift = page_shift(page_size);
+  const int64_t by_request = static_cast<int64_t>(requests) * groups;
+  const int64_t by_token = static_cast<int64_t>(tokens) * heads / 16 + requests;
+  const int64_t items = by_request < by_token ? by_request : by_token;
   const int64_t room = static_cast<int64_t>(table_width) << shift;
-  DSV2_REQUIRE(room <= INT32_MAX - kTile && items <= INT32_MAX / 2 / ((room + kTile - 1) / kTile + kItemCost), DSV2_E_SHAPE,
-               "mla_decode_paged_fp4: %d requests of up to %lld tokens, %d column groups each", requests, (long long)room,
-               groups);
+  DSV2_REQUIRE(room <= INT32_MAX - kTile && items <= kMostPlaces / ((room + kTile - 1) / kTile + kItemCost), DSV2_E_SHAPE,
+               "mla_decode_paged_fp4: %lld groups of 16 (query token, head) pairs over up to %lld tokens each",
+               (long long)items, (long long)room);
   DSV2_REQUIRE(workspace && dsv2_aligned16(workspace) &&
                    workspace_bytes >= dsv2_mla_paged_workspace_size(),
                DSV2_E_SHAPE, "mla_decode_paged_fp4: workspace of %lld bytes", (long long)workspace_bytes);
@@ -708,8 +714,8 @@ extern "C" int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_
   const PagedAttnArgs a{(const bf16_t*)q, q_ts, q_hs, tokens, heads,
                         heads == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + heads - 1) / heads),
                         (const uint8_t*)pages, page_stride, n_pages, shift, block_table, table_stride,
-                        table_width, lens, cu_q, max_q, requests, groups, softmax_scale * 1.4426950408889634f, (bf16_t*)out, out_ts, out_hs, part_o, part_ml, cuts,
-                        status};
+                        table_width, lens, cu_q, max_q, requests, softmax_scale * 1.4426950408889634f, (bf16_t*)out, out_ts,
+                        out_hs, part_o, part_ml, cuts, status};
   const int64_t tiles = (room + kTile - 1) / kTile, most = items * (tiles + kItemCost);
   const int wgs = static_cast<int>(most / kMinStretch + 1 < kWgs ? most / kMinStretch + 1 : kWgs);
   constexpr int kLds = kWaves * kWaveLds + kQLds;

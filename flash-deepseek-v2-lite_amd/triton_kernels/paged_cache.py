@@ -286,7 +286,8 @@ def attention_decode_paged_fp4(q: torch.Tensor, pages: torch.Tensor, block_table
     b owns query tokens cu_q[b] .. cu_q[b + 1], at most ``max_q`` of them, and they are its last
     cached tokens: the last one sees all, each one before it a token less.  A query that sees nothing
     gives zeros; query tokens past cu_q[B] are not written (in a fresh ``out`` they are undefined).
-    Up to 128 heads; q and out may have any token and head strides that are multiples of 8."""
+    Up to 128 heads; q and out may have any token and head strides that are multiples of 8 (out's rows apart).
+    Up to 65,535 requests and ``max_q``; (T * H / 16 + B) * (table width * page size / 16 + 32) up to 2^30."""
     name = "attention_decode_paged_fp4"
     index = _device(name, q, pages, block_table, lens)
     if q.dtype is not _BF16:

@@ -546,7 +546,9 @@ int dsv2_paged_take_status(int32_t* bits, int32_t* status, void* stream);
  * of softmax_scale * q[t, h] . row_s, softmax_scale in (0, 1e30].  Request b owns the query tokens [cu_q[b], cu_q[b + 1]), at most
  * max_q of them (cu_q NULL: token b); they are its last cached ones: query j of n sees the tokens below
  * lens[b] - n + j + 1.  A query that sees nothing gives zeros; query tokens of no request are left alone.
- * The rows of out must not overlap.
+ * The rows of out must not overlap.  requests and max_q up to 65,535; the groups of 16 (query token, head)
+ * pairs that there may be (requests * ceil(max_q * heads / 16), at most tokens * heads / 16 + requests) times
+ * (the table's room in tokens / 16 + 32) up to 2^30.
  * Table entries that name no page stand for tokens of zeros (and set DSV2_DEVERR_BAD_SLOT); a request with
  * more than max_q query tokens has the first max_q done (and sets DSV2_DEVERR_TOKENS).
  * workspace: dsv2_mla_paged_workspace_size bytes, 16-byte aligned, not shared by calls that may overlap. */

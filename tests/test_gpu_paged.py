@@ -410,6 +410,28 @@ def test_attention_numbers_of_requests(requests, drafts):
     check(rnd(sum(nq) if drafts else requests, 4, R.ROW, seed=requests, std=0.3), pages, table, lens, keys, nq)
 
 
+def test_attention_of_a_chunk_among_many_requests_with_wide_tables():
+    """A prompt's chunk beside decoding rows: 250 requests with room for 163,840 tokens each, 600 queries at most,
+    700 of them in all."""
+    B, width, ps = 250, 2560, 64
+    lens = [(37 * b) % 90 if b % 3 else 0 for b in range(B)]
+    nq = [1 if n else 0 for n in lens]
+    lens[100], nq[100] = 900, 533
+    pages, table, keys = batch(lens, ps, seed=3)
+    wide = torch.full((B, width), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    q = rnd(sum(nq), 16, R.ROW, seed=9, std=0.3)
+    cu = i32([sum(nq[:b]) for b in range(B + 1)])
+    got = P.attention_decode_paged_fp4(q, pages, wide, i32(lens), SCALE, cu, 600)
+    t = 0
+    for b, n in enumerate(nq):
+        for j in range(n):
+            if n == 1 or j % 41 == 0 or j == n - 1:
+                want, tol = R.attention(q[t], keys[b], lens[b] - n + j + 1, SCALE)
+                assert ((got[t].double() - want).abs() <= tol).all(), (b, j)
+            t += 1
+
+
 @pytest.mark.parametrize("std", [0.0, 3.0, 30.0])
 def test_attention_flat_and_sharp(std):
     """Equal scores, and scores whose softmax has one token left; a scale of its own."""

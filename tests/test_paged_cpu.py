@@ -186,6 +186,20 @@ def test_entry_points_refuse_bad_arguments_without_launching():
         refused(match, "dsv2_mla_decode_paged_fp4", *attn[:at], value, *attn[at + 1:])
 
 
+def test_attention_refuses_more_work_than_its_line_holds():
+    one, size = 1 << 20, _hip.lib.dsv2_mla_paged_workspace_size()
+
+    def refused(tokens, heads, requests, width, max_q):
+        with pytest.raises(_hip.HipKernelError, match="groups of 16"):
+            _hip.call("dsv2_mla_decode_paged_fp4", one, heads * 576, 576, tokens, heads, one, 6400, 6, 16, one, width,
+                      width, one, requests, one, max_q, 0.1, one, heads * 512, 512, one, size, None, None)
+
+    refused(65535, 128, 65535, 10000, 65535)
+    refused(2 ** 20, 128, 1, 10000, 65535)     # one request's columns
+    refused(2 ** 20, 16, 65535, 1000, 3000)    # all query tokens'
+    refused(1, 1, 1, 2 ** 27 - 1, 1)           # a table past int32 tokens
+
+
 def test_take_status_refuses_null_pointers():
     for args in ((None, 1 << 20), (1 << 20, None)):
         with pytest.raises(_hip.HipKernelError, match="paged_take_status: null"):
