@@ -28,7 +28,8 @@ from triton_kernels import paged_cache as ops
 
 class PagedLatentCache:
     def __init__(self, n_layers: int, requests: int, max_len: int, n_pages: int, page_size: int = 64, device="cuda"):
-        """Room for ``requests`` requests of up to ``max_len`` tokens, ``n_pages * page_size`` tokens in all."""
+        """Room for ``requests`` requests of up to ``max_len`` tokens (whole pages: the next multiple of
+        ``page_size``), ``n_pages * page_size`` tokens in all."""
         if min(n_layers, requests, max_len, n_pages) <= 0:
             raise ValueError("n_layers, requests, max_len and n_pages must be positive")
         if requests > ops.MAX_REQUESTS:
@@ -51,7 +52,8 @@ class PagedLatentCache:
     def step(self, delta: torch.Tensor, max_tokens: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """Change every request's length by ``delta`` (int32 [requests]; negative: tokens dropped from its end, at
         most all, which ends it) and give the new tokens, requests in order, their (slots, positions, rows), -1
-        behind the last one.  A request that does not fit keeps its length (``check_status``)."""
+        behind the last one.  A request that does not fit keeps its length (``check_status``), and those behind it
+        that need what it asked for are refused with it."""
         after, slots, positions, rows = ops.paged_cache_step(self.state, delta, self.block_table, self.free_pages,
                                                              self.page_size, max_tokens, self.status)
         self.state.copy_(after)

@@ -12,9 +12,11 @@ Slot ``p * page_size + i`` names token i of page p.  Token t of request b lies i
 ``block_table[b, t // page_size]``; one table serves all layers.
 
 Errors that only the device can see (no free page, a full block table, a slot outside the pool)
-skip what they concern and are reported by ``check_paged_status``.  They are kept in ``status``, an int32
-[1] tensor of zeros on the same GPU that callers who share it pass to each call; without one the calls of
-a device share a word of the module's, whose first use has to be outside graph capture.
+skip what they concern and are reported by ``check_paged_status``; attention takes table entries that
+name no page for tokens of zeros.  Lengths are held to what the table has room for, a negative one to
+zero, without a report.  Errors are kept in ``status``, an int32 [1] tensor of zeros on the same GPU
+that the callers who share it pass to each call; without one the calls of a device share a word of the
+module's, whose first use has to be outside graph capture.
 """
 
 from __future__ import annotations
@@ -170,8 +172,10 @@ def paged_cache_step(state: torch.Tensor, delta: torch.Tensor, block_table: torc
     on); both tensors change in place, in places that the step does not read, so the call repeated
     on the same ``state`` does the same.  New token i, requests in order, has slots[i],
     positions[i] and rows[i] (its request); entries from the last new token to ``max_tokens`` are
-    -1.  A request whose tokens do not fit the table, ``max_tokens`` or the free pages that the
-    requests before it leave keeps its length; its tokens get -1 and check_paged_status raises."""
+    -1.  A request whose tokens do not fit the table, ``max_tokens`` or the free pages keeps its
+    length; its tokens get -1 and check_paged_status raises.  Both are counted in the requests' order, what
+    was refused with the rest: behind a request refused for tokens all that grow are refused, behind one
+    refused for pages all that need a page.  One that would outgrow the table counts its tokens, no pages."""
     name = "paged_cache_step"
     index = _device(name, state, delta, block_table, free_pages)
     n = _int32(name, "delta", delta)
@@ -284,8 +288,11 @@ def attention_decode_paged_fp4(q: torch.Tensor, pages: torch.Tensor, block_table
 
     Without ``cu_q`` query token b belongs to request b.  With it (int32 [B + 1], ascending) request
     b owns query tokens cu_q[b] .. cu_q[b + 1], at most ``max_q`` of them, and they are its last
-    cached tokens: the last one sees all, each one before it a token less.  A query that sees nothing
+    cached tokens: the last one sees all, each one before it a token less.  Where ``cu_q``'s tokens are a
+    step's new ones, a request that does not grow has none, so rows are not the requests' numbers
+    (``dsv2lite.PagedLatentCache.query_starts`` forms it).  A query that sees nothing
     gives zeros; query tokens past cu_q[B] are not written (in a fresh ``out`` they are undefined).
+    Sums are fp32 with weights up to 2^8, so latents past some 2^100 may overflow to infinity.
     Up to 128 heads; q and out may have any token and head strides that are multiples of 8 (out's rows apart).
     Up to 65,535 requests and ``max_q``; (T * H / 16 + B) * (table width * page size / 16 + 32) up to 2^30."""
     name = "attention_decode_paged_fp4"

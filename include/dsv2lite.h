@@ -513,7 +513,10 @@ int dsv2_moe_combine_parts(const void* ysorted, const int32_t* route_pos, const 
  * gives the same.  New token i (requests in order, each one's tokens in order) gets slots[i],
  * positions[i] and rows[i] = its request, i < max_tokens; entries past the last new token are -1.
  * A request whose tokens do not fit the table's width, max_tokens or (a page needed) the free pages
- * left by all requests before it keeps its length, its tokens get -1 and a DSV2_DEVERR_* bit is set.
+ * keeps its length, its tokens get -1 and a DSV2_DEVERR_* bit is set.  Tokens and pages are counted in the
+ * requests' order, those of refused requests with the rest (past the table's width: its tokens, no
+ * pages), so behind one refused for tokens all that grow are refused, behind one refused for pages all that
+ * need a page.  A length outside the table's room counts as the nearest one inside.
  * requests <= 4096. */
 int dsv2_paged_step(const int32_t* state, const int32_t* delta, int requests, int32_t* block_table,
                     int64_t table_stride, int table_width, int32_t* free_pages, int n_pages, int page_size,
@@ -546,7 +549,8 @@ int dsv2_paged_take_status(int32_t* bits, int32_t* status, void* stream);
  * of softmax_scale * q[t, h] . row_s, softmax_scale in (0, 1e30].  Request b owns the query tokens [cu_q[b], cu_q[b + 1]), at most
  * max_q of them (cu_q NULL: token b); they are its last cached ones: query j of n sees the tokens below
  * lens[b] - n + j + 1.  A query that sees nothing gives zeros; query tokens of no request are left alone.
- * The rows of out must not overlap.  requests and max_q up to 65,535; the groups of 16 (query token, head)
+ * A length past the table's room counts as that room (and so for what its queries see), a negative one as 0.
+ * The rows of out must not overlap.  Sums are fp32, weights up to 2^8.  requests and max_q up to 65,535; the groups of 16 (query token, head)
  * pairs that there may be (requests * ceil(max_q * heads / 16), at most tokens * heads / 16 + requests) times
  * (the table's room in tokens / 16 + 32) up to 2^30.
  * Table entries that name no page stand for tokens of zeros (and set DSV2_DEVERR_BAD_SLOT); a request with
