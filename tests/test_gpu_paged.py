@@ -155,6 +155,25 @@ def test_the_same_row_written_to_one_slot_many_times():
     assert torch.equal(pages, want)
 
 
+@pytest.mark.parametrize("n", [8191, 8192, 8193, 8207, 20000])
+def test_reads_of_many_rows(n):
+    """Rows by the fours and their remainders, slots of no row and past the pool among them, into a wider matrix."""
+    ps, n_pages = 32, 700
+    pages = pool(n_pages, ps)
+    g = torch.Generator(device=DEV).manual_seed(n)
+    slots = torch.randint(0, n_pages * ps, (n,), device=DEV, generator=g).int()
+    slots[::97] = -1 - slots[::97]
+    slots[[0, 5, 4098, n - 2]] = i32([n_pages * ps, 2 ** 31 - 1, n_pages * ps + 7, n_pages * ps])
+    out = torch.full((n + 1, 600), 5.0, dtype=BF, device=DEV)
+    got = P.paged_cache_read_fp4(pages, slots, out=out[:n, 8:8 + R.ROW])
+    live = (slots >= 0) & (slots < n_pages * ps)
+    want = torch.where(live[:, None], R.stored(pages, slots.clamp(0, n_pages * ps - 1), ps), 0.0)
+    assert torch.equal(got.double(), want)
+    assert int((out[:, :8] != 5).sum()) + int((out[:, 8 + R.ROW:] != 5).sum()) + int((out[n] != 5).sum()) == 0
+    with pytest.raises(RuntimeError, match="outside the pool"):
+        P.check_paged_status()
+
+
 def test_more_rows_than_a_launch_has_threads_for():
     """2^26 + 1 slots of one row: the first, some around each 2^25 and the last are slots of the pool."""
     n, pages = 2 ** 26 + 1, pool(2, 16, fill=9)
@@ -430,6 +449,66 @@ def test_attention_of_a_chunk_among_many_requests_with_wide_tables():
                 want, tol = R.attention(q[t], keys[b], lens[b] - n + j + 1, SCALE)
                 assert ((got[t].double() - want).abs() <= tol).all(), (b, j)
             t += 1
+
+
+def _numbered(b, n):
+    """Rows whose every 16 tokens have a value in a latent channel of their own (shared by each 512th such tile, the
+    values taking turns), and rotary keys that spell the token's number in +-1, each bit three times."""
+    t = torch.arange(n, device=DEV)
+    x = torch.zeros(n, R.ROW, device=DEV)
+    tile = t // 16
+    x[t, tile % 512] = torch.tensor(R.VALUES[1:], device=DEV)[(tile // 512 + tile + b) % 7]
+    bits = (t[:, None] >> torch.arange(20, device=DEV)) & 1
+    x[:, 512:572] = (2.0 * bits - 1).repeat(1, 3)
+    return x.to(BF)
+
+
+CUT = [([4000, 2500, 7003], [9, 3, 5], 8), ([4000, 2500, 7003], [9, 3, 5], 17), ([1999, 8000], [7, 4], 40),
+       ([20000], None, 16), ([9000, 10, 15001], None, 16), ([150001], None, 16), ([70003], [3], 16),
+       ([300, 6000, 40], [1, 200, 1], 16), ([2048] * 60, None, 16), ([700] * 600, None, 16)]
+
+
+@pytest.mark.parametrize("lens,nq,heads", CUT)
+def test_attention_counts_every_tile_once(lens, nq, heads):
+    """All scores equal: an output channel is the sum of its tiles' values over the tokens seen, and one tile more or
+    less shows.  Items of one and of many column groups, cut into up to 256 pieces."""
+    pages, table, keys = batch(lens, 64, seed=len(lens), fill=_numbered)
+    T = sum(nq) if nq else len(lens)
+    cu = i32([sum(nq[:b]) for b in range(len(lens) + 1)]) if nq else None
+    got = P.attention_decode_paged_fp4(torch.zeros(T, heads, R.ROW, dtype=BF, device=DEV), pages, table, i32(lens),
+                                       SCALE, cu, max(nq) if nq else 1)
+    t = 0
+    for b, n in enumerate(nq or [1] * len(lens)):
+        for j in range(n):
+            seen = lens[b] - n + j + 1
+            want = keys[b][:seen, :512].sum(0) / seen
+            # weights of exactly 1, sums of halves below 2^23: the division's rounding and the output's
+            off = (got[t].double() - want).abs()
+            assert (off <= (2.0 ** -8 + 2.0 ** -20) * want).all(), (b, j, float((off / want.clamp(min=1e-9)).max()))
+            t += 1
+
+
+@pytest.mark.parametrize("lens,nq,heads", CUT)
+def test_attention_finds_one_token_each(lens, nq, heads):
+    """Every (query token, head) asks for one token, by its number: its output is that token's latent, whichever
+    piece, column group and request it is in."""
+    rng = random.Random(heads)
+    pages, table, keys = batch(lens, 64, seed=len(lens), fill=lambda b, n: torch.cat(
+        [rnd(n, 512, seed=b), _numbered(b, n)[:, 512:]], 1))
+    at, want = [], []
+    for b, n in enumerate(nq or [1] * len(lens)):
+        for j in range(n):
+            seen = lens[b] - n + j + 1
+            pick = [rng.choice([rng.randrange(seen), 16 * rng.randrange(-(-seen // 16)), seen - 1]) for _ in range(heads)]
+            at.append(pick)
+            want.append(keys[b][pick, :512])
+    q = torch.zeros(len(at), heads, R.ROW, device=DEV)
+    bits = (torch.tensor(at, device=DEV)[..., None] >> torch.arange(20, device=DEV)) & 1
+    # a token of another number scores at least 2 * 3 * 128 * SCALE = 88 less
+    q[..., 512:572] = 128 * (2.0 * bits - 1).repeat(1, 1, 3)
+    cu = i32([sum(nq[:b]) for b in range(len(lens) + 1)]) if nq else None
+    got = P.attention_decode_paged_fp4(q.to(BF), pages, table, i32(lens), SCALE, cu, max(nq) if nq else 1)
+    assert torch.equal(got.double(), torch.stack(want))
 
 
 @pytest.mark.parametrize("std", [0.0, 3.0, 30.0])
