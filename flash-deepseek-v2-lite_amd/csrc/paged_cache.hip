@@ -87,6 +87,7 @@ struct PlanArgs {
   int32_t* slots;
   int32_t* positions;
   int32_t* rows;
+  int32_t* cu_q;  // STEP: the requests' first new tokens, or null
   int32_t* status;
 };
 }  // namespace
@@ -171,6 +172,7 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(const PlanArgs a) 
       meta[b] = ok ? m : len;
       if (blockIdx.x == 0) {
         const int d = a.delta[b];
+        if (a.cu_q) a.cu_q[b + 1] = static_cast<int>(min(t_end, 0x7fffffffu));
         a.state_out[b] = d < 0 ? static_cast<int>(max(static_cast<int64_t>(len) + d, static_cast<int64_t>(0))) : (ok ? len + d : len);
       }
     } else if (t_end > static_cast<uint32_t>(a.tokens) && grows) {
@@ -187,6 +189,7 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(const PlanArgs a) 
   const int given = STEP ? static_cast<int>(min(total[K - 1], static_cast<uint32_t>(a.pages - count))) : 0;
   if (blockIdx.x == 0) {
     if (STEP && tid == 0) {
+      if (a.cu_q) a.cu_q[0] = 0;
       const int64_t h = static_cast<int64_t>(head) + used;
       a.state_out[a.n] = static_cast<int>(h >= a.pages ? h - a.pages : h);
       a.state_out[a.n + 1] = count - used + given;
@@ -292,6 +295,15 @@ extern "C" int dsv2_paged_step(const int32_t* state, const int32_t* delta, int r
                                int64_t table_stride, int table_width, int32_t* free_pages, int n_pages, int page_size,
                                int max_tokens, int32_t* state_out, int32_t* slots, int32_t* positions, int32_t* rows,
                                int32_t* status, void* stream) {
+  return dsv2_paged_step_queries(state, delta, requests, block_table, table_stride, table_width, free_pages, n_pages,
+                                 page_size, max_tokens, state_out, slots, positions, rows, nullptr, status, stream);
+}
+
+extern "C" int dsv2_paged_step_queries(const int32_t* state, const int32_t* delta, int requests, int32_t* block_table,
+                                       int64_t table_stride, int table_width, int32_t* free_pages, int n_pages,
+                                       int page_size, int max_tokens, int32_t* state_out, int32_t* slots,
+                                       int32_t* positions, int32_t* rows, int32_t* cu_q, int32_t* status,
+                                       void* stream) {
   DSV2_REQUIRE(state && delta && block_table && free_pages && state_out && (max_tokens == 0 || (slots && positions && rows)),
                DSV2_E_NULL, "paged_step: null pointer");
   const int shift = page_shift(page_size);
@@ -300,7 +312,7 @@ extern "C" int dsv2_paged_step(const int32_t* state, const int32_t* delta, int r
   DSV2_REQUIRE(state_out + requests + 2 <= state || state + requests + 2 <= state_out, DSV2_E_SHAPE,
                "paged_step: state_out overlaps state");
   const PlanArgs a{state, delta, requests, block_table, table_stride, table_width, free_pages, n_pages,
-                   shift, max_tokens, state_out, slots, positions, rows, status};
+                   shift, max_tokens, state_out, slots, positions, rows, cu_q, status};
   return plan_launch("paged_step", true, a, page_size, stream);
 }
 
@@ -310,7 +322,7 @@ extern "C" int dsv2_paged_slots(const int32_t* starts, const int32_t* counts, in
   DSV2_REQUIRE(starts && counts && block_table && (max_tokens == 0 || (slots && positions && rows)), DSV2_E_NULL,
                "paged_slots: null pointer");
   const PlanArgs a{starts, counts, requests, const_cast<int32_t*>(block_table), table_stride, table_width, nullptr, 0,
-                   page_shift(page_size), max_tokens, nullptr, slots, positions, rows, status};
+                   page_shift(page_size), max_tokens, nullptr, slots, positions, rows, nullptr, status};
   return plan_launch("paged_slots", false, a, page_size, stream);
 }
 

@@ -9,13 +9,12 @@ functions are in ``triton_kernels.paged_cache``; this class keeps their tensors 
 A serving step, which may be captured in a graph (``delta`` and the rows then keep their tensors):
 
     slots, positions, rows = cache.step(delta, max_tokens)     # lengths, pages, where the tokens go
-    cu_q = cache.query_starts(delta)                           # which of them are whose
     for each layer:
         cache.write(layer, new_rows, slots)                    # [max_tokens, 576], as dsv2_mla_prepare writes them
-        latent = cache.attend(layer, q, softmax_scale, cu_q, max_q)  # [max_tokens, heads, 512], what W_UV takes
+        latent = cache.attend(layer, q, softmax_scale, cache.cu_q, max_q)  # [max_tokens, heads, 512], what W_UV takes
 
 ``new_rows`` and ``q`` are the new tokens', in the order of ``slots``: one request after the other, none of a
-request whose length does not grow.
+request whose length does not grow; ``cache.cu_q`` says which are whose.
 
 The reference keeps one expanded bf16 tensor of fixed length instead (src/run.py:81-99)."""
 
@@ -47,6 +46,10 @@ class PagedLatentCache:
         self.state = torch.zeros(requests + 2, dtype=torch.int32, device=device)
         self.state[-1] = n_pages
         self.lens = self.state[:requests]
+        # attend's cu_q for a query of each new token of the last step: request b's are cu_q[b] .. cu_q[b + 1], at
+        # most max(delta) many.  One that the step refused keeps its places; what comes out there means nothing, as
+        # rows[i] = -1 tells
+        self.cu_q = torch.zeros(requests + 1, dtype=torch.int32, device=device)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)  # what this cache's calls had to skip
 
     def step(self, delta: torch.Tensor, max_tokens: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -55,17 +58,9 @@ class PagedLatentCache:
         behind the last one.  A request that does not fit keeps its length (``check_status``), and those behind it
         that need what it asked for are refused with it."""
         after, slots, positions, rows = ops.paged_cache_step(self.state, delta, self.block_table, self.free_pages,
-                                                             self.page_size, max_tokens, self.status)
+                                                             self.page_size, max_tokens, self.status, self.cu_q)
         self.state.copy_(after)
         return slots, positions, rows
-
-    @staticmethod
-    def query_starts(delta: torch.Tensor) -> torch.Tensor:
-        """``attend``'s cu_q (int32 [requests + 1]) for a query of each new token of a step: request b's are
-        cu_q[b] .. cu_q[b + 1], at most max(delta) many.  One that the step refused keeps its places; what comes out
-        there means nothing, as rows[i] = -1 tells."""
-        ends = delta.clamp(min=0).cumsum(0).clamp(max=2 ** 31 - 1)  # the sums in 64 bits
-        return torch.cat([ends.new_zeros(1), ends]).int()
 
     def slots_of(self, starts: torch.Tensor, counts: torch.Tensor, max_tokens: int) -> tuple[torch.Tensor, ...]:
         """(slots, positions, rows) of the cached tokens [starts[b], starts[b] + counts[b]) of every request."""
@@ -82,7 +77,7 @@ class PagedLatentCache:
     def attend(self, layer: int, q: torch.Tensor, softmax_scale: float, cu_q: torch.Tensor | None = None,
                max_q: int = 1, out: torch.Tensor | None = None) -> torch.Tensor:
         """Latent attention outputs [tokens, heads, 512] of absorbed queries [tokens, heads, 576] over a layer: the
-        requests' last cached tokens, ``cu_q[b]`` .. ``cu_q[b + 1]`` of them request b's (``query_starts``), or without
+        requests' last cached tokens, ``cu_q[b]`` .. ``cu_q[b + 1]`` of them request b's (``self.cu_q`` after a step), or without
         it row b for request b, idle requests included.  Rows past ``cu_q[-1]`` are not written."""
         return ops.attention_decode_paged_fp4(q, self.pages[layer], self.block_table, self.lens, softmax_scale, cu_q,
                                               max_q, out, self.status)

@@ -88,6 +88,7 @@ _SIGS = {
     "dsv2_moe_grouped_down_shared_fp8": ([_p, _i32, _p, _p, _i32, _i32, _p, _p, _p, _p, _p, _i32, _p, _p, _p], _i32),
     "dsv2_moe_combine_parts": ([_p, _p, _p, _i32, _p, _p, _p, _p, _f32, _p, _p], _i32),
     "dsv2_paged_step": ([_p, _p, _i32, _p, _i64, _i32, _p, _i32, _i32, _i32, _p, _p, _p, _p, _p, _p], _i32),
+    "dsv2_paged_step_queries": ([_p, _p, _i32, _p, _i64, _i32, _p, _i32, _i32, _i32, _p, _p, _p, _p, _p, _p, _p], _i32),
     "dsv2_paged_slots": ([_p, _p, _i32, _p, _i64, _i32, _i32, _i32, _p, _p, _p, _p, _p], _i32),
     "dsv2_paged_write_fp4": ([_p, _i64, _i32, _p, _p, _i64, _i32, _i32, _p, _p], _i32),
     "dsv2_paged_read_fp4": ([_p, _i64, _i32, _i32, _p, _i32, _p, _i64, _p, _p], _i32),

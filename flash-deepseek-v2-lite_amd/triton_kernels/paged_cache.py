@@ -36,7 +36,7 @@ MAX_TOKENS = 2 ** 31 - 1
 # torch.empty 1.3, an attribute of a tensor 0.05 to 0.1.
 _BF16, _I32, _U8 = torch.bfloat16, torch.int32, torch.uint8
 _PAGE_SIZES = frozenset(1 << i for i in range(11))
-_ENTRY = {n: getattr(_hip.lib, n) for n in ("dsv2_paged_step", "dsv2_paged_slots", "dsv2_paged_write_fp4",
+_ENTRY = {n: getattr(_hip.lib, n) for n in ("dsv2_paged_step_queries", "dsv2_paged_slots", "dsv2_paged_write_fp4",
                                             "dsv2_paged_read_fp4", "dsv2_mla_decode_paged_fp4", "dsv2_paged_take_status")}
 _WORKSPACE = _hip.lib.dsv2_mla_paged_workspace_size()  # bytes
 _STATUS: dict = {}  # device index -> (int32 [1] status word of the functions below, its address)
@@ -161,7 +161,8 @@ def _page_size(name: str, page_size: int) -> None:
 
 
 def paged_cache_step(state: torch.Tensor, delta: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
-                     page_size: int, max_tokens: int, status: torch.Tensor | None = None) -> tuple[torch.Tensor, ...]:
+                     page_size: int, max_tokens: int, status: torch.Tensor | None = None,
+                     cu_q: torch.Tensor | None = None) -> tuple[torch.Tensor, ...]:
     """One step of the requests' lengths; returns (state after the step, slots, positions, rows).
 
     ``state`` int32 [B + 2]: the B lengths, then head and count of the ring ``free_pages`` (int32
@@ -175,7 +176,10 @@ def paged_cache_step(state: torch.Tensor, delta: torch.Tensor, block_table: torc
     -1.  A request whose tokens do not fit the table, ``max_tokens`` or the free pages keeps its
     length; its tokens get -1 and check_paged_status raises.  Both are counted in the requests' order, what
     was refused with the rest: behind a request refused for tokens all that grow are refused, behind one
-    refused for pages all that need a page.  One that would outgrow the table counts its tokens, no pages."""
+    refused for pages all that need a page.  One that would outgrow the table counts its tokens, no pages.
+
+    ``cu_q`` int32 [B + 1], if given, receives where each request's new tokens begin and the last one's end,
+    refused ones' among them: ``attention_decode_paged_fp4``'s argument for a query of each new token."""
     name = "paged_cache_step"
     index = _device(name, state, delta, block_table, free_pages)
     n = _int32(name, "delta", delta)
@@ -185,14 +189,21 @@ def paged_cache_step(state: torch.Tensor, delta: torch.Tensor, block_table: torc
     ts, width = _table(name, block_table, n)
     if n > MAX_REQUESTS or pages == 0 or not 0 <= max_tokens <= MAX_TOKENS:
         raise ValueError(f"{name}: {n} requests (at most {MAX_REQUESTS}), {pages} pages, max_tokens {max_tokens}")
+    cu = None
+    if cu_q is not None:
+        _device(name, state, cu_q)
+        _int32(name, "cu_q", cu_q, n + 1)
+        cu = cu_q.data_ptr()
     outs = state.new_empty(n + 2 + 3 * max_tokens)  # one allocation: the state, then the three maps
     if n == 0:
         outs.fill_(-1)[:2] = state
+        if cu is not None:
+            cu_q.zero_()
     else:
         at = outs.data_ptr()
         maps, size = at + 4 * n + 8, 4 * max_tokens
-        _call(index, "dsv2_paged_step", state.data_ptr(), delta.data_ptr(), n, block_table.data_ptr(), ts, width,
-              free_pages.data_ptr(), pages, page_size, max_tokens, at, maps, maps + size, maps + 2 * size,
+        _call(index, "dsv2_paged_step_queries", state.data_ptr(), delta.data_ptr(), n, block_table.data_ptr(), ts, width,
+              free_pages.data_ptr(), pages, page_size, max_tokens, at, maps, maps + size, maps + 2 * size, cu,
               _word(name, status, index))
     return torch.unsafe_split_with_sizes(outs, (n + 2, max_tokens, max_tokens, max_tokens))
 
@@ -290,7 +301,7 @@ def attention_decode_paged_fp4(q: torch.Tensor, pages: torch.Tensor, block_table
     b owns query tokens cu_q[b] .. cu_q[b + 1], at most ``max_q`` of them, and they are its last
     cached tokens: the last one sees all, each one before it a token less.  Where ``cu_q``'s tokens are a
     step's new ones, a request that does not grow has none, so rows are not the requests' numbers
-    (``dsv2lite.PagedLatentCache.query_starts`` forms it).  A query that sees nothing
+    (``paged_cache_step`` forms it).  A query that sees nothing
     gives zeros; query tokens past cu_q[B] are not written (in a fresh ``out`` they are undefined).
     Sums are fp32 with weights up to 2^8, so latents past some 2^100 may overflow to infinity.
     Up to 128 heads; q and out may have any token and head strides that are multiples of 8 (out's rows apart).

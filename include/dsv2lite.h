@@ -523,6 +523,14 @@ int dsv2_paged_step(const int32_t* state, const int32_t* delta, int requests, in
                     int max_tokens, int32_t* state_out, int32_t* slots, int32_t* positions, int32_t* rows,
                     int32_t* status, void* stream);
 
+/* dsv2_paged_step, and cu_q [requests + 1] (NULL: none): where each request's new tokens begin, refused ones'
+ * among them, and where the last one's end: 0 and the running sums of max(delta, 0), which stop at
+ * 2^31 - 1.  It is dsv2_mla_decode_paged_fp4's cu_q for a query of each new token. */
+int dsv2_paged_step_queries(const int32_t* state, const int32_t* delta, int requests, int32_t* block_table,
+                            int64_t table_stride, int table_width, int32_t* free_pages, int n_pages, int page_size,
+                            int max_tokens, int32_t* state_out, int32_t* slots, int32_t* positions, int32_t* rows,
+                            int32_t* cu_q, int32_t* status, void* stream);
+
 /* Slots of the tokens [starts[b], starts[b] + counts[b]) of every request, one after the other, as in
  * dsv2_paged_step; -1 past the last one and for positions or pages out of range. */
 int dsv2_paged_slots(const int32_t* starts, const int32_t* counts, int requests, const int32_t* block_table,

@@ -933,7 +933,7 @@ def test_queries_of_a_step_with_idle_requests_eager_and_captured():
     def step():
         slots, _, rows = cache.step(delta, most)
         cache.write(0, new, slots)
-        cache.attend(0, q, SCALE, cache.query_starts(delta), max_q, out)
+        cache.attend(0, q, SCALE, cache.cu_q, max_q, out)
         return rows
 
     side = torch.cuda.Stream()
@@ -973,7 +973,7 @@ def test_queries_of_a_step_with_idle_requests_eager_and_captured():
     x = rnd(full + 3, R.ROW, seed=61)
     slots, _, rows_now = cache.step(delta, full + 3)
     cache.write(0, x, slots)
-    got = cache.attend(0, big, SCALE, cache.query_starts(delta), full)
+    got = cache.attend(0, big, SCALE, cache.cu_q, full)
     assert rows_now.tolist() == [0, 1] + [-1] * full + [4]
     for at, b in ((0, 0), (1, 1), (full + 2, 4)):
         keys[b] = torch.cat([keys[b], R.held(x[at:at + 1])])
@@ -981,6 +981,27 @@ def test_queries_of_a_step_with_idle_requests_eager_and_captured():
         assert ((got[at].double() - want).abs() <= tol).all(), b
     with pytest.raises(RuntimeError, match="outgrew"):
         cache.check_status()
+
+
+@pytest.mark.parametrize("n", [0, 1, 5, 300, 513, 4096])
+def test_step_says_where_each_requests_new_tokens_begin(n):
+    """Idle, shrinking, refused and huge requests; the step's other outputs as without it."""
+    rng = random.Random(n)
+    delta = [rng.choice([0, 1, 1, 3, -2, 40]) for _ in range(n)]
+    for later in ([], [2 ** 31 - 1, 5, 2 ** 31 - 1, 0, 7]):
+        delta[n - len(later):] = later[:n]
+        ends = [0]
+        for d in delta:
+            ends.append(min(ends[-1] + max(d, 0), 2 ** 31 - 1))
+        state, free = i32([1] * n + [0, 9]), i32(list(range(9)) + [-1] * n)
+        table = (torch.arange(n, device=DEV) + 9).int()[:, None].repeat(1, 2)
+        cu = torch.full((n + 3,), 7, dtype=torch.int32, device=DEV)
+        got = P.paged_cache_step(state, i32(delta), table.clone(), free.clone(), 16, 50, cu_q=cu[1:-1])
+        plain = P.paged_cache_step(state, i32(delta), table.clone(), free.clone(), 16, 50)
+        assert cu.tolist() == [7] + ends + [7] and all(torch.equal(x, y) for x, y in zip(got, plain))
+    if n:
+        with pytest.raises(RuntimeError, match="outgrew"):
+            P.check_paged_status()
 
 
 def test_a_cache_reports_its_own_errors_only():

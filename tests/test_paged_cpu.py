@@ -248,14 +248,18 @@ def test_paged_latent_cache_shapes_and_refusals():
             PagedLatentCache(**{**dict(n_layers=1, requests=2, max_len=10, n_pages=3, page_size=32, device="cpu"), **kw})
 
 
-def test_query_starts_of_idle_shrinking_and_huge_steps():
-    from dsv2lite import PagedLatentCache
-
-    most = 2 ** 31 - 1
-    starts = PagedLatentCache.query_starts(torch.tensor([2, 0, -7, 3, 1], dtype=torch.int32))
-    assert starts.tolist() == [0, 2, 2, 2, 5, 6] and starts.dtype == torch.int32
-    starts = PagedLatentCache.query_starts(torch.tensor([1, most, 0, most, 5], dtype=torch.int32))
-    assert starts.tolist() == [0, 1] + [most] * 4
+def test_step_refuses_other_query_starts(monkeypatch):
+    monkeypatch.setattr(P, "_device", lambda *a: 0)
+    calls = []
+    monkeypatch.setattr(P, "_call", lambda index, entry, *args: calls.append(args[-2]))
+    args, cu = good()["paged_cache_step"], i32(5)
+    P.paged_cache_step(*args, cu_q=cu)
+    P.paged_cache_step(*args)
+    assert calls == [cu.data_ptr(), None]
+    for bad, error in ((i32(4), ValueError), (i32(5).long(), NotImplementedError), (i32(10)[::2], NotImplementedError)):
+        with pytest.raises(error, match="cu_q must be"):
+            P.paged_cache_step(*args, cu_q=bad)
+    assert len(calls) == 2
 
 
 # --------------------------------------------------------------------------- the attention's line of items
