@@ -270,9 +270,10 @@ static int plan_launch(const char* what, bool step, const PlanArgs& a, int page_
   DSV2_REQUIRE(a.width > 0 && a.width <= (INT32_MAX >> a.shift) && a.ts >= a.width, DSV2_E_SHAPE,
                "%s: block table of %d columns", what, a.width);
   DSV2_REQUIRE(a.tokens >= 0, DSV2_E_SHAPE, "%s: max_tokens %d", what, a.tokens);
-  // Every workgroup repeats the scan, so many requests go with few, large workgroups (MI355X, scans by
-  // shuffles then: 1,024 requests with 263,000 new tokens: 512 workgroups of 256 threads 13.2 us, 2,048 13.0, 256 of
-  // 1,024 10.0; 64 requests with 64,000 tokens 3.8 with 1,024 threads, 3.4 with 256).  What a step takes back only the device knows:
+  // Every workgroup repeats the scan, so many requests go with few, large workgroups (MI355X, us with 256 and with
+  // 1,024 threads; steps whose every fourth request gains up to 2,048 tokens: 256 requests 4.7 / 4.7, 400 5.3 / 5.2, 512
+  // 5.6 / 5.1, 768 6.8 / 5.7; with one token each 64 3.9 / 4.1, 512 5.6 / 5.7, 768 6.2 / 6.4; ranges of up to 2,000
+  // tokens: 128 3.3 / 3.6, 512 5.6 / 5.6, 768 7.5 / 7.3, 1,024 9.8 / 8.9).  What a step takes back only the device knows:
   // room for 8 pages a request (1,000 requests, 62 of which end with 62 pages: 7.7 us, with none 10.7).
   const bool many = a.n > kManyRequests;
   const int threads = many ? 1024 : 256, most = many ? 256 : 1024;
@@ -377,8 +378,9 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const bf16_t* __restri
 }
 
 // From kManyRows rows a wave reads four at once and its stores pass the caches by, below it one and plain
-// stores (MI355X: 65,536 rows 21.4 -> 16.8 us, 6.0 TB/s; 4,096 rows 3.20 -> 3.38, 1,024 rows 2.48 -> 3.02)
-constexpr int kManyRows = 8192;
+// stores (MI355X, us of one and of four: 1,024 rows 2.5 / 3.1, 4,096 3.2 / 3.3, 6,000 3.7 / 3.7, 8,192 4.3 / 3.8, 16,384
+// 6.9 / 5.6, 65,536 23.3 / 16.8, 6.0 TB/s)
+constexpr int kManyRows = 6000;
 
 __device__ __forceinline__ void stg16_nt(void* p, const uint4& v) {
   const u32x4_t x = {v.x, v.y, v.z, v.w};
