@@ -67,7 +67,7 @@ def check_paged_status(device: torch.device | str = "cuda", status: torch.Tensor
     torch.cuda.synchronize(index)
     # read and cleared at once: what another thread's call finds meanwhile is left for the next check
     taken = torch.empty_like(status)
-    _call(index, "dsv2_paged_take_status", taken.data_ptr(), at)
+    _call(index, "dsv2_paged_take_status", at, taken.data_ptr())
     bits = int(taken.item())
     if not bits:
         return
@@ -77,10 +77,8 @@ def check_paged_status(device: torch.device | str = "cuda", status: torch.Tensor
     raise RuntimeError("paged cache: " + "; ".join(what) + "; those tokens were skipped")
 
 
-def _word(name: str, status: torch.Tensor | None, index: int) -> int | None:
+def _word(name: str, status: torch.Tensor, index: int) -> int:
     """The address of a call's own status word."""
-    if status is None:
-        return None
     if status.dtype is not _I32 or status.numel() != 1:
         raise ValueError(f"{name}: status must be int32 [1], not {status.dtype} {list(status.shape)}")
     if status.get_device() != index:
@@ -88,15 +86,15 @@ def _word(name: str, status: torch.Tensor | None, index: int) -> int | None:
     return status.data_ptr()
 
 
-def _call(index: int, entry: str, *args) -> None:
-    """The entry point on the device's current stream, with the device as the current one; the last argument is the
-    call's status word or None."""
+def _call(index: int, entry: str, word: int | None, *args) -> None:
+    """The entry point on the device's current stream, with the device as the current one; `word`: the address of the
+    call's status word, None for the device's."""
     if _current_device() != index:
         with torch.cuda.device(index):
-            return _call(index, entry, *args)
-    if args[-1] is None:
-        args = (*args[:-1], (_STATUS.get(index) or _status(index))[1])
-    rc = _ENTRY[entry](*args, _hip._raw_stream(index))
+            return _call(index, entry, word, *args)
+    if word is None:
+        word = (_STATUS.get(index) or _status(index))[1]
+    rc = _ENTRY[entry](*args, word, _hip._raw_stream(index))
     if rc:
         raise _hip.HipKernelError(f"{entry} failed (status {rc}): "
                                   f"{_hip.lib.dsv2_last_error_message().decode(errors='replace')}")
@@ -202,9 +200,9 @@ def paged_cache_step(state: torch.Tensor, delta: torch.Tensor, block_table: torc
     else:
         at = outs.data_ptr()
         maps, size = at + 4 * n + 8, 4 * max_tokens
-        _call(index, "dsv2_paged_step_queries", state.data_ptr(), delta.data_ptr(), n, block_table.data_ptr(), ts, width,
-              free_pages.data_ptr(), pages, page_size, max_tokens, at, maps, maps + size, maps + 2 * size, cu,
-              _word(name, status, index))
+        _call(index, "dsv2_paged_step_queries", None if status is None else _word(name, status, index),
+              state.data_ptr(), delta.data_ptr(), n, block_table.data_ptr(), ts, width, free_pages.data_ptr(), pages,
+              page_size, max_tokens, at, maps, maps + size, maps + 2 * size, cu)
     return torch.unsafe_split_with_sizes(outs, (n + 2, max_tokens, max_tokens, max_tokens))
 
 
@@ -227,8 +225,8 @@ def paged_slot_map(starts: torch.Tensor, counts: torch.Tensor, block_table: torc
         maps.fill_(-1)
     else:
         at, size = maps.data_ptr(), 4 * max_tokens
-        _call(index, "dsv2_paged_slots", starts.data_ptr(), counts.data_ptr(), n, block_table.data_ptr(), ts, width,
-              page_size, max_tokens, at, at + size, at + 2 * size, _word(name, status, index))
+        _call(index, "dsv2_paged_slots", None if status is None else _word(name, status, index), starts.data_ptr(),
+              counts.data_ptr(), n, block_table.data_ptr(), ts, width, page_size, max_tokens, at, at + size, at + 2 * size)
     return torch.unsafe_split_with_sizes(maps, (max_tokens, max_tokens, max_tokens))
 
 
@@ -255,8 +253,8 @@ def paged_cache_write_fp4(rows: torch.Tensor, slots: torch.Tensor, pages: torch.
     rs = _cache_rows(name, "rows", rows, n)
     page_stride, n_pages, page_size = _pool(name, pages)
     if n:
-        _call(index, "dsv2_paged_write_fp4", rows.data_ptr(), rs, n, slots.data_ptr(), pages.data_ptr(), page_stride,
-              n_pages, page_size, _word(name, status, index))
+        _call(index, "dsv2_paged_write_fp4", None if status is None else _word(name, status, index), rows.data_ptr(),
+              rs, n, slots.data_ptr(), pages.data_ptr(), page_stride, n_pages, page_size)
 
 
 def paged_cache_read_fp4(pages: torch.Tensor, slots: torch.Tensor, out: torch.Tensor | None = None,
@@ -272,8 +270,8 @@ def paged_cache_read_fp4(pages: torch.Tensor, slots: torch.Tensor, out: torch.Te
         _device(name, pages, out)
         os = _cache_rows(name, "out", out, n)
     if n:
-        _call(index, "dsv2_paged_read_fp4", pages.data_ptr(), page_stride, n_pages, page_size, slots.data_ptr(), n,
-              out.data_ptr(), os, _word(name, status, index))
+        _call(index, "dsv2_paged_read_fp4", None if status is None else _word(name, status, index), pages.data_ptr(),
+              page_stride, n_pages, page_size, slots.data_ptr(), n, out.data_ptr(), os)
     return out
 
 
@@ -355,7 +353,7 @@ def attention_decode_paged_fp4(q: torch.Tensor, pages: torch.Tensor, block_table
     if t == 0 or n == 0:
         return out
     ws = pages.new_empty(_WORKSPACE)
-    _call(index, "dsv2_mla_decode_paged_fp4", q.data_ptr(), q_ts, q_hs, t, h, pages.data_ptr(), page_stride, n_pages,
-          page_size, block_table.data_ptr(), ts, width, lens.data_ptr(), n, cu, max_q, softmax_scale, out.data_ptr(),
-          o_ts, o_hs, ws.data_ptr(), _WORKSPACE, _word(name, status, index))
+    _call(index, "dsv2_mla_decode_paged_fp4", None if status is None else _word(name, status, index), q.data_ptr(), q_ts,
+          q_hs, t, h, pages.data_ptr(), page_stride, n_pages, page_size, block_table.data_ptr(), ts, width, lens.data_ptr(),
+          n, cu, max_q, softmax_scale, out.data_ptr(), o_ts, o_hs, ws.data_ptr(), _WORKSPACE)
     return out

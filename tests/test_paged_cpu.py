@@ -134,7 +134,7 @@ def test_attention_refuses_outputs_whose_rows_overlap(monkeypatch, t, h):
 def test_functions_refuse_a_status_word_of_another_type_shape_or_device(monkeypatch, name):
     monkeypatch.setattr(P, "_device", lambda *a: -1)  # what get_device() says of a CPU tensor
     calls = []
-    monkeypatch.setattr(P, "_call", lambda index, entry, *args: calls.append(args[-1]))
+    monkeypatch.setattr(P, "_call", lambda index, entry, word, *args: calls.append(word))
     word = i32(1)
     getattr(P, name)(*good()[name], status=word)
     getattr(P, name)(*good()[name])
@@ -251,7 +251,7 @@ def test_paged_latent_cache_shapes_and_refusals():
 def test_step_refuses_other_query_starts(monkeypatch):
     monkeypatch.setattr(P, "_device", lambda *a: 0)
     calls = []
-    monkeypatch.setattr(P, "_call", lambda index, entry, *args: calls.append(args[-2]))
+    monkeypatch.setattr(P, "_call", lambda index, entry, *args: calls.append(args[-1]))
     args, cu = good()["paged_cache_step"], i32(5)
     P.paged_cache_step(*args, cu_q=cu)
     P.paged_cache_step(*args)
