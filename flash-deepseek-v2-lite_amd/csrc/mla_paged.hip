@@ -22,7 +22,7 @@
 //
 // MI355X, both launches: 128 requests of 256 to 8,192 tokens, 16 heads: 60.5 us for 221 MB (3.6 TB/s; 38.8 us at the
 // rate of a copy, 5.69 TB/s); the loop itself runs at that rate, some 20 us are launches (3), the first loads (4), the
-// waves' meeting (5) and the merge (6).  One request of 150,000: 25.6 us; of 140: 10.4.
+// waves' meeting (5) and the merge (6).  One request of 150,000: 25.6 us; of 140: 10.5.
 #include "paged.h"
 #include "paged_line.h"
 
