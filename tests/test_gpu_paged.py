@@ -1004,6 +1004,71 @@ def test_step_says_where_each_requests_new_tokens_begin(n):
             P.check_paged_status()
 
 
+def test_a_captured_step_through_the_c_abi_with_padded_rows():
+    """Lengths, new rows and queries from projected hidden states, pages and attention as a host would call them, idle
+    requests and padding (positions of -1) among the rows; the staging buffer's other rows stay as they are."""
+    from dsv2lite import DSV2Config
+    from dsv2lite.rope import cos_sin_tables
+
+    cfg, B, most, ps, n_pages, width, max_q = DSV2Config(), 4, 7, 16, 30, 6, 3
+    cos, sin = cos_sin_tables(cfg, 128, device=DEV)
+    kvw, w_ukt = (rnd(512, seed=1, std=0.1) + 1).to(BF), rnd(16, 512, 128, std=0.05, seed=2)
+    pages = torch.full((n_pages, ps * R.TOKEN), 255, dtype=torch.uint8, device=DEV)
+    table, ring = torch.full((B, width), -1, dtype=torch.int32, device=DEV), torch.arange(n_pages, device=DEV).int()
+    state, after, delta, cu, status = i32([0] * B + [0, n_pages]), i32([0] * (B + 2)), i32([0] * B), i32([0] * (B + 1)), i32([0])
+    slots, positions, rows, cap = (i32([0] * most) for _ in range(4))
+    base, index = torch.zeros(most, dtype=torch.int64, device=DEV), torch.arange(most, device=DEV)
+    qkva, staged = rnd(most, 3648), torch.zeros(most, R.ROW, dtype=BF, device=DEV)
+    q, olat = torch.zeros(most, 16, R.ROW, dtype=BF, device=DEV), torch.zeros(most, 16, 512, dtype=BF, device=DEV)
+    ws = torch.empty(_hip.lib.dsv2_mla_paged_workspace_size(), dtype=torch.uint8, device=DEV)
+    p = lambda t: t.data_ptr()  # noqa: E731
+
+    def step():
+        st = _hip.stream_ptr()
+        _hip.call("dsv2_paged_step_queries", p(state), p(delta), B, p(table), width, width, p(ring), n_pages, ps, most,
+                  p(after), p(slots), p(positions), p(rows), p(cu), p(status), st)
+        torch.sub(index, positions, out=base)
+        torch.add(positions, 1, out=cap)
+        _hip.call("dsv2_mla_prepare_qlat", p(qkva), 3648, most, p(positions), p(base), p(cap), p(kvw), 1e-6, p(cos),
+                  p(sin), 128, p(w_ukt), p(staged), p(q), None, st)
+        _hip.call("dsv2_paged_write_fp4", p(staged), R.ROW, most, p(slots), p(pages), ps * R.TOKEN, n_pages, ps,
+                  p(status), st)
+        _hip.call("dsv2_mla_decode_paged_fp4", p(q), 16 * R.ROW, R.ROW, most, 16, p(pages), ps * R.TOKEN, n_pages, ps,
+                  p(table), width, width, p(after), B, p(cu), max_q, SCALE, p(olat), 16 * 512, 512, p(ws), ws.numel(),
+                  p(status), st)
+        state.copy_(after)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    keys = [torch.zeros(0, R.ROW, dtype=torch.float64, device=DEV) for _ in range(B)]
+    for k, d in enumerate([[3, 0, 1, 2], [1, 0, 1, 1], [0, 3, -1, 1], [1, 1, 0, 1], [3, 1, 0, -2], [1, 1, 3, 1]] + [[3, 0, 3, 1]] * 5):
+        delta.copy_(i32(d))
+        qkva.copy_(rnd(most, 3648, seed=70 + k))
+        staged.fill_(3.0)
+        olat.fill_(7.0)
+        if k == 3:
+            step()
+        else:
+            graph.replay()
+        new = sum(max(x, 0) for x in d)
+        assert positions.tolist()[new:] == [-1] * (most - new) and int((staged[new:] != 3).sum()) == 0
+        assert int((staged[:new] != 3).any(1).sum()) == new and int((olat[new:] != 7).sum()) == 0
+        held, at = R.held(staged), 0
+        for b in range(B):
+            keys[b] = torch.cat([keys[b], held[at:at + d[b]]]) if d[b] > 0 else keys[b][:max(0, len(keys[b]) + d[b])]
+            for j in range(max(d[b], 0)):
+                want, tol = R.attention(q[at], keys[b], len(keys[b]) - d[b] + j + 1, SCALE)
+                assert ((olat[at].double() - want).abs() <= tol).all(), (k, b, j)
+                at += 1
+        assert state.tolist()[:B] == [len(x) for x in keys] and status.tolist() == [0]
+
+
 def test_a_cache_reports_its_own_errors_only():
     """Two caches of one device: the one that lost tokens says so, whoever is asked first, and the functions' common
     word stays clear."""
