@@ -429,6 +429,25 @@ def test_attention_numbers_of_requests(requests, drafts):
     check(rnd(sum(nq) if drafts else requests, 4, R.ROW, seed=requests, std=0.3), pages, table, lens, keys, nq)
 
 
+def test_attention_of_the_most_requests():
+    """65,535 requests of up to 40 tokens, a third of them empty, in pages of one pool that they take by turns."""
+    B, ps, n_pages = 65535, 16, 5000
+    pages = pool(n_pages, ps)
+    keys = R.stored(pages, torch.arange(n_pages * ps, device=DEV), ps)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    table = torch.randint(0, n_pages, (B, 3), device=DEV, generator=g).int()
+    lens = torch.randint(-20, 41, (B,), device=DEV, generator=g).clamp(min=0).int()
+    q = rnd(B, 2, R.ROW, seed=5, std=0.3)
+    got = P.attention_decode_paged_fp4(q, pages, table, lens, SCALE)
+    assert int((got[lens == 0] != 0).sum()) == 0
+    t = torch.arange(40, device=DEV)
+    for b in list(range(0, B, 211)) + [B - 2, B - 1]:
+        n = int(lens[b])
+        slots = table[b].long()[t[:n] // ps] * ps + t[:n] % ps
+        want, tol = R.attention(q[b], keys[slots], n, SCALE)
+        assert ((got[b].double() - want).abs() <= tol).all(), b
+
+
 def test_attention_of_a_chunk_among_many_requests_with_wide_tables():
     """A prompt's chunk beside decoding rows: 250 requests with room for 163,840 tokens each, 600 queries at most,
     700 of them in all."""
