@@ -77,8 +77,8 @@ class PagedLatentCache:
     def attend(self, layer: int, q: torch.Tensor, softmax_scale: float, cu_q: torch.Tensor | None = None,
                max_q: int = 1, out: torch.Tensor | None = None) -> torch.Tensor:
         """Latent attention outputs [tokens, heads, 512] of absorbed queries [tokens, heads, 576] over a layer: the
-        requests' last cached tokens, ``cu_q[b]`` .. ``cu_q[b + 1]`` of them request b's (``self.cu_q`` after a step), or without
-        it row b for request b, idle requests included.  Rows past ``cu_q[-1]`` are not written."""
+        requests' last cached tokens, ``cu_q[b]`` .. ``cu_q[b + 1]`` of them request b's (``self.cu_q`` after a step),
+        or without it row b for request b, idle requests included.  Rows past ``cu_q[-1]`` are not written."""
         return ops.attention_decode_paged_fp4(q, self.pages[layer], self.block_table, self.lens, softmax_scale, cu_q,
                                               max_q, out, self.status)
 

@@ -558,9 +558,9 @@ int dsv2_paged_take_status(int32_t* bits, int32_t* status, void* stream);
  * max_q of them (cu_q NULL: token b); they are its last cached ones: query j of n sees the tokens below
  * lens[b] - n + j + 1.  A query that sees nothing gives zeros; query tokens of no request are left alone.
  * A length past the table's room counts as that room (and so for what its queries see), a negative one as 0.
- * The rows of out must not overlap.  Sums are fp32, weights up to 2^8.  requests and max_q up to 65,535; the groups of 16 (query token, head)
- * pairs that there may be (requests * ceil(max_q * heads / 16), at most tokens * heads / 16 + requests) times
- * (the table's room in tokens / 16 + 32) up to 2^30.
+ * The rows of out must not overlap.  Sums are fp32, weights up to 2^8.  requests and max_q up to 65,535; the
+ * groups of 16 (query token, head) pairs that there may be (requests * ceil(max_q * heads / 16), at most
+ * tokens * heads / 16 + requests) times (the table's room in tokens / 16 + 32) up to 2^30.
  * Table entries that name no page stand for tokens of zeros (and set DSV2_DEVERR_BAD_SLOT); a request with
  * more than max_q query tokens has the first max_q done (and sets DSV2_DEVERR_TOKENS).
  * workspace: dsv2_mla_paged_workspace_size bytes, 16-byte aligned, not shared by calls that may overlap. */
