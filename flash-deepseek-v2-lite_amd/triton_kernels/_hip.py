@@ -96,6 +96,12 @@ _SIGS = {
     "dsv2_mla_paged_workspace_size": ([], _i64),
     "dsv2_mla_decode_paged_fp4": ([_p, _i64, _i64, _i32, _i32, _p, _i64, _i32, _i32, _p, _i64, _i32, _p, _i32, _p,
                                    _i32, _f32, _p, _i64, _i64, _p, _i64, _p, _p], _i32),
+    "dsv2_quantize_fp8_blocks": ([_p, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _p, _p, _p], _i32),
+    "dsv2_rmsnorm_fp8_blocks": ([_p, _i64, _p, _i64, _p, _f32, _i64, _i32, _i32, _p, _p, _p, _p], _i32),
+    "dsv2_silu_mul_fp8_blocks": ([_p, _i64, _p, _i64, _i64, _i32, _i32, _p, _p, _p], _i32),
+    "dsv2_linear_fp8_blocks": ([_p, _i64, _p, _i64, _i64, _i32, _p, _i64, _p, _i64, _i32, _p, _i64, _i32, _p], _i32),
+    "dsv2_grouped_linear_fp8_blocks": ([_p, _i64, _p, _i64, _i64, _p, _i64, _i32, _p, _i64, _i64, _p, _i64, _i64, _i32,
+                                        _i32, _p, _p, _i64, _i32, _p], _i32),
 }
 
 EXPORTS = tuple(_SIGS)

@@ -1,0 +1,267 @@
+"""8-bit floating point with a scale for each block of 128: rounding of activations and weights, RMSNorm and
+SwiGLU that end in it, and the matrix products of what comes out, dense and grouped by experts.
+
+No counterpart in the reference (bf16 throughout); these stand beside ``rmsnorm``, ``mlp_elementwise`` and
+``moe_batch`` for models whose weights come as e4m3 codes with a fp32 scale for each 128 x 128 block.
+
+Codes are OCP e4m3 (``torch.float8_e4m3fn``).  A block is 128 columns (the last one of a row may be shorter) of one
+row of activations or of 128 rows of weights.  With a its largest |v|, at least 2^-100, its scale is a / 448 and
+its codes are the e4m3 values nearest to 448 v / a, ties to even; a block with an infinity or a NaN stands for NaN
+throughout.  Activations [..., K] come with scales [..., ceil(K / 128)], weights [(E,) N, K] with scales
+[(E,) ceil(N / 128), ceil(K / 128)].
+
+Every function runs on its tensors' device and that device's current stream, takes no workspace and reads
+nothing back to the host: all may be captured into a graph.  Last dimensions have to be contiguous, rows may be any
+stride apart; whole 16-byte rows are read faster.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _hip
+
+BLOCK = 128
+MAX_ROWS = 2 ** 31 - 1
+MAX_GROUPS = 65536
+
+# These calls launch kernels of 2 to 10 us for few rows, so their own host time is looked at.
+_E4M3, _BF16, _F32, _I32 = torch.float8_e4m3fn, torch.bfloat16, torch.float32, torch.int32
+_TYPES = {_BF16: 0, _F32: 1}  # DSV2_DTYPE_*
+_ENTRY = {n: getattr(_hip.lib, n) for n in ("dsv2_quantize_fp8_blocks", "dsv2_rmsnorm_fp8_blocks",
+                                            "dsv2_silu_mul_fp8_blocks", "dsv2_linear_fp8_blocks",
+                                            "dsv2_grouped_linear_fp8_blocks")}
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _call(index: int, entry: str, *args) -> None:
+    """The entry point on the device's current stream, with the device as the current one."""
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return _call(index, entry, *args)
+    rc = _ENTRY[entry](*args, _hip._raw_stream(index))
+    if rc:
+        raise _hip.HipKernelError(f"{entry} failed (status {rc}): "
+                                  f"{_hip.lib.dsv2_last_error_message().decode(errors='replace')}")
+
+
+def _device(name: str, *ts: torch.Tensor) -> int:
+    """The index of the one GPU that all tensors are on."""
+    index = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != index or index < 0:
+            if not t.is_cuda:
+                raise NotImplementedError(f"{name} requires CUDA (HIP) tensors")
+            raise ValueError(f"{name}: tensors on {ts[0].device} and {t.device}")
+    return index
+
+
+def _type(name: str, what: str, t: torch.Tensor) -> int:
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        raise NotImplementedError(f"{name}: {what} must be bf16 or fp32, not {t.dtype}")
+    return code
+
+
+def _rows(name: str, what: str, t: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """(t as a matrix, its rows, its columns, its row stride)."""
+    if t.dim() != 2:
+        if t.dim() == 0:
+            raise ValueError(f"{name}: {what} must have rows, not be a number")
+        t = t.reshape(-1 if t.numel() else math.prod(t.shape[:-1]), t.shape[-1])
+    n, k = t.shape
+    rs, cs = t.stride()
+    if k == 0 or n > MAX_ROWS or k > MAX_ROWS - 255:
+        raise ValueError(f"{name}: {what} is {list(t.shape)}")
+    if cs != 1 and k > 1:
+        raise NotImplementedError(f"{name}: {what} must have a contiguous last dimension")
+    return t, n, k, rs
+
+
+def _outputs(like: torch.Tensor, shape, k: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return like.new_empty(shape, dtype=_E4M3), like.new_empty((*shape[:-1], -(-k // BLOCK)), dtype=_F32)
+
+
+def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of bf16 or fp32 values: activations [..., K] in blocks of one row (``block_rows`` 1) or weights
+    [N, K] or [E, N, K] in blocks of 128 rows (``block_rows`` 128; a matrix's last block may be shorter)."""
+    name = "quantize_fp8_blocks"
+    index = _device(name, x)
+    dtype = _type(name, "x", x)
+    if block_rows == 1:
+        m, n, k, rs = _rows(name, "x", x)
+        codes, scales = _outputs(x, x.shape, k)
+        gs, groups = 0, 1
+    elif block_rows == BLOCK:
+        if x.dim() not in (2, 3):
+            raise ValueError(f"{name}: weights must be [N, K] or [E, N, K], not {list(x.shape)}")
+        m = x
+        groups, gs = (1, 0) if x.dim() == 2 else (x.shape[0], x.stride(0))
+        n, k = x.shape[-2:]
+        rs, cs = x.stride()[-2:]
+        if k == 0 or max(n, groups) > MAX_ROWS or k > MAX_ROWS - 255:
+            raise ValueError(f"{name}: x is {list(x.shape)}")
+        if cs != 1 and k > 1:
+            raise NotImplementedError(f"{name}: x must have a contiguous last dimension")
+        codes = x.new_empty(x.shape, dtype=_E4M3)
+        scales = x.new_empty((*x.shape[:-2], -(-n // BLOCK), -(-k // BLOCK)), dtype=_F32)
+    else:
+        raise ValueError(f"{name}: block_rows must be 1 or {BLOCK}, not {block_rows}")
+    if n and groups:
+        _call(index, "dsv2_quantize_fp8_blocks", m.data_ptr(), rs, gs, groups, n, k, dtype, block_rows,
+              codes.data_ptr(), scales.data_ptr())
+    return codes, scales
+
+
+def rmsnorm_fp8_blocks(hidden_states: torch.Tensor, weight: torch.Tensor, eps: float,
+                       residual: torch.Tensor | None = None) -> tuple[torch.Tensor, ...]:
+    """(codes, scales) of h * weight / sqrt(mean(h^2) + eps) over the last dimension, h = ``hidden_states``; with a
+    ``residual`` of the same shape h is their sum, rounded to the inputs' type, and the third result.
+
+    bf16 or fp32, all of one type; fp32 inside, and nothing is rounded between the norm and the codes (``rmsnorm_triton``
+    rounds twice there).  The least block, 2^-100, is one of h * weight here."""
+    name = "rmsnorm_fp8_blocks"
+    if residual is None:
+        index = _device(name, hidden_states, weight)
+    else:
+        index = _device(name, hidden_states, weight, residual)
+    dtype = _type(name, "hidden_states", hidden_states)
+    x, n, k, rs = _rows(name, "hidden_states", hidden_states)
+    if weight.dtype != hidden_states.dtype:
+        raise NotImplementedError(f"{name}: weight is {weight.dtype}, hidden_states {hidden_states.dtype}")
+    if weight.shape != (k,):
+        raise ValueError(f"weight shape {tuple(weight.shape)} != ({k},)")
+    if not weight.is_contiguous():
+        raise NotImplementedError(f"{name}: weight must be contiguous")
+    if not 0.0 <= eps < math.inf:
+        raise ValueError(f"{name}: eps must be at least 0 and finite, not {eps}")
+    if residual is None:
+        res = total = None
+        res_stride = 0
+    else:
+        if residual.dtype != hidden_states.dtype:
+            raise NotImplementedError(f"{name}: residual is {residual.dtype}, hidden_states {hidden_states.dtype}")
+        if residual.shape != hidden_states.shape:
+            raise ValueError(f"{name}: residual is {list(residual.shape)}, hidden_states {list(hidden_states.shape)}")
+        res, _, _, res_stride = _rows(name, "residual", residual)
+        total = x.new_empty(hidden_states.shape)
+    codes, scales = _outputs(x, hidden_states.shape, k)
+    if n:
+        _call(index, "dsv2_rmsnorm_fp8_blocks", x.data_ptr(), rs, None if res is None else res.data_ptr(), res_stride,
+              weight.data_ptr(), eps, n, k, dtype, codes.data_ptr(), scales.data_ptr(),
+              None if total is None else total.data_ptr())
+    return (codes, scales) if total is None else (codes, scales, total)
+
+
+def silu_mul_fp8_blocks(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of silu(gate) * up, bf16 or fp32 [..., K] each (the halves of one gate_up result, as views);
+    fp32 inside, nothing is rounded before the codes."""
+    name = "silu_mul_fp8_blocks"
+    index = _device(name, gate, up)
+    if gate.shape != up.shape:
+        raise ValueError("gate and up must have the same shape")
+    dtype = _type(name, "gate", gate)
+    if up.dtype != gate.dtype:
+        raise NotImplementedError(f"{name}: gate is {gate.dtype}, up {up.dtype}")
+    g, n, k, gs = _rows(name, "gate", gate)
+    u, _, _, us = _rows(name, "up", up)
+    codes, scales = _outputs(gate, gate.shape, k)
+    if n:
+        _call(index, "dsv2_silu_mul_fp8_blocks", g.data_ptr(), gs, u.data_ptr(), us, n, k, dtype, codes.data_ptr(),
+              scales.data_ptr())
+    return codes, scales
+
+
+def _activations(name: str, x: torch.Tensor, scales: torch.Tensor) -> tuple[torch.Tensor, int, int, int, torch.Tensor, int]:
+    """(x as a matrix, rows, K, row stride, the scales as a matrix, their row stride)."""
+    if x.dtype is not _E4M3:
+        raise NotImplementedError(f"{name}: x must be float8_e4m3fn codes, not {x.dtype}")
+    if scales.dtype is not _F32:
+        raise NotImplementedError(f"{name}: x_scales must be fp32")
+    lead = x.shape[:-1]
+    x, n, k, rs = _rows(name, "x", x)
+    if scales.shape != (*lead, -(-k // BLOCK)):
+        raise ValueError(f"{name}: x_scales must be {[*lead, -(-k // BLOCK)]}, not {list(scales.shape)}")
+    scales, _, _, ss = _rows(name, "x_scales", scales)
+    return x, n, k, rs, scales, ss
+
+
+def _weights(name: str, w: torch.Tensor, scales: torch.Tensor, k: int, dims: int) -> None:
+    if w.dtype is not _E4M3:
+        raise NotImplementedError(f"{name}: weights must be float8_e4m3fn codes, not {w.dtype}")
+    if scales.dtype is not _F32:
+        raise NotImplementedError(f"{name}: weight scales must be fp32")
+    if w.dim() != dims or w.shape[-1] != k or 0 in w.shape or w.shape[-2] > MAX_ROWS - 255:
+        raise ValueError(f"{name}: weights must be {'[E, ' if dims == 3 else '['}N, {k}], not {list(w.shape)}")
+    want = (*w.shape[:-2], -(-w.shape[-2] // BLOCK), -(-k // BLOCK))
+    if scales.shape != want:
+        raise ValueError(f"{name}: weight scales must be {list(want)}, not {list(scales.shape)}")
+    if w.stride(-1) != 1 and k > 1 or scales.stride(-1) != 1 and want[-1] > 1:
+        raise NotImplementedError(f"{name}: weights and their scales must have a contiguous last dimension")
+
+
+def _out_type(name: str, dtype: torch.dtype | None) -> tuple[torch.dtype, int]:
+    if dtype is None:
+        return _BF16, 0
+    if dtype not in _TYPES:
+        raise NotImplementedError(f"{name}: output_dtype must be bf16 or fp32")
+    return dtype, _TYPES[dtype]
+
+
+def linear_fp8_blocks(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
+                      output_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """The product [..., N] of activations [..., K] (codes, scales) and weights [N, K] (codes, scales): fp32 sums, one
+    rounding to ``output_dtype`` (bf16, the default, or fp32)."""
+    name = "linear_fp8_blocks"
+    index = _device(name, x, x_scales, weight, weight_scales)
+    lead = x.shape[:-1]
+    x, n, k, xs, x_scales, xss = _activations(name, x, x_scales)
+    _weights(name, weight, weight_scales, k, 2)
+    dtype, code = _out_type(name, output_dtype)
+    out = weight.shape[0]
+    y = x.new_empty((*lead, out), dtype=dtype)
+    if n:
+        _call(index, "dsv2_linear_fp8_blocks", x.data_ptr(), xs, x_scales.data_ptr(), xss, n, k, weight.data_ptr(),
+              weight.stride(0), weight_scales.data_ptr(), weight_scales.stride(0), out, y.data_ptr(), out, code)
+    return y
+
+
+def grouped_linear_fp8_blocks(x: torch.Tensor, x_scales: torch.Tensor, weights: torch.Tensor, weight_scales: torch.Tensor,
+                              offsets: torch.Tensor, rows: torch.Tensor | None = None,
+                              output_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """The products [R, N] of rows sorted by group (expert): rows offsets[e] .. offsets[e + 1] are multiplied by
+    ``weights[e]`` of [E, N, K].  Row r is row r of ``x`` [R, K], or row ``rows[r]`` of ``x`` [T, K] (int32 [R]; a
+    row number outside x stands for zeros).
+
+    ``offsets`` int32 [E + 1] is read on the device only.  Rows of no group are not written (here: undefined); an
+    offset below the largest one before it, or outside [0, R], counts as the nearest that is not."""
+    name = "grouped_linear_fp8_blocks"
+    if rows is None:
+        index = _device(name, x, x_scales, weights, weight_scales, offsets)
+    else:
+        index = _device(name, x, x_scales, weights, weight_scales, offsets, rows)
+    if x.dim() != 2:
+        raise ValueError(f"{name}: x must be [rows, K], not {list(x.shape)}")
+    x, t, k, xs, x_scales, xss = _activations(name, x, x_scales)
+    _weights(name, weights, weight_scales, k, 3)
+    groups, out = weights.shape[:2]
+    if groups > MAX_GROUPS:
+        raise ValueError(f"{name}: at most {MAX_GROUPS} groups, not {groups}")
+    if offsets.dtype is not _I32 or rows is not None and rows.dtype is not _I32:
+        raise NotImplementedError(f"{name}: offsets and rows must be int32")
+    if offsets.shape != (groups + 1,) or rows is not None and (rows.dim() != 1 or rows.shape[0] > MAX_ROWS):
+        raise ValueError(f"{name}: offsets must be [{groups + 1}] and rows [R], not {list(offsets.shape)}"
+                         f"{'' if rows is None else f' and {list(rows.shape)}'}")
+    if not offsets.is_contiguous() or rows is not None and not rows.is_contiguous():
+        raise NotImplementedError(f"{name}: offsets and rows must be contiguous")
+    dtype, code = _out_type(name, output_dtype)
+    n = t if rows is None else rows.shape[0]
+    y = x.new_empty((n, out), dtype=dtype)
+    if n:
+        _call(index, "dsv2_grouped_linear_fp8_blocks", x.data_ptr(), xs, x_scales.data_ptr(), xss, t,
+              None if rows is None else rows.data_ptr(), n, k, weights.data_ptr(), weights.stride(0), weights.stride(1),
+              weight_scales.data_ptr(), weight_scales.stride(0), weight_scales.stride(1), out, groups,
+              offsets.data_ptr(), y.data_ptr(), out, code)
+    return y

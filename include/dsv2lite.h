@@ -47,6 +47,10 @@ extern "C" {
 #define DSV2_LINEAR_OUT_F32_EXACT 4 /* dsv2_gemm_bf16: store the fp32 accumulator unrounded
                                        (router logits: HF's fp32 gate product); no SwiGLU or residual */
 
+/* types of the values that the *_fp8_blocks functions take and the products give */
+#define DSV2_DTYPE_BF16 0
+#define DSV2_DTYPE_F32 1
+
 int dsv2_abi_version(void);
 const char* dsv2_last_error_message(void);
 
@@ -570,6 +574,47 @@ int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_hs, int tok
                               int64_t table_stride, int table_width, const int32_t* lens, int requests,
                               const int32_t* cu_q, int max_q, float softmax_scale, void* out, int64_t out_ts,
                               int64_t out_hs, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+
+/* ---- 8 bits with block scales --------------------------------------------- */
+
+/* Values in OCP e4m3 with one fp32 scale for each block of 128 columns (the last one of a row may be shorter)
+ * and 1 row (activations) or 128 rows (weights).  With a the largest |v| of a block, at least 2^-100, the scale
+ * is a / 448 and the codes are the e4m3 values nearest to 448 v / a, ties to even; a block with an infinity or a
+ * NaN stands for NaN throughout.  kb = ceil(K / 128).  No counterpart in the reference (bf16 only).
+ * Inputs may have any row stride (in elements) and alignment; rows of whole 8 values at multiples of 16 bytes
+ * are read faster.  Codes and scales come without gaps. */
+
+/* Rows x [rows, K] (block_rows 1, groups 1; scales [rows, kb]) or `groups` matrices of rows x K x_gstride
+ * apart (block_rows 128; codes [groups, rows, K], scales [groups, ceil(rows / 128), kb]). */
+int dsv2_quantize_fp8_blocks(const void* x, int64_t x_stride, int64_t x_gstride, int64_t groups, int64_t rows, int K,
+                             int dtype, int block_rows, void* codes, float* scales, void* stream);
+
+/* h = x + residual (residual NULL: x), stored in x's type to sum [rows, K]; codes and scales of h * weight / sqrt(mean(h^2) + eps), which is not rounded in between.  The
+ * least block (2^-100) is one of h * weight here. */
+int dsv2_rmsnorm_fp8_blocks(const void* x, int64_t x_stride, const void* residual, int64_t res_stride,
+                            const void* weight, float eps, int64_t rows, int K, int dtype, void* codes, float* scales,
+                            void* sum, void* stream);
+
+/* codes and scales of gate * sigmoid(gate) * up in fp32. */
+int dsv2_silu_mul_fp8_blocks(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, int64_t rows,
+                             int K, int dtype, void* codes, float* scales, void* stream);
+
+/* y[m, n] = sum over blocks b of x_scales[m, b] * w_scales[n / 128, b] * (codes x[m, b] . codes w[n, b]): sums in
+ * fp32, one rounding to out_dtype.  Strides in elements; rows of x and w need not be aligned (16-byte rows of
+ * whole 16 codes are read faster). */
+int dsv2_linear_fp8_blocks(const void* x, int64_t x_stride, const float* x_scales, int64_t x_scales_stride, int64_t rows,
+                           int K, const void* w, int64_t w_stride, const float* w_scales, int64_t w_scales_stride, int N,
+                           void* y, int64_t y_stride, int out_dtype, void* stream);
+
+/* The same with one matrix for each group of rows: row r of y, offsets[g] <= r < offsets[g + 1] (int32
+ * [groups + 1], on the device), is x's row index[r] (index NULL: r) times w[g].  index[r] outside [0, x_rows)
+ * stands for a row of zeros.  Rows of no group are left as they are.  offsets are held to [0, rows] and
+ * to the largest one before them. */
+int dsv2_grouped_linear_fp8_blocks(const void* x, int64_t x_stride, const float* x_scales, int64_t x_scales_stride,
+                                   int64_t x_rows, const int32_t* index, int64_t rows, int K, const void* w,
+                                   int64_t w_gstride, int64_t w_stride, const float* w_scales, int64_t w_scales_gstride,
+                                   int64_t w_scales_stride, int N, int groups, const int32_t* offsets, void* y,
+                                   int64_t y_stride, int out_dtype, void* stream);
 
 #ifdef __cplusplus
 }

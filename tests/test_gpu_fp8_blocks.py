@@ -1,0 +1,515 @@
+"""The 8-bit functions with block scales on the GPU against their definition in 64 bits: codes of bf16 values exactly,
+sums within the bound that their roundings give, and the functions together as a layer uses them."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    from triton_kernels import _hip
+    from triton_kernels import fp8_blocks as F
+
+import fp8_blocks_ref as R
+
+DEV = "cuda"
+BF, F32, E4 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
+U24 = R.U24
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def rnd(*shape, seed=0, dtype=BF, std=1.0):
+    return (torch.randn(*shape, generator=gen(seed), device=DEV) * std).to(dtype)
+
+
+def strided(t, gap=8, fill=math.nan, before=0):
+    """t's values as a view of rows `gap` further apart, `before` values into a buffer of `fill`."""
+    *lead, n, k = t.shape
+    buf = torch.full((math.prod(lead) * n * (k + gap) + before,), fill, device=DEV).to(t.dtype)
+    view = buf[before:].view(*lead, n, k + gap)[..., :k]
+    view.copy_(t)
+    return view
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+# ---------------------------------------------------------------- rounding
+# a bf16 value times 7/8 and the quotient are exact where the quotient is a code or half way between two; fp32 values are
+# rounded once before the quotient's rounding: two half steps
+LOOSE = {BF: 0.0, F32: 2 * U24}
+SHAPES = [(1, 1), (1, 127), (1, 128), (1, 129), (2, 8), (3, 200), (5, 136), (16, 2048), (17, 1408), (33, 2050), (64, 10944),
+          (700, 260), (4099, 64)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m,k", SHAPES)
+def test_rows_are_rounded_to_the_nearest_codes(m, k, dtype):
+    x = rnd(m, k, seed=m + k, dtype=dtype) * torch.exp(2 * rnd(m, 1, seed=k, dtype=F32)).to(dtype)
+    for v in (x, strided(x), strided(x, gap=3, before=1)):
+        codes, scales = F.quantize_fp8_blocks(v)
+        q, s = R.rounded(x.double(), 1)
+        R.check_codes(codes, q, LOOSE[dtype])
+        R.check_scales(scales, s, U24)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("shape", [(1, 1), (127, 128), (128, 128), (129, 136), (300, 200), (257, 2050), (2, 130, 136), (3, 70, 65),
+                                   (64, 16, 24)])
+def test_weights_are_rounded_in_blocks_of_128_rows(shape, dtype):
+    x = rnd(*shape, seed=sum(shape), dtype=dtype)
+    for v in (x, strided(x), strided(x, gap=3, before=1)):
+        codes, scales = F.quantize_fp8_blocks(v, 128)
+        for c, s, w in zip(codes.view(-1, *shape[-2:]), scales.view(-1, *scales.shape[-2:]), x.view(-1, *shape[-2:])):
+            q, want = R.rounded(w.double(), 128)
+            R.check_codes(c, q, LOOSE[dtype])
+            R.check_scales(s, want, U24)
+
+
+def test_every_bf16_value_against_every_kind_of_largest():
+    """All finite bf16 values below a largest one, for largest ones of all mantissas and the ends of the range: ties too."""
+    bits = torch.arange(0x7f80, dtype=torch.int32, device=DEV).to(torch.int16).view(BF)
+    tops = [0x3f80 + i for i in range(128)] + [0x0080, 0x0d80, 0x0d7f, 0x0d00, 0x2000, 0x7f7f, 0x7f00]
+    for top in tops:
+        a = torch.tensor([top], dtype=torch.int16, device=DEV).view(BF)
+        v = bits[:top + 1]
+        v = torch.cat([v, -v])
+        n = -(-v.numel() // 127) * 127
+        v = torch.cat([v, v.new_zeros(n - v.numel())]).view(-1, 127)
+        x = torch.cat([v, a.expand(v.shape[0], 1)], 1).contiguous()
+        codes, scales = F.quantize_fp8_blocks(x)
+        q, s = R.rounded(x.double(), 1)
+        R.check_codes(codes, q)
+        R.check_scales(scales, s, U24)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_blocks_of_zeros_and_of_values_that_are_none(dtype):
+    x = rnd(6, 300, seed=1, dtype=dtype)
+    x[0] = 0
+    x[1, 128:256] = 0
+    x[2, 5] = math.nan
+    x[3, 200] = math.inf
+    x[4, 299] = -math.inf
+    x[5, :128] = 2.0 ** -120
+    x[5, 130] = 2.0 ** 127
+    codes, scales = F.quantize_fp8_blocks(x)
+    q, s = R.rounded(torch.where(x.isfinite(), x, math.nan).double(), 1)
+    for r, b in ((2, 0), (3, 1), (4, 2)):
+        q[r, 128 * b:128 * b + 128] = math.nan
+    R.check_codes(codes, q, LOOSE[dtype])
+    R.check_scales(scales, s, U24)
+    codes, scales = F.quantize_fp8_blocks(x, 128)
+    assert codes[:, :256].isnan().all() and codes[:, 256:].isnan().all() and scales.isnan().all()
+    assert F.quantize_fp8_blocks(x.new_zeros(130, 130), 128)[0].float().count_nonzero() == 0
+
+
+@pytest.mark.parametrize("m", [1, 3, 1024, 1025, 1200])
+@pytest.mark.parametrize("k", [1, 64, 200, 1030, 2048, 2049, 5120, 8192, 8200, 10944])
+@pytest.mark.parametrize("dtype,residual", [(BF, True), (BF, False), (F32, True), (F32, False)])
+def test_norm(m, k, dtype, residual):
+    if m > 3 and k > 2049:
+        m = m // 8
+    x, r = rnd(m, k, seed=m + k, dtype=dtype, std=3), rnd(m, k, seed=m * k, dtype=dtype)
+    w = (1 + 0.3 * rnd(k, seed=k, dtype=F32)).to(dtype)
+    h = (x.float() + r.float()).to(dtype) if residual else x
+    hd = h.double()
+    q, s = R.rounded(hd * w.double(), 1)
+    s = s / torch.sqrt((hd * hd).mean(1, keepdim=True) + 1e-6)
+    # the sum of squares: a lane adds up to ceil(k / 512) * 8 of them one after another, then eight partial sums
+    # meet; half of that, and eight roundings of the factor and the scale
+    loose = (-(-k // 512) * 4 + 4 + 8) * U24
+    for v in (0, 1, 2):
+        a = (x, strided(x, 16), strided(x, 5, before=1))[v]
+        b = (r, strided(r, 8), strided(r, 3, before=3))[v]
+        out = F.rmsnorm_fp8_blocks(a, w, 1e-6, b if residual else None)
+        # fp32: the product h w is rounded, then as the rows
+        R.check_codes(out[0], q, LOOSE[dtype] + (U24 * 2 if dtype == F32 else 0))
+        R.check_scales(out[1], s, loose)
+        assert len(out) == 2 + residual
+        if residual:
+            assert torch.equal(out[2], h)
+
+
+def test_norm_of_rows_of_zeros_and_with_values_that_are_none():
+    for dtype in (BF, F32):
+        x = rnd(5, 300, seed=2, dtype=dtype)
+        x[0] = 0
+        x[1, 250] = math.nan
+        x[2, 3] = math.inf
+        w = torch.ones(300, device=DEV, dtype=dtype)
+        codes, scales, h = F.rmsnorm_fp8_blocks(x, w, 1e-6, torch.zeros_like(x))
+        assert not codes[0].float().any() and scales[0].isfinite().all()
+        # the row's factor is NaN, or with an infinity 0: what the scales stand for is not finite in the block that has it
+        assert scales[1].isnan().all()
+        assert codes[2, :128].isnan().all() and scales[2, 0].isnan()
+        assert codes[3:].float().isfinite().all() and scales[3:].isfinite().all()
+        # what rows do not hold is not read
+        assert torch.equal(F.rmsnorm_fp8_blocks(x[3:], w, 1e-6)[0].view(torch.uint8), codes[3:].view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m,k", SHAPES)
+def test_silu_mul(m, k, dtype):
+    both = rnd(m, 2 * k, seed=m + k, dtype=dtype, std=4)
+    both[:, ::7] *= 5  # gates down to -80
+    for gate, up in (both.chunk(2, 1), (strided(both, 1, before=1)[:, :k], both[:, k:])):
+        codes, scales = F.silu_mul_fp8_blocks(gate, up)
+        y = gate.double() * torch.sigmoid(gate.double()) * up.double()
+        q, s = R.rounded(y, 1)
+        # exp to an ulp, its correction, the sum, the quotient, two products: 8 half steps; both values of a quotient
+        R.check_codes(codes, q, 2 * 8 * U24 + 3 * U24)
+        R.check_scales(scales, s, 9 * U24)
+
+
+def test_silu_mul_at_the_ends():
+    g = torch.tensor([0.0, -0.0, 80.0, -80.0, 88.0, -88.0, 100.0, -83.2, -84.0, 1e30, -1e30, 1e-30, -87.5], device=DEV)
+    u = torch.full_like(g, 2.0)
+    for i in range(len(g)):
+        gi, ui = g[i:i + 1].view(1, 1), u[i:i + 1].view(1, 1)
+        codes, scales = F.silu_mul_fp8_blocks(gi, ui)
+        want = (gi.double() * torch.sigmoid(gi.double()) * ui.double()).item()
+        got = (codes.double() * scales.double()).item()
+        assert abs(got - want) <= 2.0 ** -20 * abs(want) + 2.0 ** -110, (g[i], got, want)
+    for bad in (math.nan, math.inf, -math.inf):
+        for pair in ((bad, 1.0), (1.0, bad)):
+            x = torch.ones(2, 2, 256, device=DEV)
+            x[0, 0, 3], x[1, 0, 3] = pair
+            codes, scales = F.silu_mul_fp8_blocks(x[0], x[1])
+            assert codes[0, :128].isnan().all() and scales[0, 0].isnan()
+            assert codes[0, 128:].float().isfinite().all() and scales[0, 1].isfinite() and scales[1].isfinite().all()
+
+
+# ---------------------------------------------------------------- products
+def matrix(n, k, seed, rows, groups=None):
+    x = rnd(*(() if groups is None else (groups,)), n, k, seed=seed, dtype=F32)
+    x = x * torch.exp(rnd(*x.shape[:-1], 1, seed=seed + 1, dtype=F32))
+    return F.quantize_fp8_blocks(x, rows)
+
+
+def guarded(codes, scales, gap, before):
+    """Codes and scales as views between NaNs."""
+    *lead, n, k = codes.shape
+    buf = torch.full((math.prod(lead) * n * (k + gap) + before + 64,), 0x7f, dtype=torch.uint8, device=DEV)
+    c = buf[before:before + math.prod(lead) * n * (k + gap)].view(*lead, n, k + gap)[..., :k]
+    c.copy_(codes.view(torch.uint8))
+    return c.view(E4), strided(scales, 3)
+
+
+MS = [1, 2, 15, 16, 17, 33, 64, 65, 129, 300]
+NK = [(1, 1), (16, 128), (17, 127), (130, 129), (64, 16), (300, 144), (100, 2048), (3648, 2048), (257, 1408), (50, 10944),
+      (1000, 2000), (129, 4099)]
+
+
+@pytest.mark.parametrize("n,k", NK)
+@pytest.mark.parametrize("m", MS)
+def test_linear(m, n, k):
+    x, sx = matrix(m, k, m + k, 1)
+    w, sw = matrix(n, k, n * k, 128)
+    for dtype in (BF, F32):
+        R.check_product(F.linear_fp8_blocks(x, sx, w, sw, dtype), x, sx, w, sw)
+    for gap, before in ((16, 0), (5, 3)):
+        got = F.linear_fp8_blocks(*guarded(x, sx, gap, before), *guarded(w, sw, gap, before), F32)
+        R.check_product(got, x, sx, w, sw)
+
+
+@pytest.mark.parametrize("m,n,k", [(1025, 2816, 2048), (2048, 2050, 1408), (4099, 300, 656), (513, 10944, 256), (700, 21888, 128),
+                                   (3000, 3000, 300)])
+def test_linear_large(m, n, k):
+    x, sx = matrix(m, k, m + k, 1)
+    w, sw = matrix(n, k, n * k, 128)
+    for dtype in (BF, F32):
+        R.check_product(F.linear_fp8_blocks(x, sx, w, sw, dtype), x, sx, w, sw)
+
+
+@pytest.mark.parametrize("m", [1, 20, 100, 600])
+def test_linear_sums_whole_numbers_exactly(m):
+    """Codes that are small whole numbers and scales that are powers of two: every sum is exact in fp32, so each row
+    has to meet each weight and each block its own two scales, without a tolerance."""
+    g = gen(m)
+    n, k = 515, 1200
+    x = torch.randint(-4, 5, (m, k), device=DEV, generator=g).float()
+    w = torch.randint(-4, 5, (n, k), device=DEV, generator=g).float()
+    sx = torch.exp2(torch.randint(-2, 3, (m, R.blocks(k)), device=DEV, generator=g).float())
+    sw = torch.exp2(torch.randint(-2, 3, (R.blocks(n), R.blocks(k)), device=DEV, generator=g).float())
+    got = F.linear_fp8_blocks(x.to(E4), sx, w.to(E4), sw, F32)
+    want, _ = R.product(x.to(E4), sx, w.to(E4), sw)
+    assert torch.equal(got.double(), want)
+    assert torch.equal(F.linear_fp8_blocks(x.to(E4), sx, w.to(E4), sw), want.to(BF))
+
+
+def test_linear_of_every_code_and_of_none():
+    """The 254 finite codes times one, NaN codes, infinite and NaN scales."""
+    codes = torch.arange(256, dtype=torch.uint8, device=DEV).view(256, 1).view(E4)
+    one, s1 = torch.ones(1, 1, device=DEV).to(E4), torch.ones(1, 1, device=DEV)
+    sx = torch.ones(256, 1, device=DEV)
+    got = F.linear_fp8_blocks(codes, sx, one, s1, F32)[:, 0]
+    want = codes.view(256).float()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+    x, xs = matrix(40, 300, 3, 1)
+    w, ws = matrix(200, 300, 4, 128)
+    clean = F.linear_fp8_blocks(x, xs, w, ws)
+    xs[3, 1] = math.nan
+    xs[7, 2] = math.inf
+    ws[1, 0] = math.nan
+    got = F.linear_fp8_blocks(x, xs, w, ws)
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[3], bad[7], bad[:, 128:] = True, True, True
+    assert not got[bad].isfinite().any() and got[3].isnan().all() and got[:, 128:].isnan().all()
+    assert torch.equal(got[~bad], clean[~bad])
+
+
+def test_products_leave_what_is_not_theirs():
+    """Through the C ABI with rows of y further apart than N: the gaps and the rows of no group stay."""
+    x, sx = matrix(70, 300, 5, 1)
+    w, sw = matrix(130, 300, 6, 128, groups=3)
+    for dtype, code in ((BF, 0), (F32, 1)):
+        for ys, at in ((136, 0), (131, 1)):
+            buf = torch.full((70 * ys + 9,), 7.0, device=DEV).to(dtype)
+            y = buf[at:at + 70 * ys].view(70, ys)
+            _hip.call("dsv2_linear_fp8_blocks", x.data_ptr(), 300, sx.data_ptr(), 3, 70, 300, w.data_ptr(), 300,
+                      sw.data_ptr(), 3, 130, y.data_ptr(), ys, code, _hip.stream_ptr())
+            R.check_product(y[:, :130], x, sx, w[0], sw[0])
+            assert (y[:, 130:] == 7).all() and (buf[:at] == 7).all() and (buf[at + 70 * ys:] == 7).all()
+            buf.fill_(7.0)
+            offsets = i32([4, 20, 20, 66])
+            _hip.call("dsv2_grouped_linear_fp8_blocks", x.data_ptr(), 300, sx.data_ptr(), 3, 70, None, 70, 300, w.data_ptr(),
+                      130 * 300, 300, sw.data_ptr(), 6, 3, 130, 3, offsets.data_ptr(), y.data_ptr(), ys, code,
+                      _hip.stream_ptr())
+            for e, (lo, hi) in ((0, (4, 20)), (2, (20, 66))):
+                R.check_product(y[lo:hi, :130], x[lo:hi], sx[lo:hi], w[e], sw[e])
+            assert (y[:4] == 7).all() and (y[66:] == 7).all() and (y[:, 130:] == 7).all()
+
+
+def check_grouped(y, x, sx, w, sw, offsets, rows=None):
+    for e, (lo, hi) in enumerate(zip(offsets, offsets[1:])):
+        if hi > lo:
+            at = torch.arange(lo, hi, device=DEV) if rows is None else rows[lo:hi].long()
+            there = (at >= 0) & (at < x.shape[0])
+            at = at.clamp(0, max(x.shape[0] - 1, 0))
+            xe = x.view(torch.uint8)[at].view(E4)
+            R.check_product(y[lo:hi], xe, torch.where(there[:, None], sx[at], 0), w[e], sw[e])
+
+
+def offsets_of(counts):
+    return [sum(counts[:i]) for i in range(len(counts) + 1)]
+
+
+@pytest.mark.parametrize("n,k", [(130, 300), (64, 128), (2816, 2048), (257, 1413), (1, 1)])
+@pytest.mark.parametrize("counts", [[1], [0, 1], [5, 0, 70, 1, 0], [0] * 70 + [3] + [0] * 60 + [65], [1] * 64, [16] * 20,
+                                    [300, 2, 129, 64], [0, 0, 700]], ids=str)
+def test_grouped(counts, n, k):
+    if n == 2816:
+        counts = counts[-5:]
+    offsets, groups = offsets_of(counts), len(counts)
+    total, tokens = offsets[-1], max(1, offsets[-1] // 3)
+    w, sw = matrix(n, k, n + k, 128, groups)
+    x, sx = matrix(total, k, total, 1)
+    for dtype in (BF, F32):
+        check_grouped(F.grouped_linear_fp8_blocks(x, sx, w, sw, i32(offsets), None, dtype), x, sx, w, sw, offsets)
+    rows = torch.randint(0, tokens, (total,), generator=gen(k), device=DEV).int()
+    x, sx = matrix(tokens, k, total, 1)
+    check_grouped(F.grouped_linear_fp8_blocks(x, sx, w, sw, i32(offsets), rows, F32), x, sx, w, sw, offsets, rows)
+    for gap, before in ((16, 0), (5, 3)):
+        got = F.grouped_linear_fp8_blocks(*guarded(x, sx, gap, before), *guarded(w, sw, gap, before), i32(offsets), rows)
+        check_grouped(got, x, sx, w, sw, offsets, rows)
+
+
+@pytest.mark.parametrize("counts", [[700, 3000, 0, 1500, 12, 1700], [1100] * 8])
+def test_grouped_large(counts):
+    offsets = offsets_of(counts)
+    for n, k, gather in ((2816, 2048, True), (2048, 1408, False), (700, 300, True)):
+        w, sw = matrix(n, k, n + k, 128, len(counts))
+        tokens = 1500 if gather else offsets[-1]
+        x, sx = matrix(tokens, k, 1, 1)
+        rows = torch.randint(0, tokens, (offsets[-1],), generator=gen(k), device=DEV).int() if gather else None
+        check_grouped(F.grouped_linear_fp8_blocks(x, sx, w, sw, i32(offsets), rows), x, sx, w, sw, offsets, rows)
+
+
+@pytest.mark.parametrize("k", [300, 304, 512])
+def test_grouped_holds_offsets_and_row_numbers_to_their_ranges(k):
+    w, sw = matrix(70, k, 1, 128, 4)
+    x, sx = matrix(50, k, 2, 1)
+    for given, taken in [([0, 30, 10, 20, 50], [0, 30, 30, 30, 50]), ([-5, 9, 2 ** 31 - 1, 60, 3], [0, 9, 50, 50, 50]),
+                         ([50, 40, 30, 20, 10], [50, 50, 50, 50, 50]), ([-2 ** 31, -1, 5, 5, 5], [0, 0, 5, 5, 5])]:
+        check_grouped(F.grouped_linear_fp8_blocks(x, sx, w, sw, i32(given), None, F32), x, sx, w, sw, taken)
+    rows = torch.arange(50, device=DEV).int()
+    rows[::3] = -1
+    rows[1::6] = 50
+    rows[5], rows[8] = 2 ** 31 - 1, -2 ** 31
+    sx[0] = math.nan  # nor does the first row stand in for one that there is not
+    rows[rows == 0] = 1
+    got = F.grouped_linear_fp8_blocks(x, sx, w, sw, i32([0, 10, 10, 33, 50]), rows, F32)
+    check_grouped(got, x, torch.where(sx.isnan(), 0, sx), w, sw, [0, 10, 10, 33, 50], rows)
+    assert not got[::3].any()
+    none, nosx = F.quantize_fp8_blocks(torch.zeros(0, k, device=DEV))
+    assert not F.grouped_linear_fp8_blocks(none, nosx, w, sw, i32([0, 10, 10, 33, 50]), rows).any()
+
+
+@pytest.mark.parametrize("groups", [130, 4096])
+def test_grouped_with_many_groups(groups):
+    counts = [(i * 7) % 5 if i % 3 == 0 else 0 for i in range(groups)]
+    offsets = offsets_of(counts)
+    w, sw = matrix(24, 136, 1, 128, groups)
+    x, sx = matrix(offsets[-1], 136, 2, 1)
+    check_grouped(F.grouped_linear_fp8_blocks(x, sx, w, sw, i32(offsets), None, F32), x, sx, w, sw, offsets)
+
+
+def test_a_groups_rows_do_not_depend_on_other_rows():
+    """The same group with the same rows gives the same bits in another place among other groups."""
+    w, sw = matrix(300, 1408, 1, 128, 3)
+    x, sx = matrix(200, 1408, 2, 1)
+    a = F.grouped_linear_fp8_blocks(x, sx, w, sw, i32([0, 40, 150, 200]))
+    b = F.grouped_linear_fp8_blocks(x, sx, w, sw, i32([0, 40, 40, 200]), torch.arange(200, device=DEV).int())
+    assert torch.equal(a[:40], b[:40]) and torch.equal(a[150:], b[150:])
+    c = F.grouped_linear_fp8_blocks(x, sx, w, sw, i32([0, 40, 150, 200]))
+    assert torch.equal(a, c)
+
+
+def test_offsets_past_32_bits():
+    """Rows of x, w and y whose byte offsets pass 2^31 and 2^32; few of each are looked at."""
+    m, n, k = 70001, 33000, 160
+    x, sx = matrix(m, k, 1, 1)
+    w, sw = matrix(n, k, 2, 128)
+    y = F.linear_fp8_blocks(x, sx, w, sw, BF)  # 4.6 GB
+    at = torch.tensor([0, 1, 35000, 65077, 65078, m - 1], device=DEV)
+    R.check_product(y[at], x.view(torch.uint8)[at].view(E4), sx[at], w, sw)
+    del y
+    far = 2 ** 27 + 16
+    buf = torch.zeros(40 * far, dtype=torch.uint8, device=DEV)  # 5.4 GB
+    wide = buf.view(40, far)[:, :k].view(E4)
+    wide.view(torch.uint8).copy_(x[:40].view(torch.uint8))
+    R.check_product(F.linear_fp8_blocks(wide, sx[:40], w[:300], sw[:3], F32), x[:40], sx[:40], w[:300], sw[:3])
+    wide.view(torch.uint8).copy_(w[:40].view(torch.uint8))
+    R.check_product(F.linear_fp8_blocks(x[:50], sx[:50], wide, sw[:1], F32), x[:50], sx[:50], w[:40], sw[:1])
+    rows = torch.tensor([39, 0, 17, 38], device=DEV).int()
+    wide.view(torch.uint8).copy_(x[:40].view(torch.uint8))
+    got = F.grouped_linear_fp8_blocks(wide, sx[:40], w[:256].view(2, 128, k), sw[:2].view(2, 1, -1), i32([0, 2, 4]), rows, F32)
+    check_grouped(got, x[:40], sx[:40], w[:256].view(2, 128, k), sw[:2].view(2, 1, -1), [0, 2, 4], rows)
+    big = buf[:5 * 2 ** 30].view(BF).view(-1, 2560)  # 2^31 values and more
+    big[-1] = rnd(2560, seed=4)
+    codes, scales = F.quantize_fp8_blocks(big)
+    q, s = R.rounded(big[-2:].double(), 1)
+    R.check_codes(codes[-2:], q)
+    R.check_scales(scales[-2:], s, U24)
+
+
+# ---------------------------------------------------------------- as they are used
+def layer(h, r, p, ids, offsets, rows):
+    """An attention input and a routed MLP: what a layer with 8-bit weights calls."""
+    c, s, h = F.rmsnorm_fp8_blocks(h, p["norm"], 1e-6, r)
+    qkv = F.linear_fp8_blocks(c, s, p["w"], p["sw"])
+    gu = F.grouped_linear_fp8_blocks(c, s, p["gu"], p["sgu"], offsets, rows)
+    gate, up = gu.chunk(2, 1)
+    a, sa = F.silu_mul_fp8_blocks(gate, up)
+    y = F.grouped_linear_fp8_blocks(a, sa, p["down"], p["sdown"], offsets)
+    return {"c": c, "s": s, "h": h, "qkv": qkv, "gu": gu, "a": a, "sa": sa, "y": y}
+
+
+def layer_inputs(tokens, seed, hidden=512, inter=352, experts=8, top=3):
+    p = {"norm": (1 + 0.2 * rnd(hidden, seed=9, dtype=F32)).to(BF)}
+    p["w"], p["sw"] = matrix(700, hidden, 10, 128)
+    p["gu"], p["sgu"] = matrix(2 * inter, hidden, 11, 128, experts)
+    p["down"], p["sdown"] = matrix(hidden, inter, 12, 128, experts)
+    h, r = rnd(tokens, hidden, seed=seed), rnd(tokens, hidden, seed=seed + 1)
+    ids = torch.rand(tokens, experts, generator=gen(seed), device=DEV).topk(top, 1).indices.reshape(-1)
+    order = torch.sort(ids, stable=True).indices
+    counts = torch.bincount(ids, minlength=experts)
+    offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0)]).int()
+    return h, r, p, ids, offsets, (order // top).int()
+
+
+def check_layer(o, h, r, p, ids, offsets, rows):
+    """Each function's result against 64 bits from what it was given."""
+    assert torch.equal(o["h"], (h.float() + r.float()).to(BF))
+    hd = o["h"].double()
+    q, s = R.rounded(hd * p["norm"].double(), 1)
+    R.check_codes(o["c"], q)
+    R.check_scales(o["s"], s / torch.sqrt((hd * hd).mean(1, keepdim=True) + 1e-6), 24 * U24)
+    R.check_product(o["qkv"], o["c"], o["s"], p["w"], p["sw"])
+    at = offsets.tolist()
+    check_grouped(o["gu"], o["c"], o["s"], p["gu"], p["sgu"], at, rows)
+    gate, up = o["gu"].double().chunk(2, 1)
+    q, s = R.rounded(gate * torch.sigmoid(gate) * up, 1)
+    R.check_codes(o["a"], q, 19 * U24)
+    R.check_scales(o["sa"], s, 9 * U24)
+    check_grouped(o["y"], o["a"], o["sa"], p["down"], p["sdown"], at)
+
+
+@pytest.mark.parametrize("tokens", [1, 7, 64, 500])
+def test_a_layer(tokens):
+    args = layer_inputs(tokens, tokens)
+    check_layer(layer(*args), *args)
+
+
+def test_a_layer_captured_and_replayed_with_other_inputs():
+    args = list(layer_inputs(24, 5))
+    h, r, p, ids, offsets, rows = args
+    layer(*args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(*args)
+    for seed in (30, 31, 32):
+        new = layer_inputs(24, seed)
+        for a, b in zip((h, r, offsets, rows), (new[0], new[1], new[4], new[5])):
+            a.copy_(b)
+        graph.replay()
+        eager = layer(h, r, p, new[3], offsets, rows)
+        torch.cuda.synchronize()
+        for name in out:
+            assert torch.equal(out[name].view(torch.uint8), eager[name].view(torch.uint8)), name
+        check_layer(out, h, r, p, new[3], offsets, rows)
+
+
+def test_two_streams_at_once():
+    a, b = layer_inputs(100, 1), layer_inputs(300, 2)
+    want = [layer(*a), layer(*b)]
+    torch.cuda.synchronize()
+    s = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(4):
+        for i, args in enumerate((a, b)):
+            with torch.cuda.stream(s[i]):
+                got[i].append(layer(*args))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o in got[i]:
+            for name in o:
+                assert torch.equal(o[name].view(torch.uint8), want[i][name].view(torch.uint8)), name
+
+
+def test_more_leading_dimensions_and_single_rows():
+    x = rnd(2, 3, 300, seed=1)
+    w, sw = matrix(140, 300, 2, 128)
+    norm = torch.ones(300, device=DEV, dtype=BF)
+    for v in (x, x[0, 0], x[:, 1], x.transpose(0, 1)):
+        flat = v.reshape(-1, 300)
+        for got, want in ((F.quantize_fp8_blocks(v), F.quantize_fp8_blocks(flat)),
+                          (F.silu_mul_fp8_blocks(v, v), F.silu_mul_fp8_blocks(flat, flat)),
+                          (F.rmsnorm_fp8_blocks(v, norm, 1e-6, v), F.rmsnorm_fp8_blocks(flat, norm, 1e-6, flat))):
+            for a, b in zip(got, want):
+                assert a.shape[:-1] == v.shape[:-1]
+                assert torch.equal(a.contiguous().view(torch.uint8).reshape(-1), b.view(torch.uint8).reshape(-1))
+        c, s = F.quantize_fp8_blocks(v)
+        y = F.linear_fp8_blocks(c, s, w, sw)
+        assert y.shape == (*v.shape[:-1], 140)
+        assert torch.equal(y.reshape(-1, 140), F.linear_fp8_blocks(*F.quantize_fp8_blocks(flat), w, sw))
+
+
+def test_no_rows():
+    w, sw = matrix(140, 300, 2, 128)
+    x = torch.zeros(0, 300, device=DEV, dtype=BF)
+    c, s = F.quantize_fp8_blocks(x)
+    assert F.linear_fp8_blocks(c, s, w, sw).shape == (0, 140)
+    assert F.rmsnorm_fp8_blocks(x, x.new_ones(300), 1e-6)[1].shape == (0, 3)
+    assert F.silu_mul_fp8_blocks(x, x)[0].shape == (0, 300)
+    assert F.grouped_linear_fp8_blocks(c, s, w[None], sw[None], i32([0, 0])).shape == (0, 140)
