@@ -41,54 +41,101 @@ struct Args {
   int wide;       // y's rows begin at multiples of 16 bytes
 };
 
-// this workgroup's tile: neighbours in the order of tiles run on one XCD (workgroup i runs on XCD i % 8) and
-// share its L2; within a band of kBand token tiles the tiles of one feature block follow each other
+// Tile t in the order that shares most: within a band of kBand token tiles the tiles of one feature block follow
+// each other.
 constexpr int kBand = 8;
-__device__ __forceinline__ bool tile_of(const Args& a, int& tm, int& tn) {
-  const int64_t total = (int64_t)a.mt * a.nt, per = (total + 7) / 8;
-  const int64_t t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= per || t >= total) return false;
-  const int64_t band = t / ((int64_t)kBand * a.nt);
-  const int r = static_cast<int>(t - band * kBand * a.nt), high = min(kBand, a.mt - (int)band * kBand);
+__device__ __forceinline__ void tile_at(uint32_t t, int mt, int nt, int& tm, int& tn) {
+  const uint32_t band = t / ((uint32_t)kBand * nt), r = t - band * kBand * nt;
+  const uint32_t high = min((uint32_t)kBand, mt - band * kBand);
   tn = r / high;
-  tm = (int)band * kBand + r - tn * high;
+  tm = band * kBand + r - tn * high;
+}
+
+// Up to 64 groups' rows and token tiles, a group a lane.  Offsets are held to [0, rows] and ascending.
+struct Groups {
+  int lo, hi;  // rows lo .. hi - 1
+  int tiles;   // of this group and those before it in the 64
+};
+template <int BM>
+__device__ __forceinline__ Groups scan_groups(const Args& a, int base, int least) {
+  const int lane = threadIdx.x & 63, rows = static_cast<int>(a.rows), e = min(base + lane, a.groups - 1);
+  Groups g;
+  g.lo = max(min(max(a.offsets[e], 0), rows), least);
+  const int end = min(max(a.offsets[e + 1], 0), rows);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) g.lo = max(g.lo, __shfl_up(g.lo, o, 64));  // the lowest lanes: their own
+  g.hi = max(end, g.lo);
+  g.tiles = base + lane < a.groups ? (g.hi - g.lo + BM - 1) / BM : 0;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int s = __shfl_up(g.tiles, o, 64);
+    if (lane >= o) g.tiles += s;
+  }
+  return g;
+}
+
+// the group and rows of the 64 groups' token tile tm, if it is one of theirs
+template <int BM>
+__device__ __forceinline__ bool find_tile(const Groups& g, int tm, int& l, int64_t& m0, int& count) {
+  const uint64_t past = __ballot(g.tiles > tm);
+  if (!past) return false;
+  l = __builtin_ctzll(past);
+  const int before = l ? __builtin_amdgcn_readlane(g.tiles, l - 1) : 0;
+  const int r0 = __builtin_amdgcn_readlane(g.lo, l) + (tm - before) * BM;
+  m0 = r0;
+  count = min(BM, __builtin_amdgcn_readlane(g.hi, l) - r0);
   return true;
 }
 
-// The group and rows of token tile tm: offsets held to [0, rows] and ascending; every wave scans them for itself,
-// 64 groups at a time.  False where there are fewer tiles.
+// all groups' token tiles; `last`: what the last 64 (up to 64: all) groups are
 template <int BM>
-__device__ __forceinline__ bool group_of(const Args& a, int tm, int& group, int64_t& m0, int& count) {
-  const int lane = threadIdx.x & 63, rows = static_cast<int>(a.rows);
-  int before = 0, least = 0;  // tiles of the groups before, the largest offset so far
+__device__ __forceinline__ int all_tiles(const Args& a, Groups& last) {
+  int sum = 0, least = 0;
   for (int base = 0; base < a.groups; base += 64) {
-    const int e = min(base + lane, a.groups - 1);
-    int lo = min(max(a.offsets[e], 0), rows), hi = min(max(a.offsets[e + 1], 0), rows);
-    lo = max(lo, least);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) lo = max(lo, __shfl_up(lo, o, 64));  // lane 0's own: shfl_up returns it
-    hi = max(hi, lo);
-    const int tiles = base + lane < a.groups ? (hi - lo + BM - 1) / BM : 0;
-    int sum = tiles;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int s = __shfl_up(sum, o, 64);
-      if (lane >= o) sum += s;
-    }
-    const uint64_t past = __ballot(before + sum > tm);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      group = base + l;
-      const int in = tm - before - __builtin_amdgcn_readlane(sum - tiles, l);
-      const int r0 = __builtin_amdgcn_readlane(lo, l) + in * BM;
-      m0 = r0;
-      count = min(BM, __builtin_amdgcn_readlane(hi, l) - r0);
-      return true;
-    }
-    before += __builtin_amdgcn_readlane(sum, 63);
-    least = __builtin_amdgcn_readlane(hi, 63);
+    last = scan_groups<BM>(a, base, least);
+    sum += __builtin_amdgcn_readlane(last.tiles, 63);
+    least = __builtin_amdgcn_readlane(last.hi, 63);
   }
-  return false;
+  return sum;
+}
+
+// token tile tm of all groups (there is one); `all`: the groups, where they are up to 64
+template <int BM>
+__device__ __forceinline__ void group_of(const Args& a, const Groups& all, int tm, int& group, int64_t& m0, int& count) {
+  if (a.groups <= 64) {
+    find_tile<BM>(all, tm, group, m0, count);
+    return;
+  }
+  int least = 0;
+  for (int base = 0; base < a.groups; base += 64) {
+    const Groups g = scan_groups<BM>(a, base, least);
+    if (find_tile<BM>(g, tm, group, m0, count)) {
+      group += base;
+      return;
+    }
+    tm -= __builtin_amdgcn_readlane(g.tiles, 63);
+    least = __builtin_amdgcn_readlane(g.hi, 63);
+  }
+}
+
+// This workgroup's tile, if it has one: neighbours in tile_at's order run on one XCD (workgroup i runs on XCD
+// i % 8) and share its L2.
+template <int BM, bool GROUPED>
+__device__ __forceinline__ bool tile_of(const Args& a, int& tn, int& group, int64_t& m0, int& count) {
+  Groups all;
+  const int mt = GROUPED ? all_tiles<BM>(a, all) : a.mt;
+  const uint32_t total = (uint32_t)mt * a.nt, per = (total + 7) / 8;
+  const uint32_t t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= per || t >= total) return false;
+  int tm;
+  tile_at(t, mt, a.nt, tm, tn);
+  if constexpr (GROUPED) {
+    group_of<BM>(a, all, tm, group, m0, count);
+  } else {
+    m0 = (int64_t)tm * BM;
+    count = static_cast<int>(min((int64_t)BM, a.rows - m0));
+  }
+  return true;
 }
 
 __device__ __forceinline__ void store4(const Args& a, int64_t m, int n, const floatx4_t& v) {
@@ -168,15 +215,9 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Args a) {
   using Operand = std::conditional_t<EXACT, Decoded, Codes>;
   __shared__ __attribute__((aligned(16))) uint8_t lds[(BM + BN) * 128];
   __shared__ float lsx[BM];
-  int tm, tn, group = 0, count;
+  int tn, group = 0, count;
   int64_t m0;
-  if (!tile_of(a, tm, tn)) return;
-  if constexpr (GROUPED) {
-    if (!group_of<BM>(a, tm, group, m0, count)) return;
-  } else {
-    m0 = (int64_t)tm * BM;
-    count = static_cast<int>(min((int64_t)BM, a.rows - m0));
-  }
+  if (!tile_of<BM, GROUPED>(a, tn, group, m0, count)) return;
   const int n0 = tn * BN, lane = threadIdx.x & 63, wv = threadIdx.x >> 6, wm = wv % WM, wn = wv / WM;
   const int li = lane & 15, kg = lane >> 4, nch = (a.K + kFp8Block - 1) / kFp8Block;
   const float* sw = a.sw + group * a.swgs + (n0 / kFp8Block) * a.sws;
@@ -245,19 +286,524 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Args a) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// The same product with both operands streamed into LDS without registers (global_load_lds), for rows of whole
+// 16 codes at multiples of 16 bytes.  KW groups of WM x WN waves share the tile and take every KW-th block of
+// K; each group has a ring of ST stages of its own, ST - 1 of them requested ahead.  The scales of a stage's
+// block come the same way, 64 a load.  A group of one wave needs no barrier: its own waits order its loads
+// and reads.  At the end the groups' sums meet in LDS, in fixed order.
+// ---------------------------------------------------------------------------
+// 16 (4) bytes a lane from src to LDS, lane after lane from dst; in functions of their own: with the builtin in a
+// template hipcc drops the kernel's host launch stub
+__device__ __forceinline__ void load_lds16(const void* src, uint8_t* dst) {
+  __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+// with the non-temporal hint: bytes that nothing reads again soon
+__device__ __forceinline__ void load_lds16_nt(const void* src, uint8_t* dst) {
+  __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)dst, 16, 0, 2);
+}
+__device__ __forceinline__ void load_lds4(const void* src, uint8_t* dst) {
+  __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)dst, 4, 0, 0);
+}
+
+// 16 bytes a lane at base + voffset + soffset to LDS; zeros where voffset is past the resource's size
+__device__ __forceinline__ void buffer_lds16(__amdgpu_buffer_rsrc_t base, uint8_t* dst, int voffset, int soffset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (__attribute__((address_space(3))) void*)dst, 16, voffset, soffset, 0, 0);
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(bytes), 0x00020000);
+}
+
+template <int WM, int WN, int TT, int FT, int KW, int ST>
+struct Ring {
+  static constexpr int BM = 16 * TT * WM, BN = 16 * FT * WN, NW = WM * WN;
+  static constexpr int DI = (BM + BN) / 8 / NW;               // loads of codes a wave and stage
+  static constexpr int NB = BN > 128 ? BN / 128 : 1;           // scales of features
+  static constexpr int XS = (BM + NB + 63) / 64;               // loads of scales: the tokens', then the features'
+  static constexpr int SI = (XS + NW - 1) / NW;                // loads of scales a wave and stage
+  static constexpr int kCodes = (BM + BN) * 128, kStage = kCodes + SI * NW * 256;
+  static constexpr int kRing = KW * ST * kStage;
+  static constexpr int kLds = KW > 1 && KW * NW * TT * FT * 1024 > kRing ? KW * NW * TT * FT * 1024 : kRing;
+  static constexpr int kThreads = 64 * NW * KW;
+  static_assert((BM + BN) % (8 * NW) == 0 && BM % 8 == 0 && kLds <= 160 * 1024, "tile");
+  static_assert(BN <= 128 ? 128 % BN == 0 : BN % 128 == 0, "a tile's features are whole blocks or in one");
+  static_assert(ST >= 2 && (ST - 2) * (DI + SI) < 64, "vmcnt counts to 63");
+};
+
+template <int WM, int WN, int TT, int FT, int KW, int ST, bool NT, bool EXACT, bool GROUPED>
+__global__ __launch_bounds__(64 * WM * WN * KW) void ring_kernel(const Args a) {
+  using R = Ring<WM, WN, TT, FT, KW, ST>;
+  using Operand = std::conditional_t<EXACT, Decoded, Codes>;
+  static_assert(!NT || WM * WN == 1, "a load is of tokens or of features");
+  constexpr int BM = R::BM, BN = R::BN, NW = R::NW, DI = R::DI, SI = R::SI;
+  extern __shared__ __attribute__((aligned(16))) uint8_t ring[];
+  int tn, group = 0, count;
+  int64_t m0;
+  if (!tile_of<BM, GROUPED>(a, tn, group, m0, count)) return;
+  const int n0 = tn * BN, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kw = wave / NW, wv = wave % NW, wm = wv % WM, wn = wv / WM;
+  const int li = lane & 15, kg = lane >> 4, nch = (a.K + kFp8Block - 1) / kFp8Block;
+  // the row of x behind row t of the tile; -1: none, and zeros are read for it
+  auto x_row = [&](int t) -> int64_t {
+    if (t >= count) return -1;
+    if (!GROUPED || !a.index) return m0 + t;
+    const int64_t r = a.index[m0 + t];
+    return r >= 0 && r < a.xrows ? r : -1;
+  };
+  const uint8_t* zeros = reinterpret_cast<const uint8_t*>(kZeros);
+  const uint8_t* src[DI];
+  int lim[DI];  // codes of the row from src on
+#pragma unroll
+  for (int j = 0; j < DI; ++j) {
+    const int r = (wv * DI + j) * 8 + (lane >> 3), q = r - BM;
+    const int key = r < BM ? r & 7 : (q & 3) | (q / (4 * FT) & 1) << 2, at = ((lane & 7) ^ key) * 16;
+    const int64_t row = r < BM ? x_row(r) : min(n0 + q, a.N - 1);
+    src[j] = (r < BM ? a.x + row * a.xs : a.w + group * a.wgs + row * a.ws) + at;
+    lim[j] = row < 0 ? 0 : a.K - at;
+  }
+  const float* ssrc[SI];
+#pragma unroll
+  for (int j = 0; j < SI; ++j) {
+    const int i = (wv + NW * j) * 64 + lane;  // one more scale a lane than needed costs a line of memory each
+    ssrc[j] = nullptr;
+    if (i < BM) {
+      const int64_t row = x_row(i);
+      if (row >= 0) ssrc[j] = a.sx + row * a.sxs;
+    } else if (i < BM + R::NB) {
+      ssrc[j] = a.sw + group * a.swgs + min(n0 / kFp8Block + i - BM, (a.N - 1) / kFp8Block) * a.sws;
+    }
+  }
+  uint8_t* const mine = ring + kw * ST * R::kStage;
+  auto issue = [&](int c, int stage) {
+    uint8_t* const to = mine + stage * R::kStage;
+#pragma unroll
+    for (int j = 0; j < DI; ++j) {
+      const uint8_t* const from = c * kFp8Block < lim[j] ? src[j] + c * kFp8Block : zeros;
+      if (NT && j * 8 >= BM) load_lds16_nt(from, to + (wv * DI + j) * 1024);
+      else load_lds16(from, to + (wv * DI + j) * 1024);
+    }
+    const int cs = min(c, nch - 1);
+#pragma unroll
+    for (int j = 0; j < SI; ++j)
+      load_lds4(ssrc[j] ? ssrc[j] + cs : reinterpret_cast<const float*>(zeros), to + R::kCodes + (wv + NW * j) * 256);
+  };
+  floatx4_t acc[TT][FT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+#pragma unroll
+    for (int f = 0; f < FT; ++f) acc[t][f] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+  const int piece = (kg ^ (li & 7)) * 16;
+  const int xat = (wm * TT * 16 + li) * 128, wat = (BM + wn * FT * 16 + (li >> 2) * 4 * FT + (li & 3)) * 128;
+  const int sxat = R::kCodes + (wm * TT * 16 + li) * 4, swat = R::kCodes + (BM + wn * FT * 16 / kFp8Block) * 4;
+  const int steps = (nch + KW - 1) / KW;
+#pragma unroll
+  for (int s = 0; s + 1 < ST; ++s) issue(s * KW + kw, s);
+  int st = 0;
+  for (int i = 0; i < steps; ++i) {
+    // this wave's loads of stage st have landed and its reads of the stage before are done, then every wave's
+    __builtin_amdgcn_s_waitcnt(vmcnt_only((ST - 2) * (DI + SI)) & ~0xf00);
+    asm volatile("" ::: "memory");
+    if constexpr (NW > 1) {
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    }
+    const int c = i * KW + kw;
+    issue(c + (ST - 1) * KW, st == 0 ? ST - 1 : st - 1);
+    if (c < nch) {
+      const uint8_t* const from = mine + st * R::kStage;
+      auto frag = [&](int at) {
+        const int4v u = *reinterpret_cast<const int4v*>(from + at + piece);
+        const int4v v = *reinterpret_cast<const int4v*>(from + at + (piece ^ 64));
+        return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+      };
+      Operand wf[FT];
+#pragma unroll
+      for (int f = 0; f < FT; ++f) operand(frag(wat + f * 4 * 128), wf[f]);
+      const float s = *reinterpret_cast<const float*>(from + swat);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        Operand xf;
+        operand(frag(xat + t * 16 * 128), xf);
+        const float f0 = s * *reinterpret_cast<const float*>(from + sxat + t * 64);
+#pragma unroll
+        for (int f = 0; f < FT; ++f) {
+          const floatx4_t p = block_sum(wf[f], xf);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[t][f][e] = __builtin_fmaf(f0, p[e], acc[t][f][e]);
+        }
+      }
+    }
+    st = st + 1 == ST ? 0 : st + 1;
+  }
+  // what was requested past the last block must land before the ring is used again or released
+  __builtin_amdgcn_s_waitcnt(vmcnt_only(0) & ~0xf00);
+  const int col = n0 + wn * FT * 16 + kg * 4 * FT;
+  if constexpr (KW == 1) {
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      const int m = wm * TT * 16 + t * 16 + li;
+      if (m < count) {
+#pragma unroll
+        for (int f = 0; f < FT; ++f) store4(a, m0 + m, col + f * 4, acc[t][f]);
+      }
+    }
+  } else {
+    // every group leaves its sums; group i adds up and stores the wave's pieces i, i + KW, ...
+    floatx4_t* const sums = reinterpret_cast<floatx4_t*>(ring) + wv * TT * FT * 64 + lane;
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+      for (int f = 0; f < FT; ++f) sums[(kw * NW * TT * FT + t * FT + f) * 64] = acc[t][f];
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < TT * FT; b += KW) {
+      const int i = b + kw;
+      if (TT * FT % KW != 0 && i >= TT * FT) break;
+      floatx4_t v = sums[i * 64];
+#pragma unroll
+      for (int k = 1; k < KW; ++k) {
+        const floatx4_t u = sums[(k * NW * TT * FT + i) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += u[e];
+      }
+      const int m = wm * TT * 16 + i / FT * 16 + li;
+      if (m < count) store4(a, m0 + m, col + i % FT * 4, v);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: 256 tokens x 256 features by 8 waves of 128 x 64, K in blocks through two LDS stages of 64 KB; up to 256
+// workgroups go through the tiles.  The one barrier of a block stands before its last two token tiles: all waves'
+// fragments of the block are in registers then, so its stage takes the loads of the block after the next, and the
+// next block's first fragments are read under the matrix instructions that are left.  Sums are added three
+// instructions behind.  The next tile's first two blocks follow this one's last two without a gap.
+// ---------------------------------------------------------------------------
+struct Big {
+  static constexpr int BM = 256, BN = 256, kThreads = 512, kWgs = 256;
+  static constexpr int kStage = (BM + BN) * 128;
+  // scales of eight blocks: of the tokens [256][8], the places of tokens 8 i + 8 .. 8 i + 15, i even, exchanged by xor 4 (banks),
+  // then of the features' two blocks [2][8], four copies; two such windows, and the addresses of the tokens' scales
+  static constexpr int kWindow = BM * 32 + 4 * 256, kScales = 2 * kStage, kRows = kScales + 2 * kWindow;
+  static constexpr int kGroups = kRows + BM * 8, kUnused = kGroups + 64 * 12, kLds = kUnused + 8 * 256;
+};
+
 template <bool GROUPED>
-int launch(Args a, hipStream_t st) {
-  constexpr int BM = 64, BN = 64;
-  const int64_t mt = GROUPED ? (a.rows + min(a.rows, (int64_t)a.groups) * (BM - 1)) / BM : (a.rows + BM - 1) / BM;
-  const int64_t nt = (a.N + BN - 1) / BN;
-  // a launch has fewer than 2^32 threads
-  DSV2_REQUIRE(mt * nt <= 0xfffff8, DSV2_E_SHAPE, "linear_fp8_blocks: %lld rows of %d", (long long)a.rows, a.N);
+__global__ __launch_bounds__(512) void big_kernel(const Args a) {
+  constexpr int BM = Big::BM, BN = Big::BN;
+  extern __shared__ __attribute__((aligned(16))) uint8_t ring[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave & 1, wn = wave >> 1, li = lane & 15, kg = lane >> 4, nch = (a.K + kFp8Block - 1) / kFp8Block;
+  const bool gather = GROUPED && a.index;
+  // the tiles of this XCD's workgroups: neighbours in tile_at's order
+  int mt = a.mt;
+  Groups* const all = reinterpret_cast<Groups*>(ring + Big::kGroups);  // up to 64 groups
+  if constexpr (GROUPED) {
+    Groups g;
+    mt = all_tiles<BM>(a, g);
+    if (wave == 0) all[lane] = g;
+    __syncthreads();
+  }
+  const uint32_t total = (uint32_t)mt * a.nt, per = (total + 7) / 8, last = min(((blockIdx.x & 7) + 1) * per, total);
+  uint32_t at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (at >= last) return;
+
+  // the tile whose blocks are requested
+  int group = 0, count = 0, n0 = 0;
+  int64_t m0 = 0;
+  // Loads: waves 0 to 3 the tokens' rows, 4 to 7 the features', 64 each, by offsets that lie past the buffer for what
+  // is not there (zeros).  The lane's 16-byte piece of its rows: of even and odd eights of rows, for tokens the same.
+  const int at0 = ((lane & 7) ^ (wave < 4 ? lane >> 3 : lane >> 3 & 3)) * 16, at1 = wave < 4 ? at0 : at0 ^ 64;
+  constexpr uint32_t kPast = 0x80000000u;
+  __amdgpu_buffer_rsrc_t codes;
+  uint32_t voff[8];
+  uint64_t swrow = 0;  // of waves 4 to 7
+  const uint64_t own = wave < 4 ? ~0ull : 0ull;
+  // the addresses of the tokens' scales; for a row that x does not have that of a zero, plus 1
+  uint64_t* const srows = reinterpret_cast<uint64_t*>(ring + Big::kRows);
+  auto enter = [&](uint32_t tile) {
+    int tm, tn;
+    tile_at(tile, mt, a.nt, tm, tn);
+    if constexpr (GROUPED) {
+      group_of<BM>(a, all[lane], tm, group, m0, count);
+    } else {
+      m0 = (int64_t)tm * BM;
+      count = static_cast<int>(min((int64_t)BM, a.rows - m0));
+    }
+    n0 = tn * BN;
+    codes = buffer(wave >= 4 ? a.w + group * a.wgs + n0 * a.ws : gather ? a.x : a.x + m0 * a.xs, kPast);
+    const uint32_t stride = static_cast<uint32_t>(wave >= 4 ? a.ws : a.xs);
+    const int most = wave >= 4 ? a.N - 1 - n0 : count - 1;  // rows past the tile's: its last one
+    if (gather && wave < 4) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = a.index[m0 + min(wave * 64 + j * 8 + (lane >> 3), most)];
+        voff[j] = r >= 0 && r < a.xrows ? r * stride + (j & 1 ? at1 : at0) : kPast;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        voff[j] = min((wave & 3) * 64 + j * 8 + (lane >> 3), most) * stride + (j & 1 ? at1 : at0);
+    }
+    swrow = ~own & reinterpret_cast<uint64_t>(
+                       a.sw + group * a.swgs + min(n0 / kFp8Block + (lane >> 3 & 1), (a.N - 1) / kFp8Block) * a.sws);
+    if (threadIdx.x < BM) {
+      int64_t row = m0 + min((int)threadIdx.x, count - 1);
+      if (gather) row = a.index[row];
+      srows[threadIdx.x] = row < 0 || row >= a.xrows ? reinterpret_cast<uint64_t>(kZeros) + 1 : reinterpret_cast<uint64_t>(a.sx + row * a.sxs);
+    }
+  };
+  // no branch in these two: in the middle of a block's instructions one costs the loop over 100 spilled registers
+  auto issue = [&](int c, int stage) {
+    uint8_t* const to = ring + stage * Big::kStage;
+    const int k = c * kFp8Block;
+    // pieces past the rows' end lie past the buffer: zeros
+    const uint32_t out0 = k + at0 < a.K ? 0u : kPast, out1 = k + at1 < a.K ? 0u : kPast;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) buffer_lds16(codes, to + (wave * 8 + j) * 1024, voff[j] | (j & 1 ? out1 : out0), k);
+  };
+  // an eighth of a window: waves 0 to 3 eight tokens' scales each, the others the features' (each its own copy)
+  const int swap = wave < 4 ? (wave & 1) << 2 : 0;
+  auto scales = [&](int part, int window0) {  // part: counted over the tile's windows
+    const int in = part & 7, first = part & ~7, t = in * 32 + (wave & 3) * 8 + (lane >> 3);
+    const uint64_t row = srows[t] & own | swrow;
+    const int b = row & 1 ? 0 : min(first + ((lane & 7) ^ swap), nch - 1);
+    const int window = Big::kScales + ((part >> 3) + window0 & 1) * Big::kWindow;
+    const int to = wave < 4 ? (in * 4 + wave) * 256 : BM * 32 + (wave - 4) * 256;
+    // a window past the last block's goes where nothing is read, not into the next tile's first
+    load_lds4(reinterpret_cast<const float*>(row & ~1ull) + b, ring + (first < nch ? window + to : Big::kUnused + wave * 256));
+  };
+  floatx4_t acc[8][4];
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+#pragma unroll
+    for (int f = 0; f < 4; ++f) acc[t][f] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+  const int piece = (kg ^ (li & 7)) * 16;
+  const int xat = (wm * 128 + li) * 128, wat = (BM + wn * 64 + (li >> 2) * 8 + (li & 3)) * 128;
+  const int sxat = (wm * 128 + li) * 32, sxkey = li >> 3 << 2, swat = BM * 32 + (wn >> 1) * 32;
+  auto frag = [&](const uint8_t* from, int at) {
+    const int4v u = *reinterpret_cast<const int4v*>(from + at + piece);
+    const int4v v = *reinterpret_cast<const int4v*>(from + at + (piece ^ 64));
+    return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  // This wave's loads have landed and its reads are done, then every wave's.  Behind a tile's end its 16 stores may be on
+  // their way still (the branch is written out: the compiler's would cut the block's instructions in two).
+  int stores = 0;
+  auto meet = [&] {
+    asm volatile(
+        "s_cmp_lg_u32 %0, 0\n\ts_cbranch_scc1 .Lstores%=\n\ts_waitcnt vmcnt(0)\n.Lstores%=:\n\t"
+        "s_waitcnt vmcnt(16) lgkmcnt(0)\n\ts_barrier" ::"s"(stores)
+        : "memory", "scc");
+  };
+  int8v wf[4], xf[3];
+  float nx[8], nw;
+  auto first_reads = [&](const uint8_t* from, int c, int window0) {
+#pragma unroll
+    for (int f = 0; f < 4; ++f) wf[f] = frag(from, wat + (f >> 1) * 4096 + (f & 1) * 512);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) xf[t] = frag(from, xat + t * 2048);
+    const uint8_t* const win = ring + Big::kScales + ((c >> 3) + window0 & 1) * Big::kWindow;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) nx[t] = *reinterpret_cast<const float*>(win + sxat + ((c & 7) ^ sxkey) * 4 + t * 512);
+    nw = *reinterpret_cast<const float*>(win + swat + (c & 7) * 4);
+  };
+  enter(at);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 9; ++i) scales(i, 0);
+  issue(0, 0);
+  meet();
+  issue(1, 1);
+  int stage = 0, window = 0;  // the block's stage, the tile's first window's place
+  int kc = 2, kwin = 0;       // the block that is requested (of this tile or the next), its tile's first window
+  first_reads(ring, 0, 0);
+  for (;;) {
+    const int64_t om0 = m0;
+    const int ocount = count, on0 = n0;
+    for (int c = 0; c < nch; ++c) {
+      if (c == nch - 2) {  // what is requested from here on is the next tile's
+        at += (gridDim.x + 7) >> 3;
+        kc = 0;
+        kwin = window + ((nch - 1) >> 3) + 1 & 1;  // not where this tile's last scales are
+        if (at < last) {
+          enter(at);
+          __builtin_amdgcn_s_waitcnt(vmcnt_only(63) & ~0xf00);
+          __builtin_amdgcn_s_barrier();  // srows is written
+          asm volatile("" ::: "memory");
+#pragma unroll
+          for (int i = 0; i < 7; ++i) scales(i, kwin);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) voff[j] = kPast;
+        }
+      }
+      const uint8_t* const from = ring + stage * Big::kStage;
+      float sx[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) sx[t] = nx[t] * nw;
+      floatx4_t p[4];
+#pragma unroll
+      for (int i = 0; i < 32 + 3; ++i) {
+        const int t = i >> 2, f = i & 3;
+        __builtin_amdgcn_sched_barrier(0);
+        if (i < 32) {
+          p[i & 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[f], xf[t % 3], floatx4_t{0.f, 0.f, 0.f, 0.f}, 0, 0,
+                                                                      0, 0, 0, 0);
+          if (f == 0 && t < 6) xf[(t + 2) % 3] = frag(from, xat + (t + 2) * 2048);
+          if (i == 23) {
+            meet();
+            stores = 0;
+            issue(kc, stage);
+            scales(kc + 7, kwin);
+          }
+        }
+        if (i >= 3) {
+          const int tt = (i - 3) >> 2, ff = (i - 3) & 3;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[tt][ff][e] = __builtin_fmaf(sx[tt], p[(i - 3) & 3][e], acc[tt][ff][e]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      stage ^= 1;
+      ++kc;
+      const bool end = c + 1 == nch;
+      first_reads(ring + stage * Big::kStage, end ? 0 : c + 1, end ? kwin : window);
+    }
+    window = kwin;
+    // lane group kg holds features 8 kg .. 8 kg + 7 of each half of the wave's 64
+    int r0 = wm * 128 + li;
+    asm volatile("" : "+v"(r0));  // here: kept over the loop the rows' offsets are spilled, and a reload waits for the stores
+    const int col = on0 + wn * 64 + kg * 8;
+    // as many stores for every wave, so that the next block's wait may leave them on their way; what is not the tile's
+    // lies past the buffer
+    const __amdgpu_buffer_rsrc_t out = buffer(static_cast<bf16_t*>(a.y) + om0 * a.ys, kPast);
+    const uint32_t out0 = col < a.N ? col * 2 : kPast, out1 = col + 32 < a.N ? col * 2 + 64 : kPast;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const int m = r0 + t * 16;
+      const uint32_t row = m < ocount ? m * (uint32_t)a.ys * 2 : kPast;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const floatx4_t u = acc[t][2 * i], v = acc[t][2 * i + 1];
+        const u32x4_t w = {pack2(u[0], u[1]), pack2(u[2], u[3]), pack2(v[0], v[1]), pack2(v[2], v[3])};
+        __builtin_amdgcn_raw_buffer_store_b128(w, out, row + (i ? out1 : out0) | (row | (i ? out1 : out0)) & kPast, 0, 0);
+      }
+    }
+    stores = 16;
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) acc[t][f] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+    if (at >= last) break;
+  }
+  __builtin_amdgcn_s_waitcnt(vmcnt_only(0));  // what was requested past the last block must land before the ring is released
+}
+
+// ---------------------------------------------------------------------------
+// Which of them.  A launch of n tiles takes about a + b k us, and for each 256 tiles (one a CU) past the first
+// c + d k more, k the blocks of K (measured at 32 to 6,144 tiles of 4, 16 and 64 blocks on MI355X, off by 3 to 10%
+// on the mean): many waves on small tiles where the launch is short of tiles, larger tiles, which read the
+// operands less often, where it is not.  The least of the estimates is taken.
+// ---------------------------------------------------------------------------
+constexpr int64_t kStreamed = 64ll << 20;
+struct Cost {
+  int bm, bn;
+  float a, b, c, d;
+};
+enum Shape { kFew, kFew32, kTall32, kWide32, kMid, kMid128, kTile128, kLong128, kBig, kShapes };
+constexpr Cost kCost[kShapes] = {
+    {16, 16, 3.4f, 0.06f, 0.69f, 0.09f},    // 8 waves along K
+    {32, 16, 3.8f, 0.06f, 1.85f, 0.07f},    // 8 along K
+    {32, 32, 3.4f, 0.12f, 0.78f, 0.10f},    // 4 along K
+    {32, 64, 4.0f, 0.35f, 0.80f, 0.16f},    // 2 along K
+    {64, 64, 4.2f, 0.27f, 2.25f, 0.31f},    // 4 on the tile, 2 along K
+    {128, 64, 5.2f, 0.44f, 3.18f, 0.51f},   // 4 on the tile, 2 along K
+    {128, 128, 5.7f, 0.68f, 3.86f, 0.74f},  // 8 on the tile
+    {128, 256, 8.0f, 1.10f, 7.89f, 1.22f},  // 8 on the tile
+    {256, 256, 9.3f, 1.51f, 9.12f, 1.71f},  // big_kernel
+};
+
+// token tiles: the most there may be, and as many as are likely (groups of like sizes)
+int64_t most_tiles(const Args& a, bool grouped, int bm) {
+  return grouped ? (a.rows + min(a.rows, (int64_t)a.groups) * (bm - 1)) / bm : (a.rows + bm - 1) / bm;
+}
+float likely_tiles(const Args& a, bool grouped, int bm) {
+  if (!grouped) return static_cast<float>((a.rows + bm - 1) / bm);
+  const float rows = static_cast<float>(a.rows), hit = a.groups * (1.f - expf(-rows / a.groups));
+  return fmaxf(hit, rows / bm + 0.5f * hit);
+}
+
+Shape choose(const Args& a, bool grouped, bool big) {
+  const float k = static_cast<float>((a.K + kFp8Block - 1) / kFp8Block);
+  Shape best = kFew;
+  float least = 3e38f;
+  for (int s = 0; s < (big ? kShapes : kBig); ++s) {
+    const Cost& c = kCost[s];
+    float n = likely_tiles(a, grouped, c.bm) * ((a.N + c.bn - 1) / c.bn) * (1.f / 256);
+    if (s == kBig) n = ceilf(n);
+    const float t = c.a + c.b * k + fmaxf(n - 1.f, 0.f) * (c.c + c.d * k);
+    if (t < least) least = t, best = static_cast<Shape>(s);
+  }
+  return best;
+}
+
+bool set_tiles(Args& a, bool grouped, int bm, int bn, int threads) {
+  const int64_t mt = most_tiles(a, grouped, bm), nt = (a.N + bn - 1) / bn;
   a.mt = (int)mt;
   a.nt = (int)nt;
-  const dim3 grid((unsigned)((mt * nt + 7) / 8 * 8));
-  if (a.out_f32) product_kernel<2, 2, 2, 2, true, GROUPED><<<grid, 256, 0, st>>>(a);
-  else product_kernel<2, 2, 2, 2, false, GROUPED><<<grid, 256, 0, st>>>(a);
+  if (mt * nt <= (1ll << 32) / threads - 8) return true;  // a launch has fewer than 2^32 threads
+  dsv2_set_error("linear_fp8_blocks: %lld rows of %d", (long long)a.rows, a.N);
+  return false;
+}
+dim3 grid_of(const Args& a) { return dim3((unsigned)(((int64_t)a.mt * a.nt + 7) / 8 * 8)); }
+
+template <int WM, int WN, int TT, int FT, int KW, int ST, bool NT, bool EXACT, bool GROUPED>
+int launch_ring(Args a, hipStream_t st) {
+  using R = Ring<WM, WN, TT, FT, KW, ST>;
+  if (!set_tiles(a, GROUPED, R::BM, R::BN, R::kThreads)) return DSV2_E_SHAPE;
+  ring_kernel<WM, WN, TT, FT, KW, ST, NT, EXACT, GROUPED><<<grid_of(a), R::kThreads, R::kLds, st>>>(a);
   return dsv2_launch_status(GROUPED ? "grouped_linear_fp8_blocks" : "linear_fp8_blocks");
+}
+
+template <bool GROUPED>
+int launch_big(Args a, hipStream_t st) {
+  if (!set_tiles(a, GROUPED, Big::BM, Big::BN, Big::kThreads)) return DSV2_E_SHAPE;
+  dim3 grid = grid_of(a);
+  grid.x = min(grid.x, (unsigned)Big::kWgs);
+  big_kernel<GROUPED><<<grid, Big::kThreads, Big::kLds, st>>>(a);
+  return dsv2_launch_status(GROUPED ? "grouped_linear_fp8_blocks" : "linear_fp8_blocks");
+}
+
+template <bool EXACT, bool GROUPED>
+int launch(Args a, hipStream_t st) {
+  const bool rows16 = a.K % 16 == 0 && dsv2_aligned16(a.x) && dsv2_aligned16(a.w) && a.xs % 16 == 0 && a.ws % 16 == 0 &&
+                      a.wgs % 16 == 0;
+  if (!rows16) {
+    if (!set_tiles(a, GROUPED, 64, 64, 256)) return DSV2_E_SHAPE;
+    product_kernel<2, 2, 2, 2, EXACT, GROUPED><<<grid_of(a), 256, 0, st>>>(a);
+    return dsv2_launch_status(GROUPED ? "grouped_linear_fp8_blocks" : "linear_fp8_blocks");
+  }
+  // Weights that are read once and do not stay in the 256 MB of the last-level cache: one wave a tile, many
+  // workgroups a CU, and the non-temporal hint.
+  if (a.rows <= 16 * (GROUPED ? (int64_t)a.groups : 1) && (int64_t)a.groups * a.N * a.K >= kStreamed)
+    return launch_ring<1, 1, 1, 2, 1, 3, true, EXACT, GROUPED>(a, st);
+  // big_kernel's offsets are 31 bits: those of its tile's rows, or of all of x where rows are taken by number
+  constexpr int64_t kReach = 1ll << 31;
+  const bool big = !EXACT && a.wide && a.N % 8 == 0 && a.K > kFp8Block && a.xrows > 0 &&
+                   256 * a.ws + a.K < kReach && 512 * a.ys < kReach &&
+                   (a.index ? a.xrows : 256) * a.xs + a.K < kReach;
+  switch (choose(a, GROUPED, big)) {
+    case kFew: return launch_ring<1, 1, 1, 1, 8, 2, false, EXACT, GROUPED>(a, st);
+    case kFew32: return launch_ring<1, 1, 2, 1, 8, 2, false, EXACT, GROUPED>(a, st);
+    case kTall32: return launch_ring<1, 1, 2, 2, 4, 2, false, EXACT, GROUPED>(a, st);
+    case kWide32: return launch_ring<1, 1, 2, 4, 2, 2, false, EXACT, GROUPED>(a, st);
+    case kMid: return launch_ring<2, 2, 2, 2, 2, 3, false, EXACT, GROUPED>(a, st);
+    case kMid128: return launch_ring<2, 2, 4, 2, 2, 3, false, EXACT, GROUPED>(a, st);
+    case kTile128: return launch_ring<2, 4, 4, 2, 1, 4, false, EXACT, GROUPED>(a, st);
+    case kLong128: return launch_ring<2, 4, 4, 4, 1, 3, false, EXACT, GROUPED>(a, st);
+    default: return launch_big<GROUPED>(a, st);
+  }
 }
 
 bool aligned(const void* p, int to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
@@ -284,7 +830,8 @@ int dsv2_linear_fp8_blocks(const void* x, int64_t x_stride, const float* x_scale
   Args a{static_cast<const uint8_t*>(x), x_scales, nullptr, static_cast<const uint8_t*>(w), w_scales, nullptr, y,
          x_stride, x_scales_stride, rows, 0, w_stride, 0, w_scales_stride, y_stride, rows, K, N, 1, 0, 0,
          out_dtype == DSV2_DTYPE_F32, dsv2_aligned16(y) && y_stride * size % 16 == 0};
-  return launch<false>(a, static_cast<hipStream_t>(stream));
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  return a.out_f32 ? launch<true, false>(a, st) : launch<false, false>(a, st);
 }
 
 int dsv2_grouped_linear_fp8_blocks(const void* x, int64_t x_stride, const float* x_scales, int64_t x_scales_stride,
@@ -303,5 +850,6 @@ int dsv2_grouped_linear_fp8_blocks(const void* x, int64_t x_stride, const float*
   Args a{static_cast<const uint8_t*>(x), x_scales, index, static_cast<const uint8_t*>(w), w_scales, offsets, y,
          x_stride, x_scales_stride, x_rows, w_gstride, w_stride, w_scales_gstride, w_scales_stride, y_stride, rows, K, N,
          groups, 0, 0, out_dtype == DSV2_DTYPE_F32, dsv2_aligned16(y) && y_stride * size % 16 == 0};
-  return launch<true>(a, static_cast<hipStream_t>(stream));
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  return a.out_f32 ? launch<true, true>(a, st) : launch<false, true>(a, st);
 }
