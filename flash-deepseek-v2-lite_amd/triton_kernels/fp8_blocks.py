@@ -27,13 +27,15 @@ BLOCK = 128
 MAX_ROWS = 2 ** 31 - 1
 MAX_GROUPS = 65536
 
-# These calls launch kernels of 2 to 10 us for few rows, so their own host time is looked at.
+# These calls launch kernels of 2 to 10 us for few rows, so their own host time is looked at: a launch takes 3 us of it,
+# an attribute of a tensor 0.05 to 0.1, new_empty 1.5, torch's allocation by shape, strides and type alone 0.7.
 _E4M3, _BF16, _F32, _I32 = torch.float8_e4m3fn, torch.bfloat16, torch.float32, torch.int32
 _TYPES = {_BF16: 0, _F32: 1}  # DSV2_DTYPE_*
 _ENTRY = {n: getattr(_hip.lib, n) for n in ("dsv2_quantize_fp8_blocks", "dsv2_rmsnorm_fp8_blocks",
                                             "dsv2_silu_mul_fp8_blocks", "dsv2_linear_fp8_blocks",
                                             "dsv2_grouped_linear_fp8_blocks")}
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
 
 
 def _call(index: int, entry: str, *args) -> None:
@@ -58,6 +60,13 @@ def _device(name: str, *ts: torch.Tensor) -> int:
     return index
 
 
+def _matrix(like: torch.Tensor, n: int, k: int, dtype: torch.dtype) -> torch.Tensor:
+    """An uninitialised [n, k] on the device of `like`."""
+    if _empty_strided is None or not like.is_cuda or _current_device() != like.get_device():
+        return like.new_empty((n, k), dtype=dtype)
+    return _empty_strided((n, k), (k, 1), dtype)
+
+
 def _type(name: str, what: str, t: torch.Tensor) -> int:
     code = _TYPES.get(t.dtype)
     if code is None:
@@ -67,21 +76,25 @@ def _type(name: str, what: str, t: torch.Tensor) -> int:
 
 def _rows(name: str, what: str, t: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
     """(t as a matrix, its rows, its columns, its row stride)."""
-    if t.dim() != 2:
-        if t.dim() == 0:
+    shape = t.shape
+    if len(shape) != 2:
+        if not shape:
             raise ValueError(f"{name}: {what} must have rows, not be a number")
-        t = t.reshape(-1 if t.numel() else math.prod(t.shape[:-1]), t.shape[-1])
-    n, k = t.shape
+        t = t.reshape(math.prod(shape[:-1]), shape[-1])
+        shape = t.shape
+    n, k = shape
     rs, cs = t.stride()
     if k == 0 or n > MAX_ROWS or k > MAX_ROWS - 255:
-        raise ValueError(f"{name}: {what} is {list(t.shape)}")
+        raise ValueError(f"{name}: {what} is {list(shape)}")
     if cs != 1 and k > 1:
         raise NotImplementedError(f"{name}: {what} must have a contiguous last dimension")
     return t, n, k, rs
 
 
-def _outputs(like: torch.Tensor, shape, k: int) -> tuple[torch.Tensor, torch.Tensor]:
-    return like.new_empty(shape, dtype=_E4M3), like.new_empty((*shape[:-1], -(-k // BLOCK)), dtype=_F32)
+def _shaped(like: torch.Tensor, *results: torch.Tensor) -> tuple[torch.Tensor, ...]:
+    """Matrices with the leading dimensions of `like`."""
+    lead = like.shape[:-1]
+    return results if len(lead) == 1 else tuple(r.view(*lead, r.shape[1]) for r in results)
 
 
 def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
@@ -92,12 +105,14 @@ def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Ten
     dtype = _type(name, "x", x)
     if block_rows == 1:
         m, n, k, rs = _rows(name, "x", x)
-        codes, scales = _outputs(x, x.shape, k)
-        gs, groups = 0, 1
-    elif block_rows == BLOCK:
+        codes, scales = _matrix(m, n, k, _E4M3), _matrix(m, n, (k + 127) // BLOCK, _F32)
+        if n:
+            _call(index, "dsv2_quantize_fp8_blocks", m.data_ptr(), rs, 0, 1, n, k, dtype, 1, codes.data_ptr(),
+                  scales.data_ptr())
+        return _shaped(x, codes, scales)
+    if block_rows == BLOCK:
         if x.dim() not in (2, 3):
             raise ValueError(f"{name}: weights must be [N, K] or [E, N, K], not {list(x.shape)}")
-        m = x
         groups, gs = (1, 0) if x.dim() == 2 else (x.shape[0], x.stride(0))
         n, k = x.shape[-2:]
         rs, cs = x.stride()[-2:]
@@ -110,8 +125,8 @@ def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Ten
     else:
         raise ValueError(f"{name}: block_rows must be 1 or {BLOCK}, not {block_rows}")
     if n and groups:
-        _call(index, "dsv2_quantize_fp8_blocks", m.data_ptr(), rs, gs, groups, n, k, dtype, block_rows,
-              codes.data_ptr(), scales.data_ptr())
+        _call(index, "dsv2_quantize_fp8_blocks", x.data_ptr(), rs, gs, groups, n, k, dtype, BLOCK, codes.data_ptr(),
+              scales.data_ptr())
     return codes, scales
 
 
@@ -123,13 +138,10 @@ def rmsnorm_fp8_blocks(hidden_states: torch.Tensor, weight: torch.Tensor, eps: f
     bf16 or fp32, all of one type; fp32 inside, and nothing is rounded between the norm and the codes (``rmsnorm_triton``
     rounds twice there).  The least block, 2^-100, is one of h * weight here."""
     name = "rmsnorm_fp8_blocks"
-    if residual is None:
-        index = _device(name, hidden_states, weight)
-    else:
-        index = _device(name, hidden_states, weight, residual)
+    index = _device(name, hidden_states, weight) if residual is None else _device(name, hidden_states, weight, residual)
     dtype = _type(name, "hidden_states", hidden_states)
     x, n, k, rs = _rows(name, "hidden_states", hidden_states)
-    if weight.dtype != hidden_states.dtype:
+    if weight.dtype is not hidden_states.dtype:
         raise NotImplementedError(f"{name}: weight is {weight.dtype}, hidden_states {hidden_states.dtype}")
     if weight.shape != (k,):
         raise ValueError(f"weight shape {tuple(weight.shape)} != ({k},)")
@@ -137,22 +149,22 @@ def rmsnorm_fp8_blocks(hidden_states: torch.Tensor, weight: torch.Tensor, eps: f
         raise NotImplementedError(f"{name}: weight must be contiguous")
     if not 0.0 <= eps < math.inf:
         raise ValueError(f"{name}: eps must be at least 0 and finite, not {eps}")
+    codes, scales = _matrix(x, n, k, _E4M3), _matrix(x, n, (k + 127) // BLOCK, _F32)
     if residual is None:
-        res = total = None
-        res_stride = 0
-    else:
-        if residual.dtype != hidden_states.dtype:
-            raise NotImplementedError(f"{name}: residual is {residual.dtype}, hidden_states {hidden_states.dtype}")
-        if residual.shape != hidden_states.shape:
-            raise ValueError(f"{name}: residual is {list(residual.shape)}, hidden_states {list(hidden_states.shape)}")
-        res, _, _, res_stride = _rows(name, "residual", residual)
-        total = x.new_empty(hidden_states.shape)
-    codes, scales = _outputs(x, hidden_states.shape, k)
+        if n:
+            _call(index, "dsv2_rmsnorm_fp8_blocks", x.data_ptr(), rs, None, 0, weight.data_ptr(), eps, n, k, dtype,
+                  codes.data_ptr(), scales.data_ptr(), None)
+        return _shaped(hidden_states, codes, scales)
+    if residual.dtype is not hidden_states.dtype:
+        raise NotImplementedError(f"{name}: residual is {residual.dtype}, hidden_states {hidden_states.dtype}")
+    if residual.shape != hidden_states.shape:
+        raise ValueError(f"{name}: residual is {list(residual.shape)}, hidden_states {list(hidden_states.shape)}")
+    res, _, _, res_stride = _rows(name, "residual", residual)
+    total = _matrix(x, n, k, x.dtype)
     if n:
-        _call(index, "dsv2_rmsnorm_fp8_blocks", x.data_ptr(), rs, None if res is None else res.data_ptr(), res_stride,
-              weight.data_ptr(), eps, n, k, dtype, codes.data_ptr(), scales.data_ptr(),
-              None if total is None else total.data_ptr())
-    return (codes, scales) if total is None else (codes, scales, total)
+        _call(index, "dsv2_rmsnorm_fp8_blocks", x.data_ptr(), rs, res.data_ptr(), res_stride, weight.data_ptr(), eps, n, k,
+              dtype, codes.data_ptr(), scales.data_ptr(), total.data_ptr())
+    return _shaped(hidden_states, codes, scales, total)
 
 
 def silu_mul_fp8_blocks(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -167,11 +179,11 @@ def silu_mul_fp8_blocks(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.Ten
         raise NotImplementedError(f"{name}: gate is {gate.dtype}, up {up.dtype}")
     g, n, k, gs = _rows(name, "gate", gate)
     u, _, _, us = _rows(name, "up", up)
-    codes, scales = _outputs(gate, gate.shape, k)
+    codes, scales = _matrix(g, n, k, _E4M3), _matrix(g, n, (k + 127) // BLOCK, _F32)
     if n:
         _call(index, "dsv2_silu_mul_fp8_blocks", g.data_ptr(), gs, u.data_ptr(), us, n, k, dtype, codes.data_ptr(),
               scales.data_ptr())
-    return codes, scales
+    return _shaped(gate, codes, scales)
 
 
 def _activations(name: str, x: torch.Tensor, scales: torch.Tensor) -> tuple[torch.Tensor, int, int, int, torch.Tensor, int]:
@@ -180,26 +192,30 @@ def _activations(name: str, x: torch.Tensor, scales: torch.Tensor) -> tuple[torc
         raise NotImplementedError(f"{name}: x must be float8_e4m3fn codes, not {x.dtype}")
     if scales.dtype is not _F32:
         raise NotImplementedError(f"{name}: x_scales must be fp32")
-    lead = x.shape[:-1]
-    x, n, k, rs = _rows(name, "x", x)
-    if scales.shape != (*lead, -(-k // BLOCK)):
-        raise ValueError(f"{name}: x_scales must be {[*lead, -(-k // BLOCK)]}, not {list(scales.shape)}")
+    codes, n, k, rs = _rows(name, "x", x)
+    want = (*x.shape[:-1], (k + 127) // BLOCK)
+    if scales.shape != want:
+        raise ValueError(f"{name}: x_scales must be {list(want)}, not {list(scales.shape)}")
     scales, _, _, ss = _rows(name, "x_scales", scales)
-    return x, n, k, rs, scales, ss
+    return codes, n, k, rs, scales, ss
 
 
-def _weights(name: str, w: torch.Tensor, scales: torch.Tensor, k: int, dims: int) -> None:
+def _weights(name: str, w: torch.Tensor, scales: torch.Tensor, k: int, dims: int) -> tuple[tuple[int, ...], ...]:
+    """(shape, strides, the scales' strides)."""
     if w.dtype is not _E4M3:
         raise NotImplementedError(f"{name}: weights must be float8_e4m3fn codes, not {w.dtype}")
     if scales.dtype is not _F32:
         raise NotImplementedError(f"{name}: weight scales must be fp32")
-    if w.dim() != dims or w.shape[-1] != k or 0 in w.shape or w.shape[-2] > MAX_ROWS - 255:
-        raise ValueError(f"{name}: weights must be {'[E, ' if dims == 3 else '['}N, {k}], not {list(w.shape)}")
-    want = (*w.shape[:-2], -(-w.shape[-2] // BLOCK), -(-k // BLOCK))
+    shape = w.shape
+    if len(shape) != dims or shape[-1] != k or 0 in shape or shape[-2] > MAX_ROWS - 255:
+        raise ValueError(f"{name}: weights must be {'[E, ' if dims == 3 else '['}N, {k}], not {list(shape)}")
+    want = (*shape[:-2], (shape[-2] + 127) // BLOCK, (k + 127) // BLOCK)
     if scales.shape != want:
         raise ValueError(f"{name}: weight scales must be {list(want)}, not {list(scales.shape)}")
-    if w.stride(-1) != 1 and k > 1 or scales.stride(-1) != 1 and want[-1] > 1:
+    strides, scale_strides = w.stride(), scales.stride()
+    if strides[-1] != 1 and k > 1 or scale_strides[-1] != 1 and want[-1] > 1:
         raise NotImplementedError(f"{name}: weights and their scales must have a contiguous last dimension")
+    return shape, strides, scale_strides
 
 
 def _out_type(name: str, dtype: torch.dtype | None) -> tuple[torch.dtype, int]:
@@ -216,16 +232,14 @@ def linear_fp8_blocks(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Ten
     rounding to ``output_dtype`` (bf16, the default, or fp32)."""
     name = "linear_fp8_blocks"
     index = _device(name, x, x_scales, weight, weight_scales)
-    lead = x.shape[:-1]
-    x, n, k, xs, x_scales, xss = _activations(name, x, x_scales)
-    _weights(name, weight, weight_scales, k, 2)
+    codes, n, k, xs, x_scales, xss = _activations(name, x, x_scales)
+    (out, _), (ws, _), (wss, _) = _weights(name, weight, weight_scales, k, 2)
     dtype, code = _out_type(name, output_dtype)
-    out = weight.shape[0]
-    y = x.new_empty((*lead, out), dtype=dtype)
+    y = _matrix(codes, n, out, dtype)
     if n:
-        _call(index, "dsv2_linear_fp8_blocks", x.data_ptr(), xs, x_scales.data_ptr(), xss, n, k, weight.data_ptr(),
-              weight.stride(0), weight_scales.data_ptr(), weight_scales.stride(0), out, y.data_ptr(), out, code)
-    return y
+        _call(index, "dsv2_linear_fp8_blocks", codes.data_ptr(), xs, x_scales.data_ptr(), xss, n, k, weight.data_ptr(), ws,
+              weight_scales.data_ptr(), wss, out, y.data_ptr(), out, code)
+    return _shaped(x, y)[0]
 
 
 def grouped_linear_fp8_blocks(x: torch.Tensor, x_scales: torch.Tensor, weights: torch.Tensor, weight_scales: torch.Tensor,
@@ -245,8 +259,7 @@ def grouped_linear_fp8_blocks(x: torch.Tensor, x_scales: torch.Tensor, weights: 
     if x.dim() != 2:
         raise ValueError(f"{name}: x must be [rows, K], not {list(x.shape)}")
     x, t, k, xs, x_scales, xss = _activations(name, x, x_scales)
-    _weights(name, weights, weight_scales, k, 3)
-    groups, out = weights.shape[:2]
+    (groups, out, _), (wgs, ws, _), (wsgs, wss, _) = _weights(name, weights, weight_scales, k, 3)
     if groups > MAX_GROUPS:
         raise ValueError(f"{name}: at most {MAX_GROUPS} groups, not {groups}")
     if offsets.dtype is not _I32 or rows is not None and rows.dtype is not _I32:
@@ -258,10 +271,9 @@ def grouped_linear_fp8_blocks(x: torch.Tensor, x_scales: torch.Tensor, weights: 
         raise NotImplementedError(f"{name}: offsets and rows must be contiguous")
     dtype, code = _out_type(name, output_dtype)
     n = t if rows is None else rows.shape[0]
-    y = x.new_empty((n, out), dtype=dtype)
+    y = _matrix(x, n, out, dtype)
     if n:
         _call(index, "dsv2_grouped_linear_fp8_blocks", x.data_ptr(), xs, x_scales.data_ptr(), xss, t,
-              None if rows is None else rows.data_ptr(), n, k, weights.data_ptr(), weights.stride(0), weights.stride(1),
-              weight_scales.data_ptr(), weight_scales.stride(0), weight_scales.stride(1), out, groups,
-              offsets.data_ptr(), y.data_ptr(), out, code)
+              None if rows is None else rows.data_ptr(), n, k, weights.data_ptr(), wgs, ws, weight_scales.data_ptr(), wsgs,
+              wss, out, groups, offsets.data_ptr(), y.data_ptr(), out, code)
     return y
