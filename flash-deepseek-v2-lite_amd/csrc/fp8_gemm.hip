@@ -520,7 +520,7 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
   uint32_t voff[8];
   uint64_t swrow = 0;  // of waves 4 to 7
   const uint64_t own = wave < 4 ? ~0ull : 0ull;
-  // the addresses of the tokens' scales; for a row that x does not have that of a zero, plus 1
+  // the addresses of the tokens' scales; for a row that is not there that of a zero, plus 1
   uint64_t* const srows = reinterpret_cast<uint64_t*>(ring + Big::kRows);
   auto enter = [&](uint32_t tile) {
     int tm, tn;
@@ -534,23 +534,25 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
     n0 = tn * BN;
     codes = buffer(wave >= 4 ? a.w + group * a.wgs + n0 * a.ws : gather ? a.x : a.x + m0 * a.xs, kPast);
     const uint32_t stride = static_cast<uint32_t>(wave >= 4 ? a.ws : a.xs);
-    const int most = wave >= 4 ? a.N - 1 - n0 : count - 1;  // rows past the tile's: its last one
+    const int rows = wave >= 4 ? a.N - n0 : count;
     if (gather && wave < 4) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int r = a.index[m0 + min(wave * 64 + j * 8 + (lane >> 3), most)];
+        const int i = wave * 64 + j * 8 + (lane >> 3), r = i < rows ? a.index[m0 + i] : -1;
         voff[j] = r >= 0 && r < a.xrows ? r * stride + (j & 1 ? at1 : at0) : kPast;
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        voff[j] = min((wave & 3) * 64 + j * 8 + (lane >> 3), most) * stride + (j & 1 ? at1 : at0);
+      for (int j = 0; j < 8; ++j) {
+        const int i = (wave & 3) * 64 + j * 8 + (lane >> 3);
+        voff[j] = i < rows ? i * stride + (j & 1 ? at1 : at0) : kPast;
+      }
     }
     swrow = ~own & reinterpret_cast<uint64_t>(
                        a.sw + group * a.swgs + min(n0 / kFp8Block + (lane >> 3 & 1), (a.N - 1) / kFp8Block) * a.sws);
     if (threadIdx.x < BM) {
-      int64_t row = m0 + min((int)threadIdx.x, count - 1);
-      if (gather) row = a.index[row];
+      int64_t row = (int)threadIdx.x < count ? m0 + threadIdx.x : -1;
+      if (gather && row >= 0) row = a.index[row];
       srows[threadIdx.x] = row < 0 || row >= a.xrows ? reinterpret_cast<uint64_t>(kZeros) + 1 : reinterpret_cast<uint64_t>(a.sx + row * a.sxs);
     }
   };
@@ -598,16 +600,13 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
   };
   int8v wf[4], xf[3];
   float nx[8], nw;
-  auto first_reads = [&](const uint8_t* from, int c, int window0) {
-#pragma unroll
-    for (int f = 0; f < 4; ++f) wf[f] = frag(from, wat + (f >> 1) * 4096 + (f & 1) * 512);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) xf[t] = frag(from, xat + t * 2048);
+  auto read_scales = [&](int c, int window0) {
     const uint8_t* const win = ring + Big::kScales + ((c >> 3) + window0 & 1) * Big::kWindow;
 #pragma unroll
     for (int t = 0; t < 8; ++t) nx[t] = *reinterpret_cast<const float*>(win + sxat + ((c & 7) ^ sxkey) * 4 + t * 512);
     nw = *reinterpret_cast<const float*>(win + swat + (c & 7) * 4);
   };
+  auto read_w = [&](const uint8_t* from, int f) { wf[f] = frag(from, wat + (f >> 1) * 4096 + (f & 1) * 512); };
   enter(at);
   __syncthreads();
 #pragma unroll
@@ -617,7 +616,16 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
   issue(1, 1);
   int stage = 0, window = 0;  // the block's stage, the tile's first window's place
   int kc = 2, kwin = 0;       // the block that is requested (of this tile or the next), its tile's first window
-  first_reads(ring, 0, 0);
+  read_scales(0, 0);
+#pragma unroll
+  for (int f = 0; f < 4; ++f) read_w(ring, f);
+  xf[0] = frag(ring, xat);
+  xf[1] = frag(ring, xat + 2048);
+  // the sums on their way: of the last three instructions, added in the next block
+  floatx4_t p[4];
+  float sx7 = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = floatx4_t{0.f, 0.f, 0.f, 0.f};
   for (;;) {
     const int64_t om0 = m0;
     const int ocount = count, on0 = n0;
@@ -639,38 +647,48 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
         }
       }
       const uint8_t* const from = ring + stage * Big::kStage;
+      const uint8_t* const next = ring + (stage ^ 1) * Big::kStage;
+      const bool end = c + 1 == nch;
       float sx[8];
 #pragma unroll
       for (int t = 0; t < 8; ++t) sx[t] = nx[t] * nw;
-      floatx4_t p[4];
 #pragma unroll
-      for (int i = 0; i < 32 + 3; ++i) {
+      for (int i = 0; i < 32; ++i) {
         const int t = i >> 2, f = i & 3;
         __builtin_amdgcn_sched_barrier(0);
-        if (i < 32) {
-          p[i & 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[f], xf[t % 3], floatx4_t{0.f, 0.f, 0.f, 0.f}, 0, 0,
-                                                                      0, 0, 0, 0);
-          if (f == 0 && t < 6) xf[(t + 2) % 3] = frag(from, xat + (t + 2) * 2048);
-          if (i == 23) {
-            meet();
-            stores = 0;
-            issue(kc, stage);
-            scales(kc + 7, kwin);
-          }
+        p[i & 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[f], xf[t % 3], floatx4_t{0.f, 0.f, 0.f, 0.f}, 0, 0,
+                                                                    0, 0, 0, 0);
+        if (f == 0 && t < 6) xf[(t + 2) % 3] = frag(from, xat + (t + 2) * 2048);
+        if (i == 23) {
+          meet();
+          stores = 0;
+          issue(kc, stage);
         }
-        if (i >= 3) {
-          const int tt = (i - 3) >> 2, ff = (i - 3) & 3;
+        if (i == 24) scales(kc + 7, kwin);
+        // the next block's first fragments, each behind the last use of the one whose place it takes
+        if (i == 25) read_scales(end ? 0 : c + 1, end ? kwin : window);
+        if (i == 28) xf[0] = frag(next, xat);
+        if (i >= 29) read_w(next, i - 29);
+        if (i == 31) {
+          read_w(next, 3);
+          xf[1] = frag(next, xat + 2048);
+        }
+        const int tt = i >= 3 ? (i - 3) >> 2 : 7, ff = (i - 3) & 3;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[tt][ff][e] = __builtin_fmaf(sx[tt], p[(i - 3) & 3][e], acc[tt][ff][e]);
-        }
+        for (int e = 0; e < 4; ++e)
+          acc[tt][ff][e] = __builtin_fmaf(i >= 3 ? sx[tt] : sx7, p[(i - 3) & 3][e], acc[tt][ff][e]);
       }
       __builtin_amdgcn_sched_barrier(0);
+      sx7 = sx[7];
       stage ^= 1;
       ++kc;
-      const bool end = c + 1 == nch;
-      first_reads(ring + stage * Big::kStage, end ? 0 : c + 1, end ? kwin : window);
     }
     window = kwin;
+#pragma unroll
+    for (int f = 1; f < 4; ++f)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[7][f][e] = __builtin_fmaf(sx7, p[f][e], acc[7][f][e]);
+    sx7 = 0.f;
     // lane group kg holds features 8 kg .. 8 kg + 7 of each half of the wave's 64
     int r0 = wm * 128 + li;
     asm volatile("" : "+v"(r0));  // here: kept over the loop the rows' offsets are spilled, and a reload waits for the stores
@@ -711,7 +729,7 @@ struct Cost {
   int bm, bn;
   float a, b, c, d;
 };
-enum Shape { kFew, kFew32, kTall32, kWide32, kMid, kMid128, kTile128, kLong128, kBig, kShapes };
+enum Shape { kFew, kFew32, kTall32, kWide32, kMid, kMid128, kTile128, kLong128, kBig, kShapes, kStream, kAny };
 constexpr Cost kCost[kShapes] = {
     {16, 16, 3.4f, 0.06f, 0.69f, 0.09f},    // 8 waves along K
     {32, 16, 3.8f, 0.06f, 1.85f, 0.07f},    // 8 along K
@@ -775,25 +793,23 @@ int launch_big(Args a, hipStream_t st) {
   return dsv2_launch_status(GROUPED ? "grouped_linear_fp8_blocks" : "linear_fp8_blocks");
 }
 
-template <bool EXACT, bool GROUPED>
-int launch(Args a, hipStream_t st) {
-  const bool rows16 = a.K % 16 == 0 && dsv2_aligned16(a.x) && dsv2_aligned16(a.w) && a.xs % 16 == 0 && a.ws % 16 == 0 &&
-                      a.wgs % 16 == 0;
-  if (!rows16) {
-    if (!set_tiles(a, GROUPED, 64, 64, 256)) return DSV2_E_SHAPE;
-    product_kernel<2, 2, 2, 2, EXACT, GROUPED><<<grid_of(a), 256, 0, st>>>(a);
-    return dsv2_launch_status(GROUPED ? "grouped_linear_fp8_blocks" : "linear_fp8_blocks");
-  }
+// the kernel and tiles of a call
+Shape shape_of(const Args& a, bool grouped) {
+  if (a.K % 16 != 0 || !dsv2_aligned16(a.x) || !dsv2_aligned16(a.w) || a.xs % 16 != 0 || a.ws % 16 != 0 || a.wgs % 16 != 0)
+    return kAny;
   // Weights that are read once and do not stay in the 256 MB of the last-level cache: one wave a tile, many
   // workgroups a CU, and the non-temporal hint.
-  if (a.rows <= 16 * (GROUPED ? (int64_t)a.groups : 1) && (int64_t)a.groups * a.N * a.K >= kStreamed)
-    return launch_ring<1, 1, 1, 2, 1, 3, true, EXACT, GROUPED>(a, st);
+  if (a.rows <= 16 * (grouped ? (int64_t)a.groups : 1) && (int64_t)a.groups * a.N * a.K >= kStreamed) return kStream;
   // big_kernel's offsets are 31 bits: those of its tile's rows, or of all of x where rows are taken by number
   constexpr int64_t kReach = 1ll << 31;
-  const bool big = !EXACT && a.wide && a.N % 8 == 0 && a.K > kFp8Block && a.xrows > 0 &&
-                   256 * a.ws + a.K < kReach && 512 * a.ys < kReach &&
-                   (a.index ? a.xrows : 256) * a.xs + a.K < kReach;
-  switch (choose(a, GROUPED, big)) {
+  const bool big = !a.out_f32 && a.wide && a.N % 8 == 0 && a.K > kFp8Block && 256 * a.ws + a.K < kReach &&
+                   512 * a.ys < kReach && (a.index ? a.xrows : 256) * a.xs + a.K < kReach;
+  return choose(a, grouped, big);
+}
+
+template <bool EXACT, bool GROUPED>
+int launch(Args a, hipStream_t st) {
+  switch (shape_of(a, GROUPED)) {
     case kFew: return launch_ring<1, 1, 1, 1, 8, 2, false, EXACT, GROUPED>(a, st);
     case kFew32: return launch_ring<1, 1, 2, 1, 8, 2, false, EXACT, GROUPED>(a, st);
     case kTall32: return launch_ring<1, 1, 2, 2, 4, 2, false, EXACT, GROUPED>(a, st);
@@ -802,8 +818,15 @@ int launch(Args a, hipStream_t st) {
     case kMid128: return launch_ring<2, 2, 4, 2, 2, 3, false, EXACT, GROUPED>(a, st);
     case kTile128: return launch_ring<2, 4, 4, 2, 1, 4, false, EXACT, GROUPED>(a, st);
     case kLong128: return launch_ring<2, 4, 4, 4, 1, 3, false, EXACT, GROUPED>(a, st);
-    default: return launch_big<GROUPED>(a, st);
+    case kStream: return launch_ring<1, 1, 1, 2, 1, 3, true, EXACT, GROUPED>(a, st);
+    case kBig:
+      if constexpr (!EXACT) return launch_big<GROUPED>(a, st);
+      break;
+    default: break;
   }
+  if (!set_tiles(a, GROUPED, 64, 64, 256)) return DSV2_E_SHAPE;
+  product_kernel<2, 2, 2, 2, EXACT, GROUPED><<<grid_of(a), 256, 0, st>>>(a);
+  return dsv2_launch_status(GROUPED ? "grouped_linear_fp8_blocks" : "linear_fp8_blocks");
 }
 
 bool aligned(const void* p, int to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
@@ -852,4 +875,18 @@ int dsv2_grouped_linear_fp8_blocks(const void* x, int64_t x_stride, const float*
          groups, 0, 0, out_dtype == DSV2_DTYPE_F32, dsv2_aligned16(y) && y_stride * size % 16 == 0};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   return a.out_f32 ? launch<true, true>(a, st) : launch<false, true>(a, st);
+}
+
+int dsv2_linear_fp8_blocks_tiles(int64_t rows, int K, int N, int groups, int out_dtype) {
+  Args a{};
+  a.xs = a.ws = K;
+  a.wgs = (int64_t)N * K;
+  a.ys = N;
+  a.rows = a.xrows = rows;
+  a.K = K;
+  a.N = N;
+  a.groups = groups > 0 ? groups : 1;
+  a.out_f32 = out_dtype == DSV2_DTYPE_F32;
+  a.wide = (int64_t)N * (a.out_f32 ? 4 : 2) % 16 == 0;
+  return shape_of(a, groups > 0);
 }

@@ -102,6 +102,7 @@ _SIGS = {
     "dsv2_linear_fp8_blocks": ([_p, _i64, _p, _i64, _i64, _i32, _p, _i64, _p, _i64, _i32, _p, _i64, _i32, _p], _i32),
     "dsv2_grouped_linear_fp8_blocks": ([_p, _i64, _p, _i64, _i64, _p, _i64, _i32, _p, _i64, _i64, _p, _i64, _i64, _i32,
                                         _i32, _p, _p, _i64, _i32, _p], _i32),
+    "dsv2_linear_fp8_blocks_tiles": ([_i64, _i32, _i32, _i32, _i32], _i32),
 }
 
 EXPORTS = tuple(_SIGS)

@@ -334,6 +334,82 @@ def test_grouped_large(counts):
         check_grouped(F.grouped_linear_fp8_blocks(x, sx, w, sw, i32(offsets), rows), x, sx, w, sw, offsets, rows)
 
 
+def rows_for(shape, n, k, groups, f32):
+    """The fewest rows of a list with which a product takes that kernel, or None."""
+    for m in (1, 11, 20, 48, 100, 130, 256, 300, 520, 700, 1030, 2100, 4100, 9000):
+        if _hip.lib.dsv2_linear_fp8_blocks_tiles(m, k, n, groups, int(f32)) == shape:
+            return m
+    return None
+
+
+# kernel (dsv2_linear_fp8_blocks_tiles): features with which it is taken, dense and of eight groups
+KERNELS = {0: (331, 331), 1: (2809, 331), 2: (8191, 1003), 3: (None, 16384), 4: (16381, 2051), 5: (16384, 2051), 6: (16384, 2811),
+           7: (16381, 8189), 8: (16376, 8184), 10: (65536, 65536), 11: (300, 300)}
+CASES = [(s, g, k) for s, (dense, of8) in KERNELS.items() for g, n in ((0, dense), (8, of8)) if n
+         for k in ((1040, 1104, 2064) if s == 1 else (144, 272, 1040, 1104, 2064) if s < 9 else (1040, 2064) if s == 10 else (135, 1041))]
+
+
+@pytest.mark.parametrize("shape,groups,k", CASES)
+def test_every_kernel(shape, groups, k):
+    """Each at lengths that end within a block, between NaNs, results of both types where it gives them."""
+    n = KERNELS[shape][groups > 0]
+    ran = 0
+    for f32 in (False, True):
+        m = rows_for(shape, n, k, groups, f32)
+        if m is None:
+            continue
+        ran += 1
+        dtype = F32 if f32 else BF
+        w, sw = matrix(n, k, n + k, 128, groups or None)
+        if shape == 11:
+            gw, gsw = w, sw
+        else:
+            gw, gsw = guarded(w, sw, 16, 0)
+        if not groups:
+            x, sx = matrix(m, k, m + k, 1)
+            gx, gsx = (x, sx) if shape == 11 else guarded(x, sx, 16, 0)
+            R.check_product(F.linear_fp8_blocks(gx, gsx, gw, gsw, dtype), x, sx, w, sw)
+            continue
+        cuts = torch.randint(0, m + 1, (groups - 1,), generator=gen(k), device=DEV).sort().values.tolist()
+        cuts[2] = cuts[1]  # a group without rows
+        offsets = [0, *cuts, m]
+        x, sx = matrix(m, k, m + k, 1)
+        gx, gsx = (x, sx) if shape == 11 else guarded(x, sx, 16, 0)
+        check_grouped(F.grouped_linear_fp8_blocks(gx, gsx, gw, gsw, i32(offsets), None, dtype), x, sx, w, sw, offsets)
+        rows = torch.randint(-1, m + 1, (m,), generator=gen(m), device=DEV).int()
+        sx[m // 2:] = torch.where(torch.rand_like(sx[m // 2:]) < 0.01, 0, sx[m // 2:])
+        check_grouped(F.grouped_linear_fp8_blocks(x, sx, gw, gsw, i32(offsets), rows, dtype), x, sx, w, sw, offsets, rows)
+    assert ran, "no call reaches it"
+
+
+@pytest.mark.parametrize("m,n,k", [(4200, 16376, 272), (700, 33000, 144), (9000, 4104, 1296), (4000, 8200, 2176)])
+def test_large_tiles_one_after_another(m, n, k):
+    """More 256 x 256 tiles than workgroups: the next tile's first blocks are read behind the last of the one before, with
+    its scales beside them (2, 3, 11 and 17 blocks: within and past their windows of eight)."""
+    assert _hip.lib.dsv2_linear_fp8_blocks_tiles(m, k, n, 0, 0) == 8 and -(-m // 256) * -(-n // 256) > 256
+    x, sx = matrix(m, k, m + k, 1)
+    w, sw = matrix(n, k, n * k, 128)
+    y = F.linear_fp8_blocks(x, sx, w, sw)
+    R.check_product(y, x, sx, w, sw)
+    for _ in range(3):
+        assert torch.equal(F.linear_fp8_blocks(x, sx, w, sw), y)
+
+
+@pytest.mark.parametrize("groups,n,k", [(8, 8184, 1104), (70, 2048, 272), (3, 16384, 2064)])
+def test_large_tiles_of_groups(groups, n, k):
+    m = 9000
+    assert _hip.lib.dsv2_linear_fp8_blocks_tiles(m, k, n, groups, 0) == (8 if groups < 64 else 7)
+    cuts = torch.randint(0, m + 1, (groups - 1,), generator=gen(k), device=DEV).sort().values.tolist()
+    offsets = [5, *[max(c, 5) for c in cuts], m - 7]
+    w, sw = matrix(n, k, n + k, 128, groups)
+    x, sx = matrix(2000, k, 1, 1)
+    rows = torch.randint(-3, 2003, (m,), generator=gen(m), device=DEV).int()
+    y = F.grouped_linear_fp8_blocks(x, sx, w, sw, i32(offsets), rows)
+    check_grouped(y, x, sx, w, sw, offsets, rows)
+    again = F.grouped_linear_fp8_blocks(x, sx, w, sw, i32(offsets), rows)
+    assert torch.equal(again[5:m - 7], y[5:m - 7])
+
+
 @pytest.mark.parametrize("k", [300, 304, 512])
 def test_grouped_holds_offsets_and_row_numbers_to_their_ranges(k):
     w, sw = matrix(70, k, 1, 128, 4)
