@@ -25,17 +25,32 @@ from . import _hip
 
 BLOCK = 128
 MAX_ROWS = 2 ** 31 - 1
+MAX_COLS = 2 ** 31 - 256
 MAX_GROUPS = 65536
 
 # These calls launch kernels of 2 to 10 us for few rows, so their own host time is looked at: a launch takes 3 us of it,
-# an attribute of a tensor 0.05 to 0.1, new_empty 1.5, torch's allocation by shape, strides and type alone 0.7.
+# an attribute of a tensor 0.05 to 0.1, new_empty 1.5, torch's allocation by shape, strides and type alone 0.7.  The
+# plain case (matrices, as they should be, on the current device) is therefore found by one condition at the head of a
+# function; whatever does not meet it goes through the checks one by one.
 _E4M3, _BF16, _F32, _I32 = torch.float8_e4m3fn, torch.bfloat16, torch.float32, torch.int32
 _TYPES = {_BF16: 0, _F32: 1}  # DSV2_DTYPE_*
 _ENTRY = {n: getattr(_hip.lib, n) for n in ("dsv2_quantize_fp8_blocks", "dsv2_rmsnorm_fp8_blocks",
                                             "dsv2_silu_mul_fp8_blocks", "dsv2_linear_fp8_blocks",
                                             "dsv2_grouped_linear_fp8_blocks")}
+_QUANTIZE, _RMSNORM, _SILU, _LINEAR = tuple(_ENTRY.values())[:4]
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+
+
+def _check(rc: int, entry: str) -> None:
+    if rc:
+        raise _hip.HipKernelError(f"{entry} failed (status {rc}): "
+                                  f"{_hip.lib.dsv2_last_error_message().decode(errors='replace')}")
+
+
+def _plain(index: int) -> bool:
+    """Tensors of that device may be allocated and used without a change of the current one."""
+    return index >= 0 and _empty_strided is not None and _current_device() == index
 
 
 def _call(index: int, entry: str, *args) -> None:
@@ -43,10 +58,7 @@ def _call(index: int, entry: str, *args) -> None:
     if _current_device() != index:
         with torch.cuda.device(index):
             return _call(index, entry, *args)
-    rc = _ENTRY[entry](*args, _hip._raw_stream(index))
-    if rc:
-        raise _hip.HipKernelError(f"{entry} failed (status {rc}): "
-                                  f"{_hip.lib.dsv2_last_error_message().decode(errors='replace')}")
+    _check(_ENTRY[entry](*args, _hip._raw_stream(index)), entry)
 
 
 def _device(name: str, *ts: torch.Tensor) -> int:
@@ -62,9 +74,7 @@ def _device(name: str, *ts: torch.Tensor) -> int:
 
 def _matrix(like: torch.Tensor, n: int, k: int, dtype: torch.dtype) -> torch.Tensor:
     """An uninitialised [n, k] on the device of `like`."""
-    if _empty_strided is None or not like.is_cuda or _current_device() != like.get_device():
-        return like.new_empty((n, k), dtype=dtype)
-    return _empty_strided((n, k), (k, 1), dtype)
+    return like.new_empty((n, k), dtype=dtype)
 
 
 def _type(name: str, what: str, t: torch.Tensor) -> int:
@@ -84,7 +94,7 @@ def _rows(name: str, what: str, t: torch.Tensor) -> tuple[torch.Tensor, int, int
         shape = t.shape
     n, k = shape
     rs, cs = t.stride()
-    if k == 0 or n > MAX_ROWS or k > MAX_ROWS - 255:
+    if k == 0 or n > MAX_ROWS or k > MAX_COLS:
         raise ValueError(f"{name}: {what} is {list(shape)}")
     if cs != 1 and k > 1:
         raise NotImplementedError(f"{name}: {what} must have a contiguous last dimension")
@@ -101,6 +111,16 @@ def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Ten
     """(codes, scales) of bf16 or fp32 values: activations [..., K] in blocks of one row (``block_rows`` 1) or weights
     [N, K] or [E, N, K] in blocks of 128 rows (``block_rows`` 128; a matrix's last block may be shorter)."""
     name = "quantize_fp8_blocks"
+    if block_rows == 1 and x.dim() == 2:
+        n, k = x.shape
+        rs, cs = x.stride()
+        dtype, index = _TYPES.get(x.dtype), x.get_device()
+        if dtype is not None and cs == 1 and 0 < n <= MAX_ROWS and 0 < k <= MAX_COLS and _plain(index):
+            kb = (k + 127) // BLOCK
+            codes, scales = _empty_strided((n, k), (k, 1), _E4M3), _empty_strided((n, kb), (kb, 1), _F32)
+            _check(_QUANTIZE(x.data_ptr(), rs, 0, 1, n, k, dtype, 1, codes.data_ptr(), scales.data_ptr(),
+                             _hip._raw_stream(index)), name)
+            return codes, scales
     index = _device(name, x)
     dtype = _type(name, "x", x)
     if block_rows == 1:
@@ -116,7 +136,7 @@ def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Ten
         groups, gs = (1, 0) if x.dim() == 2 else (x.shape[0], x.stride(0))
         n, k = x.shape[-2:]
         rs, cs = x.stride()[-2:]
-        if k == 0 or max(n, groups) > MAX_ROWS or k > MAX_ROWS - 255:
+        if k == 0 or max(n, groups) > MAX_ROWS or k > MAX_COLS:
             raise ValueError(f"{name}: x is {list(x.shape)}")
         if cs != 1 and k > 1:
             raise NotImplementedError(f"{name}: x must have a contiguous last dimension")
@@ -138,6 +158,26 @@ def rmsnorm_fp8_blocks(hidden_states: torch.Tensor, weight: torch.Tensor, eps: f
     bf16 or fp32, all of one type; fp32 inside, and nothing is rounded between the norm and the codes (``rmsnorm_triton``
     rounds twice there).  The least block, 2^-100, is one of h * weight here."""
     name = "rmsnorm_fp8_blocks"
+    x, index = hidden_states, hidden_states.get_device()
+    if x.dim() == 2 and _plain(index) and weight.get_device() == index:
+        n, k = x.shape
+        rs, cs = x.stride()
+        dtype, t = x.dtype, _TYPES.get(x.dtype)
+        if (t is not None and cs == 1 and 0 < n <= MAX_ROWS and 0 < k <= MAX_COLS and 0.0 <= eps < math.inf and
+                weight.dtype is dtype and weight.shape == (k,) and weight.is_contiguous()):
+            kb = (k + 127) // BLOCK
+            if residual is None:
+                codes, scales = _empty_strided((n, k), (k, 1), _E4M3), _empty_strided((n, kb), (kb, 1), _F32)
+                _check(_RMSNORM(x.data_ptr(), rs, None, 0, weight.data_ptr(), eps, n, k, t, codes.data_ptr(),
+                                scales.data_ptr(), None, _hip._raw_stream(index)), name)
+                return codes, scales
+            if (residual.dtype is dtype and residual.get_device() == index and residual.shape == (n, k) and
+                    residual.stride(1) == 1):
+                codes, scales = _empty_strided((n, k), (k, 1), _E4M3), _empty_strided((n, kb), (kb, 1), _F32)
+                total = _empty_strided((n, k), (k, 1), dtype)
+                _check(_RMSNORM(x.data_ptr(), rs, residual.data_ptr(), residual.stride(0), weight.data_ptr(), eps, n, k, t,
+                                codes.data_ptr(), scales.data_ptr(), total.data_ptr(), _hip._raw_stream(index)), name)
+                return codes, scales, total
     index = _device(name, hidden_states, weight) if residual is None else _device(name, hidden_states, weight, residual)
     dtype = _type(name, "hidden_states", hidden_states)
     x, n, k, rs = _rows(name, "hidden_states", hidden_states)
@@ -171,6 +211,17 @@ def silu_mul_fp8_blocks(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.Ten
     """(codes, scales) of silu(gate) * up, bf16 or fp32 [..., K] each (the halves of one gate_up result, as views);
     fp32 inside, nothing is rounded before the codes."""
     name = "silu_mul_fp8_blocks"
+    index = gate.get_device()
+    if gate.dim() == 2 and up.dim() == 2 and _plain(index) and up.get_device() == index:
+        n, k = shape = gate.shape
+        (gs, gc), (us, uc), t = gate.stride(), up.stride(), _TYPES.get(gate.dtype)
+        if (t is not None and up.dtype is gate.dtype and up.shape == shape and gc == uc == 1 and 0 < n <= MAX_ROWS and
+                0 < k <= MAX_COLS):
+            kb = (k + 127) // BLOCK
+            codes, scales = _empty_strided((n, k), (k, 1), _E4M3), _empty_strided((n, kb), (kb, 1), _F32)
+            _check(_SILU(gate.data_ptr(), gs, up.data_ptr(), us, n, k, t, codes.data_ptr(), scales.data_ptr(),
+                         _hip._raw_stream(index)), name)
+            return codes, scales
     index = _device(name, gate, up)
     if gate.shape != up.shape:
         raise ValueError("gate and up must have the same shape")
@@ -207,7 +258,7 @@ def _weights(name: str, w: torch.Tensor, scales: torch.Tensor, k: int, dims: int
     if scales.dtype is not _F32:
         raise NotImplementedError(f"{name}: weight scales must be fp32")
     shape = w.shape
-    if len(shape) != dims or shape[-1] != k or 0 in shape or shape[-2] > MAX_ROWS - 255:
+    if len(shape) != dims or shape[-1] != k or 0 in shape or shape[-2] > MAX_COLS:
         raise ValueError(f"{name}: weights must be {'[E, ' if dims == 3 else '['}N, {k}], not {list(shape)}")
     want = (*shape[:-2], (shape[-2] + 127) // BLOCK, (k + 127) // BLOCK)
     if scales.shape != want:
@@ -231,6 +282,20 @@ def linear_fp8_blocks(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Ten
     """The product [..., N] of activations [..., K] (codes, scales) and weights [N, K] (codes, scales): fp32 sums, one
     rounding to ``output_dtype`` (bf16, the default, or fp32)."""
     name = "linear_fp8_blocks"
+    index = x.get_device()
+    if (x.dim() == 2 and x_scales.dim() == 2 and weight.dim() == 2 and weight_scales.dim() == 2 and _plain(index) and
+            x_scales.get_device() == index and weight.get_device() == index and weight_scales.get_device() == index):
+        n, k = x.shape
+        out, wk = weight.shape
+        kb, t = (k + 127) // BLOCK, 0 if output_dtype is None else _TYPES.get(output_dtype)
+        (xs, xc), (xss, xsc), (ws, wc), (wss, wsc) = x.stride(), x_scales.stride(), weight.stride(), weight_scales.stride()
+        if (x.dtype is _E4M3 and weight.dtype is _E4M3 and x_scales.dtype is _F32 and weight_scales.dtype is _F32 and
+                t is not None and wk == k and xc == wc == xsc == wsc == 1 and 0 < n <= MAX_ROWS and 0 < k <= MAX_COLS and
+                0 < out <= MAX_COLS and x_scales.shape == (n, kb) and weight_scales.shape == ((out + 127) // BLOCK, kb)):
+            y = _empty_strided((n, out), (out, 1), output_dtype or _BF16)
+            _check(_LINEAR(x.data_ptr(), xs, x_scales.data_ptr(), xss, n, k, weight.data_ptr(), ws, weight_scales.data_ptr(),
+                           wss, out, y.data_ptr(), out, t, _hip._raw_stream(index)), name)
+            return y
     index = _device(name, x, x_scales, weight, weight_scales)
     codes, n, k, xs, x_scales, xss = _activations(name, x, x_scales)
     (out, _), (ws, _), (wss, _) = _weights(name, weight, weight_scales, k, 2)

@@ -15,6 +15,7 @@ if torch.cuda.is_available():
     from triton_kernels import fp8_blocks as F
 
 import fp8_blocks_ref as R
+import test_fp8_blocks_cpu as C
 
 DEV = "cuda"
 BF, F32, E4 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
@@ -579,6 +580,45 @@ def test_more_leading_dimensions_and_single_rows():
         y = F.linear_fp8_blocks(c, s, w, sw)
         assert y.shape == (*v.shape[:-1], 140)
         assert torch.equal(y.reshape(-1, 140), F.linear_fp8_blocks(*F.quantize_fp8_blocks(flat), w, sw))
+
+
+def on_gpu(args):
+    """Arguments of the refusal tests on the GPU, with their strides."""
+    def there(a):
+        if not isinstance(a, torch.Tensor):
+            return a
+        u = a.view(torch.uint8) if a.dtype.itemsize == 1 else a
+        moved = torch.empty_strided(u.shape, u.stride(), dtype=u.dtype, device=DEV).zero_()
+        return moved.view(a.dtype)
+    return [there(a) for a in args]
+
+
+@pytest.mark.parametrize("name,at,value,error,text", C.REFUSED)
+def test_bad_arguments_are_refused_on_the_gpu_too(name, at, value, error, text):
+    args = on_gpu(C.good()[name])
+    getattr(F, name)(*args)
+    args[at] = on_gpu([value])[0]
+    with pytest.raises(error, match=text):
+        getattr(F, name)(*args)
+
+
+@pytest.mark.parametrize("name", sorted(C.good()))
+def test_tensors_of_two_devices_are_refused(name):
+    args = on_gpu(C.good()[name])
+    for i, a in enumerate(args):
+        if isinstance(a, torch.Tensor) and not (name == "quantize_fp8_blocks"):
+            with pytest.raises((NotImplementedError, ValueError), match="requires CUDA|tensors on"):
+                getattr(F, name)(*args[:i], a.cpu(), *args[i + 1:])
+
+
+def test_the_plain_case_and_the_checks_one_by_one_agree(monkeypatch):
+    """The head of each function and what follows it give the same."""
+    args = layer_inputs(24, 5)
+    want = layer(*args)
+    monkeypatch.setattr(F, "_plain", lambda index: False)
+    got = layer(*args)
+    for name in want:
+        assert torch.equal(got[name].view(torch.uint8), want[name].view(torch.uint8)), name
 
 
 def test_no_rows():
