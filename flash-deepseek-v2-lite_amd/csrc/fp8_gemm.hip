@@ -524,6 +524,10 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
   uint64_t* const srows = reinterpret_cast<uint64_t*>(ring + Big::kRows);
   auto enter = [&](uint32_t tile) {
     int tm, tn;
+    // in here: kept over the loop what follows from it is spilled
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));
+    const int lane = thread & 63;
     tile_at(tile, mt, a.nt, tm, tn);
     if constexpr (GROUPED) {
       group_of<BM>(a, all[lane], tm, group, m0, count);
@@ -550,20 +554,23 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
     }
     swrow = ~own & reinterpret_cast<uint64_t>(
                        a.sw + group * a.swgs + min(n0 / kFp8Block + (lane >> 3 & 1), (a.N - 1) / kFp8Block) * a.sws);
-    if (threadIdx.x < BM) {
-      int64_t row = (int)threadIdx.x < count ? m0 + threadIdx.x : -1;
+    if (thread < BM) {
+      int64_t row = thread < count ? m0 + thread : -1;
       if (gather && row >= 0) row = a.index[row];
-      srows[threadIdx.x] = row < 0 || row >= a.xrows ? reinterpret_cast<uint64_t>(kZeros) + 1 : reinterpret_cast<uint64_t>(a.sx + row * a.sxs);
+      srows[thread] = row < 0 || row >= a.xrows ? reinterpret_cast<uint64_t>(kZeros) + 1 : reinterpret_cast<uint64_t>(a.sx + row * a.sxs);
     }
+  };
+  // pieces past the rows' end: of the last block, which is the tile's last to be requested
+  auto cut = [&] {
+    const int k = (nch - 1) * kFp8Block;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) voff[j] |= k + (j & 1 ? at1 : at0) < a.K ? 0u : kPast;
   };
   // no branch in these two: in the middle of a block's instructions one costs the loop over 100 spilled registers
   auto issue = [&](int c, int stage) {
     uint8_t* const to = ring + stage * Big::kStage;
-    const int k = c * kFp8Block;
-    // pieces past the rows' end lie past the buffer: zeros
-    const uint32_t out0 = k + at0 < a.K ? 0u : kPast, out1 = k + at1 < a.K ? 0u : kPast;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) buffer_lds16(codes, to + (wave * 8 + j) * 1024, voff[j] | (j & 1 ? out1 : out0), k);
+    for (int j = 0; j < 8; ++j) buffer_lds16(codes, to + (wave * 8 + j) * 1024, voff[j], c * kFp8Block);
   };
   // an eighth of a window: waves 0 to 3 eight tokens' scales each, the others the features' (each its own copy)
   const int swap = wave < 4 ? (wave & 1) << 2 : 0;
@@ -613,6 +620,7 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
   for (int i = 0; i < 9; ++i) scales(i, 0);
   issue(0, 0);
   meet();
+  if (nch == 2) cut();
   issue(1, 1);
   int stage = 0, window = 0;  // the block's stage, the tile's first window's place
   int kc = 2, kwin = 0;       // the block that is requested (of this tile or the next), its tile's first window
@@ -646,6 +654,7 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
           for (int j = 0; j < 8; ++j) voff[j] = kPast;
         }
       }
+      if (kc == nch - 1) cut();
       const uint8_t* const from = ring + stage * Big::kStage;
       const uint8_t* const next = ring + (stage ^ 1) * Big::kStage;
       const bool end = c + 1 == nch;
