@@ -10,15 +10,21 @@
 namespace {
 
 
+template <bool NT>
+__device__ __forceinline__ uint4 load16(const void* p) {
+  if constexpr (NT) return ldg16_nt(p);
+  else return ldg16(p);
+}
+
 // a lane's 8 values from p: VEC: two or one 16-byte loads, all or none of them in the row; else one by one
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool NT = false>
 __device__ __forceinline__ void load8(const T* __restrict__ p, int n, float (&f)[8]) {
   if constexpr (VEC) {
+    const uint4 z = make_uint4(0, 0, 0, 0);
     if constexpr (sizeof(T) == 2) {
-      unpack8(n > 0 ? ldg16(p) : make_uint4(0, 0, 0, 0), f);
+      unpack8(n > 0 ? load16<NT>(p) : z, f);
     } else {
-      const uint4 z = make_uint4(0, 0, 0, 0);
-      const uint4 a = n > 0 ? ldg16(p) : z, b = n > 0 ? ldg16(p + 4) : z;
+      const uint4 a = n > 0 ? load16<NT>(p) : z, b = n > 0 ? load16<NT>(p + 4) : z;
       f[0] = __uint_as_float(a.x), f[1] = __uint_as_float(a.y), f[2] = __uint_as_float(a.z), f[3] = __uint_as_float(a.w);
       f[4] = __uint_as_float(b.x), f[5] = __uint_as_float(b.y), f[6] = __uint_as_float(b.z), f[7] = __uint_as_float(b.w);
     }
@@ -103,24 +109,35 @@ __device__ __forceinline__ float swiglu(float g, float u) {
   return g * q * u;
 }
 
-template <typename T, bool SILU, bool VEC>
+// NB blocks for each 16 lanes, 16 NB a workgroup
+template <typename T, bool SILU, bool VEC, int NB, bool NT>
 __global__ __launch_bounds__(256) void block_kernel(const BlockArgs a) {
-  const int64_t b0 = blockIdx.x * (int64_t)16, row0 = b0 / a.kb, b = b0 + (threadIdx.x >> 4);
-  if (b >= a.n_blocks) return;  // whole 16-lane rows leave: the DPP steps stay within one
-  const uint32_t at = static_cast<uint32_t>(b0 - row0 * a.kb) + (threadIdx.x >> 4), down = at / (uint32_t)a.kb;
-  const int64_t row = row0 + down;
-  const int c = static_cast<int>(at - down * a.kb) * kFp8Block + (threadIdx.x & 15) * 8, n = a.K - c;
-  float f[8];
-  load8<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.x_stride + c, n, f);
-  if constexpr (SILU) {
-    float u[8];
-    load8<T, VEC>(reinterpret_cast<const T*>(a.up) + row * a.up_stride + c, n, u);
+  const int64_t b0 = blockIdx.x * (int64_t)(16 * NB), row0 = b0 / a.kb;
+  const T* const x = reinterpret_cast<const T*>(a.x);
+  float f[NB][8], u[SILU ? NB : 1][8];
+  int64_t row[NB];
+  int c[NB];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = swiglu(f[i], u[i]);
+  for (int i = 0; i < NB; ++i) {
+    const uint32_t at = static_cast<uint32_t>(b0 - row0 * a.kb) + (threadIdx.x >> 4) + 16 * i, down = at / (uint32_t)a.kb;
+    row[i] = row0 + down;
+    c[i] = static_cast<int>(at - down * a.kb) * kFp8Block + (threadIdx.x & 15) * 8;
+    const int n = b0 + (threadIdx.x >> 4) + 16 * i < a.n_blocks ? a.K - c[i] : 0;
+    load8<T, VEC, NT>(x + row[i] * a.x_stride + c[i], n, f[i]);
+    if constexpr (SILU) load8<T, VEC, NT>(reinterpret_cast<const T*>(a.up) + row[i] * a.up_stride + c[i], n, u[i]);
   }
-  const uint32_t m = max(row_max(max8(f)), kLeastBits);
-  store_codes<VEC>(a.codes + row * a.K + c, n, Fp8Rounding(m), f);
-  if ((threadIdx.x & 15) == 0) a.scales[b] = fp8_scale(m);
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    const int64_t b = b0 + (threadIdx.x >> 4) + 16 * i;
+    if (b >= a.n_blocks) return;  // whole 16-lane rows leave: the DPP steps stay within one
+    if constexpr (SILU) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[i][j] = swiglu(f[i][j], u[i][j]);
+    }
+    const uint32_t m = max(row_max(max8(f[i])), kLeastBits);
+    store_codes<VEC>(a.codes + row[i] * a.K + c[i], a.K - c[i], Fp8Rounding(m), f[i]);
+    if ((threadIdx.x & 15) == 0) a.scales[b] = fp8_scale(m);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -272,11 +289,22 @@ void launch_norm(const NormArgs& a, bool vec, hipStream_t st) {
   }
 }
 
+template <typename T, bool SILU, int NB, bool NT>
+void launch_blocks(const BlockArgs& a, bool vec, hipStream_t st) {
+  const dim3 grid((unsigned)((a.n_blocks + 16 * NB - 1) / (16 * NB)));
+  if (vec) block_kernel<T, SILU, true, NB, NT><<<grid, 256, 0, st>>>(a);
+  else block_kernel<T, SILU, false, NB, false><<<grid, 256, 0, st>>>(a);
+}
+
+// One block for each 16 lanes (MI355X: 1,024 blocks 2.0 us, two 2.3; 33,000 SwiGLU 5.4 / 5.6), two where there are
+// many workgroups either way (262,144 18.4 / 16.7; 180,000 SwiGLU 25.3 / 24.7).  Non-temporal loads of what
+// cannot stay in the 256 MB of the last-level cache (49,152 x 1,408 SwiGLU 65.6 -> 62.7; in it 16.9 -> 19.7).
 template <typename T, bool SILU>
 void launch_blocks(const BlockArgs& a, bool vec, hipStream_t st) {
-  const dim3 grid((unsigned)((a.n_blocks + 15) / 16));
-  if (vec) block_kernel<T, SILU, true><<<grid, 256, 0, st>>>(a);
-  else block_kernel<T, SILU, false><<<grid, 256, 0, st>>>(a);
+  const int64_t bytes = a.n_blocks * kFp8Block * (int64_t)sizeof(T) * (SILU ? 2 : 1);
+  if (bytes > 256ll << 20) launch_blocks<T, SILU, 2, true>(a, vec, st);
+  else if (a.n_blocks > 98304) launch_blocks<T, SILU, 2, false>(a, vec, st);
+  else launch_blocks<T, SILU, 1, false>(a, vec, st);
 }
 
 // rows that a kernel's 16-byte loads may take: whole groups of 8 values at multiples of 16 bytes

@@ -48,7 +48,8 @@ def i32(x):
 # rounded once before the quotient's rounding: two half steps
 LOOSE = {BF: 0.0, F32: 2 * U24}
 SHAPES = [(1, 1), (1, 127), (1, 128), (1, 129), (2, 8), (3, 200), (5, 136), (16, 2048), (17, 1408), (33, 2050), (64, 10944),
-          (700, 260), (4099, 64)]
+          (700, 260), (4099, 64), (33001, 264), (9001, 1411)]  # the last: two blocks a lane
+LARGE = [(70003, 1408), (130001, 136)]  # past the last-level cache
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
@@ -168,6 +169,19 @@ def test_silu_mul(m, k, dtype):
         q, s = R.rounded(y, 1)
         # exp to an ulp, its correction, the sum, the quotient, two products: 8 half steps; both values of a quotient
         R.check_codes(codes, q, 2 * 8 * U24 + 3 * U24)
+        R.check_scales(scales, s, 9 * U24)
+
+
+@pytest.mark.parametrize("m,k", LARGE)
+def test_rows_past_the_last_level_cache(m, k):
+    both = rnd(m, 2 * k, seed=k, dtype=F32 if k < 200 else BF, std=2)
+    if k < 200:
+        both = strided(both, 1030)[:, :2 * k]  # far apart: 1.3 GB between the first and the last
+    gate, up = both.chunk(2, 1)
+    for codes, scales, y, loose in ((*F.silu_mul_fp8_blocks(gate, up), gate.double() * torch.sigmoid(gate.double()) * up, 19 * U24),
+                                    (*F.quantize_fp8_blocks(both), both.double(), LOOSE[both.dtype])):
+        q, s = R.rounded(y.double(), 1)
+        R.check_codes(codes, q, loose)
         R.check_scales(scales, s, 9 * U24)
 
 
