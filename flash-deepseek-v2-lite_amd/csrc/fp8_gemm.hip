@@ -161,11 +161,11 @@ __device__ __forceinline__ void store4(const Args& a, int64_t m, int n, const fl
   }
 }
 
-// 16 codes from p, of which n are in the row
+// 16 codes from p, at any alignment, of which n are in the row
 __device__ __forceinline__ uint4 codes16(const uint8_t* p, int n) {
   uint4 v = make_uint4(0, 0, 0, 0);
   if (n >= 16) {
-    __builtin_memcpy(&v, p, 16);  // any alignment
+    __builtin_memcpy(&v, p, 16);
   } else if (n > 0) {
     uint32_t d[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -204,94 +204,16 @@ __device__ __forceinline__ floatx4_t block_sum(const Decoded& w, const Decoded& 
   return p;
 }
 
-// A workgroup of WM x WN waves, each TT x FT MFMA tiles of 16 tokens x 16 features; K in chunks of one block.
-// The chunk's rows of 128 bytes lie in LDS with their 16-byte pieces exchanged by row (piece p of row r at
-// place p ^ key(r)), so that 8 lanes reading one piece of 8 rows hit different banks.  Row i of a wave's MFMA
-// tile f is its feature 4 FT (i / 4) + 4 f + i % 4: a lane ends with 4 FT neighbouring features.
-template <int WM, int WN, int TT, int FT, bool EXACT, bool GROUPED>
-__global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Args a) {
-  constexpr int BM = 16 * TT * WM, BN = 16 * FT * WN, NW = WM * WN, DI = (BM + BN) / 8 / NW;
-  static_assert((BM + BN) % (8 * NW) == 0 && 128 % BN == 0, "tile");
-  using Operand = std::conditional_t<EXACT, Decoded, Codes>;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[(BM + BN) * 128];
-  __shared__ float lsx[BM];
-  int tn, group = 0, count;
-  int64_t m0;
-  if (!tile_of<BM, GROUPED>(a, tn, group, m0, count)) return;
-  const int n0 = tn * BN, lane = threadIdx.x & 63, wv = threadIdx.x >> 6, wm = wv % WM, wn = wv / WM;
-  const int li = lane & 15, kg = lane >> 4, nch = (a.K + kFp8Block - 1) / kFp8Block;
-  const float* sw = a.sw + group * a.swgs + (n0 / kFp8Block) * a.sws;
-  // rows past the tile's are its last one again: their sums are not stored
-  auto x_row = [&](int t) -> int64_t {
-    const int64_t m = m0 + min(t, count - 1);
-    if (!GROUPED || !a.index) return m;
-    const int64_t r = a.index[m];
-    return r >= 0 && r < a.xrows ? r : -1;
-  };
-  const uint8_t* src[DI];
-  int lim[DI];
-#pragma unroll
-  for (int j = 0; j < DI; ++j) {
-    const int r = (wv * DI + j) * 8 + (lane >> 3), q = r - BM;
-    const int key = r < BM ? r & 7 : (q & 3) | (q / (4 * FT) & 1) << 2, at = ((lane & 7) ^ key) * 16;
-    const int64_t row = r < BM ? x_row(r) : min(n0 + q, a.N - 1);
-    src[j] = (r < BM ? a.x + max(row, (int64_t)0) * a.xs : a.w + group * a.wgs + row * a.ws) + at;
-    lim[j] = row < 0 ? 0 : a.K - at;
-  }
-  const int64_t srow = x_row(min((int)threadIdx.x, BM - 1));
-  floatx4_t acc[TT][FT];
-#pragma unroll
-  for (int t = 0; t < TT; ++t)
-#pragma unroll
-    for (int f = 0; f < FT; ++f) acc[t][f] = floatx4_t{0.f, 0.f, 0.f, 0.f};
-  const int piece = (kg ^ (li & 7)) * 16;
-  const uint8_t* lx = lds + (wm * TT * 16 + li) * 128;
-  const uint8_t* lw = lds + (BM + wn * FT * 16 + (li >> 2) * 4 * FT + (li & 3)) * 128;
-  auto frag = [&](const uint8_t* p) {
-    const int4v a = *reinterpret_cast<const int4v*>(p + piece), b = *reinterpret_cast<const int4v*>(p + (piece ^ 64));
-    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-  };
-  for (int c = 0; c < nch; ++c) {
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < DI; ++j)
-      *reinterpret_cast<uint4*>(lds + ((wv * DI + j) * 8) * 128 + lane * 16) =
-          codes16(src[j] + c * kFp8Block, lim[j] - c * kFp8Block);
-    if (threadIdx.x < BM) lsx[threadIdx.x] = srow < 0 ? 0.f : a.sx[srow * a.sxs + c];
-    __syncthreads();
-    Operand wf[FT];
-#pragma unroll
-    for (int f = 0; f < FT; ++f) operand(frag(lw + f * 4 * 128), wf[f]);
-    const float s = sw[c];
-#pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      Operand xf;
-      operand(frag(lx + t * 16 * 128), xf);
-      const float st = s * lsx[wm * TT * 16 + t * 16 + li];
-#pragma unroll
-      for (int f = 0; f < FT; ++f) {
-        const floatx4_t p = block_sum(wf[f], xf);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][f][i] = __builtin_fmaf(st, p[i], acc[t][f][i]);
-      }
-    }
-  }
-#pragma unroll
-  for (int t = 0; t < TT; ++t) {
-    const int m = wm * TT * 16 + t * 16 + li;
-    if (m < count) {
-#pragma unroll
-      for (int f = 0; f < FT; ++f) store4(a, m0 + m, n0 + wn * FT * 16 + kg * 4 * FT + f * 4, acc[t][f]);
-    }
-  }
-}
-
 // ---------------------------------------------------------------------------
-// The same product with both operands streamed into LDS without registers (global_load_lds), for rows of whole
-// 16 codes at multiples of 16 bytes.  KW groups of WM x WN waves share the tile and take every KW-th block of
-// K; each group has a ring of ST stages of its own, ST - 1 of them requested ahead.  The scales of a stage's
-// block come the same way, 64 a load.  A group of one wave needs no barrier: its own waits order its loads
-// and reads.  At the end the groups' sums meet in LDS, in fixed order.
+// A tile by KW groups of WM x WN waves, each wave TT x FT MFMA tiles of 16 tokens x 16 features; group i takes every
+// KW-th block of K from block i on.  A block's rows of 128 bytes lie in LDS with their 16-byte pieces exchanged
+// by row (piece p of row r at place p ^ key(r)), so that 8 lanes reading one piece of 8 rows hit different banks.  Row i
+// of a wave's MFMA tile f is its feature 4 FT (i / 4) + 4 f + i % 4: a lane ends with 4 FT neighbouring features.
+//
+// Rows of whole 16 codes at multiples of 16 bytes (ANY false) are streamed into LDS without registers
+// (global_load_lds): each group has a ring of ST stages, ST - 1 of them requested ahead, and a block's scales come the same
+// way, 64 a load.  Other rows go through registers, one block ahead of two stages.  A group of one wave needs no
+// barrier: its own waits order its loads and reads.  At the end the groups' sums meet in LDS, in fixed order.
 // ---------------------------------------------------------------------------
 // 16 (4) bytes a lane from src to LDS, lane after lane from dst; in functions of their own: with the builtin in a
 // template hipcc drops the kernel's host launch stub
@@ -330,11 +252,12 @@ struct Ring {
   static_assert(ST >= 2 && (ST - 2) * (DI + SI) < 64, "vmcnt counts to 63");
 };
 
-template <int WM, int WN, int TT, int FT, int KW, int ST, bool NT, bool EXACT, bool GROUPED>
+template <int WM, int WN, int TT, int FT, int KW, int ST, bool NT, bool ANY, bool EXACT, bool GROUPED>
 __global__ __launch_bounds__(64 * WM * WN * KW) void ring_kernel(const Args a) {
   using R = Ring<WM, WN, TT, FT, KW, ST>;
   using Operand = std::conditional_t<EXACT, Decoded, Codes>;
   static_assert(!NT || WM * WN == 1, "a load is of tokens or of features");
+  static_assert(!ANY || ST == 2, "one block in registers");
   constexpr int BM = R::BM, BN = R::BN, NW = R::NW, DI = R::DI, SI = R::SI;
   extern __shared__ __attribute__((aligned(16))) uint8_t ring[];
   int tn, group = 0, count;
@@ -374,18 +297,36 @@ __global__ __launch_bounds__(64 * WM * WN * KW) void ring_kernel(const Args a) {
     }
   }
   uint8_t* const mine = ring + kw * ST * R::kStage;
+  uint4 held[ANY ? DI : 1];
+  float factors[ANY ? SI : 1];
+  // block c to the stage, or (ANY) into registers and from there to the stage
   auto issue = [&](int c, int stage) {
     uint8_t* const to = mine + stage * R::kStage;
+    const int k = c * kFp8Block, cs = min(c, nch - 1);
 #pragma unroll
     for (int j = 0; j < DI; ++j) {
-      const uint8_t* const from = c * kFp8Block < lim[j] ? src[j] + c * kFp8Block : zeros;
-      if (NT && j * 8 >= BM) load_lds16_nt(from, to + (wv * DI + j) * 1024);
-      else load_lds16(from, to + (wv * DI + j) * 1024);
+      if constexpr (ANY) {
+        held[j] = codes16(src[j] + k, lim[j] - k);
+      } else {
+        const uint8_t* const from = k < lim[j] ? src[j] + k : zeros;
+        if (NT && j * 8 >= BM) load_lds16_nt(from, to + (wv * DI + j) * 1024);
+        else load_lds16(from, to + (wv * DI + j) * 1024);
+      }
     }
-    const int cs = min(c, nch - 1);
+#pragma unroll
+    for (int j = 0; j < SI; ++j) {
+      const float* const from = ssrc[j] ? ssrc[j] + cs : reinterpret_cast<const float*>(zeros);
+      if constexpr (ANY) factors[j] = *from;
+      else load_lds4(from, to + R::kCodes + (wv + NW * j) * 256);
+    }
+  };
+  auto put = [&](int stage) {
+    uint8_t* const to = mine + stage * R::kStage;
+#pragma unroll
+    for (int j = 0; j < DI; ++j) *reinterpret_cast<uint4*>(to + (wv * DI + j) * 1024 + lane * 16) = held[j];
 #pragma unroll
     for (int j = 0; j < SI; ++j)
-      load_lds4(ssrc[j] ? ssrc[j] + cs : reinterpret_cast<const float*>(zeros), to + R::kCodes + (wv + NW * j) * 256);
+      *reinterpret_cast<float*>(to + R::kCodes + (wv + NW * j) * 256 + lane * 4) = factors[j];
   };
   floatx4_t acc[TT][FT];
 #pragma unroll
@@ -398,10 +339,11 @@ __global__ __launch_bounds__(64 * WM * WN * KW) void ring_kernel(const Args a) {
   const int steps = (nch + KW - 1) / KW;
 #pragma unroll
   for (int s = 0; s + 1 < ST; ++s) issue(s * KW + kw, s);
+  if constexpr (ANY) put(0);
   int st = 0;
   for (int i = 0; i < steps; ++i) {
-    // this wave's loads of stage st have landed and its reads of the stage before are done, then every wave's
-    __builtin_amdgcn_s_waitcnt(vmcnt_only((ST - 2) * (DI + SI)) & ~0xf00);
+    // this wave's loads of stage st have landed (its writes are done) and its reads of the stage before, then every wave's
+    __builtin_amdgcn_s_waitcnt(vmcnt_only(ANY ? 63 : (ST - 2) * (DI + SI)) & ~0xf00);
     asm volatile("" ::: "memory");
     if constexpr (NW > 1) {
       __builtin_amdgcn_s_barrier();
@@ -434,6 +376,7 @@ __global__ __launch_bounds__(64 * WM * WN * KW) void ring_kernel(const Args a) {
       }
     }
     st = st + 1 == ST ? 0 : st + 1;
+    if constexpr (ANY) put(st);
   }
   // what was requested past the last block must land before the ring is used again or released
   __builtin_amdgcn_s_waitcnt(vmcnt_only(0) & ~0xf00);
@@ -761,11 +704,13 @@ float likely_tiles(const Args& a, bool grouped, int bm) {
   return fmaxf(hit, rows / bm + 0.5f * hit);
 }
 
-Shape choose(const Args& a, bool grouped, bool big) {
+// the least estimate among the shapes whose bits are set
+Shape choose(const Args& a, bool grouped, unsigned among) {
   const float k = static_cast<float>((a.K + kFp8Block - 1) / kFp8Block);
   Shape best = kFew;
   float least = 3e38f;
-  for (int s = 0; s < (big ? kShapes : kBig); ++s) {
+  for (int s = 0; s < kShapes; ++s) {
+    if (!(among >> s & 1)) continue;
     const Cost& c = kCost[s];
     float n = likely_tiles(a, grouped, c.bm) * ((a.N + c.bn - 1) / c.bn) * (1.f / 256);
     if (s == kBig) n = ceilf(n);
@@ -785,11 +730,11 @@ bool set_tiles(Args& a, bool grouped, int bm, int bn, int threads) {
 }
 dim3 grid_of(const Args& a) { return dim3((unsigned)(((int64_t)a.mt * a.nt + 7) / 8 * 8)); }
 
-template <int WM, int WN, int TT, int FT, int KW, int ST, bool NT, bool EXACT, bool GROUPED>
+template <int WM, int WN, int TT, int FT, int KW, int ST, bool NT, bool ANY, bool EXACT, bool GROUPED>
 int launch_ring(Args a, hipStream_t st) {
   using R = Ring<WM, WN, TT, FT, KW, ST>;
   if (!set_tiles(a, GROUPED, R::BM, R::BN, R::kThreads)) return DSV2_E_SHAPE;
-  ring_kernel<WM, WN, TT, FT, KW, ST, NT, EXACT, GROUPED><<<grid_of(a), R::kThreads, R::kLds, st>>>(a);
+  ring_kernel<WM, WN, TT, FT, KW, ST, NT, ANY, EXACT, GROUPED><<<grid_of(a), R::kThreads, R::kLds, st>>>(a);
   return dsv2_launch_status(GROUPED ? "grouped_linear_fp8_blocks" : "linear_fp8_blocks");
 }
 
@@ -802,10 +747,10 @@ int launch_big(Args a, hipStream_t st) {
   return dsv2_launch_status(GROUPED ? "grouped_linear_fp8_blocks" : "linear_fp8_blocks");
 }
 
-// the kernel and tiles of a call
-Shape shape_of(const Args& a, bool grouped) {
+// the tiles of a call; kAny is added where its rows go through registers
+int shape_of(const Args& a, bool grouped) {
   if (a.K % 16 != 0 || !dsv2_aligned16(a.x) || !dsv2_aligned16(a.w) || a.xs % 16 != 0 || a.ws % 16 != 0 || a.wgs % 16 != 0)
-    return kAny;
+    return kAny + choose(a, grouped, 1 << kFew | 1 << kTall32 | 1 << kMid | 1 << kTile128);
   // Weights that are read once and do not stay in the 256 MB of the last-level cache: one wave a tile, many
   // workgroups a CU, and the non-temporal hint.
   if (a.rows <= 16 * (grouped ? (int64_t)a.groups : 1) && (int64_t)a.groups * a.N * a.K >= kStreamed) return kStream;
@@ -813,29 +758,29 @@ Shape shape_of(const Args& a, bool grouped) {
   constexpr int64_t kReach = 1ll << 31;
   const bool big = !a.out_f32 && a.wide && a.N % 8 == 0 && a.K > kFp8Block && 256 * a.ws + a.K < kReach &&
                    512 * a.ys < kReach && (a.index ? a.xrows : 256) * a.xs + a.K < kReach;
-  return choose(a, grouped, big);
+  return choose(a, grouped, (1 << kShapes) - 1 - (big ? 0 : 1 << kBig));
 }
 
 template <bool EXACT, bool GROUPED>
-int launch(Args a, hipStream_t st) {
+int launch(const Args& a, hipStream_t st) {
   switch (shape_of(a, GROUPED)) {
-    case kFew: return launch_ring<1, 1, 1, 1, 8, 2, false, EXACT, GROUPED>(a, st);
-    case kFew32: return launch_ring<1, 1, 2, 1, 8, 2, false, EXACT, GROUPED>(a, st);
-    case kTall32: return launch_ring<1, 1, 2, 2, 4, 2, false, EXACT, GROUPED>(a, st);
-    case kWide32: return launch_ring<1, 1, 2, 4, 2, 2, false, EXACT, GROUPED>(a, st);
-    case kMid: return launch_ring<2, 2, 2, 2, 2, 3, false, EXACT, GROUPED>(a, st);
-    case kMid128: return launch_ring<2, 2, 4, 2, 2, 3, false, EXACT, GROUPED>(a, st);
-    case kTile128: return launch_ring<2, 4, 4, 2, 1, 4, false, EXACT, GROUPED>(a, st);
-    case kLong128: return launch_ring<2, 4, 4, 4, 1, 3, false, EXACT, GROUPED>(a, st);
-    case kStream: return launch_ring<1, 1, 1, 2, 1, 3, true, EXACT, GROUPED>(a, st);
-    case kBig:
-      if constexpr (!EXACT) return launch_big<GROUPED>(a, st);
-      break;
+    case kFew: return launch_ring<1, 1, 1, 1, 8, 2, false, false, EXACT, GROUPED>(a, st);
+    case kFew32: return launch_ring<1, 1, 2, 1, 8, 2, false, false, EXACT, GROUPED>(a, st);
+    case kTall32: return launch_ring<1, 1, 2, 2, 4, 2, false, false, EXACT, GROUPED>(a, st);
+    case kWide32: return launch_ring<1, 1, 2, 4, 2, 2, false, false, EXACT, GROUPED>(a, st);
+    case kMid: return launch_ring<2, 2, 2, 2, 2, 3, false, false, EXACT, GROUPED>(a, st);
+    case kMid128: return launch_ring<2, 2, 4, 2, 2, 3, false, false, EXACT, GROUPED>(a, st);
+    case kTile128: return launch_ring<2, 4, 4, 2, 1, 4, false, false, EXACT, GROUPED>(a, st);
+    case kLong128: return launch_ring<2, 4, 4, 4, 1, 3, false, false, EXACT, GROUPED>(a, st);
+    case kStream: return launch_ring<1, 1, 1, 2, 1, 3, true, false, EXACT, GROUPED>(a, st);
+    case kAny + kFew: return launch_ring<1, 1, 1, 1, 8, 2, false, true, EXACT, GROUPED>(a, st);
+    case kAny + kTall32: return launch_ring<1, 1, 2, 2, 4, 2, false, true, EXACT, GROUPED>(a, st);
+    case kAny + kMid: return launch_ring<2, 2, 2, 2, 2, 2, false, true, EXACT, GROUPED>(a, st);
+    case kAny + kTile128: return launch_ring<2, 4, 4, 2, 1, 2, false, true, EXACT, GROUPED>(a, st);
     default: break;
   }
-  if (!set_tiles(a, GROUPED, 64, 64, 256)) return DSV2_E_SHAPE;
-  product_kernel<2, 2, 2, 2, EXACT, GROUPED><<<grid_of(a), 256, 0, st>>>(a);
-  return dsv2_launch_status(GROUPED ? "grouped_linear_fp8_blocks" : "linear_fp8_blocks");
+  if constexpr (!EXACT) return launch_big<GROUPED>(a, st);
+  else return DSV2_E_FLAGS;  // not reached: kBig is for bf16 results
 }
 
 bool aligned(const void* p, int to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
@@ -845,7 +790,7 @@ bool aligned(const void* p, int to) { return reinterpret_cast<uintptr_t>(p) % to
 #define CHECK_PRODUCT(name)                                                                                       \
   DSV2_REQUIRE(out_dtype == DSV2_DTYPE_BF16 || out_dtype == DSV2_DTYPE_F32, DSV2_E_FLAGS, name ": out_dtype %d", \
                out_dtype);                                                                                        \
-  DSV2_REQUIRE(rows >= 0 && rows <= 0x7fffffff && K > 0 && K <= 0x7fffff00 && N > 0 && N <= 0x7fffff00, DSV2_E_SHAPE, \
+  DSV2_REQUIRE(rows >= 0 && rows <= 0x7fffffff && K > 0 && K <= 1 << 30 && N > 0 && N <= 0x7fffff00, DSV2_E_SHAPE, \
                name ": %lld rows, K %d, N %d", (long long)rows, K, N);                                           \
   if (rows == 0) return DSV2_OK;                                                                                  \
   DSV2_REQUIRE((rows == 1 || y_stride >= N) && x_stride >= 0 && x_scales_stride >= 0 && w_stride >= 0 &&          \

@@ -15,8 +15,19 @@ __device__ __forceinline__ uint4 load16(const void* p) {
   if constexpr (NT) return ldg16_nt(p);
   else return ldg16(p);
 }
+__device__ __forceinline__ uint4 load16_any(const void* p) {  // of any alignment
+  uint4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
 
-// a lane's 8 values from p: VEC: two or one 16-byte loads, all or none of them in the row; else one by one
+__device__ __forceinline__ void floats(const uint4& a, const uint4& b, float (&f)[8]) {
+  f[0] = __uint_as_float(a.x), f[1] = __uint_as_float(a.y), f[2] = __uint_as_float(a.z), f[3] = __uint_as_float(a.w);
+  f[4] = __uint_as_float(b.x), f[5] = __uint_as_float(b.y), f[6] = __uint_as_float(b.z), f[7] = __uint_as_float(b.w);
+}
+
+// a lane's 8 values from p, of which n are in the row.  VEC: all or none, at multiples of 16 bytes; else all of them by
+// the same loads at any alignment (a lane's bytes then lie in two lines now and then), a row's last few one by one
 template <typename T, bool VEC, bool NT = false>
 __device__ __forceinline__ void load8(const T* __restrict__ p, int n, float (&f)[8]) {
   if constexpr (VEC) {
@@ -25,9 +36,11 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, int n, float (&f)
       unpack8(n > 0 ? load16<NT>(p) : z, f);
     } else {
       const uint4 a = n > 0 ? load16<NT>(p) : z, b = n > 0 ? load16<NT>(p + 4) : z;
-      f[0] = __uint_as_float(a.x), f[1] = __uint_as_float(a.y), f[2] = __uint_as_float(a.z), f[3] = __uint_as_float(a.w);
-      f[4] = __uint_as_float(b.x), f[5] = __uint_as_float(b.y), f[6] = __uint_as_float(b.z), f[7] = __uint_as_float(b.w);
+      floats(a, b, f);
     }
+  } else if (n >= 8) {
+    if constexpr (sizeof(T) == 2) unpack8(load16_any(p), f);
+    else floats(load16_any(p), load16_any(p + 4), f);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -42,17 +55,22 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, int n, float (&f)
 
 template <typename T, bool VEC>
 __device__ __forceinline__ void store8(T* __restrict__ p, int n, const float (&f)[8]) {
-  if constexpr (VEC) {
-    if (n <= 0) return;
+  if (VEC ? n > 0 : n >= 8) {
     if constexpr (sizeof(T) == 2) {
-      *reinterpret_cast<uint4*>(p) = pack8(f);
+      const uint4 v = pack8(f);
+      if constexpr (VEC) *reinterpret_cast<uint4*>(p) = v;
+      else __builtin_memcpy(p, &v, 16);
     } else {
-      reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-      reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+      if constexpr (VEC) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+      } else {
+        __builtin_memcpy(p, f, 32);
+      }
     }
-  } else {
+  } else if constexpr (!VEC) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 7; ++i)
       if (i < n) {
         if constexpr (sizeof(T) == 2) p[i] = f2bf(f[i]);
         else p[i] = f[i];
@@ -62,13 +80,14 @@ __device__ __forceinline__ void store8(T* __restrict__ p, int n, const float (&f
 
 template <bool VEC>
 __device__ __forceinline__ void store_codes(uint8_t* __restrict__ p, int n, const Fp8Rounding& q, const float (&f)[8]) {
-  const uint32_t lo = fp8x4(q(f[0]), q(f[1]), q(f[2]), q(f[3])), hi = fp8x4(q(f[4]), q(f[5]), q(f[6]), q(f[7]));
-  if constexpr (VEC) {
-    if (n > 0) *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
-  } else {
+  const uint2 v = make_uint2(fp8x4(q(f[0]), q(f[1]), q(f[2]), q(f[3])), fp8x4(q(f[4]), q(f[5]), q(f[6]), q(f[7])));
+  if (VEC ? n > 0 : n >= 8) {
+    if constexpr (VEC) *reinterpret_cast<uint2*>(p) = v;
+    else __builtin_memcpy(p, &v, 8);
+  } else if constexpr (!VEC) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = static_cast<uint8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));
+    for (int i = 0; i < 7; ++i)
+      if (i < n) p[i] = static_cast<uint8_t>((i < 4 ? v.x : v.y) >> (8 * (i & 3)));
   }
 }
 
@@ -271,6 +290,8 @@ void launch_norm(const NormArgs& a, hipStream_t st) {
     norm_kernel<T, 1, 4, RES, VEC><<<dim3((unsigned)((a.rows + 3) / 4)), 256, 0, st>>>(a);
   } else if (a.K <= 2048) {
     norm_kernel<T, 4, 1, RES, VEC><<<dim3((unsigned)a.rows), 256, 0, st>>>(a);
+  } else if (a.K <= 4096) {
+    norm_kernel<T, 4, 2, RES, VEC><<<dim3((unsigned)a.rows), 256, 0, st>>>(a);
   } else if (a.K <= 8192) {
     norm_kernel<T, 4, 4, RES, VEC><<<dim3((unsigned)a.rows), 256, 0, st>>>(a);
   } else {

@@ -359,9 +359,10 @@ def rows_for(shape, n, k, groups, f32):
 
 # kernel (dsv2_linear_fp8_blocks_tiles): features with which it is taken, dense and of eight groups
 KERNELS = {0: (331, 331), 1: (2809, 331), 2: (8191, 1003), 3: (None, 16384), 4: (16381, 2051), 5: (16384, 2051), 6: (16384, 2811),
-           7: (16381, 8189), 8: (16376, 8184), 10: (65536, 65536), 11: (300, 300)}
+           7: (16381, 8189), 8: (16376, 8184), 10: (65536, 65536), 11: (300, 300), 13: (8191, 1003), 15: (16381, 2051),
+           17: (16381, 2811)}
 CASES = [(s, g, k) for s, (dense, of8) in KERNELS.items() for g, n in ((0, dense), (8, of8)) if n
-         for k in ((1040, 1104, 2064) if s == 1 else (144, 272, 1040, 1104, 2064) if s < 9 else (1040, 2064) if s == 10 else (135, 1041))]
+         for k in ((1040, 1104, 2064) if s == 1 else (144, 272, 1040, 1104, 2064) if s < 9 else (1040, 2064) if s == 10 else (135, 1041, 1288))]
 
 
 @pytest.mark.parametrize("shape,groups,k", CASES)
@@ -376,20 +377,20 @@ def test_every_kernel(shape, groups, k):
         ran += 1
         dtype = F32 if f32 else BF
         w, sw = matrix(n, k, n + k, 128, groups or None)
-        if shape == 11:
+        if shape >= 11:
             gw, gsw = w, sw
         else:
             gw, gsw = guarded(w, sw, 16, 0)
         if not groups:
             x, sx = matrix(m, k, m + k, 1)
-            gx, gsx = (x, sx) if shape == 11 else guarded(x, sx, 16, 0)
+            gx, gsx = (x, sx) if shape >= 11 else guarded(x, sx, 16, 0)
             R.check_product(F.linear_fp8_blocks(gx, gsx, gw, gsw, dtype), x, sx, w, sw)
             continue
         cuts = torch.randint(0, m + 1, (groups - 1,), generator=gen(k), device=DEV).sort().values.tolist()
         cuts[2] = cuts[1]  # a group without rows
         offsets = [0, *cuts, m]
         x, sx = matrix(m, k, m + k, 1)
-        gx, gsx = (x, sx) if shape == 11 else guarded(x, sx, 16, 0)
+        gx, gsx = (x, sx) if shape >= 11 else guarded(x, sx, 16, 0)
         check_grouped(F.grouped_linear_fp8_blocks(gx, gsx, gw, gsw, i32(offsets), None, dtype), x, sx, w, sw, offsets)
         rows = torch.randint(-1, m + 1, (m,), generator=gen(m), device=DEV).int()
         sx[m // 2:] = torch.where(torch.rand_like(sx[m // 2:]) < 0.01, 0, sx[m // 2:])
