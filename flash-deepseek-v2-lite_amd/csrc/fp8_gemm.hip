@@ -138,26 +138,38 @@ __device__ __forceinline__ bool tile_of(const Args& a, int& tn, int& group, int6
   return true;
 }
 
+// features n .. n + 3 of row m; rows may begin at any multiple of a value
 __device__ __forceinline__ void store4(const Args& a, int64_t m, int n, const floatx4_t& v) {
-  if (n >= a.N) return;
   if (a.out_f32) {
-    float* p = static_cast<float*>(a.y) + m * a.ys + n;
-    if (a.wide && n + 4 <= a.N) {
-      *reinterpret_cast<floatx4_t*>(p) = v;
+    float* const p = static_cast<float*>(a.y) + m * a.ys + n;
+    if (n + 4 <= a.N) {
+      __builtin_memcpy(p, &v, 16);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 3; ++i)
         if (n + i < a.N) p[i] = v[i];
     }
   } else {
-    bf16_t* p = static_cast<bf16_t*>(a.y) + m * a.ys + n;
-    if (a.wide && n + 4 <= a.N) {
-      *reinterpret_cast<uint2*>(p) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+    bf16_t* const p = static_cast<bf16_t*>(a.y) + m * a.ys + n;
+    const uint2 w = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+    if (n + 4 <= a.N) {
+      __builtin_memcpy(p, &w, 8);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i < a.N) p[i] = f2bf(v[i]);
+      for (int i = 0; i < 3; ++i)
+        if (n + i < a.N) p[i] = static_cast<bf16_t>((i < 2 ? w.x : w.y) >> (16 * (i & 1)));
     }
+  }
+}
+
+// features n .. n + 7 of a row of N, at any alignment
+__device__ __forceinline__ void store8_any(bf16_t* row, int n, int N, const u32x4_t& v) {
+  if (n + 8 <= N) {
+    __builtin_memcpy(row + n, &v, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+      if (n + i < N) row[n + i] = static_cast<bf16_t>(v[i >> 1] >> (16 * (i & 1)));
   }
 }
 
@@ -438,7 +450,7 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t ring[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave & 1, wn = wave >> 1, li = lane & 15, kg = lane >> 4, nch = (a.K + kFp8Block - 1) / kFp8Block;
-  const bool gather = GROUPED && a.index;
+  const bool gather = GROUPED && a.index, whole = a.wide && a.N % 8 == 0;
   // the tiles of this XCD's workgroups: neighbours in tile_at's order
   int mt = a.mt;
   Groups* const all = reinterpret_cast<Groups*>(ring + Big::kGroups);  // up to 64 groups
@@ -645,22 +657,36 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
     int r0 = wm * 128 + li;
     asm volatile("" : "+v"(r0));  // here: kept over the loop the rows' offsets are spilled, and a reload waits for the stores
     const int col = on0 + wn * 64 + kg * 8;
-    // as many stores for every wave, so that the next block's wait may leave them on their way; what is not the tile's
-    // lies past the buffer
-    const __amdgpu_buffer_rsrc_t out = buffer(static_cast<bf16_t*>(a.y) + om0 * a.ys, kPast);
-    const uint32_t out0 = col < a.N ? col * 2 : kPast, out1 = col + 32 < a.N ? col * 2 + 64 : kPast;
+    auto pair = [&](int t, int i) {
+      const floatx4_t u = acc[t][2 * i], v = acc[t][2 * i + 1];
+      return u32x4_t{pack2(u[0], u[1]), pack2(u[2], u[3]), pack2(v[0], v[1]), pack2(v[2], v[3])};
+    };
+    if (whole) {
+      // as many stores for every wave, so that the next block's wait may leave them on their way; what is not the
+      // tile's lies past the buffer
+      const __amdgpu_buffer_rsrc_t out = buffer(static_cast<bf16_t*>(a.y) + om0 * a.ys, kPast);
+      const uint32_t out0 = col < a.N ? col * 2 : kPast, out1 = col + 32 < a.N ? col * 2 + 64 : kPast;
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      const int m = r0 + t * 16;
-      const uint32_t row = m < ocount ? m * (uint32_t)a.ys * 2 : kPast;
+      for (int t = 0; t < 8; ++t) {
+        const int m = r0 + t * 16;
+        const uint32_t row = m < ocount ? m * (uint32_t)a.ys * 2 : kPast;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const floatx4_t u = acc[t][2 * i], v = acc[t][2 * i + 1];
-        const u32x4_t w = {pack2(u[0], u[1]), pack2(u[2], u[3]), pack2(v[0], v[1]), pack2(v[2], v[3])};
-        __builtin_amdgcn_raw_buffer_store_b128(w, out, row + (i ? out1 : out0) | (row | (i ? out1 : out0)) & kPast, 0, 0);
+        for (int i = 0; i < 2; ++i)
+          __builtin_amdgcn_raw_buffer_store_b128(pair(t, i), out,
+                                                 row + (i ? out1 : out0) | (row | (i ? out1 : out0)) & kPast, 0, 0);
+      }
+      stores = 16;
+    } else {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const int m = r0 + t * 16;
+        if (m < ocount) {
+          bf16_t* const row = static_cast<bf16_t*>(a.y) + (om0 + m) * a.ys;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) store8_any(row, col + 32 * i, a.N, pair(t, i));
+        }
       }
     }
-    stores = 16;
 #pragma unroll
     for (int t = 0; t < 8; ++t)
 #pragma unroll
@@ -756,7 +782,7 @@ int shape_of(const Args& a, bool grouped) {
   if (a.rows <= 16 * (grouped ? (int64_t)a.groups : 1) && (int64_t)a.groups * a.N * a.K >= kStreamed) return kStream;
   // big_kernel's offsets are 31 bits: those of its tile's rows, or of all of x where rows are taken by number
   constexpr int64_t kReach = 1ll << 31;
-  const bool big = !a.out_f32 && a.wide && a.N % 8 == 0 && a.K > kFp8Block && 256 * a.ws + a.K < kReach &&
+  const bool big = !a.out_f32 && a.K > kFp8Block && 256 * a.ws + a.K < kReach &&
                    512 * a.ys < kReach && (a.index ? a.xrows : 256) * a.xs + a.K < kReach;
   return choose(a, grouped, (1 << kShapes) - 1 - (big ? 0 : 1 << kBig));
 }

@@ -359,7 +359,7 @@ def rows_for(shape, n, k, groups, f32):
 
 # kernel (dsv2_linear_fp8_blocks_tiles): features with which it is taken, dense and of eight groups
 KERNELS = {0: (331, 331), 1: (2809, 331), 2: (8191, 1003), 3: (None, 16384), 4: (16381, 2051), 5: (16384, 2051), 6: (16384, 2811),
-           7: (16381, 8189), 8: (16376, 8184), 10: (65536, 65536), 11: (300, 300), 13: (8191, 1003), 15: (16381, 2051),
+           7: (16381, 8189), 8: (16381, 8187), 10: (65536, 65536), 11: (300, 300), 13: (8191, 1003), 15: (16381, 2051),
            17: (16381, 2811)}
 CASES = [(s, g, k) for s, (dense, of8) in KERNELS.items() for g, n in ((0, dense), (8, of8)) if n
          for k in ((1040, 1104, 2064) if s == 1 else (144, 272, 1040, 1104, 2064) if s < 9 else (1040, 2064) if s == 10 else (135, 1041, 1288))]
@@ -398,7 +398,8 @@ def test_every_kernel(shape, groups, k):
     assert ran, "no call reaches it"
 
 
-@pytest.mark.parametrize("m,n,k", [(4200, 16376, 272), (700, 33000, 144), (9000, 4104, 1296), (4000, 8200, 2176)])
+@pytest.mark.parametrize("m,n,k", [(4200, 16376, 272), (700, 33000, 144), (9000, 4104, 1296), (4000, 8200, 2176),
+                                   (4000, 8194, 1040), (700, 33003, 272)])
 def test_large_tiles_one_after_another(m, n, k):
     """More 256 x 256 tiles than workgroups: the next tile's first blocks are read behind the last of the one before, with
     its scales beside them (2, 3, 11 and 17 blocks: within and past their windows of eight)."""
@@ -411,7 +412,7 @@ def test_large_tiles_one_after_another(m, n, k):
         assert torch.equal(F.linear_fp8_blocks(x, sx, w, sw), y)
 
 
-@pytest.mark.parametrize("groups,n,k", [(8, 8184, 1104), (70, 2048, 272), (3, 16384, 2064)])
+@pytest.mark.parametrize("groups,n,k", [(8, 8184, 1104), (70, 2048, 272), (3, 16387, 2064)])
 def test_large_tiles_of_groups(groups, n, k):
     m = 9000
     assert _hip.lib.dsv2_linear_fp8_blocks_tiles(m, k, n, groups, 0) == (8 if groups < 64 else 7)
