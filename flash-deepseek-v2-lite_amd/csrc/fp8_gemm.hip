@@ -441,7 +441,8 @@ struct Big {
   // scales of eight blocks: of the tokens [256][8], the places of tokens 8 i + 8 .. 8 i + 15, i even, exchanged by xor 4 (banks),
   // then of the features' two blocks [2][8], four copies; two such windows, and the addresses of the tokens' scales
   static constexpr int kWindow = BM * 32 + 4 * 256, kScales = 2 * kStage, kRows = kScales + 2 * kWindow;
-  static constexpr int kGroups = kRows + BM * 8, kUnused = kGroups + 64 * 12, kLds = kUnused + 8 * 256;
+  static constexpr int kGroups = kRows + 2 * BM * 8, kUnused = kGroups + 64 * 12, kLds = kUnused + 8 * 256;
+  static_assert(kLds <= 160 * 1024, "LDS");
 };
 
 template <bool GROUPED>
@@ -475,8 +476,10 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
   uint32_t voff[8];
   uint64_t swrow = 0;  // of waves 4 to 7
   const uint64_t own = wave < 4 ? ~0ull : 0ull;
-  // the addresses of the tokens' scales; for a row that is not there that of a zero, plus 1
-  uint64_t* const srows = reinterpret_cast<uint64_t*>(ring + Big::kRows);
+  // the addresses of the tokens' scales, of this tile and of the next by turns (a slow wave may still read this one's
+  // when the next one's are written); for a row that is not there that of a zero, plus 1
+  int turn = 0;
+  auto srow = [&](int t) { return reinterpret_cast<uint64_t*>(ring + Big::kRows + turn) + t; };
   auto enter = [&](uint32_t tile) {
     int tm, tn;
     // in here: kept over the loop what follows from it is spilled
@@ -509,10 +512,11 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
     }
     swrow = ~own & reinterpret_cast<uint64_t>(
                        a.sw + group * a.swgs + min(n0 / kFp8Block + (lane >> 3 & 1), (a.N - 1) / kFp8Block) * a.sws);
+    turn ^= BM * 8;
     if (thread < BM) {
       int64_t row = thread < count ? m0 + thread : -1;
       if (gather && row >= 0) row = a.index[row];
-      srows[thread] = row < 0 || row >= a.xrows ? reinterpret_cast<uint64_t>(kZeros) + 1 : reinterpret_cast<uint64_t>(a.sx + row * a.sxs);
+      *srow(thread) = row < 0 || row >= a.xrows ? reinterpret_cast<uint64_t>(kZeros) + 1 : reinterpret_cast<uint64_t>(a.sx + row * a.sxs);
     }
   };
   // pieces past the rows' end: of the last block, which is the tile's last to be requested
@@ -531,7 +535,7 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
   const int swap = wave < 4 ? (wave & 1) << 2 : 0;
   auto scales = [&](int part, int window0) {  // part: counted over the tile's windows
     const int in = part & 7, first = part & ~7, t = in * 32 + (wave & 3) * 8 + (lane >> 3);
-    const uint64_t row = srows[t] & own | swrow;
+    const uint64_t row = *srow(t) & own | swrow;
     const int b = row & 1 ? 0 : min(first + ((lane & 7) ^ swap), nch - 1);
     const int window = Big::kScales + ((part >> 3) + window0 & 1) * Big::kWindow;
     const int to = wave < 4 ? (in * 4 + wave) * 256 : BM * 32 + (wave - 4) * 256;
@@ -600,7 +604,7 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
         if (at < last) {
           enter(at);
           __builtin_amdgcn_s_waitcnt(vmcnt_only(63) & ~0xf00);
-          __builtin_amdgcn_s_barrier();  // srows is written
+          __builtin_amdgcn_s_barrier();  // the scales' addresses are written
           asm volatile("" ::: "memory");
 #pragma unroll
           for (int i = 0; i < 7; ++i) scales(i, kwin);
