@@ -734,7 +734,12 @@ float likely_tiles(const Args& a, bool grouped, int bm) {
   return fmaxf(hit, rows / bm + 0.5f * hit);
 }
 
-// the least estimate among the shapes whose bits are set
+// a launch has fewer than 2^32 threads
+bool launchable(const Args& a, bool grouped, int bm, int bn, int threads) {
+  return most_tiles(a, grouped, bm) <= ((1ll << 32) / threads - 8) / ((a.N + (int64_t)bn - 1) / bn);
+}
+
+// the least estimate among the shapes whose bits are set and that have not too many tiles
 Shape choose(const Args& a, bool grouped, unsigned among) {
   const float k = static_cast<float>((a.K + kFp8Block - 1) / kFp8Block);
   Shape best = kFew;
@@ -742,6 +747,7 @@ Shape choose(const Args& a, bool grouped, unsigned among) {
   for (int s = 0; s < kShapes; ++s) {
     if (!(among >> s & 1)) continue;
     const Cost& c = kCost[s];
+    if (!launchable(a, grouped, c.bm, c.bn, 512)) continue;
     float n = likely_tiles(a, grouped, c.bm) * ((a.N + c.bn - 1) / c.bn) * (1.f / 256);
     if (s == kBig) n = ceilf(n);
     const float t = c.a + c.b * k + fmaxf(n - 1.f, 0.f) * (c.c + c.d * k);
@@ -751,10 +757,9 @@ Shape choose(const Args& a, bool grouped, unsigned among) {
 }
 
 bool set_tiles(Args& a, bool grouped, int bm, int bn, int threads) {
-  const int64_t mt = most_tiles(a, grouped, bm), nt = (a.N + bn - 1) / bn;
-  a.mt = (int)mt;
-  a.nt = (int)nt;
-  if (mt * nt <= (1ll << 32) / threads - 8) return true;  // a launch has fewer than 2^32 threads
+  a.mt = (int)most_tiles(a, grouped, bm);
+  a.nt = (a.N + bn - 1) / bn;
+  if (launchable(a, grouped, bm, bn, threads)) return true;
   dsv2_set_error("linear_fp8_blocks: %lld rows of %d", (long long)a.rows, a.N);
   return false;
 }
@@ -783,7 +788,8 @@ int shape_of(const Args& a, bool grouped) {
     return kAny + choose(a, grouped, 1 << kFew | 1 << kTall32 | 1 << kMid | 1 << kTile128);
   // Weights that are read once and do not stay in the 256 MB of the last-level cache: one wave a tile, many
   // workgroups a CU, and the non-temporal hint.
-  if (a.rows <= 16 * (grouped ? (int64_t)a.groups : 1) && (int64_t)a.groups * a.N * a.K >= kStreamed) return kStream;
+  if (a.rows <= 16 * (grouped ? (int64_t)a.groups : 1) && (int64_t)a.groups * a.N >= (kStreamed + a.K - 1) / a.K)
+    return kStream;
   // big_kernel's offsets are 31 bits: those of its tile's rows, or of all of x where rows are taken by number
   constexpr int64_t kReach = 1ll << 31;
   const bool big = !a.out_f32 && a.K > kFp8Block && 256 * a.ws + a.K < kReach &&
@@ -820,7 +826,7 @@ bool aligned(const void* p, int to) { return reinterpret_cast<uintptr_t>(p) % to
 #define CHECK_PRODUCT(name)                                                                                       \
   DSV2_REQUIRE(out_dtype == DSV2_DTYPE_BF16 || out_dtype == DSV2_DTYPE_F32, DSV2_E_FLAGS, name ": out_dtype %d", \
                out_dtype);                                                                                        \
-  DSV2_REQUIRE(rows >= 0 && rows <= 0x7fffffff && K > 0 && K <= 1 << 30 && N > 0 && N <= 0x7fffff00, DSV2_E_SHAPE, \
+  DSV2_REQUIRE(rows >= 0 && rows <= 0x7fffffff && K > 0 && K <= 1 << 30 && N > 0 && N <= 1 << 30, DSV2_E_SHAPE, \
                name ": %lld rows, K %d, N %d", (long long)rows, K, N);                                           \
   if (rows == 0) return DSV2_OK;                                                                                  \
   DSV2_REQUIRE((rows == 1 || y_stride >= N) && x_stride >= 0 && x_scales_stride >= 0 && w_stride >= 0 &&          \

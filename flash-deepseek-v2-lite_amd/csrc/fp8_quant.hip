@@ -342,7 +342,7 @@ bool fits(const void* p, int64_t stride, int size) { return reinterpret_cast<uin
 
 #define CHECK_COMMON(name)                                                                                      \
   DSV2_REQUIRE(dtype == DSV2_DTYPE_BF16 || dtype == DSV2_DTYPE_F32, DSV2_E_FLAGS, name ": dtype %d", dtype);    \
-  DSV2_REQUIRE(rows >= 0 && K > 0 && K <= 0x7fffff00, DSV2_E_SHAPE, name ": %lld rows of %d", (long long)rows, K);                 \
+  DSV2_REQUIRE(rows >= 0 && K > 0 && K <= 1 << 30, DSV2_E_SHAPE, name ": %lld rows of %d", (long long)rows, K); \
   if (rows == 0) return DSV2_OK;
 
 int dsv2_quantize_fp8_blocks(const void* x, int64_t x_stride, int64_t x_gstride, int64_t groups, int64_t rows, int K,

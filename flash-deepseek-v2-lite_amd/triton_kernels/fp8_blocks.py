@@ -25,7 +25,7 @@ from . import _hip
 
 BLOCK = 128
 MAX_ROWS = 2 ** 31 - 1
-MAX_COLS = 2 ** 31 - 256
+MAX_COLS = 2 ** 30  # and features of a product
 MAX_GROUPS = 65536
 
 # These calls launch kernels of 2 to 10 us for few rows, so their own host time is looked at: a launch takes 3 us of it,

@@ -136,18 +136,18 @@ def test_entry_points_refuse_bad_arguments_without_launching():
     refused("dsv2_quantize_fp8_blocks", [one, 200, 0, 1, 5, 200, 0, 1, one, one],
             (0, None, "null"), (0, one + 1, "alignment"), (1, -8, "alignment"), (3, 2, "groups"), (4, -1, "rows"),
             (5, 0, "rows"), (5, 2 ** 31 - 1, "rows"), (6, 2, "dtype"), (7, 64, "blocks of 64"), (8, None, "null"),
-            (9, one + 2, "alignment"), (4, 2 ** 40, "rows"))
+            (9, one + 2, "alignment"), (4, 2 ** 40, "rows"), (5, 2 ** 30 + 1, "rows of"))
     refused("dsv2_quantize_fp8_blocks", [one, 200, 0, 1, 5, 200, 1, 128, one, one],
             (0, one + 2, "alignment"), (4, 2 ** 40, "matrices"), (3, 2 ** 31, "matrices"), (3, -1, "groups"))
     refused("dsv2_rmsnorm_fp8_blocks", [one, 200, one, 200, one, 1e-6, 5, 200, 0, one, one, one],
             (0, None, "null"), (4, None, "null"), (11, None, "null"), (9, None, "null"), (6, 2 ** 31, "rows"),
-            (7, 0, "rows"), (8, 3, "dtype"), (4, one + 1, "alignment"), (11, one + 1, "alignment"))
+            (7, 0, "rows"), (7, 2 ** 30 + 1, "rows of"), (8, 3, "dtype"), (4, one + 1, "alignment"), (11, one + 1, "alignment"))
     refused("dsv2_silu_mul_fp8_blocks", [one, 200, one, 200, 5, 200, 0, one, one],
             (0, None, "null"), (2, None, "null"), (2, one + 1, "alignment"), (4, -1, "rows"), (4, 2 ** 40, "rows"),
-            (6, -1, "dtype"))
+            (5, 2 ** 30 + 1, "rows of"), (6, -1, "dtype"))
     product = [one, 200, one, 2, 5, 200, one, 200, one, 2, 300, one, 300, 0]
     refused("dsv2_linear_fp8_blocks", product,
-            (0, None, "null"), (2, one + 2, "alignment"), (4, -1, "rows"), (4, 2 ** 31, "rows"), (5, 0, "K 0"),
+            (0, None, "null"), (2, one + 2, "alignment"), (4, -1, "rows"), (4, 2 ** 31, "rows"), (5, 0, "K 0"), (5, 2 ** 30 + 1, "K"), (10, 2 ** 30 + 1, "N"),
             (8, None, "null"), (10, 0, "N 0"), (11, one + 1, "alignment"), (12, 299, "strides"), (7, -1, "strides"),
             (13, 2, "out_dtype"))
     with pytest.raises(_hip.HipKernelError, match="rows of"):  # more tiles than a launch has workgroups
@@ -157,6 +157,17 @@ def test_entry_points_refuse_bad_arguments_without_launching():
     refused("dsv2_grouped_linear_fp8_blocks", grouped,
             (0, None, "null"), (4, -1, "rows of x"), (5, None, "rows of x"), (5, one + 2, "alignment"), (6, -1, "rows"),
             (9, -1, "strides"), (15, 0, "0 groups"), (15, 65537, "groups"), (16, None, "null"), (17, one + 2, "alignment"))
+
+
+@pytest.mark.parametrize("rows,k,n,groups,f32", [(600_000_000, 16, 16, 0, 1), (1_000_000_000, 1, 3, 0, 0), (1, 16, 2 ** 30, 0, 0),
+                                                 (1, 16, 2 ** 30, 1, 1), (65536, 16, 30_000, 65536, 0)])
+def test_calls_of_very_many_tiles_take_tiles_that_a_launch_has_room_for(rows, k, n, groups, f32):
+    shape = _hip.lib.dsv2_linear_fp8_blocks_tiles(rows, k, n, groups, f32)
+    bm, bn, threads = {0: (16, 16, 512), 1: (32, 16, 512), 2: (32, 32, 256), 3: (32, 64, 128), 4: (64, 64, 512),
+                       5: (128, 64, 512), 6: (128, 128, 512), 7: (128, 256, 512), 8: (256, 256, 512), 10: (16, 32, 64),
+                       11: (16, 16, 512), 13: (32, 32, 256), 15: (64, 64, 512), 17: (128, 128, 512)}[shape]
+    tiles = (rows + min(rows, groups) * (bm - 1)) // bm if groups else -(-rows // bm)
+    assert tiles * -(-n // bn) * threads < 2 ** 32
 
 
 def test_definition_of_the_rounding():
