@@ -284,10 +284,14 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a) {
   }
 }
 
+// A wave a row where it holds the row in one chunk, else four (MI355X, bf16 with a residual, a wave / four: 8,192 x
+// 512 7.4 / 9.1 us, 65,536 x 128 21 / 45; in four chunks 8,192 x 2,048 19.3 / 18.8, 64 x 2,048 4.1 / 2.7).  Maxima in
+// registers or scales read back: 64 x 2,048 2.7 / 3.1, 64 x 4,096 3.2 / 3.5, 64 x 8,192 4.3 / 4.9, 4,096 x 8,192
+// 38.8 / 39.4.  8,192 x 2,048 moves 118 MB at 6.1 TB/s, more than a copy past the caches (5.7): some of it stays in them.
 template <typename T, bool RES, bool VEC>
 void launch_norm(const NormArgs& a, hipStream_t st) {
-  if (a.K <= 2048 && a.rows > 1024) {
-    norm_kernel<T, 1, 4, RES, VEC><<<dim3((unsigned)((a.rows + 3) / 4)), 256, 0, st>>>(a);
+  if (a.K <= 512) {
+    norm_kernel<T, 1, 1, RES, VEC><<<dim3((unsigned)((a.rows + 3) / 4)), 256, 0, st>>>(a);
   } else if (a.K <= 2048) {
     norm_kernel<T, 4, 1, RES, VEC><<<dim3((unsigned)a.rows), 256, 0, st>>>(a);
   } else if (a.K <= 4096) {

@@ -115,7 +115,7 @@ def test_blocks_of_zeros_and_of_values_that_are_none(dtype):
 
 
 @pytest.mark.parametrize("m", [1, 3, 1024, 1025, 1200])
-@pytest.mark.parametrize("k", [1, 64, 200, 1030, 2048, 2049, 5120, 8192, 8200, 10944])
+@pytest.mark.parametrize("k", [1, 64, 200, 512, 513, 1030, 2048, 2049, 5120, 8192, 8200, 10944])
 @pytest.mark.parametrize("dtype,residual", [(BF, True), (BF, False), (F32, True), (F32, False)])
 def test_norm(m, k, dtype, residual):
     if m > 3 and k > 2049:
