@@ -807,7 +807,7 @@ int launch(const Args& a, hipStream_t st) {
     case kMid: return launch_ring<2, 2, 2, 2, 2, 3, false, false, EXACT, GROUPED>(a, st);
     case kMid128: return launch_ring<2, 2, 4, 2, 2, 3, false, false, EXACT, GROUPED>(a, st);
     case kTile128: return launch_ring<2, 4, 4, 2, 1, 4, false, false, EXACT, GROUPED>(a, st);
-    case kLong128: return launch_ring<2, 4, 4, 4, 1, 3, false, false, EXACT, GROUPED>(a, st);
+    case kLong128: return launch_ring<EXACT ? 2 : 4, 4, EXACT ? 4 : 2, 4, 1, 3, false, false, EXACT, GROUPED>(a, st);
     case kStream: return launch_ring<1, 1, 1, 2, 1, 3, true, false, EXACT, GROUPED>(a, st);
     case kAny + kFew: return launch_ring<1, 1, 1, 1, 8, 2, false, true, EXACT, GROUPED>(a, st);
     case kAny + kTall32: return launch_ring<1, 1, 2, 2, 4, 2, false, true, EXACT, GROUPED>(a, st);
