@@ -701,10 +701,12 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
 }
 
 // ---------------------------------------------------------------------------
-// Which of them.  A launch of n tiles takes about a + b k us, and for each 256 tiles (one a CU) past the first
-// c + d k more, k the blocks of K (measured at 32 to 6,144 tiles of 4, 16 and 64 blocks on MI355X, off by 3 to 10%
-// on the mean): many waves on small tiles where the launch is short of tiles, larger tiles, which read the
-// operands less often, where it is not.  The least of the estimates is taken.
+// Which of them.  A launch of up to 256 tiles (one a CU) takes about a + b k us, k the blocks of K, and each further
+// round of them c + d k more; the last round takes as long with one tile as with 256.  (Measured on MI355X: 135 products
+// of 1 to 4,096 rows, 512 to 10,944 columns, off by 3 to 9% on the mean.  The shape that is taken was 0.7% slower
+// on the mean than the best one, with fp32 results 0.5%; estimates without whole rounds 7%.)  Groups' tiles also wait for
+// memory: what they load together takes at least 3 us and 8 TB/s (31 products of 4 to 4,000 tokens of 8 to 128
+// groups: 2% slower than the best, without this 5%).
 // ---------------------------------------------------------------------------
 constexpr int64_t kStreamed = 64ll << 20;
 struct Cost {
@@ -713,15 +715,15 @@ struct Cost {
 };
 enum Shape { kFew, kFew32, kTall32, kWide32, kMid, kMid128, kTile128, kLong128, kBig, kShapes, kStream, kAny };
 constexpr Cost kCost[kShapes] = {
-    {16, 16, 3.4f, 0.06f, 0.69f, 0.09f},    // 8 waves along K
-    {32, 16, 3.8f, 0.06f, 1.85f, 0.07f},    // 8 along K
-    {32, 32, 3.4f, 0.12f, 0.78f, 0.10f},    // 4 along K
-    {32, 64, 4.0f, 0.35f, 0.80f, 0.16f},    // 2 along K
-    {64, 64, 4.2f, 0.27f, 2.25f, 0.31f},    // 4 on the tile, 2 along K
-    {128, 64, 5.2f, 0.44f, 3.18f, 0.51f},   // 4 on the tile, 2 along K
-    {128, 128, 5.7f, 0.68f, 3.86f, 0.74f},  // 8 on the tile
-    {128, 256, 8.0f, 1.10f, 7.89f, 1.22f},  // 8 on the tile
-    {256, 256, 9.3f, 1.51f, 9.12f, 1.71f},  // big_kernel
+    {16, 16, 2.95f, 0.07f, 0.79f, 0.04f},   // 8 waves along K
+    {32, 16, 3.18f, 0.08f, 1.74f, 0.07f},   // 8 along K
+    {32, 32, 2.86f, 0.15f, 0.83f, 0.09f},   // 4 along K
+    {32, 64, 3.34f, 0.36f, 0.79f, 0.13f},   // 2 along K
+    {64, 64, 3.95f, 0.28f, 2.32f, 0.28f},   // 4 on the tile, 2 along K
+    {128, 64, 4.71f, 0.48f, 3.24f, 0.48f},  // 4 on the tile, 2 along K
+    {128, 128, 4.95f, 0.70f, 3.50f, 0.72f},  // 8 on the tile
+    {128, 256, 6.27f, 1.07f, 6.80f, 1.09f},  // 16 on the tile (fp32 results: 8)
+    {256, 256, 7.27f, 1.52f, 6.03f, 1.50f},  // big_kernel
 };
 
 // token tiles: the most there may be, and as many as are likely (groups of like sizes)
@@ -748,9 +750,9 @@ Shape choose(const Args& a, bool grouped, unsigned among) {
     if (!(among >> s & 1)) continue;
     const Cost& c = kCost[s];
     if (!launchable(a, grouped, c.bm, c.bn, 512)) continue;
-    float n = likely_tiles(a, grouped, c.bm) * ((a.N + c.bn - 1) / c.bn) * (1.f / 256);
-    if (s == kBig) n = ceilf(n);
-    const float t = c.a + c.b * k + fmaxf(n - 1.f, 0.f) * (c.c + c.d * k);
+    const float n = likely_tiles(a, grouped, c.bm) * ((a.N + c.bn - 1) / c.bn);
+    float t = c.a + c.b * k + fmaxf(ceilf(n * (1.f / 256)) - 1.f, 0.f) * (c.c + c.d * k);
+    if (grouped) t = fmaxf(t, 3.f + n * (c.bm + c.bn) * a.K * (1.f / 8e6f));
     if (t < least) least = t, best = static_cast<Shape>(s);
   }
   return best;

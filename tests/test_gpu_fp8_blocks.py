@@ -358,8 +358,8 @@ def rows_for(shape, n, k, groups, f32):
 
 
 # kernel (dsv2_linear_fp8_blocks_tiles): features with which it is taken, dense and of eight groups
-KERNELS = {0: (331, 331), 1: (2809, 331), 2: (8191, 1003), 3: (None, 16384), 4: (16381, 2051), 5: (16384, 2051), 6: (16384, 2811),
-           7: (16381, 8189), 8: (16381, 8187), 10: (65536, 65536), 11: (300, 300), 13: (8191, 1003), 15: (16381, 2051),
+KERNELS = {0: (331, 331), 1: (2809, 331), 2: (8191, 1003), 3: (9003, 20003), 4: (16381, 1003), 5: (16384, 1003), 6: (16384, 2811),
+           7: (16381, 8189), 8: (16381, 8187), 10: (65536, 65536), 11: (300, 300), 13: (8191, 1003), 15: (16381, 6001),
            17: (16381, 2811)}
 CASES = [(s, g, k) for s, (dense, of8) in KERNELS.items() for g, n in ((0, dense), (8, of8)) if n
          for k in ((1040, 1104, 2064) if s == 1 else (144, 272, 1040, 1104, 2064) if s < 9 else (1040, 2064) if s == 10 else (135, 1041, 1288))]
@@ -415,7 +415,7 @@ def test_large_tiles_one_after_another(m, n, k):
 @pytest.mark.parametrize("groups,n,k", [(8, 8184, 1104), (70, 2048, 272), (3, 16387, 2064)])
 def test_large_tiles_of_groups(groups, n, k):
     m = 9000
-    assert _hip.lib.dsv2_linear_fp8_blocks_tiles(m, k, n, groups, 0) == (8 if groups < 64 else 7)
+    assert _hip.lib.dsv2_linear_fp8_blocks_tiles(m, k, n, groups, 0) == 8
     cuts = torch.randint(0, m + 1, (groups - 1,), generator=gen(k), device=DEV).sort().values.tolist()
     offsets = [5, *[max(c, 5) for c in cuts], m - 7]
     w, sw = matrix(n, k, n + k, 128, groups)
