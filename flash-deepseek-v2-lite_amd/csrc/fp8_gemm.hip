@@ -219,13 +219,17 @@ __device__ __forceinline__ floatx4_t block_sum(const Decoded& w, const Decoded& 
 // ---------------------------------------------------------------------------
 // A tile by KW groups of WM x WN waves, each wave TT x FT MFMA tiles of 16 tokens x 16 features; group i takes every
 // KW-th block of K from block i on.  A block's rows of 128 bytes lie in LDS with their 16-byte pieces exchanged
-// by row (piece p of row r at place p ^ key(r)), so that 8 lanes reading one piece of 8 rows hit different banks.  Row i
-// of a wave's MFMA tile f is its feature 4 FT (i / 4) + 4 f + i % 4: a lane ends with 4 FT neighbouring features.
+// by row (piece p of row r at place p ^ key(r)), so that 8 lanes reading one piece of 8 rows hit different banks.  Row
+// i of a wave's MFMA tile f is its feature 4 FT (i / 4) + 4 f + i % 4: a lane ends with 4 FT neighbouring features.
 //
 // Rows of whole 16 codes at multiples of 16 bytes (ANY false) are streamed into LDS without registers
-// (global_load_lds): each group has a ring of ST stages, ST - 1 of them requested ahead, and a block's scales come the same
-// way, 64 a load.  Other rows go through registers, one block ahead of two stages.  A group of one wave needs no
+// (global_load_lds): each group has a ring of ST stages, ST - 1 of them requested ahead, and a block's scales come the
+// same way, 64 a load.  Other rows go through registers, one block ahead of two stages.  A group of one wave needs no
 // barrier: its own waits order its loads and reads.  At the end the groups' sums meet in LDS, in fixed order.
+//
+// Few rows are bound by what a CU can load, 50 to 55 bytes a ns on MI355X whatever the depth of the ring (2 to 8), the
+// waves or the tile: 64 x 2,048 x 10,944 takes 11 us, 9.5 of them for 525 KB a CU.  So tiles are small enough for 256
+// CUs first, and large only beyond (1 x 3,648 x 2,048 3.3 us, 1.7 of them an empty launch; 1,024 x 2,816 x 2,048 17).
 // ---------------------------------------------------------------------------
 // 16 (4) bytes a lane from src to LDS, lane after lane from dst; in functions of their own: with the builtin in a
 // template hipcc drops the kernel's host launch stub
@@ -354,7 +358,8 @@ __global__ __launch_bounds__(64 * WM * WN * KW) void ring_kernel(const Args a) {
   if constexpr (ANY) put(0);
   int st = 0;
   for (int i = 0; i < steps; ++i) {
-    // this wave's loads of stage st have landed (its writes are done) and its reads of the stage before, then every wave's
+    // this wave's loads of stage st have landed (its writes are done) and its reads of the stage before, then every
+    // wave's
     __builtin_amdgcn_s_waitcnt(vmcnt_only(ANY ? 63 : (ST - 2) * (DI + SI)) & ~0xf00);
     asm volatile("" ::: "memory");
     if constexpr (NW > 1) {
@@ -434,12 +439,18 @@ __global__ __launch_bounds__(64 * WM * WN * KW) void ring_kernel(const Args a) {
 // fragments of the block are in registers then, so its stage takes the loads of the block after the next, and the
 // next block's first fragments are read under the matrix instructions that are left.  Sums are added three
 // instructions behind.  The next tile's first two blocks follow this one's last two without a gap.
+//
+// Bound by the issue of instructions and by power: a wave issues some 215 vector instructions a block, 32 of them
+// matrix, and the matrix cores are busy for 48 to 52% of the cycles, at 1.8 GHz (LDS 30%).  MI355X: 8,192 x 21,888 x
+// 2,048 355 us (2.07 PFLOP/s), 8,192^3 475 (2.31); 128 x 256 tiles of ring_kernel 580 and 660, but 26 for 32 with 1,024
+// x 2,816 x 2,048.  Groups: 49,152 rows of 64, 2,816 x 2,048, 350 us, 1.17 times their rows in tiles.
 // ---------------------------------------------------------------------------
 struct Big {
   static constexpr int BM = 256, BN = 256, kThreads = 512, kWgs = 256;
   static constexpr int kStage = (BM + BN) * 128;
-  // scales of eight blocks: of the tokens [256][8], the places of tokens 8 i + 8 .. 8 i + 15, i even, exchanged by xor 4 (banks),
-  // then of the features' two blocks [2][8], four copies; two such windows, and the addresses of the tokens' scales
+  // scales of eight blocks: of the tokens [256][8], the places of tokens 8 i + 8 .. 8 i + 15, i even, exchanged by xor 4
+  // (banks), then of the features' two blocks [2][8], four copies; two such windows, and the addresses of the tokens'
+  // scales, twice
   static constexpr int kWindow = BM * 32 + 4 * 256, kScales = 2 * kStage, kRows = kScales + 2 * kWindow;
   static constexpr int kGroups = kRows + 2 * BM * 8, kUnused = kGroups + 64 * 12, kLds = kUnused + 8 * 256;
   static_assert(kLds <= 160 * 1024, "LDS");
@@ -516,7 +527,8 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
     if (thread < BM) {
       int64_t row = thread < count ? m0 + thread : -1;
       if (gather && row >= 0) row = a.index[row];
-      *srow(thread) = row < 0 || row >= a.xrows ? reinterpret_cast<uint64_t>(kZeros) + 1 : reinterpret_cast<uint64_t>(a.sx + row * a.sxs);
+      *srow(thread) = row < 0 || row >= a.xrows ? reinterpret_cast<uint64_t>(kZeros) + 1
+                                                : reinterpret_cast<uint64_t>(a.sx + row * a.sxs);
     }
   };
   // pieces past the rows' end: of the last block, which is the tile's last to be requested
@@ -540,7 +552,8 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
     const int window = Big::kScales + ((part >> 3) + window0 & 1) * Big::kWindow;
     const int to = wave < 4 ? (in * 4 + wave) * 256 : BM * 32 + (wave - 4) * 256;
     // a window past the last block's goes where nothing is read, not into the next tile's first
-    load_lds4(reinterpret_cast<const float*>(row & ~1ull) + b, ring + (first < nch ? window + to : Big::kUnused + wave * 256));
+    load_lds4(reinterpret_cast<const float*>(row & ~1ull) + b,
+              ring + (first < nch ? window + to : Big::kUnused + wave * 256));
   };
   floatx4_t acc[8][4];
 #pragma unroll
@@ -788,8 +801,10 @@ int launch_big(Args a, hipStream_t st) {
 int shape_of(const Args& a, bool grouped) {
   if (a.K % 16 != 0 || !dsv2_aligned16(a.x) || !dsv2_aligned16(a.w) || a.xs % 16 != 0 || a.ws % 16 != 0 || a.wgs % 16 != 0)
     return kAny + choose(a, grouped, 1 << kFew | 1 << kTall32 | 1 << kMid | 1 << kTile128);
-  // Weights that are read once and do not stay in the 256 MB of the last-level cache: one wave a tile, many
-  // workgroups a CU, and the non-temporal hint.
+  // Weights that are read once and do not stay in the 256 MB of the last-level cache (a model's others are read in
+  // between): one wave a tile, many workgroups a CU, and the non-temporal hint (MI355X: 5 x 102,400 x 2,048, fp32, 36.6
+  // us, 5.8 TB/s, the best of the others 49.6; 64 tokens x 6 of 64 groups of 2,816 x 2,048 62.4 / 75.6).  Smaller ones
+  // the other way: 64 x 2,048 x 10,944 (22 MB) 30 / 11, 1 x 3,648 x 2,048 (7 MB) 8 / 3.5.
   if (a.rows <= 16 * (grouped ? (int64_t)a.groups : 1) && (int64_t)a.groups * a.N >= (kStreamed + a.K - 1) / a.K)
     return kStream;
   // big_kernel's offsets are 31 bits: those of its tile's rows, or of all of x where rows are taken by number

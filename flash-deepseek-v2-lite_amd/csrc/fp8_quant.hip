@@ -4,11 +4,11 @@
 //
 // A block of a row is 16 lanes of 8 values: one 16-byte load a lane of bf16, the largest value by four
 // DPP steps, one 8-byte store of codes.  All of it is bound by memory (2 to 9 bytes a value for some 10
-// to 30 instructions), for few rows by the launch and one trip to memory.
+// to 30 instructions), for few rows by the launch and one trip to memory.  MI355X, bf16: 64 x 2,048 1.9 us, an empty
+// launch 1.7; SwiGLU of 49,152 x 1,408 60.5 us, 5.8 TB/s, the rate of a large copy; 384 x 1,408 2.6.
 #include "fp8_blocks.h"
 
 namespace {
-
 
 template <bool NT>
 __device__ __forceinline__ uint4 load16(const void* p) {
@@ -160,7 +160,8 @@ __global__ __launch_bounds__(256) void block_kernel(const BlockArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Weights: one workgroup a 128 x 128 block, its values in registers between the maximum and the codes.
+// Weights: one workgroup a 128 x 128 block, its values in registers between the maximum and the codes, so that memory
+// is read once (MI355X: 21,888 x 2,048 bf16 25.3 us, 5.3 TB/s).
 // ---------------------------------------------------------------------------
 struct WeightArgs {
   const void* x;

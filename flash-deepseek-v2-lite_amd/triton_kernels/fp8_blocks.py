@@ -280,7 +280,8 @@ def _out_type(name: str, dtype: torch.dtype | None) -> tuple[torch.dtype, int]:
 def linear_fp8_blocks(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
                       output_dtype: torch.dtype | None = None) -> torch.Tensor:
     """The product [..., N] of activations [..., K] (codes, scales) and weights [N, K] (codes, scales): fp32 sums, one
-    rounding to ``output_dtype`` (bf16, the default, or fp32)."""
+    rounding to ``output_dtype`` (bf16, the default, or fp32).  A block's two scales are multiplied first, in fp32: their
+    product has to be in its range."""
     name = "linear_fp8_blocks"
     index = x.get_device()
     if (x.dim() == 2 and x_scales.dim() == 2 and weight.dim() == 2 and weight_scales.dim() == 2 and _plain(index) and

@@ -582,15 +582,16 @@ int dsv2_mla_decode_paged_fp4(const void* q, int64_t q_ts, int64_t q_hs, int tok
  * is a / 448 and the codes are the e4m3 values nearest to 448 v / a, ties to even; a block with an infinity or a
  * NaN stands for NaN throughout.  kb = ceil(K / 128).  No counterpart in the reference (bf16 only).
  * Inputs may have any row stride (in elements) and alignment; rows of whole 8 values at multiples of 16 bytes
- * are read faster.  Codes and scales come without gaps. */
+ * are read faster.  Codes and scales come without gaps and overlap nothing that is read.  K up to 2^30. */
 
 /* Rows x [rows, K] (block_rows 1, groups 1; scales [rows, kb]) or `groups` matrices of rows x K x_gstride
  * apart (block_rows 128; codes [groups, rows, K], scales [groups, ceil(rows / 128), kb]). */
 int dsv2_quantize_fp8_blocks(const void* x, int64_t x_stride, int64_t x_gstride, int64_t groups, int64_t rows, int K,
                              int dtype, int block_rows, void* codes, float* scales, void* stream);
 
-/* h = x + residual (residual NULL: x), stored in x's type to sum [rows, K]; codes and scales of h * weight / sqrt(mean(h^2) + eps), which is not rounded in between.  The
- * least block (2^-100) is one of h * weight here. */
+/* h = x + residual (residual NULL: x), rounded to x's type and stored to sum [rows, K]; codes and scales of
+ * h * weight / sqrt(mean(h^2) + eps), which is not rounded in between.  The least block (2^-100) is one of
+ * h * weight here. */
 int dsv2_rmsnorm_fp8_blocks(const void* x, int64_t x_stride, const void* residual, int64_t res_stride,
                             const void* weight, float eps, int64_t rows, int K, int dtype, void* codes, float* scales,
                             void* sum, void* stream);
@@ -600,8 +601,8 @@ int dsv2_silu_mul_fp8_blocks(const void* gate, int64_t gate_stride, const void* 
                              int K, int dtype, void* codes, float* scales, void* stream);
 
 /* y[m, n] = sum over blocks b of x_scales[m, b] * w_scales[n / 128, b] * (codes x[m, b] . codes w[n, b]): sums in
- * fp32, one rounding to out_dtype.  Strides in elements; rows of x and w need not be aligned (16-byte rows of
- * whole 16 codes are read faster). */
+ * fp32, one rounding to out_dtype.  A block's two scales are multiplied first, in fp32.  K and N up to 2^30.
+ * Strides in elements; rows of x and w need not be aligned (16-byte rows of whole 16 codes are read faster). */
 int dsv2_linear_fp8_blocks(const void* x, int64_t x_stride, const float* x_scales, int64_t x_scales_stride, int64_t rows,
                            int K, const void* w, int64_t w_stride, const float* w_scales, int64_t w_scales_stride, int N,
                            void* y, int64_t y_stride, int out_dtype, void* stream);
