@@ -276,8 +276,8 @@ __global__ __launch_bounds__(64 * WM * WN * KW) void ring_kernel(const Args a) {
   static_assert(!ANY || ST == 2, "one block in registers");
   constexpr int BM = R::BM, BN = R::BN, NW = R::NW, DI = R::DI, SI = R::SI;
   extern __shared__ __attribute__((aligned(16))) uint8_t ring[];
-  int tn, group = 0, count;
-  int64_t m0;
+  int tn, group = 0, count = 0;  // no rows, should the offsets change between two looks at them
+  int64_t m0 = 0;
   if (!tile_of<BM, GROUPED>(a, tn, group, m0, count)) return;
   const int n0 = tn * BN, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kw = wave / NW, wv = wave % NW, wm = wv % WM, wn = wv / WM;
@@ -885,6 +885,9 @@ int dsv2_grouped_linear_fp8_blocks(const void* x, int64_t x_stride, const float*
 }
 
 int dsv2_linear_fp8_blocks_tiles(int64_t rows, int K, int N, int groups, int out_dtype) {
+  DSV2_REQUIRE(rows > 0 && rows <= 0x7fffffff && K > 0 && K <= 1 << 30 && N > 0 && N <= 1 << 30 && groups >= 0 &&
+                   groups <= 65536, DSV2_E_SHAPE, "linear_fp8_blocks_tiles: %lld rows, K %d, N %d, %d groups",
+               (long long)rows, K, N, groups);
   Args a{};
   a.xs = a.ws = K;
   a.wgs = (int64_t)N * K;

@@ -619,7 +619,8 @@ int dsv2_grouped_linear_fp8_blocks(const void* x, int64_t x_stride, const float*
 
 /* The kernel that a product without gaps between its rows takes (groups 0: dense): 0 16 tokens x 16 features,
  * 1 32 x 16, 2 32 x 32, 3 32 x 64, 4 64 x 64, 5 128 x 64, 6 128 x 128, 7 128 x 256, 8 256 x 256, 10 streamed weights
- * (16 x 32); of rows that are not whole 16s 11 16 x 16, 13 32 x 32, 15 64 x 64, 17 128 x 128.  Host arithmetic only. */
+ * (16 x 32); of rows that are not whole 16s 11 16 x 16, 13 32 x 32, 15 64 x 64, 17 128 x 128.
+ * Host arithmetic only; DSV2_E_SHAPE for sizes that no product has. */
 int dsv2_linear_fp8_blocks_tiles(int64_t rows, int K, int N, int groups, int out_dtype);
 
 #ifdef __cplusplus

@@ -170,6 +170,13 @@ def test_calls_of_very_many_tiles_take_tiles_that_a_launch_has_room_for(rows, k,
     assert tiles * -(-n // bn) * threads < 2 ** 32
 
 
+@pytest.mark.parametrize("args", [(0, 128, 128, 0, 0), (-1, 128, 128, 0, 0), (2 ** 31, 128, 128, 0, 0), (5, 0, 128, 0, 0),
+                                  (5, -16, 128, 2, 0), (5, 128, 0, 0, 1), (5, 2 ** 30 + 1, 128, 0, 0), (5, 128, 128, -1, 0),
+                                  (5, 128, 128, 65537, 0)])
+def test_the_tiles_of_sizes_that_no_product_has_are_an_error(args):
+    assert _hip.lib.dsv2_linear_fp8_blocks_tiles(*args) == -2
+
+
 def test_definition_of_the_rounding():
     """The 64-bit form against torch's conversion, and against every code and every tie."""
     q = torch.arange(256, dtype=torch.uint8).view(E4).float()
