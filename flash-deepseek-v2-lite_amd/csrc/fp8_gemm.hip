@@ -275,6 +275,11 @@ __global__ __launch_bounds__(64 * WM * WN * KW) void ring_kernel(const Args a) {
   static_assert(!NT || WM * WN == 1, "a load is of tokens or of features");
   static_assert(!ANY || ST == 2, "one block in registers");
   constexpr int BM = R::BM, BN = R::BN, NW = R::NW, DI = R::DI, SI = R::SI;
+  // With many matrix instructions a block its fragments are read before the next loads are issued, which holds a wave
+  // back, and sums are added two instructions behind (MI355X: 1,024 x 2,816 x 2,048 17.6 -> 16.9 us, 2,048 x 2,816 x 2,048
+  // 25.0 -> 23.9, 128 x 64 tiles 47 -> 44).  With few of them the loads' way is the longer one and they go first (32 x
+  // 32 tiles at 128 x 2,048 x 10,944 16.1 us, behind the fragments 18.5), as do those through registers to bf16 results.
+  constexpr bool kLate = TT * FT >= 8 && (EXACT || !ANY);
   extern __shared__ __attribute__((aligned(16))) uint8_t ring[];
   int tn, group = 0, count = 0;  // no rows, should the offsets change between two looks at them
   int64_t m0 = 0;
@@ -367,30 +372,49 @@ __global__ __launch_bounds__(64 * WM * WN * KW) void ring_kernel(const Args a) {
       asm volatile("" ::: "memory");
     }
     const int c = i * KW + kw;
-    issue(c + (ST - 1) * KW, st == 0 ? ST - 1 : st - 1);
-    if (c < nch) {
+    if constexpr (!kLate) issue(c + (ST - 1) * KW, st == 0 ? ST - 1 : st - 1);
+    if (KW == 1 || c < nch) {
       const uint8_t* const from = mine + st * R::kStage;
       auto frag = [&](int at) {
         const int4v u = *reinterpret_cast<const int4v*>(from + at + piece);
         const int4v v = *reinterpret_cast<const int4v*>(from + at + (piece ^ 64));
         return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
       };
-      Operand wf[FT];
+      int8v wc[FT], xc[TT];
+      float f0[TT];
 #pragma unroll
-      for (int f = 0; f < FT; ++f) operand(frag(wat + f * 4 * 128), wf[f]);
+      for (int f = 0; f < FT; ++f) wc[f] = frag(wat + f * 4 * 128);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) xc[t] = frag(xat + t * 16 * 128);
       const float s = *reinterpret_cast<const float*>(from + swat);
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        Operand xf;
-        operand(frag(xat + t * 16 * 128), xf);
-        const float f0 = s * *reinterpret_cast<const float*>(from + sxat + t * 64);
-#pragma unroll
-        for (int f = 0; f < FT; ++f) {
-          const floatx4_t p = block_sum(wf[f], xf);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[t][f][e] = __builtin_fmaf(f0, p[e], acc[t][f][e]);
-        }
+      for (int t = 0; t < TT; ++t) f0[t] = *reinterpret_cast<const float*>(from + sxat + t * 64);
+      if constexpr (kLate) {
+        __builtin_amdgcn_sched_barrier(0);
+        issue(c + (ST - 1) * KW, st == 0 ? ST - 1 : st - 1);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      Operand wf[FT];
+#pragma unroll
+      for (int f = 0; f < FT; ++f) operand(wc[f], wf[f]);
+      floatx4_t p[3];
+#pragma unroll
+      for (int j = 0; j < TT * FT + 2; ++j) {
+        if (j < TT * FT) {
+          Operand xf;
+          operand(xc[j / FT], xf);
+          p[j % 3] = block_sum(wf[j % FT], xf);
+        }
+        if (j >= 2) {
+          const int u = j - 2, t = u / FT, f = u % FT;
+          if (f == 0) f0[t] *= s;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[t][f][e] = __builtin_fmaf(f0[t], p[u % 3][e], acc[t][f][e]);
+        }
+        if constexpr (kLate && !EXACT) __builtin_amdgcn_sched_barrier(0);
+      }
+    } else if constexpr (kLate) {
+      issue(c + (ST - 1) * KW, st == 0 ? ST - 1 : st - 1);
     }
     st = st + 1 == ST ? 0 : st + 1;
     if constexpr (ANY) put(st);
@@ -442,7 +466,7 @@ __global__ __launch_bounds__(64 * WM * WN * KW) void ring_kernel(const Args a) {
 //
 // Bound by the issue of instructions and by power: a wave issues some 215 vector instructions a block, 32 of them
 // matrix, and the matrix cores are busy for 48 to 52% of the cycles, at 1.8 GHz (LDS 30%).  MI355X: 8,192 x 21,888 x
-// 2,048 355 us (2.07 PFLOP/s), 8,192^3 475 (2.31); 128 x 256 tiles of ring_kernel 580 and 660, but 26 for 32 with 1,024
+// 2,048 355 us (2.07 PFLOP/s), 8,192^3 475 (2.31); 128 x 256 tiles of ring_kernel 552 and 648, but 23 for 31 with 1,024
 // x 2,816 x 2,048.  Groups: 49,152 rows of 64, 2,816 x 2,048, 350 us, 1.17 times their rows in tiles.
 // ---------------------------------------------------------------------------
 struct Big {
@@ -716,8 +740,8 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
 // ---------------------------------------------------------------------------
 // Which of them.  A launch of up to 256 tiles (one a CU) takes about a + b k us, k the blocks of K, and each further
 // round of them c + d k more; the last round takes as long with one tile as with 256.  (Measured on MI355X: 135 products
-// of 1 to 4,096 rows, 512 to 10,944 columns, off by 3 to 9% on the mean.  The shape that is taken was 0.7% slower
-// on the mean than the best one, with fp32 results 0.5%; estimates without whole rounds 7%.)  Groups' tiles also wait for
+// of 1 to 4,096 rows, 512 to 10,944 columns, off by 3 to 8% on the mean.  The shape that is taken was 0.4% slower
+// on the mean than the best one, with fp32 results 1%; estimates without whole rounds 7%.)  Groups' tiles also wait for
 // memory: what they load together takes at least 3 us and 8 TB/s (31 products of 4 to 4,000 tokens of 8 to 128
 // groups: 2% slower than the best, without this 5%).
 // ---------------------------------------------------------------------------
@@ -728,15 +752,15 @@ struct Cost {
 };
 enum Shape { kFew, kFew32, kTall32, kWide32, kMid, kMid128, kTile128, kLong128, kBig, kShapes, kStream, kAny };
 constexpr Cost kCost[kShapes] = {
-    {16, 16, 2.95f, 0.07f, 0.79f, 0.04f},   // 8 waves along K
-    {32, 16, 3.18f, 0.08f, 1.74f, 0.07f},   // 8 along K
-    {32, 32, 2.86f, 0.15f, 0.83f, 0.09f},   // 4 along K
-    {32, 64, 3.34f, 0.36f, 0.79f, 0.13f},   // 2 along K
-    {64, 64, 3.95f, 0.28f, 2.32f, 0.28f},   // 4 on the tile, 2 along K
-    {128, 64, 4.71f, 0.48f, 3.24f, 0.48f},  // 4 on the tile, 2 along K
-    {128, 128, 4.95f, 0.70f, 3.50f, 0.72f},  // 8 on the tile
-    {128, 256, 6.27f, 1.07f, 6.80f, 1.09f},  // 16 on the tile (fp32 results: 8)
-    {256, 256, 7.27f, 1.52f, 6.03f, 1.50f},  // big_kernel
+    {16, 16, 2.85f, 0.069f, 0.81f, 0.043f},    // 8 waves along K
+    {32, 16, 3.22f, 0.083f, 1.78f, 0.071f},    // 8 along K
+    {32, 32, 2.71f, 0.149f, 0.83f, 0.093f},    // 4 along K
+    {32, 64, 3.11f, 0.333f, 0.83f, 0.135f},    // 2 along K
+    {64, 64, 3.92f, 0.275f, 2.31f, 0.269f},    // 4 on the tile, 2 along K
+    {128, 64, 4.45f, 0.446f, 3.18f, 0.438f},   // 4 on the tile, 2 along K
+    {128, 128, 4.75f, 0.671f, 3.35f, 0.704f},  // 8 on the tile
+    {128, 256, 6.42f, 0.965f, 7.45f, 1.024f},  // 16 on the tile (fp32 results: 8)
+    {256, 256, 7.28f, 1.525f, 6.08f, 1.588f},  // big_kernel
 };
 
 // token tiles: the most there may be, and as many as are likely (groups of like sizes)

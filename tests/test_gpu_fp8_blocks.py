@@ -358,7 +358,7 @@ def rows_for(shape, n, k, groups, f32):
 
 
 # kernel (dsv2_linear_fp8_blocks_tiles): features with which it is taken, dense and of eight groups
-KERNELS = {0: (331, 331), 1: (2809, 331), 2: (8191, 1003), 3: (9003, 20003), 4: (16381, 1003), 5: (16384, 1003), 6: (16384, 2811),
+KERNELS = {0: (331, 331), 1: (2809, 201), 2: (8191, 1003), 3: (9003, 20003), 4: (16381, 1003), 5: (16384, 1003), 6: (16384, 2811),
            7: (16381, 8189), 8: (16381, 8187), 10: (65536, 65536), 11: (300, 300), 13: (8191, 1003), 15: (16381, 6001),
            17: (16381, 2811)}
 CASES = [(s, g, k) for s, (dense, of8) in KERNELS.items() for g, n in ((0, dense), (8, of8)) if n
