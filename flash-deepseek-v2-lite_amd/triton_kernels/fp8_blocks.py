@@ -37,7 +37,7 @@ _TYPES = {_BF16: 0, _F32: 1}  # DSV2_DTYPE_*
 _ENTRY = {n: getattr(_hip.lib, n) for n in ("dsv2_quantize_fp8_blocks", "dsv2_rmsnorm_fp8_blocks",
                                             "dsv2_silu_mul_fp8_blocks", "dsv2_linear_fp8_blocks",
                                             "dsv2_grouped_linear_fp8_blocks")}
-_QUANTIZE, _RMSNORM, _SILU, _LINEAR = tuple(_ENTRY.values())[:4]
+_QUANTIZE, _RMSNORM, _SILU, _LINEAR, _GROUPED = _ENTRY.values()
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
 
@@ -111,14 +111,14 @@ def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Ten
     """(codes, scales) of bf16 or fp32 values: activations [..., K] in blocks of one row (``block_rows`` 1) or weights
     [N, K] or [E, N, K] in blocks of 128 rows (``block_rows`` 128; a matrix's last block may be shorter)."""
     name = "quantize_fp8_blocks"
-    if block_rows == 1 and x.dim() == 2:
+    if x.dim() == 2 and (block_rows == 1 or block_rows == BLOCK):
         n, k = x.shape
         rs, cs = x.stride()
         dtype, index = _TYPES.get(x.dtype), x.get_device()
         if dtype is not None and cs == 1 and 0 < n <= MAX_ROWS and 0 < k <= MAX_COLS and _plain(index):
-            kb = (k + 127) // BLOCK
-            codes, scales = _empty_strided((n, k), (k, 1), _E4M3), _empty_strided((n, kb), (kb, 1), _F32)
-            _check(_QUANTIZE(x.data_ptr(), rs, 0, 1, n, k, dtype, 1, codes.data_ptr(), scales.data_ptr(),
+            kb, nb = (k + 127) // BLOCK, n if block_rows == 1 else (n + 127) // BLOCK
+            codes, scales = _empty_strided((n, k), (k, 1), _E4M3), _empty_strided((nb, kb), (kb, 1), _F32)
+            _check(_QUANTIZE(x.data_ptr(), rs, 0, 1, n, k, dtype, block_rows, codes.data_ptr(), scales.data_ptr(),
                              _hip._raw_stream(index)), name)
             return codes, scales
     index = _device(name, x)
@@ -318,6 +318,27 @@ def grouped_linear_fp8_blocks(x: torch.Tensor, x_scales: torch.Tensor, weights: 
     ``offsets`` int32 [E + 1] is read on the device only.  Rows of no group are not written (here: undefined); an
     offset below the largest one before it, or outside [0, R], counts as the nearest that is not."""
     name = "grouped_linear_fp8_blocks"
+    index = x.get_device()
+    if (x.dim() == 2 and x_scales.dim() == 2 and weights.dim() == 3 and weight_scales.dim() == 3 and offsets.dim() == 1 and
+            _plain(index) and x_scales.get_device() == index and weights.get_device() == index and
+            weight_scales.get_device() == index and offsets.get_device() == index and
+            (rows is None or rows.get_device() == index and rows.dim() == 1)):
+        (r, k), (groups, out, wk) = x.shape, weights.shape
+        n = r if rows is None else rows.shape[0]
+        kb, t = (k + 127) // BLOCK, 0 if output_dtype is None else _TYPES.get(output_dtype)
+        (xs, xc), (xss, xsc) = x.stride(), x_scales.stride()
+        (wgs, ws, wc), (wsgs, wss, wsc) = weights.stride(), weight_scales.stride()
+        if (x.dtype is _E4M3 and weights.dtype is _E4M3 and x_scales.dtype is _F32 and weight_scales.dtype is _F32 and
+                offsets.dtype is _I32 and t is not None and wk == k and xc == wc == xsc == wsc == 1 and
+                0 < n <= MAX_ROWS and 0 < r <= MAX_ROWS and 0 < k <= MAX_COLS and 0 < out <= MAX_COLS and
+                0 < groups <= MAX_GROUPS and x_scales.shape == (r, kb) and offsets.shape == (groups + 1,) and
+                weight_scales.shape == (groups, (out + 127) // BLOCK, kb) and offsets.is_contiguous() and
+                (rows is None or rows.dtype is _I32 and rows.is_contiguous())):
+            y = _empty_strided((n, out), (out, 1), output_dtype or _BF16)
+            _check(_GROUPED(x.data_ptr(), xs, x_scales.data_ptr(), xss, r, None if rows is None else rows.data_ptr(), n, k,
+                            weights.data_ptr(), wgs, ws, weight_scales.data_ptr(), wsgs, wss, out, groups,
+                            offsets.data_ptr(), y.data_ptr(), out, t, _hip._raw_stream(index)), name)
+            return y
     if rows is None:
         index = _device(name, x, x_scales, weights, weight_scales, offsets)
     else:

@@ -637,6 +637,27 @@ def test_the_plain_case_and_the_checks_one_by_one_agree(monkeypatch):
         assert torch.equal(got[name].view(torch.uint8), want[name].view(torch.uint8)), name
 
 
+def test_weights_by_the_plain_case_and_by_the_checks_one_by_one(monkeypatch):
+    x = torch.randn(300, 200, device=DEV, generator=gen(3))
+    inputs = [x, x.to(BF), x[:, 3:], x[::2], x[:, :1], x.expand(1, 300, 200)[0]]
+    w, sw = matrix(140, 300, 2, 128, 3)
+    c, s = matrix(20, 300, 1, 1)
+    rows = torch.tensor([3, 3, 19, 0, -1, 7, 20, 5, 5], device=DEV).int()
+
+    def results():
+        for v in inputs:
+            yield from F.quantize_fp8_blocks(v, 128)
+        for dtype in (None, BF, F32):
+            yield F.grouped_linear_fp8_blocks(c, s, w, sw, i32([0, 4, 4, 20]), None, dtype)
+            yield F.grouped_linear_fp8_blocks(c, s, w, sw, i32([0, 2, 9, 9]), rows, dtype)
+
+    want = list(results())
+    monkeypatch.setattr(F, "_plain", lambda index: False)
+    for a, b in zip(results(), want):
+        assert a.shape == b.shape and a.dtype == b.dtype and a.is_contiguous() and b.is_contiguous()
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_no_rows():
     w, sw = matrix(140, 300, 2, 128)
     x = torch.zeros(0, 300, device=DEV, dtype=BF)
