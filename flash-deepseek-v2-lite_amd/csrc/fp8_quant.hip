@@ -116,15 +116,16 @@ struct BlockArgs {
 __device__ __forceinline__ float swiglu(float g, float u) {
   constexpr float l2e = 1.44269504088896f, l2e_lo = 1.92596299e-8f, ln2 = 0.693147180559945f;
   const float t = g * l2e, r = __builtin_fmaf(g, l2e_lo, __builtin_fmaf(g, l2e, -t)) * ln2;
-  float q;
-  if (t < -120.f) {  // 1 + exp(-g) = exp(-g) in fp32, and soon past its range
-    const float e = __builtin_amdgcn_exp2f(t);
-    q = __builtin_fmaf(r, e, e);
-  } else {
-    const float e = __builtin_amdgcn_exp2f(-t), d = 1.f + __builtin_fmaf(-r, e, e);
-    q = __builtin_amdgcn_rcpf(d);
-    q = __builtin_fmaf(__builtin_fmaf(-q, d, 1.f), q, q);
+  if (t < -120.f) {
+    // 1 + exp(-g) = exp(-g) in fp32, and soon past its range: 2^130 exp(g) instead, a normal number as long as the largest
+    // u brings the product to a code; u takes half of the factor back before the product, which has to stay in range
+    if (t < -300.f && g > -__builtin_inff()) return 0.f * g * u;
+    const float e = __builtin_amdgcn_exp2f(t + 130.f);
+    return g * __builtin_fmaf(r, e, e) * (u * 0x1p-64f) * 0x1p-66f;
   }
+  const float e = __builtin_amdgcn_exp2f(-t), d = 1.f + __builtin_fmaf(-r, e, e);
+  float q = __builtin_amdgcn_rcpf(d);
+  q = __builtin_fmaf(__builtin_fmaf(-q, d, 1.f), q, q);
   return g * q * u;
 }
 

@@ -203,6 +203,21 @@ def test_silu_mul_at_the_ends():
             assert codes[0, 128:].float().isfinite().all() and scales[0, 1].isfinite() and scales[1].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_silu_mul_where_the_exponential_is_no_normal_number(dtype):
+    """Gates down to -3e38, with factors that bring the product back to codes: blocks of one value and of 128."""
+    g = torch.cat([torch.arange(-200, -80, 0.25), torch.tensor([-250.0, -1000.0, -1e30, -3e38, -3.3e38])])
+    u = 2.0 ** torch.arange(0, 128, 3.0)
+    gate, up = (v.reshape(-1, 1).to(DEV, dtype) for v in torch.meshgrid(g, u, indexing="ij"))
+    for cols in (1, 128):
+        n = gate.numel() // cols * cols
+        a, b = gate[:n].view(-1, cols), up[:n].view(-1, cols)
+        codes, scales = F.silu_mul_fp8_blocks(a, b)
+        q, s = R.rounded(a.double() * torch.sigmoid(a.double()) * b.double(), 1)
+        R.check_codes(codes, q, 2 * 8 * U24 + 3 * U24)
+        R.check_scales(scales, s, 9 * U24)
+
+
 # ---------------------------------------------------------------- products
 def matrix(n, k, seed, rows, groups=None):
     x = rnd(*(() if groups is None else (groups,)), n, k, seed=seed, dtype=F32)
