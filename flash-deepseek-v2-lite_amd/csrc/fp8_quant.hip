@@ -5,7 +5,8 @@
 // A block of a row is 16 lanes of 8 values: one 16-byte load a lane of bf16, the largest value by four
 // DPP steps, one 8-byte store of codes.  All of it is bound by memory (2 to 9 bytes a value for some 10
 // to 30 instructions), for few rows by the launch and one trip to memory.  MI355X, bf16: 64 x 2,048 1.9 us, an empty
-// launch 1.7; SwiGLU of 49,152 x 1,408 60.5 us, 5.8 TB/s, the rate of a large copy; 384 x 1,408 2.6.
+// launch 1.7; SwiGLU of 49,152 x 1,408 57.5 us, 6.0 TB/s (a large copy 5.7: some of it stays in the last-level
+// cache); 384 x 1,408 2.6.
 #include "fp8_blocks.h"
 
 namespace {
@@ -323,14 +324,16 @@ void launch_blocks(const BlockArgs& a, bool vec, hipStream_t st) {
   else block_kernel<T, SILU, false, NB, false><<<grid, 256, 0, st>>>(a);
 }
 
-// One block for each 16 lanes (MI355X: 1,024 blocks 2.0 us, two 2.3; 33,000 SwiGLU 5.4 / 5.6), two where there are
-// many workgroups either way (262,144 18.4 / 16.7; 180,000 SwiGLU 25.3 / 24.7).  Non-temporal loads of what
-// cannot stay in the 256 MB of the last-level cache (49,152 x 1,408 SwiGLU 65.6 -> 62.7; in it 16.9 -> 19.7).
+// One block for each 16 lanes, two where there are many workgroups either way (MI355X, one / two: 1,024 blocks of rows
+// 3.1 / 3.6 us, 65,536 6.7 / 6.7, 131,072 11.1 / 10.4, 640,000 45 / 40), but not of SwiGLU, which hides its loads by
+// its own instructions (33,000 blocks 7.0 / 7.9, 330,000 37.7 / 39.1).  Two with non-temporal loads for what cannot stay
+// in the 256 MB of the last-level cache (80,000 x 2,048 rows 85 -> 77; 49,152 x 1,408 SwiGLU 61.4 -> 56.5; in the
+// cache 17.1 -> 19.8 and 22.1 -> 23.6).
 template <typename T, bool SILU>
 void launch_blocks(const BlockArgs& a, bool vec, hipStream_t st) {
   const int64_t bytes = a.n_blocks * kFp8Block * (int64_t)sizeof(T) * (SILU ? 2 : 1);
   if (bytes > 256ll << 20) launch_blocks<T, SILU, 2, true>(a, vec, st);
-  else if (a.n_blocks > 98304) launch_blocks<T, SILU, 2, false>(a, vec, st);
+  else if (!SILU && a.n_blocks > 98304) launch_blocks<T, false, 2, false>(a, vec, st);
   else launch_blocks<T, SILU, 1, false>(a, vec, st);
 }
 
