@@ -693,7 +693,10 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
     for (int f = 1; f < 4; ++f)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[7][f][e] = __builtin_fmaf(sx7, p[f][e], acc[7][f][e]);
+    // the next tile's first block adds these once more: nothing of them may be left, a NaN would outlast a factor of zero
     sx7 = 0.f;
+#pragma unroll
+    for (int f = 1; f < 4; ++f) p[f] = floatx4_t{0.f, 0.f, 0.f, 0.f};
     // lane group kg holds features 8 kg .. 8 kg + 7 of each half of the wave's 64
     int r0 = wm * 128 + li;
     asm volatile("" : "+v"(r0));  // here: kept over the loop the rows' offsets are spilled, and a reload waits for the stores

@@ -442,6 +442,64 @@ def test_large_tiles_of_groups(groups, n, k):
     assert torch.equal(again[5:m - 7], y[5:m - 7])
 
 
+def with_nans(codes, first, share, seed):
+    """The codes with a NaN in some rows (`share` of them), in a column from `first` on; and which rows."""
+    *lead, k = codes.shape
+    bad = torch.rand(*lead, generator=gen(seed), device=DEV) < share
+    at = torch.randint(first, k, lead, generator=gen(seed + 1), device=DEV)
+    out = codes.view(torch.uint8).clone()
+    here = bad[..., None] & (at[..., None] == torch.arange(k, device=DEV))
+    return torch.where(here, torch.full_like(out, 0x7f), out).view(E4), bad
+
+
+def check_nans(got, clean, bad):
+    """NaN where a row of x or of w has one, and nowhere else a bit of another value."""
+    assert torch.equal(got.isnan(), bad)
+    assert torch.equal(torch.where(bad, 0, got), torch.where(bad, 0, clean))
+
+
+@pytest.mark.parametrize("m,n,k", [(4200, 16376, 272), (700, 33000, 144), (9000, 4104, 1296), (700, 33003, 272)])
+def test_large_tiles_keep_nans_to_their_rows_and_features(m, n, k):
+    """The sums of a tile's last instructions are added behind its end: none of them may reach the next tile."""
+    assert _hip.lib.dsv2_linear_fp8_blocks_tiles(m, k, n, 0, 0) == 8 and -(-m // 256) * -(-n // 256) > 256
+    x, sx = matrix(m, k, m + k, 1)
+    w, sw = matrix(n, k, n * k, 128)
+    clean = F.linear_fp8_blocks(x, sx, w, sw)
+    last = (k - 1) // 128 * 128
+    nx, xbad = with_nans(x, last, 0.02, 1)
+    nw, wbad = with_nans(w, last, 0.02, 2)
+    no = torch.zeros_like
+    for a, ab, b, bb in ((nx, xbad, w, no(wbad)), (x, no(xbad), nw, wbad), (nx, xbad, nw, wbad)):
+        check_nans(F.linear_fp8_blocks(a, sx, b, sw), clean, ab[:, None] | bb)
+    # one tile's last 16 rows of each half alone
+    nx = x.view(torch.uint8).clone()
+    xbad = no(xbad)
+    for at in (112, 240):
+        nx[256 + at:256 + at + 16, k - 1] = 0x7f
+        xbad[256 + at:256 + at + 16] = True
+    check_nans(F.linear_fp8_blocks(nx.view(E4), sx, w, sw), clean, xbad[:, None] | no(wbad))
+
+
+@pytest.mark.parametrize("groups,n,k", [(8, 8184, 1104), (70, 2048, 272), (3, 16387, 2064)])
+def test_large_tiles_of_groups_keep_nans_to_their_rows_and_features(groups, n, k):
+    m = 9000
+    assert _hip.lib.dsv2_linear_fp8_blocks_tiles(m, k, n, groups, 0) == 8
+    cuts = torch.randint(0, m + 1, (groups - 1,), generator=gen(k), device=DEV).sort().values.tolist()
+    offsets = i32([0, *cuts, m])
+    group = torch.searchsorted(offsets[1:].contiguous(), torch.arange(m, device=DEV), right=True)
+    w, sw = matrix(n, k, n + k, 128, groups)
+    x, sx = matrix(2000, k, 1, 1)
+    rows = torch.randint(0, 2000, (m,), generator=gen(m), device=DEV).int()
+    clean = F.grouped_linear_fp8_blocks(x, sx, w, sw, offsets, rows)
+    last = (k - 1) // 128 * 128
+    nx, xbad = with_nans(x, last, 0.02, 1)
+    nw, wbad = with_nans(w, last, 0.02, 2)
+    xbad = xbad[rows.long()]
+    no = torch.zeros_like
+    for a, ab, b, bb in ((nx, xbad, w, no(wbad)), (x, no(xbad), nw, wbad), (nx, xbad, nw, wbad)):
+        check_nans(F.grouped_linear_fp8_blocks(a, sx, b, sw, offsets, rows), clean, ab[:, None] | bb[group])
+
+
 @pytest.mark.parametrize("k", [300, 304, 512])
 def test_grouped_holds_offsets_and_row_numbers_to_their_ranges(k):
     w, sw = matrix(70, k, 1, 128, 4)
