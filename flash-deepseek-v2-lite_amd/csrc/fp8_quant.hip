@@ -116,7 +116,9 @@ struct BlockArgs {
 // rounding lost: v_exp_f32 of t alone is off by |t| / 2 ulp.  The quotient by v_rcp_f32 with one residual.
 __device__ __forceinline__ float swiglu(float g, float u) {
   constexpr float l2e = 1.44269504088896f, l2e_lo = 1.92596299e-8f, ln2 = 0.693147180559945f;
-  const float t = g * l2e, r = __builtin_fmaf(g, l2e_lo, __builtin_fmaf(g, l2e, -t)) * ln2;
+  // a gate past 2.3e38 takes t out of range and r to -inf, which times exp2(-t) = 0 would be NaN; where the exponential
+  // counts r is within 2^-15
+  const float t = g * l2e, lost = __builtin_fmaf(g, l2e_lo, __builtin_fmaf(g, l2e, -t)), r = __builtin_fmaxf(lost, -1.f) * ln2;
   if (t < -120.f) {
     // 1 + exp(-g) = exp(-g) in fp32, and soon past its range: 2^130 exp(g) instead, a normal number as long as the largest
     // u brings the product to a code; u takes half of the factor back before the product, which has to stay in range

@@ -218,6 +218,23 @@ def test_silu_mul_where_the_exponential_is_no_normal_number(dtype):
         R.check_scales(scales, s, 9 * U24)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_silu_mul_of_gates_up_to_the_largest(dtype):
+    """Gates up to the type's largest, with factors that leave their product in range: blocks of one value and of 128."""
+    g = torch.cat([torch.tensor([60.0, 88.0, 90.0, 104.0, 128.0, 1e4, 1e20, 2.3e38, 2.35e38, 2.36e38, 2.4e38, 3e38, 3.3e38]),
+                   torch.tensor([torch.finfo(dtype).max])])
+    u = torch.cat([s * 2.0 ** -torch.arange(0, 127, 3.0) for s in (1.0, -1.0)])
+    gate, up = (v.reshape(-1, 1).to(DEV, dtype) for v in torch.meshgrid(g, u, indexing="ij"))
+    assert gate.isfinite().all()
+    for cols in (1, 128):
+        n = gate.numel() // cols * cols
+        a, b = gate[:n].view(-1, cols), up[:n].view(-1, cols)
+        codes, scales = F.silu_mul_fp8_blocks(a, b)
+        q, s = R.rounded(a.double() * torch.sigmoid(a.double()) * b.double(), 1)
+        R.check_codes(codes, q, 2 * 8 * U24 + 3 * U24)
+        R.check_scales(scales, s, 9 * U24)
+
+
 # ---------------------------------------------------------------- products
 def matrix(n, k, seed, rows, groups=None):
     x = rnd(*(() if groups is None else (groups,)), n, k, seed=seed, dtype=F32)
