@@ -235,6 +235,23 @@ def test_silu_mul_of_gates_up_to_the_largest(dtype):
         R.check_scales(scales, s, 9 * U24)
 
 
+def test_silu_mul_rounds_the_quotient_once():
+    """Blocks of one value, up = 1: the scale is silu(g) / 448.  1 + exp(-g) is rounded by up to half a step of numbers
+    from 1 to 2 and holds exp(-g) to 8 half steps; then the quotient's rounding and the scale's, half a step of each."""
+    gate = torch.linspace(8, 12, 2 ** 20, dtype=torch.float64, device=DEV).float().view(-1, 1)
+    codes, scales = F.silu_mul_fp8_blocks(gate, torch.ones_like(gate))
+    assert (codes.float() == 448).all()
+    e = torch.exp(-gate.double())
+    y = gate.double() / (1 + e)
+
+    def half(v):  # half a step at v, relative; of the larger step where v is next to a power of two
+        return torch.exp2(torch.floor(torch.log2(v * (1 + 2.0 ** -20)))) * U24 / v
+
+    bound = (U24 / (1 + e) + 8 * U24 * e + half(y) + half(y / 448)) * (1 + 2.0 ** -20)
+    off = (scales.double() * 448 / y - 1).abs()
+    assert (off <= bound).all(), (off / bound).max()
+
+
 # ---------------------------------------------------------------- products
 def matrix(n, k, seed, rows, groups=None):
     x = rnd(*(() if groups is None else (groups,)), n, k, seed=seed, dtype=F32)
