@@ -750,21 +750,24 @@ __global__ __launch_bounds__(512) void big_kernel(const Args a) {
 // ---------------------------------------------------------------------------
 constexpr int64_t kStreamed = 64ll << 20;
 struct Cost {
-  int bm, bn;
+  int bm, bn, threads;  // of a workgroup
   float a, b, c, d;
 };
 enum Shape { kFew, kFew32, kTall32, kWide32, kMid, kMid128, kTile128, kLong128, kBig, kShapes, kStream, kAny };
 constexpr Cost kCost[kShapes] = {
-    {16, 16, 2.85f, 0.069f, 0.81f, 0.043f},    // 8 waves along K
-    {32, 16, 3.22f, 0.083f, 1.78f, 0.071f},    // 8 along K
-    {32, 32, 2.71f, 0.149f, 0.83f, 0.093f},    // 4 along K
-    {32, 64, 3.11f, 0.333f, 0.83f, 0.135f},    // 2 along K
-    {64, 64, 3.92f, 0.275f, 2.31f, 0.269f},    // 4 on the tile, 2 along K
-    {128, 64, 4.45f, 0.446f, 3.18f, 0.438f},   // 4 on the tile, 2 along K
-    {128, 128, 4.75f, 0.671f, 3.35f, 0.704f},  // 8 on the tile
-    {128, 256, 6.42f, 0.965f, 7.45f, 1.024f},  // 16 on the tile (fp32 results: 8)
-    {256, 256, 7.28f, 1.525f, 6.08f, 1.588f},  // big_kernel
+    {16, 16, 512, 2.85f, 0.069f, 0.81f, 0.043f},     // 8 waves along K
+    {32, 16, 512, 3.22f, 0.083f, 1.78f, 0.071f},     // 8 along K
+    {32, 32, 256, 2.71f, 0.149f, 0.83f, 0.093f},     // 4 along K
+    {32, 64, 128, 3.11f, 0.333f, 0.83f, 0.135f},     // 2 along K
+    {64, 64, 512, 3.92f, 0.275f, 2.31f, 0.269f},     // 4 on the tile, 2 along K
+    {128, 64, 512, 4.45f, 0.446f, 3.18f, 0.438f},    // 4 on the tile, 2 along K
+    {128, 128, 512, 4.75f, 0.671f, 3.35f, 0.704f},   // 8 on the tile
+    {128, 256, 1024, 6.42f, 0.965f, 7.45f, 1.024f},  // 16 on the tile (fp32 results: 8)
+    {256, 256, 512, 7.28f, 1.525f, 6.08f, 1.588f},   // big_kernel
 };
+constexpr Cost kStreamed32 = {16, 32, 64, 0.f, 0.f, 0.f, 0.f};  // chosen by another rule
+constexpr const Cost& tile_of_shape(int s) { return s == kStream ? kStreamed32 : kCost[s % kAny]; }
+constexpr int threads_of(int s, bool f32) { return s == kLong128 && f32 ? 512 : tile_of_shape(s).threads; }
 
 // token tiles: the most there may be, and as many as are likely (groups of like sizes)
 int64_t most_tiles(const Args& a, bool grouped, int bm) {
@@ -777,8 +780,10 @@ float likely_tiles(const Args& a, bool grouped, int bm) {
 }
 
 // a launch has fewer than 2^32 threads
-bool launchable(const Args& a, bool grouped, int bm, int bn, int threads) {
-  return most_tiles(a, grouped, bm) <= ((1ll << 32) / threads - 8) / ((a.N + (int64_t)bn - 1) / bn);
+bool launchable(const Args& a, bool grouped, int shape) {
+  const Cost& c = tile_of_shape(shape);
+  return most_tiles(a, grouped, c.bm) <=
+         ((1ll << 32) / threads_of(shape, a.out_f32) - 8) / ((a.N + (int64_t)c.bn - 1) / c.bn);
 }
 
 // the least estimate among the shapes whose bits are set and that have not too many tiles
@@ -789,7 +794,7 @@ Shape choose(const Args& a, bool grouped, unsigned among) {
   for (int s = 0; s < kShapes; ++s) {
     if (!(among >> s & 1)) continue;
     const Cost& c = kCost[s];
-    if (!launchable(a, grouped, c.bm, c.bn, 512)) continue;
+    if (!launchable(a, grouped, s)) continue;
     const float n = likely_tiles(a, grouped, c.bm) * ((a.N + c.bn - 1) / c.bn);
     float t = c.a + c.b * k + fmaxf(ceilf(n * (1.f / 256)) - 1.f, 0.f) * (c.c + c.d * k);
     if (grouped) t = fmaxf(t, 3.f + n * (c.bm + c.bn) * a.K * (1.f / 8e6f));
@@ -798,26 +803,30 @@ Shape choose(const Args& a, bool grouped, unsigned among) {
   return best;
 }
 
-bool set_tiles(Args& a, bool grouped, int bm, int bn, int threads) {
-  a.mt = (int)most_tiles(a, grouped, bm);
-  a.nt = (a.N + bn - 1) / bn;
-  if (launchable(a, grouped, bm, bn, threads)) return true;
+bool set_tiles(Args& a, bool grouped, int shape) {
+  const Cost& c = tile_of_shape(shape);
+  a.mt = (int)most_tiles(a, grouped, c.bm);
+  a.nt = (a.N + c.bn - 1) / c.bn;
+  if (launchable(a, grouped, shape)) return true;
   dsv2_set_error("linear_fp8_blocks: %lld rows of %d", (long long)a.rows, a.N);
   return false;
 }
 dim3 grid_of(const Args& a) { return dim3((unsigned)(((int64_t)a.mt * a.nt + 7) / 8 * 8)); }
 
-template <int WM, int WN, int TT, int FT, int KW, int ST, bool NT, bool ANY, bool EXACT, bool GROUPED>
+template <int SHAPE, int WM, int WN, int TT, int FT, int KW, int ST, bool NT, bool ANY, bool EXACT, bool GROUPED>
 int launch_ring(Args a, hipStream_t st) {
   using R = Ring<WM, WN, TT, FT, KW, ST>;
-  if (!set_tiles(a, GROUPED, R::BM, R::BN, R::kThreads)) return DSV2_E_SHAPE;
+  static_assert(R::BM == tile_of_shape(SHAPE).bm && R::BN == tile_of_shape(SHAPE).bn &&
+                R::kThreads == threads_of(SHAPE, EXACT), "what the choice goes by");
+  if (!set_tiles(a, GROUPED, SHAPE)) return DSV2_E_SHAPE;
   ring_kernel<WM, WN, TT, FT, KW, ST, NT, ANY, EXACT, GROUPED><<<grid_of(a), R::kThreads, R::kLds, st>>>(a);
   return dsv2_launch_status(GROUPED ? "grouped_linear_fp8_blocks" : "linear_fp8_blocks");
 }
 
 template <bool GROUPED>
 int launch_big(Args a, hipStream_t st) {
-  if (!set_tiles(a, GROUPED, Big::BM, Big::BN, Big::kThreads)) return DSV2_E_SHAPE;
+  static_assert(Big::BM == kCost[kBig].bm && Big::BN == kCost[kBig].bn && Big::kThreads == kCost[kBig].threads, "the same");
+  if (!set_tiles(a, GROUPED, kBig)) return DSV2_E_SHAPE;
   dim3 grid = grid_of(a);
   grid.x = min(grid.x, (unsigned)Big::kWgs);
   big_kernel<GROUPED><<<grid, Big::kThreads, Big::kLds, st>>>(a);
@@ -832,7 +841,8 @@ int shape_of(const Args& a, bool grouped) {
   // between): one wave a tile, many workgroups a CU, and the non-temporal hint (MI355X: 5 x 102,400 x 2,048, fp32, 36.6
   // us, 5.8 TB/s, the best of the others 49.6; 64 tokens x 6 of 64 groups of 2,816 x 2,048 62.4 / 75.6).  Smaller ones
   // the other way: 64 x 2,048 x 10,944 (22 MB) 30 / 11, 1 x 3,648 x 2,048 (7 MB) 8 / 3.5.
-  if (a.rows <= 16 * (grouped ? (int64_t)a.groups : 1) && (int64_t)a.groups * a.N >= (kStreamed + a.K - 1) / a.K)
+  if (a.rows <= 16 * (grouped ? (int64_t)a.groups : 1) && (int64_t)a.groups * a.N >= (kStreamed + a.K - 1) / a.K &&
+      launchable(a, grouped, kStream))
     return kStream;
   // big_kernel's offsets are 31 bits: those of its tile's rows, or of all of x where rows are taken by number
   constexpr int64_t kReach = 1ll << 31;
@@ -844,19 +854,19 @@ int shape_of(const Args& a, bool grouped) {
 template <bool EXACT, bool GROUPED>
 int launch(const Args& a, hipStream_t st) {
   switch (shape_of(a, GROUPED)) {
-    case kFew: return launch_ring<1, 1, 1, 1, 8, 2, false, false, EXACT, GROUPED>(a, st);
-    case kFew32: return launch_ring<1, 1, 2, 1, 8, 2, false, false, EXACT, GROUPED>(a, st);
-    case kTall32: return launch_ring<1, 1, 2, 2, 4, 2, false, false, EXACT, GROUPED>(a, st);
-    case kWide32: return launch_ring<1, 1, 2, 4, 2, 2, false, false, EXACT, GROUPED>(a, st);
-    case kMid: return launch_ring<2, 2, 2, 2, 2, 3, false, false, EXACT, GROUPED>(a, st);
-    case kMid128: return launch_ring<2, 2, 4, 2, 2, 3, false, false, EXACT, GROUPED>(a, st);
-    case kTile128: return launch_ring<2, 4, 4, 2, 1, 4, false, false, EXACT, GROUPED>(a, st);
-    case kLong128: return launch_ring<EXACT ? 2 : 4, 4, EXACT ? 4 : 2, 4, 1, 3, false, false, EXACT, GROUPED>(a, st);
-    case kStream: return launch_ring<1, 1, 1, 2, 1, 3, true, false, EXACT, GROUPED>(a, st);
-    case kAny + kFew: return launch_ring<1, 1, 1, 1, 8, 2, false, true, EXACT, GROUPED>(a, st);
-    case kAny + kTall32: return launch_ring<1, 1, 2, 2, 4, 2, false, true, EXACT, GROUPED>(a, st);
-    case kAny + kMid: return launch_ring<2, 2, 2, 2, 2, 2, false, true, EXACT, GROUPED>(a, st);
-    case kAny + kTile128: return launch_ring<2, 4, 4, 2, 1, 2, false, true, EXACT, GROUPED>(a, st);
+    case kFew: return launch_ring<kFew, 1, 1, 1, 1, 8, 2, false, false, EXACT, GROUPED>(a, st);
+    case kFew32: return launch_ring<kFew32, 1, 1, 2, 1, 8, 2, false, false, EXACT, GROUPED>(a, st);
+    case kTall32: return launch_ring<kTall32, 1, 1, 2, 2, 4, 2, false, false, EXACT, GROUPED>(a, st);
+    case kWide32: return launch_ring<kWide32, 1, 1, 2, 4, 2, 2, false, false, EXACT, GROUPED>(a, st);
+    case kMid: return launch_ring<kMid, 2, 2, 2, 2, 2, 3, false, false, EXACT, GROUPED>(a, st);
+    case kMid128: return launch_ring<kMid128, 2, 2, 4, 2, 2, 3, false, false, EXACT, GROUPED>(a, st);
+    case kTile128: return launch_ring<kTile128, 2, 4, 4, 2, 1, 4, false, false, EXACT, GROUPED>(a, st);
+    case kLong128: return launch_ring<kLong128, EXACT ? 2 : 4, 4, EXACT ? 4 : 2, 4, 1, 3, false, false, EXACT, GROUPED>(a, st);
+    case kStream: return launch_ring<kStream, 1, 1, 1, 2, 1, 3, true, false, EXACT, GROUPED>(a, st);
+    case kAny + kFew: return launch_ring<kAny + kFew, 1, 1, 1, 1, 8, 2, false, true, EXACT, GROUPED>(a, st);
+    case kAny + kTall32: return launch_ring<kAny + kTall32, 1, 1, 2, 2, 4, 2, false, true, EXACT, GROUPED>(a, st);
+    case kAny + kMid: return launch_ring<kAny + kMid, 2, 2, 2, 2, 2, 2, false, true, EXACT, GROUPED>(a, st);
+    case kAny + kTile128: return launch_ring<kAny + kTile128, 2, 4, 4, 2, 1, 2, false, true, EXACT, GROUPED>(a, st);
     default: break;
   }
   if constexpr (!EXACT) return launch_big<GROUPED>(a, st);

@@ -170,6 +170,35 @@ def test_calls_of_very_many_tiles_take_tiles_that_a_launch_has_room_for(rows, k,
     assert tiles * -(-n // bn) * threads < 2 ** 32
 
 
+# kernel: tokens and features of a tile, threads of a workgroup (kernel 7: with bf16 and with fp32 results)
+TILES = {0: (16, 16, 512), 1: (32, 16, 512), 2: (32, 32, 256), 3: (32, 64, 128), 4: (64, 64, 512), 5: (128, 64, 512),
+         6: (128, 128, 512), 7: (128, 256, (1024, 512)), 8: (256, 256, 512), 10: (16, 32, 64), 11: (16, 16, 512),
+         13: (32, 32, 256), 15: (64, 64, 512), 17: (128, 128, 512)}
+
+
+def room(shape, rows, n, groups, f32):
+    """Workgroups that the kernel has, and that a launch of its workgroups has room for (beyond 2^32 threads there are none;
+    a launch is rounded up to eights)."""
+    bm, bn, threads = TILES[shape]
+    threads = threads if isinstance(threads, int) else threads[f32]
+    tiles = (rows + min(rows, groups) * (bm - 1)) // bm if groups else -(-rows // bm)
+    return tiles * -(-n // bn), 2 ** 32 // threads - 8
+
+
+@pytest.mark.parametrize("rows,k,n,groups,f32", [(1114112, 512, 14400, 65536, 0), (2 ** 21, 16, 13312, 65536, 0),
+                                                 (2 ** 20, 16, 20000, 65536, 0), (2 ** 20, 16, 20000, 65536, 1),
+                                                 (2 ** 20, 16, 16000, 65536, 1), (1114112, 512, 14400, 65536, 1)])
+def test_the_kernel_of_a_huge_grouped_call_is_one_that_a_launch_has_room_for(rows, k, n, groups, f32):
+    """Where some kernel has room, the one that is taken has it."""
+    shape = _hip.lib.dsv2_linear_fp8_blocks_tiles(rows, k, n, groups, f32)
+    able = []
+    for s in TILES:
+        needed, most = room(s, rows, n, groups, f32)
+        if s < 11 and not (s == 8 and (f32 or k <= 128)) and needed <= most:
+            able.append(s)
+    assert able and shape in able
+
+
 @pytest.mark.parametrize("args", [(0, 128, 128, 0, 0), (-1, 128, 128, 0, 0), (2 ** 31, 128, 128, 0, 0), (5, 0, 128, 0, 0),
                                   (5, -16, 128, 2, 0), (5, 128, 0, 0, 1), (5, 2 ** 30 + 1, 128, 0, 0), (5, 128, 128, -1, 0),
                                   (5, 128, 128, 65537, 0)])
