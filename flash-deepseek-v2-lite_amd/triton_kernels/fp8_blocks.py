@@ -13,6 +13,11 @@ throughout.  Activations [..., K] come with scales [..., ceil(K / 128)], weights
 Every function runs on its tensors' device and that device's current stream, takes no workspace and reads
 nothing back to the host: all may be captured into a graph.  Last dimensions have to be contiguous, rows may be any
 stride apart; whole 16-byte rows are read faster.
+
+Products with fp32 results are sums in fp32.  bf16 results (the default) take the 8-bit matrix instruction for the sum
+within a block: it aligns the products of 8 neighbouring columns to the largest of them and drops what lies 2^-13 below
+it, 1.3e-5 of the sum for normal values.  Where large terms cancel that can be more than bf16's rounding of what is left:
+ask for fp32 results there.  Blocks are added up in fp32 either way.
 """
 
 from __future__ import annotations
@@ -279,9 +284,10 @@ def _out_type(name: str, dtype: torch.dtype | None) -> tuple[torch.dtype, int]:
 
 def linear_fp8_blocks(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
                       output_dtype: torch.dtype | None = None) -> torch.Tensor:
-    """The product [..., N] of activations [..., K] (codes, scales) and weights [N, K] (codes, scales): fp32 sums, one
-    rounding to ``output_dtype`` (bf16, the default, or fp32).  A block's two scales are multiplied first, in fp32: their
-    product has to be in its range."""
+    """The product [..., N] of activations [..., K] (codes, scales) and weights [N, K] (codes, scales), rounded once to
+    ``output_dtype`` (bf16, the default, or fp32).  Sums are in fp32, for bf16 results with a narrower adder inside a block
+    (above): large terms that cancel need fp32 results.  A block's two scales are multiplied first, in fp32: their product
+    has to be in its range."""
     name = "linear_fp8_blocks"
     index = x.get_device()
     if (x.dim() == 2 and x_scales.dim() == 2 and weight.dim() == 2 and weight_scales.dim() == 2 and _plain(index) and
@@ -313,7 +319,7 @@ def grouped_linear_fp8_blocks(x: torch.Tensor, x_scales: torch.Tensor, weights: 
                               output_dtype: torch.dtype | None = None) -> torch.Tensor:
     """The products [R, N] of rows sorted by group (expert): rows offsets[e] .. offsets[e + 1] are multiplied by
     ``weights[e]`` of [E, N, K].  Row r is row r of ``x`` [R, K], or row ``rows[r]`` of ``x`` [T, K] (int32 [R]; a
-    row number outside x stands for zeros).
+    row number outside x stands for zeros).  Sums are those of ``linear_fp8_blocks``.
 
     ``offsets`` int32 [E + 1] is read on the device only.  Rows of no group are not written (here: undefined); an
     offset below the largest one before it, or outside [0, R], counts as the nearest that is not."""

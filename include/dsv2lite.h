@@ -600,8 +600,12 @@ int dsv2_rmsnorm_fp8_blocks(const void* x, int64_t x_stride, const void* residua
 int dsv2_silu_mul_fp8_blocks(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, int64_t rows,
                              int K, int dtype, void* codes, float* scales, void* stream);
 
-/* y[m, n] = sum over blocks b of x_scales[m, b] * w_scales[n / 128, b] * (codes x[m, b] . codes w[n, b]): sums in
- * fp32, one rounding to out_dtype.  A block's two scales are multiplied first, in fp32.  K and N up to 2^30.
+/* y[m, n] = sum over blocks b of x_scales[m, b] * w_scales[n / 128, b] * (codes x[m, b] . codes w[n, b]), rounded once to
+ * out_dtype.  Blocks are added up in fp32.  The sum within a block is in fp32 for fp32 results; for bf16 results it is the
+ * 8-bit matrix instruction's, which aligns the products of 8 neighbouring columns to the largest of them and drops what
+ * lies 2^-13 below it: 1.3e-5 of the sum for normal values, but where large terms cancel it can be more than bf16's
+ * rounding of what is left (take fp32 results there).  A block's two scales are multiplied first, in fp32.  K and N up to
+ * 2^30.
  * Strides in elements; rows of x and w need not be aligned (16-byte rows of whole 16 codes are read faster). */
 int dsv2_linear_fp8_blocks(const void* x, int64_t x_stride, const float* x_scales, int64_t x_scales_stride, int64_t rows,
                            int K, const void* w, int64_t w_stride, const float* w_scales, int64_t w_scales_stride, int N,

@@ -310,6 +310,25 @@ def test_linear_sums_whole_numbers_exactly(m):
     assert torch.equal(F.linear_fp8_blocks(x.to(E4), sx, w.to(E4), sw), want.to(BF))
 
 
+@pytest.mark.parametrize("m", [1, 40, 600])
+def test_linear_whose_largest_terms_cancel(m):
+    """Two terms of 448 * 448 and opposite sign, the others multiples of 2^-6 up to 1: what is left after them is exact in
+    fp32 results, whose every partial sum has 24 bits.  bf16 results may lose 15 * 2^-13 of each of the two."""
+    g = gen(m)
+    n, k = 150, 300
+    small = lambda rows: torch.randint(-8, 9, (rows, k), device=DEV, generator=g) / 8
+    sx, sw = torch.ones(m, R.blocks(k), device=DEV), torch.ones(R.blocks(n), R.blocks(k), device=DEV)
+    for a, b in ((0, 1), (3, 18), (5, 69), (0, 127), (200, 299), (100, 140)):
+        x, w = small(m), small(n)
+        x[:, a] = x[:, b] = w[:, a] = 448
+        w[:, b] = -448
+        x, w = x.to(E4), w.to(E4)
+        want, size = R.product(x, sx, w, sw)
+        assert torch.equal(F.linear_fp8_blocks(x, sx, w, sw, F32).double(), want)
+        off = (F.linear_fp8_blocks(x, sx, w, sw).double() - want).abs()
+        assert (off <= 15 * 2.0 ** -13 * size + 2.0 ** -8 * want.abs() * 1.01).all()
+
+
 def test_linear_of_every_code_and_of_none():
     """The 254 finite codes times one, NaN codes, infinite and NaN scales."""
     codes = torch.arange(256, dtype=torch.uint8, device=DEV).view(256, 1).view(E4)
