@@ -372,6 +372,32 @@ def test_products_leave_what_is_not_theirs():
             assert (y[:4] == 7).all() and (y[66:] == 7).all() and (y[:, 130:] == 7).all()
 
 
+@pytest.mark.parametrize("inter", [200, 203, 256])
+def test_gate_and_up_with_scales_of_their_own_into_one_buffer(inter):
+    """Through the C ABI: halves that are no whole blocks of 128 rows, as two products with the row stride of both; whole
+    blocks one behind the other, as one."""
+    r, h, kb, ib = 33, 300, 3, R.blocks(inter)
+    x, sx = matrix(r, h, 5, 1)
+    gate, up = matrix(inter, h, 6, 128), matrix(inter, h, 7, 128)
+    y = torch.zeros(r, 2 * inter, device=DEV, dtype=BF)
+    for (w, sw), at in ((gate, 0), (up, inter)):
+        _hip.call("dsv2_linear_fp8_blocks", x.data_ptr(), h, sx.data_ptr(), kb, r, h, w.data_ptr(), h, sw.data_ptr(), kb,
+                  inter, y.data_ptr() + 2 * at, 2 * inter, 0, _hip.stream_ptr())
+    for (w, sw), half in zip((gate, up), y.chunk(2, 1)):
+        R.check_product(half, x, sx, w, sw)
+    if inter % 128 == 0:
+        w = torch.cat([gate[0].view(torch.uint8), up[0].view(torch.uint8)]).view(E4)
+        assert torch.equal(F.linear_fp8_blocks(x, sx, w, torch.cat([gate[1], up[1]])), y)
+    codes = torch.empty(r, inter, device=DEV, dtype=E4)
+    scales = torch.empty(r, ib, device=DEV)
+    _hip.call("dsv2_silu_mul_fp8_blocks", y.data_ptr(), 2 * inter, y.data_ptr() + 2 * inter, 2 * inter, r, inter, 0,
+              codes.data_ptr(), scales.data_ptr(), _hip.stream_ptr())
+    g, u = y.double().chunk(2, 1)
+    q, s = R.rounded(g * torch.sigmoid(g) * u, 1)
+    R.check_codes(codes, q, 19 * U24)
+    R.check_scales(scales, s, 9 * U24)
+
+
 def check_grouped(y, x, sx, w, sw, offsets, rows=None):
     for e, (lo, hi) in enumerate(zip(offsets, offsets[1:])):
         if hi > lo:
