@@ -492,6 +492,40 @@ def test_every_kernel(shape, groups, k):
     assert ran, "no call reaches it"
 
 
+@pytest.mark.parametrize("shape,groups", [(s, g) for s in KERNELS for g in (0, 8)])
+def test_every_kernel_keeps_nans_to_their_rows_and_features(shape, groups):
+    """NaN codes and scales that are no numbers, in any block."""
+    n, k = KERNELS[shape][groups > 0], 1041 if shape >= 11 else 2064 if shape == 10 else 1040
+    ran = 0
+    for f32 in (False, True):
+        m = rows_for(shape, n, k, groups, f32)
+        if m is None:
+            continue
+        ran += 1
+        dtype = F32 if f32 else BF
+        w, sw = matrix(n, k, n + k, 128, groups or None)
+        x, sx = matrix(m, k, m + k, 1)
+        nx, xbad = with_nans(x, 0, 0.05, 1)
+        nw, wbad = with_nans(w, 0, 0.01, 2)
+        nsx = sx.clone()
+        nsx[m // 2, 3] = math.inf
+        nsx[m - 1, R.blocks(k) - 1] = math.nan
+        xbad[m // 2], xbad[m - 1] = True, True
+        nsw = sw.clone()
+        nsw[..., 1, R.blocks(k) - 1] = math.nan
+        wbad[..., 128:256] = True
+        if groups:
+            cuts = torch.randint(0, m + 1, (groups - 1,), generator=gen(k), device=DEV).sort().values.tolist()
+            offsets = i32([0, *cuts, m])
+            wbad = wbad[torch.searchsorted(offsets[1:].contiguous(), torch.arange(m, device=DEV), right=True)]
+            clean = F.grouped_linear_fp8_blocks(x, sx, w, sw, offsets, None, dtype)
+            got = F.grouped_linear_fp8_blocks(nx, nsx, nw, nsw, offsets, None, dtype)
+        else:
+            clean, got = F.linear_fp8_blocks(x, sx, w, sw, dtype), F.linear_fp8_blocks(nx, nsx, nw, nsw, dtype)
+        check_nans(torch.where(got.isfinite(), got, math.nan), clean, xbad[:, None] | wbad)
+    assert ran, "no call reaches it"
+
+
 @pytest.mark.parametrize("m,n,k", [(4200, 16376, 272), (700, 33000, 144), (9000, 4104, 1296), (4000, 8200, 2176),
                                    (4000, 8194, 1040), (700, 33003, 272)])
 def test_large_tiles_one_after_another(m, n, k):
