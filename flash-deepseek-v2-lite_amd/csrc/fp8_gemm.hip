@@ -228,9 +228,11 @@ __device__ __forceinline__ floatx4_t block_sum(const Decoded& w, const Decoded& 
 // same way, 64 a load.  Other rows go through registers, one block ahead of two stages.  A group of one wave needs no
 // barrier: its own waits order its loads and reads.  At the end the groups' sums meet in LDS, in fixed order.
 //
-// Few rows are bound by what a CU can load, 50 to 55 bytes a ns on MI355X whatever the depth of the ring (2 to 8), the
-// waves or the tile: 64 x 2,048 x 10,944 takes 11 us, 9.5 of them for 525 KB a CU.  So tiles are small enough for 256
-// CUs first, and large only beyond (1 x 3,648 x 2,048 3.3 us, 1.7 of them an empty launch; 1,024 x 2,816 x 2,048 17).
+// Few rows over a long K load 50 to 55 bytes a ns and CU on MI355X whatever the depth of the ring (2 to 8), the waves or
+// the tile: 64 x 2,048 x 10,944 takes 11.3 us, 9.5 of them for 525 KB a CU.  What holds them there is not known, but not
+// the CU's load rate: 128 x 128 tiles load 68, and loads alone reach 150 from L2 (80 where rows straddle lines, which
+// costs a twentieth here: rows 11,008 apart take 11.0).  Half the bytes a CU gain a tenth.  Tiles are small enough for
+// 256 CUs first, and large only beyond (1 x 3,648 x 2,048 3.6 us, 1.7 of them an empty launch; 1,024 x 2,816 x 2,048 17).
 // ---------------------------------------------------------------------------
 // 16 (4) bytes a lane from src to LDS, lane after lane from dst; in functions of their own: with the builtin in a
 // template hipcc drops the kernel's host launch stub
@@ -465,10 +467,10 @@ __global__ __launch_bounds__(64 * WM * WN * KW) void ring_kernel(const Args a) {
 // next block's first fragments are read under the matrix instructions that are left.  Sums are added three
 // instructions behind.  The next tile's first two blocks follow this one's last two without a gap.
 //
-// Bound by the issue of instructions and by power: a wave issues some 215 vector instructions a block, 32 of them
-// matrix, and the matrix cores are busy for 48 to 52% of the cycles, at 1.8 GHz (LDS 30%).  MI355X: 8,192 x 21,888 x
-// 2,048 355 us (2.07 PFLOP/s), 8,192^3 475 (2.31); 128 x 256 tiles of ring_kernel 552 and 648, but 23 for 31 with 1,024
-// x 2,816 x 2,048.  Groups: 49,152 rows of 64, 2,816 x 2,048, 350 us, 1.17 times their rows in tiles.
+// Bound by the issue of instructions and by power: a wave issues some 216 vector instructions a block, 32 of them
+// matrix, and the matrix cores are busy for 47% of the cycles, at 1.9 to 2.0 GHz (LDS 24%).  MI355X: 8,192 x 21,888 x
+// 2,048 354 to 363 us (2.02 to 2.07 PFLOP/s), 8,192^3 479 (2.29); 128 x 256 tiles of ring_kernel 552 and 648, but 23 for 31
+// with 1,024 x 2,816 x 2,048.  Groups: 49,152 rows of 64, 2,816 x 2,048, 352 to 366 us, 1.17 times their rows in tiles.
 // ---------------------------------------------------------------------------
 struct Big {
   static constexpr int BM = 256, BN = 256, kThreads = 512, kWgs = 256;
@@ -841,7 +843,8 @@ int shape_of(const Args& a, bool grouped) {
   // Weights that are read once and do not stay in the 256 MB of the last-level cache (a model's others are read in
   // between): one wave a tile, many workgroups a CU, and the non-temporal hint (MI355X: 5 x 102,400 x 2,048, fp32, 36.6
   // us, 5.8 TB/s, the best of the others 49.6; 64 tokens x 6 of 64 groups of 2,816 x 2,048 62.4 / 75.6).  Smaller ones
-  // the other way: 64 x 2,048 x 10,944 (22 MB) 30 / 11, 1 x 3,648 x 2,048 (7 MB) 8 / 3.5.
+  // the other way: 64 x 2,048 x 10,944 (22 MB) 30 / 11, 1 x 3,648 x 2,048 (7 MB) 8 / 3.5.  Groups go by their mean, which
+  // is all that the host knows: 1,020 rows of 64 groups 94 us where most groups have some, 48 where one has them all.
   if (a.rows <= 16 * (grouped ? (int64_t)a.groups : 1) && (int64_t)a.groups * a.N >= (kStreamed + a.K - 1) / a.K &&
       launchable(a, grouped, kStream))
     return kStream;

@@ -4,9 +4,9 @@
 //
 // A block of a row is 16 lanes of 8 values: one 16-byte load a lane of bf16, the largest value by four
 // DPP steps, one 8-byte store of codes.  All of it is bound by memory (2 to 9 bytes a value for some 10
-// to 30 instructions), for few rows by the launch and one trip to memory.  MI355X, bf16: 64 x 2,048 1.9 us, an empty
-// launch 1.7; SwiGLU of 49,152 x 1,408 57.5 us, 6.0 TB/s (a large copy 5.7: some of it stays in the last-level
-// cache); 384 x 1,408 2.6.
+// to 30 instructions), for few rows by the launch and one trip to memory.  MI355X, bf16, a call in a replayed graph over
+// three sets of tensors: 64 x 2,048 2.2 us, an empty launch 1.7; SwiGLU of 49,152 x 1,408 58 to 61 us, 5.7 to 6.0 TB/s (a
+// large copy 5.7: some of it stays in the last-level cache); 384 x 1,408 2.9.
 #include "fp8_blocks.h"
 
 namespace {
@@ -292,7 +292,8 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a) {
 // A wave a row where it holds the row in one chunk, else four (MI355X, bf16 with a residual, a wave / four: 8,192 x
 // 512 7.4 / 9.1 us, 65,536 x 128 21 / 45; in four chunks 8,192 x 2,048 19.3 / 18.8, 64 x 2,048 4.1 / 2.7).  Maxima in
 // registers or scales read back: 64 x 2,048 2.7 / 3.1, 64 x 4,096 3.2 / 3.5, 64 x 8,192 4.3 / 4.9, 4,096 x 8,192
-// 38.8 / 39.4.  8,192 x 2,048 moves 118 MB at 6.1 TB/s, more than a copy past the caches (5.7): some of it stays in them.
+// 38.8 / 39.4.  8,192 x 2,048 moves 118 MB in 18.6 to 21.8 us, 5.4 to 6.3 TB/s (a copy past the caches 5.7: some of it
+// stays in them).
 template <typename T, bool RES, bool VEC>
 void launch_norm(const NormArgs& a, hipStream_t st) {
   if (a.K <= 512) {
@@ -326,11 +327,12 @@ void launch_blocks(const BlockArgs& a, bool vec, hipStream_t st) {
   else block_kernel<T, SILU, false, NB, false><<<grid, 256, 0, st>>>(a);
 }
 
-// One block for each 16 lanes, two where there are many workgroups either way (MI355X, one / two: 1,024 blocks of rows
-// 3.1 / 3.6 us, 65,536 6.7 / 6.7, 131,072 11.1 / 10.4, 640,000 45 / 40), but not of SwiGLU, which hides its loads by
-// its own instructions (33,000 blocks 7.0 / 7.9, 330,000 37.7 / 39.1).  Two with non-temporal loads for what cannot stay
-// in the 256 MB of the last-level cache (80,000 x 2,048 rows 85 -> 77; 49,152 x 1,408 SwiGLU 61.4 -> 56.5; in the
-// cache 17.1 -> 19.8 and 22.1 -> 23.6).
+// One block for each 16 lanes, two where there are many workgroups either way (MI355X, calls in a replayed graph over
+// three sets of tensors, one / two: 16,384 blocks of rows 3.1 / 3.2 us, 65,536 6.6 / 6.5, 131,072 10.9 / 10.4, 640,000
+// 47 / 41), but not of SwiGLU, which hides its loads by its own instructions (33,000 blocks 6.9 / 7.7; at
+// 330,000 the two are even, 41.3 / 39.9 and over one set 35.4 / 35.1).  Two with non-temporal loads for what cannot stay in
+// the 256 MB of the last-level cache (80,000 x 2,048 rows 85.5 -> 77.3; 49,152 x 1,408 SwiGLU 63.9 -> 60.0; in the
+// cache, 8,192 rows 10.3 -> 11.5, 30,000 of SwiGLU over one set 35.1 -> 40.7).
 template <typename T, bool SILU>
 void launch_blocks(const BlockArgs& a, bool vec, hipStream_t st) {
   const int64_t bytes = a.n_blocks * kFp8Block * (int64_t)sizeof(T) * (SILU ? 2 : 1);
